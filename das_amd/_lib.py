@@ -10,10 +10,11 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, 'csrc', 'libdas_hip.so')
 
 DAS_OK, DAS_ERR_ARG, DAS_ERR_LAUNCH = 0, 1, 2
-DAS_F32, DAS_BF16 = 0, 1
+DAS_F32, DAS_BF16, DAS_F16 = 0, 1, 2
+DAS_NS_MAX_STEPS = 16
 DAS_MAX_LEVELS = 5
 
-vp, i32, f32, i64 = C.c_void_p, C.c_int, C.c_float, C.c_longlong
+vp, i32, f32, i64, f64 = C.c_void_p, C.c_int, C.c_float, C.c_longlong, C.c_double
 
 
 class DasConvDesc(C.Structure):
@@ -67,6 +68,21 @@ class DasPhotometric(C.Structure):
 class DasRleDesc(C.Structure):
     _fields_ = [('J', i32), ('sets', i32), ('npos', i32), ('pose_ps', i32), ('aux_ps', i32), ('stride2', i32),
                 ('stride3', i32), ('amp', f32), ('beta', f32)]
+
+
+class DasNsShape(C.Structure):
+    _fields_ = [('off', i64), ('count', i32), ('rows', i32), ('cols', i32), ('reserved', i32)]
+
+
+class DasNsPlan(C.Structure):
+    _fields_ = [('n_groups', i32), ('n_matrices', i32), ('n_chunks', i32), ('n_gram', i32), ('n_update', i32), ('steps', i32),
+                ('x_elems', i64), ('a_elems', i64), ('extent', i64),
+                ('mat_at', i64), ('chunk_at', i64), ('gram_at', i64), ('update_at', i64), ('table_bytes', i64),
+                ('coef', f32 * (3 * DAS_NS_MAX_STEPS)), ('eps', f32)]
+
+
+class DasNsSource(C.Structure):
+    _fields_ = [('base', vp), ('batch_stride', i64), ('row_stride', i64)]
 
 
 class DasDecodeDesc(C.Structure):
@@ -164,6 +180,11 @@ SIGNATURES = {
     'das_rle_backward': (i32, [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, C.POINTER(DasRleDesc), vp, vp, vp]),
     'das_grad_sumsq': (i32, [vp, i64, vp, i32, vp]),
     'das_sgd_momentum_step': (i32, [vp, vp, vp, i64, f32, f32, f32, f32, f32, vp, i32, vp]),
+    'das_ns_plan': (i32, [C.POINTER(DasNsShape), i32, i32, C.POINTER(f32), f32, C.POINTER(DasNsPlan), vp, i64]),
+    'das_ns_ws_bytes': (i64, [C.POINTER(DasNsPlan)]),
+    'das_orthogonalize': (i32, [C.POINTER(DasNsPlan), vp, C.POINTER(DasNsSource), i32, i32, vp, i32, vp, vp]),
+    'das_muon_step': (i32, [C.POINTER(DasNsPlan), vp, vp, vp, vp, f32, f32, f32, i32, i32, f32, f32, vp, vp, vp]),
+    'das_adamw_step': (i32, [vp, vp, vp, vp, i64, f64, f64, f64, f64, f64, i64, f32, f32, vp, vp]),
     'das_decode_cap': (i32, [C.POINTER(DasDecodeDesc)]),
     'das_decode_ws_bytes': (i64, [i32, i32, i32]),
     'das_decode': (i32, [C.POINTER(DasDecodeDesc), vp, vp, vp, vp, vp, vp, vp]),

@@ -1,4 +1,4 @@
-"""ctypes wrappers of the loss / target / optimizer entry points (train_loss.hip)."""
+"""ctypes wrappers of the loss / target / optimizer entry points (train_loss.hip, adamw.hip, muon.hip)."""
 import ctypes as C
 
 import torch
@@ -144,6 +144,164 @@ def sgd_momentum_step(p, g, buf, lr, momentum, weight_decay, grad_scale=1.0, max
     _lib.check(_lib.load().das_sgd_momentum_step(_ptr(p), _ptr(g), _ptr(buf), p.numel(), lr, momentum, weight_decay,
                                                  grad_scale, max_norm, _ptr(grad_sumsq_t), int(first_step), _stream()),
                'das_sgd_momentum_step')
+
+
+# ------------------------------------------------------------------ AdamW, Newton-Schulz orthogonalisation, Muon
+def _flat_buffers(what, *ts):
+    """Contiguous f32 tensors of one size on one GPU: what the flat-buffer optimizer steps take."""
+    _need_gpu(*ts)
+    for t in ts:
+        if t.dtype != torch.float32 or not t.is_contiguous() or t.numel() != ts[0].numel() or t.device != ts[0].device:
+            raise _lib.DasHipError(f'{what}: parameters, gradients and state are contiguous float32 tensors of one size on one device')
+
+
+def _clip_sum(what, max_norm, grad_sumsq_t, device):
+    if not max_norm > 0:
+        return None
+    if grad_sumsq_t is None or grad_sumsq_t.dtype != torch.float32 or grad_sumsq_t.device != device:
+        raise _lib.DasHipError(f'{what}: max_norm > 0 needs grad_sumsq_t, the f32 sum of squares of the whole gradient (grad_sumsq)')
+    return grad_sumsq_t
+
+
+def adamw_step(p, g, m, v, lr, step, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=1e-2, grad_scale=1.0, max_norm=0.0,
+               grad_sumsq_t=None):
+    """One AdamW step (decoupled weight decay, bias-corrected moments) in place on flat f32 buffers, `step` counting from 1; the
+    gradient is used times grad_scale * min(1, max_norm / (sqrt(grad_sumsq_t) * grad_scale + 1e-6)) (max_norm <= 0: no clipping). A NaN
+    norm makes every element NaN. Scalars are fixed when a call is captured into a hipGraph."""
+    _flat_buffers('adamw_step', p, g, m, v)
+    sumsq = _clip_sum('adamw_step', max_norm, grad_sumsq_t, p.device)
+    if p.numel() == 0:
+        return
+    with torch.cuda.device(p.device):
+        _lib.check(_lib.load().das_adamw_step(_ptr(p), _ptr(g), _ptr(m), _ptr(v), p.numel(), float(lr), float(beta1), float(beta2),
+                                              float(eps), float(weight_decay), int(step), float(grad_scale), float(max_norm),
+                                              _ptr(sumsq), _stream()), 'das_adamw_step')
+
+
+NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)   # quintic of the published Muon optimizer: singular values of [1e-3, 1] -> [0.7, 1.2]
+
+
+class NewtonSchulzPlan:
+    """The tables of das_orthogonalize / das_muon_step for one set of matrices: built once, usable by any number of calls, on any
+    stream (a plan is read-only; workspaces come from torch's allocator call by call).
+
+    shapes: (rows, cols) or (count, rows, cols) of equal matrices, in storage order. offsets: element offset of each entry's first
+    matrix in the flat buffers of muon_step (default: back to back; only such a plan serves orthogonalize). coefficients: (a, b, c) for every step or one triple
+    per step. Entries without elements are allowed and left alone."""
+
+    def __init__(self, shapes, device, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, offsets=None):
+        self.shapes = [(1,) + tuple(int(v) for v in s) if len(s) == 2 else tuple(int(v) for v in s) for s in shapes]
+        self.device = torch.device(device)
+        if self.device.type != 'cuda':
+            raise _lib.DasHipError('das_amd ops run on the GPU only (no CPU fallback); got device ' + str(device))
+        if self.device.index is None:
+            self.device = torch.device('cuda', torch.cuda.current_device())
+        if any(len(s) != 3 or min(s) < 0 for s in self.shapes) or not 1 <= int(steps) <= _lib.DAS_NS_MAX_STEPS:
+            raise _lib.DasHipError(f'NewtonSchulzPlan: shapes are (rows, cols) or (count, rows, cols), steps 1 ... {_lib.DAS_NS_MAX_STEPS}')
+        co = [float(v) for v in coefficients] if isinstance(coefficients[0], (int, float)) else \
+            [float(v) for t in coefficients for v in t]
+        co = co * int(steps) if len(co) == 3 else co
+        if len(co) != 3 * int(steps):
+            raise _lib.DasHipError('NewtonSchulzPlan: one (a, b, c) triple, or one for every step')
+        self.steps, self.eps = int(steps), float(eps)
+        sizes = [k * r * c for k, r, c in self.shapes]
+        if offsets is None:
+            self.offsets = [sum(sizes[:i]) for i in range(len(sizes))]
+        else:
+            self.offsets = [int(o) for o in offsets]
+            if len(self.offsets) != len(sizes):
+                raise _lib.DasHipError('NewtonSchulzPlan: one offset for every entry of shapes')
+        live = [(o, s) for o, s, n in zip(self.offsets, self.shapes, sizes) if n]
+        self._flat = self._build(live, co)
+        # orthogonalize()'s results: one flat output, every entry on a 16-byte boundary of it
+        self._out, self._out_offsets, self._out_size = None, [], 0
+        if offsets is None:
+            for n in sizes:
+                self._out_offsets.append(self._out_size)
+                self._out_size += (n + 7) // 8 * 8
+            self._out = self._flat if self._out_offsets == self.offsets else \
+                self._build([(o, s) for o, s, n in zip(self._out_offsets, self.shapes, sizes) if n], co)
+
+    def _build(self, entries, co):
+        """-> (DasNsPlan, device tables, workspace bytes), None for no entries"""
+        if not entries:
+            return None
+        lib = _lib.load()
+        arr = (_lib.DasNsShape * len(entries))()
+        for a, (o, (k, r, c)) in zip(arr, entries):
+            a.off, a.count, a.rows, a.cols = o, k, r, c
+        plan = _lib.DasNsPlan()
+        cf = (C.c_float * len(co))(*co)
+        _lib.check(lib.das_ns_plan(arr, len(entries), self.steps, cf, self.eps, C.byref(plan), None, 0), 'das_ns_plan')
+        host = torch.empty(plan.table_bytes, dtype=torch.uint8)
+        _lib.check(lib.das_ns_plan(arr, len(entries), self.steps, cf, self.eps, C.byref(plan), _ptr(host), plan.table_bytes), 'das_ns_plan')
+        return plan, host.to(self.device), lib.das_ns_ws_bytes(C.byref(plan))
+
+
+def orthogonalize(mats, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, out_dtype=torch.bfloat16, plan=None):
+    """The orthogonal factor of every matrix of a list (or of one tensor) by `steps` Newton-Schulz products: for U = mats[i],
+    X = U / (|U| + eps), then X <- (a I + b X X^T + c (X X^T)^2) X. 2-D tensors are one matrix, 3-D ones a stack; f32, bf16 or f16 (one
+    type a call), any row / stack stride, unit column stride. Returns tensors of the same shapes, bf16 (default) or f16.
+    plan: a NewtonSchulzPlan of these shapes (built here if None, which copies its tables to the device: keep one where the call
+    repeats; inside a hipGraph capture it is required). Products take f16 operands: a few 1e-3 off exact arithmetic, up to
+    5e-2 for matrices whose singular values span many orders of magnitude. Inf or NaN in a matrix makes that matrix NaN, no other."""
+    one = torch.is_tensor(mats)
+    mats = [mats] if one else list(mats)
+    _need_gpu(*mats)
+    if out_dtype not in (torch.bfloat16, torch.float16):
+        raise _lib.DasHipError('orthogonalize: out_dtype is bfloat16 or float16')
+    if not mats:
+        return []
+    dt = {torch.float32: _lib.DAS_F32, torch.bfloat16: _lib.DAS_BF16, torch.float16: _lib.DAS_F16}.get(mats[0].dtype)
+    if dt is None or any(t.dtype != mats[0].dtype or t.device != mats[0].device or t.dim() not in (2, 3) for t in mats):
+        raise _lib.DasHipError('orthogonalize: 2-D or 3-D tensors of one type (float32, bfloat16, float16) on one device')
+    shapes = [tuple(t.shape) if t.dim() == 3 else (1,) + tuple(t.shape) for t in mats]
+    dev = mats[0].device
+    if plan is None:
+        plan = NewtonSchulzPlan(shapes, dev, steps=steps, coefficients=coefficients, eps=eps)
+    if plan.shapes != shapes or plan.device != dev:
+        raise _lib.DasHipError(f'orthogonalize: the plan is for {plan.shapes} on {plan.device}, the tensors are {shapes} on {dev}')
+    mats = [t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous() for t in mats]
+    if len(plan._out_offsets) != len(shapes):
+        raise _lib.DasHipError('orthogonalize: a plan with offsets of its own is for muon_step')
+    out = torch.empty(plan._out_size, dtype=out_dtype, device=dev)
+    if plan._out is not None:
+        p, tables, ws_bytes = plan._out
+        live = [t for t in mats if t.numel()]
+        src = (_lib.DasNsSource * len(live))()
+        for s, t in zip(src, live):
+            s.base, s.row_stride, s.batch_stride = t.data_ptr(), t.stride(-2), t.stride(0) if t.dim() == 3 else 0
+        with torch.cuda.device(dev):
+            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+            _lib.check(_lib.load().das_orthogonalize(C.byref(p), _ptr(tables), src, len(live), dt, _ptr(out),
+                                                     _lib.DAS_BF16 if out_dtype == torch.bfloat16 else _lib.DAS_F16, _ptr(ws),
+                                                     _stream()), 'das_orthogonalize')
+    res = [out[o:o + t.numel()].view(t.shape) for o, t in zip(plan._out_offsets, mats)]
+    return res[0] if one else res
+
+
+def muon_step(p, g, buf, plan, lr, momentum=0.95, weight_decay=0.0, nesterov=True, lr_scale='original', grad_scale=1.0, max_norm=0.0,
+              grad_sumsq_t=None):
+    """One Muon step in place on flat f32 buffers holding the plan's matrices (parameters, gradients, momentum; what lies between them
+    is not touched): momentum average, orthogonalised direction, decoupled weight decay. lr_scale: 'original' = the
+    update of a rows x cols matrix times sqrt(max(1, rows / cols)); 'match_rms_adamw' = times 0.2 sqrt(max(rows, cols)), the size
+    of an AdamW update. Gradient scaling and clipping as in adamw_step."""
+    _flat_buffers('muon_step', p, g, buf)
+    sumsq = _clip_sum('muon_step', max_norm, grad_sumsq_t, p.device)
+    if lr_scale not in ('original', 'match_rms_adamw'):
+        raise _lib.DasHipError("muon_step: lr_scale is 'original' or 'match_rms_adamw'")
+    if plan.device != p.device:
+        raise _lib.DasHipError(f'muon_step: the plan is on {plan.device}, the buffers on {p.device}')
+    if plan._flat is None:
+        return
+    c_plan, tables, ws_bytes = plan._flat
+    if c_plan.extent > p.numel():
+        raise _lib.DasHipError(f'muon_step: the plan reaches element {c_plan.extent} of buffers of {p.numel()}')
+    with torch.cuda.device(p.device):
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=p.device)
+        _lib.check(_lib.load().das_muon_step(C.byref(c_plan), _ptr(tables), _ptr(p), _ptr(g), _ptr(buf), float(lr), float(momentum),
+                                             float(weight_decay), int(bool(nesterov)), int(lr_scale != 'original'), float(grad_scale),
+                                             float(max_norm), _ptr(sumsq), _ptr(ws), _stream()), 'das_muon_step')
 
 
 # ------------------------------------------------------------------ RealNVP log-density (RLE pose loss)

@@ -606,6 +606,62 @@ int das_sgd_momentum_step(float* p, const float* g, float* buf, long long n, flo
                           int first_step, void* stream);
 
 /* ------------------------------------------------------------------------------------
+ * Muon and AdamW: the optimizers beside SGD (no reference counterpart; the reference trains with torch.optim.SGD).
+ *
+ * Newton-Schulz orthogonalisation of a ragged set of matrices. For each matrix U (rows x cols, m = min, n = max of the two,
+ * transposed if rows > cols so that X is m x n):
+ *   X = U / (|U|_F + eps);   steps times:  A = X X^T,  B = a I + b A + c A^2,  X = B X.
+ * Products take f16 operands and sum in f32; X, A and B are rounded to f16 between products (X carries a power-of-two scale that
+ * keeps its entries in f16's normal range), so a result is a few 1e-3 off a 64-bit evaluation for the gradients of a
+ * training run, and up to 5e-2 (2-norm) for matrices whose singular values span many orders of magnitude. The sum of squares and
+ * the joint scale of each 64 x 64 block are held in f32 / f64. Results do not depend on what else is in the set, and are the
+ * same bits from run to run.
+ *
+ * A plan lists the set once: das_ns_plan() checks the shapes and the polynomial and writes the tables (host memory) that the
+ * kernels walk; the caller copies them to the device and hands both to every call. Plans hold no pointers and no results. */
+#define DAS_F16 2
+#define DAS_NS_MAX_STEPS 16
+typedef struct {
+  long long off;   /* element offset of the first matrix in the flat buffers (das_muon_step) / in `out` (das_orthogonalize) */
+  int count, rows, cols;   /* `count` equal matrices, dense, back to back */
+  int reserved;
+} DasNsShape;
+typedef struct {
+  int n_groups, n_matrices, n_chunks, n_gram, n_update, steps;
+  long long x_elems, a_elems, extent;            /* work areas (f16 elements); one past the last element of the flat buffers used */
+  long long mat_at, chunk_at, gram_at, update_at, table_bytes;   /* byte offsets of the tables */
+  float coef[3 * DAS_NS_MAX_STEPS];              /* a, b, c of each step */
+  float eps;
+} DasNsPlan;
+/* One source tensor of das_orthogonalize: `count` matrices, element (i, r, c) at base[i * batch_stride + r * row_stride + c]. */
+typedef struct {
+  const void* base;
+  long long batch_stride, row_stride;
+} DasNsSource;
+/* Fills *plan; with tables != NULL (plan->table_bytes host bytes) also the tables. DAS_ERR_ARG: n < 1, a shape without elements or
+ * with a side over 1 << 20, overlapping matrices, steps outside 1 ... DAS_NS_MAX_STEPS, a polynomial that takes [0, 1] out of
+ * [-16, 16] within `steps` steps (f16 would overflow), eps < 0, or tables too small. */
+int das_ns_plan(const DasNsShape* shapes, int n, int steps, const float* coef, float eps, DasNsPlan* plan, void* tables,
+                long long table_bytes);
+long long das_ns_ws_bytes(const DasNsPlan* plan);
+/* out (flat, out_dtype DAS_BF16 or DAS_F16, plan offsets): the orthogonalised matrices; srcs: one per group of the plan, in_dtype
+ * DAS_F32 / DAS_BF16 / DAS_F16. `ws`: das_ns_ws_bytes() of device memory, 16-byte aligned, in use until the call's kernels end. */
+int das_orthogonalize(const DasNsPlan* plan, const void* tables_dev, const DasNsSource* srcs, int n_srcs, int in_dtype, void* out,
+                      int out_dtype, void* ws, void* stream);
+/* Muon: with g' = g * grad_scale * min(1, max_norm / (sqrt(*grad_sumsq) * grad_scale + 1e-6)) (no clipping for max_norm <= 0),
+ *   buf = momentum * buf + (1 - momentum) * g';   U = nesterov ? (1 - momentum) * g' + momentum * buf : buf;
+ *   p = p * (1 - lr * weight_decay) - lr * f * orthogonalised(U),   f = sqrt(max(1, rows / cols)) (lr_scale 0) or
+ *   0.2 * sqrt(max(rows, cols)) (lr_scale 1). Elements of p, g, buf outside the plan's matrices are not touched. */
+int das_muon_step(const DasNsPlan* plan, const void* tables_dev, float* p, const float* g, float* buf, float lr, float momentum,
+                  float weight_decay, int nesterov, int lr_scale, float grad_scale, float max_norm, const float* grad_sumsq,
+                  void* ws, void* stream);
+/* AdamW on flat f32 buffers, g' as above, t = step >= 1:
+ *   m = beta1 m + (1 - beta1) g';  v = beta2 v + (1 - beta2) g'^2;
+ *   p = p (1 - lr weight_decay) - lr (m / (1 - beta1^t)) / (sqrt(v / (1 - beta2^t)) + eps). */
+int das_adamw_step(float* p, const float* g, float* m, float* v, long long n, double lr, double beta1, double beta2, double eps,
+                   double weight_decay, long long step, float grad_scale, float max_norm, const float* grad_sumsq, void* stream);
+
+/* ------------------------------------------------------------------------------------
  * Decode (das_head.py:690-796 `_get_poses_single`, pose_nms.py:51-126 oks_iou / oks_nms), fused:
  * per image  score = sigmoid(cls)*sigmoid(ctr) -> keep score > score_thr -> per level keep the
  * nms_pre best when the level has more than nms_pre locations -> center = (point - offset)/scale,

@@ -1,0 +1,320 @@
+"""Newton-Schulz orthogonalisation, the Muon step and the AdamW step against 64-bit evaluations of their formulas."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = 'cuda'
+COEF = (3.4445, -4.7750, 2.0315)
+U16 = 2.0 ** -11     # half a step of f16
+HALF = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+
+
+def gradient(r, c, seed, k=None):
+    """a sum over pixels of output gradients times rectified features, as a layer's weight gradient is"""
+    gen = torch.Generator().manual_seed(seed)
+    n = (k or 1)
+    out = []
+    for _ in range(n):
+        pix = 2 * max(r, c) + 16
+        d = torch.randn(pix, r, generator=gen) * torch.exp(torch.randn(r, generator=gen))
+        out.append(d.t() @ (torch.randn(pix, c, generator=gen) + torch.randn(pix, 1, generator=gen)).relu())
+    g = torch.stack(out).to(DEV)
+    return g if k else g[0]
+
+
+def ns64(u, coef, eps=1e-7):
+    """(result in f64, bound on the 2-norm of a f16 evaluation's error). The bound follows the roundings: f16 holds X, A and B (relative
+    U16 each, and 2^-25 absolute below its normal range; X is scaled by about sqrt(n)); an error of X grows by at most L = max |p'|
+    over the singular values' range in a step (the derivative of an odd function of a matrix is bounded, in the 2-norm over all
+    entries, by its divided differences); f32 sums over K products add K 2^-23."""
+    x = u.double()
+    x = x / (x.norm() + eps)
+    if x.shape[0] > x.shape[1]:
+        y, e = ns64(u.t(), coef, eps)
+        return y.t(), e
+    m, n = x.shape
+    tiny = 2.0 ** -25 * math.sqrt(m * n) / math.sqrt(n) * 2
+    eye = torch.eye(m, dtype=torch.float64, device=x.device)
+    err = 2 * U16 * float(x.norm()) + 2 * tiny
+    for a, b, c in coef:
+        s2 = min(float(torch.linalg.matrix_norm(x, 2)) if m <= 512 else 1.25, float(x.norm()))
+        s = torch.linspace(0, max(s2, 1e-30) * 1.01, 2048, dtype=torch.float64)
+        lip = float((a + 3 * b * s ** 2 + 5 * c * s ** 4).abs().max())
+        g = x @ x.T
+        q = a * eye + b * g + c * (g @ g)
+        y = q @ x
+        acc = (n + 2 * m) * 2.0 ** -23
+        da = (U16 + acc) * float(g.norm()) + 2.0 ** -25 * m
+        db = abs(b) * da + abs(c) * 2 * s2 * s2 * da + (U16 + acc) * (float(q.norm())) + 2.0 ** -25 * m
+        err = lip * err + db * s2 + (U16 + acc) * float(y.norm()) + tiny
+        x = y
+    return x, err
+
+
+def check(got, u, coef, eps=1e-7, what=''):
+    ref, err = ns64(u, coef, eps)
+    d = float((got.double() - ref).norm())
+    tol = 1.1 * err + HALF[got.dtype] * float(ref.norm())
+    assert torch.isfinite(got).all(), what
+    assert d <= tol, (what, d, tol, float(ref.norm()))
+
+
+SHAPES = [(1, 1), (1, 64), (64, 1), (2, 3), (45, 256), (27, 2304), (64, 64), (64, 147), (65, 63), (63, 65), (128, 1152), (129, 1023),
+          (256, 64), (333, 77), (512, 128), (500, 513), (700, 513), (256, 2304)]
+
+
+@pytest.mark.parametrize('steps', [1, 2, 5])
+@pytest.mark.parametrize('shape', SHAPES, ids=lambda s: '%dx%d' % s)
+def test_orthogonalize_one_matrix(shape, steps):
+    from das_amd import train_ops as T
+    u = gradient(*shape, seed=shape[0] * 7 + shape[1])
+    check(T.orthogonalize(u, steps=steps), u, [COEF] * steps)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('out_dtype', [torch.bfloat16, torch.float16])
+def test_orthogonalize_set(dtype, out_dtype):
+    """every matrix of a ragged set comes out as it does alone, bit for bit, and a second call gives the same bits"""
+    from das_amd import train_ops as T
+    mats = [gradient(r, c, 3 * r + c, k=k) for k, r, c in [(3, 45, 256), (1, 333, 77), (2, 64, 64), (1, 1, 256), (5, 64, 3), (1, 129, 640)]]
+    mats = [(t * (1e-3 if dtype == torch.float16 else 1)).to(dtype) for t in mats]
+    plan = T.NewtonSchulzPlan([tuple(t.shape) for t in mats], DEV)
+    got = T.orthogonalize(mats, plan=plan, out_dtype=out_dtype)
+    again = T.orthogonalize(mats, plan=plan, out_dtype=out_dtype)
+    for t, y, z in zip(mats, got, again):
+        assert y.shape == t.shape and y.dtype == out_dtype and torch.equal(y, z)
+        for i in range(t.shape[0]):
+            check(y[i], t[i], [COEF] * 5, what=tuple(t.shape))
+            assert torch.equal(y[i], T.orthogonalize(t[i], out_dtype=out_dtype))
+
+
+def test_orthogonalize_strides_and_offsets():
+    """rows and stacks of any stride, starts that no vector load could take, a transposed view"""
+    from das_amd import train_ops as T
+    base = gradient(131, 407, 5)
+    view = base[1:120, 3:400]
+    check(T.orthogonalize(view), view, [COEF] * 5)
+    stack = gradient(60, 100, 6, k=5)[::2, 1:, 1:98]
+    for i, y in enumerate(T.orthogonalize(stack)):
+        check(y, stack[i], [COEF] * 5)
+    half = base.bfloat16()[:, 1:]
+    check(T.orthogonalize(half), half, [COEF] * 5)
+    check(T.orthogonalize(base.t()), base.t(), [COEF] * 5)
+    same = base[:1].expand(64, -1)       # a row stride of zero: rank one
+    check(T.orthogonalize(same), same, [COEF] * 5)
+
+
+@pytest.mark.parametrize('mag', [1e-30, 1e-12, 1e12, 1e30])
+def test_orthogonalize_magnitudes(mag):
+    from das_amd import train_ops as T
+    u = gradient(96, 160, 9)
+    u = u / u.norm() * mag
+    check(T.orthogonalize(u, eps=0.0 if mag < 1 else 1e-7), u, [COEF] * 5, eps=0.0 if mag < 1 else 1e-7)
+
+
+def test_orthogonalize_hard_spectra():
+    """rank one, low rank, zeros, a single huge entry"""
+    from das_amd import train_ops as T
+    gen = torch.Generator().manual_seed(1)
+    a = (torch.randn(96, 8, generator=gen) @ torch.randn(8, 300, generator=gen)).to(DEV)
+    check(T.orthogonalize(a), a, [COEF] * 5)
+    one = torch.outer(torch.randn(70, generator=gen), torch.randn(200, generator=gen)).to(DEV)
+    check(T.orthogonalize(one), one, [COEF] * 5)
+    assert not T.orthogonalize(torch.zeros(40, 70, device=DEV)).any()
+    spike = 1e-6 * torch.randn(65, 130, generator=gen)
+    spike[64, 129] = 1e6
+    spike = spike.to(DEV)
+    check(T.orthogonalize(spike), spike, [COEF] * 5)
+
+
+@pytest.mark.parametrize('bad', [float('nan'), float('inf'), -float('inf')])
+def test_orthogonalize_nonfinite_stays_in_its_matrix(bad):
+    from das_amd import train_ops as T
+    a, b, c = gradient(64, 100, 1), gradient(70, 100, 2), gradient(100, 70, 3)
+    clean = T.orthogonalize([a, b, c])
+    b = b.clone()
+    b[69, 99] = bad
+    got = T.orthogonalize([a, b, c])
+    assert torch.equal(got[0], clean[0]) and torch.equal(got[2], clean[2])
+    assert torch.isnan(got[1]).all()
+
+
+def test_orthogonalize_other_polynomials_and_empty():
+    from das_amd import train_ops as T
+    u = gradient(80, 120, 4)
+    cubic = (1.5, -0.5, 0.0)
+    check(T.orthogonalize(u, steps=3, coefficients=cubic), u, [cubic] * 3)
+    per_step = [(4.0, -6.0, 2.5), (3.0, -4.0, 1.8), (2.0, -1.5, 0.5)]
+    check(T.orthogonalize(u, steps=3, coefficients=per_step), u, per_step)
+    assert T.orthogonalize([]) == []
+    e = T.orthogonalize([torch.zeros(0, 5, device=DEV), u, torch.zeros(3, 4, 0, device=DEV)])
+    assert e[0].shape == (0, 5) and e[2].shape == (3, 4, 0) and torch.equal(e[1], T.orthogonalize(u))
+
+
+def test_orthogonalize_many_tensors():
+    """more source tensors than one launch takes by value"""
+    from das_amd import train_ops as T
+    mats = [gradient(3 + i % 7, 5 + i % 11, 100 + i) for i in range(150)]
+    for t, y in zip(mats, T.orthogonalize(mats)):
+        check(y, t, [COEF] * 5)
+
+
+def test_plan_serves_two_streams_and_a_graph():
+    from das_amd import train_ops as T
+    u, v = gradient(256, 300, 1), gradient(256, 300, 2)
+    plan = T.NewtonSchulzPlan([(256, 300)], DEV)
+    want_u, want_v = T.orthogonalize([u], plan=plan)[0], T.orthogonalize([v], plan=plan)[0]
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(4):
+        with torch.cuda.stream(s1):
+            a = T.orthogonalize([u], plan=plan)[0]
+        with torch.cuda.stream(s2):
+            b = T.orthogonalize([v], plan=plan)[0]
+        got.append((a, b))
+    torch.cuda.synchronize()
+    for a, b in got:
+        assert torch.equal(a, want_u) and torch.equal(b, want_v)
+    static, g1, g2 = u.clone(), torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g1):
+        o1 = T.orthogonalize([static], plan=plan)[0]
+    with torch.cuda.graph(g2):
+        o2 = T.orthogonalize([static], plan=plan)[0]
+    for t, want in ((v, want_v), (u, want_u), (v, want_v)):
+        static.copy_(t)
+        g1.replay()
+        g2.replay()
+        extra = T.orthogonalize([t], plan=plan)[0]
+        torch.cuda.synchronize()
+        assert torch.equal(o1, want) and torch.equal(o2, want) and torch.equal(extra, want)
+
+
+def muon64(p, g, m, shapes, offsets, lr, momentum, wd, nesterov, lr_scale, coef):
+    p, g, m = p.double().clone(), g.double(), m.double().clone()
+    tol = torch.zeros_like(p)
+    for (k, r, c), o in zip(shapes, offsets):
+        for i in range(k):
+            s = slice(o + i * r * c, o + (i + 1) * r * c)
+            m[s] = momentum * m[s] + (1 - momentum) * g[s] * coef
+            u = (1 - momentum) * g[s] * coef + momentum * m[s] if nesterov else m[s]
+            x, err = ns64(u.view(r, c), [COEF] * 5)
+            f = math.sqrt(max(1.0, r / c)) if lr_scale == 'original' else 0.2 * math.sqrt(max(r, c))
+            p[s] = p[s] * (1 - lr * wd) - lr * f * x.reshape(-1)
+            tol[s] = 1.1 * lr * f * err      # (2-norm over the matrix)
+    return p, m, tol
+
+
+@pytest.mark.parametrize('nesterov,lr_scale,clip', [(True, 'original', 0.0), (False, 'match_rms_adamw', 0.0), (True, 'original', 0.5)])
+def test_muon_step(nesterov, lr_scale, clip):
+    """two steps over a flat buffer with gaps and odd starts between the matrices; the gaps keep their bytes"""
+    from das_amd import train_ops as T
+    shapes, offsets = [(2, 64, 147), (1, 300, 70), (3, 64, 3), (1, 1, 256), (1, 128, 256)], []
+    at = 5
+    for i, (k, r, c) in enumerate(shapes):
+        offsets.append(at)
+        at += k * r * c + (3, 1, 64, 17, 9)[i]
+    gen = torch.Generator().manual_seed(3)
+    p, g, m = (torch.randn(at, generator=gen).to(DEV) * s for s in (0.1, 1e-2, 1e-2))
+    inside = torch.zeros(at, dtype=torch.bool, device=DEV)
+    for (k, r, c), o in zip(shapes, offsets):
+        inside[o:o + k * r * c] = True
+    p0, m0 = p.clone(), m.clone()
+    plan = T.NewtonSchulzPlan(shapes, DEV, offsets=offsets)
+    kw = dict(lr=0.02, momentum=0.9, weight_decay=0.1, nesterov=nesterov, lr_scale=lr_scale)
+    for step in range(2):
+        sumsq = T.grad_sumsq(g)
+        norm = float(g.double().norm()) * 0.5
+        coef = 0.5 * (min(1.0, clip / (norm + 1e-6)) if clip else 1.0)
+        rp, rm, tol = muon64(p, g, m, shapes, offsets, kw['lr'], kw['momentum'], kw['weight_decay'], nesterov, lr_scale, coef)
+        T.muon_step(p, g, m, plan, grad_scale=0.5, max_norm=clip, grad_sumsq_t=sumsq, **kw)
+        # momentum: products and a sum in f32, the clip factor from a f32 sum of squares over n elements
+        assert float((m.double() - rm)[inside].abs().max()) <= (8 + 32 * (clip > 0)) * 2.0 ** -24 * float(rm.abs().max() + g.abs().max())
+        for (k, r, c), o in zip(shapes, offsets):
+            for i in range(k):
+                s = slice(o + i * r * c, o + (i + 1) * r * c)
+                slack = 4 * 2.0 ** -24 * float(p[s].double().norm()) + (1e-4 if clip else 0) * float(tol[o])
+                assert float((p[s].double() - rp[s]).norm()) <= float(tol[s][0]) + slack, (step, r, c)
+        g = torch.randn(at, generator=gen).to(DEV) * 1e-2
+    assert torch.equal(p[~inside], p0[~inside]) and torch.equal(m[~inside], m0[~inside])
+    assert not torch.equal(p[inside], p0[inside])
+
+
+@pytest.mark.parametrize('n', [1, 3, 4, 5, 255, 4099, 1 << 20, 3_000_001])
+@pytest.mark.parametrize('step,clip', [(1, 0.0), (7, 1.0), (100000, 0.0)])
+def test_adamw_step(n, step, clip):
+    from das_amd import train_ops as T
+    gen = torch.Generator().manual_seed(n + step)
+    p, g = torch.randn(n, generator=gen).to(DEV), (torch.randn(n, generator=gen) * torch.exp(3 * torch.randn(n, generator=gen))).to(DEV) * 1e-3
+    m = torch.zeros_like(p) if step == 1 else g * torch.rand(n, generator=gen).to(DEV)
+    v = torch.zeros_like(p) if step == 1 else g * g * torch.rand(n, generator=gen).to(DEV) * (1 - 0.999 ** step)
+    kw = dict(lr=1e-2, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.1)
+    sumsq = T.grad_sumsq(g)
+    coef = 0.25 * (min(1.0, clip / (float(g.double().norm()) * 0.25 + 1e-6)) if clip else 1.0)
+    gd = g.double() * coef
+    m64 = 0.9 * m.double() + 0.1 * gd
+    v64 = 0.999 * v.double() + 0.001 * gd * gd
+    upd = (m64 / (1 - 0.9 ** step)) / ((v64 / (1 - 0.999 ** step)).sqrt() + 1e-8)
+    p64 = p.double() * (1 - 1e-2 * 0.1) - 1e-2 * upd
+    mag = 0.9 * m.double().abs() + 0.1 * gd.abs()
+    T.adamw_step(p, g, m, v, step=step, grad_scale=0.25, max_norm=clip, grad_sumsq_t=sumsq, **kw)
+    u = 2.0 ** -24
+    cl = 64 * u if clip else 0.0      # the f32 sum of squares (a tree of partial sums) under the clip factor
+    assert ((m.double() - m64).abs() <= (6 * u + cl) * mag).all()
+    assert ((v.double() - v64).abs() <= (8 * u + 2 * cl) * v64 + 2.0 ** -126).all()
+    # m carries an absolute error of (6 u + cl) mag (its two terms may cancel), the quotient and the root a dozen roundings more
+    lim = (4 * u) * p64.abs() + 1e-2 * ((16 * u + 2 * cl) * upd.abs() + (6 * u + cl) * (mag / (1 - 0.9 ** step)) /
+                                        ((v64 / (1 - 0.999 ** step)).sqrt() + 1e-8)) + 4 * u * p.double().abs()
+    assert ((p.double() - p64).abs() <= lim).all()
+
+
+def test_adamw_unaligned_views_and_empty():
+    from das_amd import train_ops as T
+    base = [torch.randn(1031, device=DEV).abs() for _ in range(4)]
+    a = [t.clone() for t in base]
+    T.adamw_step(*[t[1:1030] for t in a], lr=1e-2, step=3)
+    b = [t[1:1030].clone() for t in base]
+    T.adamw_step(*b, lr=1e-2, step=3)
+    for x, y, z in zip(a, b, base):
+        assert torch.equal(x[1:1030], y) and x[0] == z[0] and x[1030] == z[1030]
+    T.adamw_step(*[torch.empty(0, device=DEV) for _ in range(4)], lr=1e-2, step=1)
+
+
+def test_nan_norm_and_nan_gradient():
+    from das_amd import train_ops as T
+    p, m, v = (torch.ones(64, device=DEV) for _ in range(3))
+    g = torch.ones(64, device=DEV)
+    g[5] = float('nan')
+    T.adamw_step(p, g, m, v, lr=1e-2, step=1)
+    assert torch.isnan(p[5]) and int(torch.isnan(p).sum()) == 1
+    T.adamw_step(p, g, m, v, lr=1e-2, step=1, max_norm=1.0, grad_sumsq_t=T.grad_sumsq(g))
+    assert torch.isnan(p).all()
+
+
+def test_refusals():
+    from das_amd import train_ops as T
+    from das_amd._lib import DasHipError
+    u = torch.ones(8, 8, device=DEV)
+    f = torch.ones(64, device=DEV)
+    plan = T.NewtonSchulzPlan([(8, 8)], DEV)
+    for bad in (lambda: T.orthogonalize(u, out_dtype=torch.float32), lambda: T.orthogonalize(u.double()),
+                lambda: T.orthogonalize([u, u.half()]), lambda: T.orthogonalize(u[0]), lambda: T.orthogonalize(u.cpu()),
+                lambda: T.orthogonalize([u, u], plan=plan), lambda: T.orthogonalize(u, steps=0), lambda: T.orthogonalize(u, steps=17),
+                lambda: T.orthogonalize(u, coefficients=(float('nan'), 0, 0)), lambda: T.orthogonalize(u, coefficients=(40., 0, 0)),
+                lambda: T.orthogonalize(u, coefficients=[(1.5, -.5, 0)] * 2), lambda: T.orthogonalize(u, eps=-1.0),
+                lambda: T.NewtonSchulzPlan([(8, 8), (8, 8)], DEV, offsets=[0, 63]), lambda: T.NewtonSchulzPlan([(8, 8)], DEV, offsets=[-1]),
+                lambda: T.NewtonSchulzPlan([(8, 8)], DEV, offsets=[0, 64]), lambda: T.NewtonSchulzPlan([(8, 8)], 'cpu'),
+                lambda: T.NewtonSchulzPlan([(8, -8)], DEV),
+                lambda: T.orthogonalize([u], plan=T.NewtonSchulzPlan([(8, 8)], DEV, offsets=[0])),
+                lambda: T.muon_step(f[:63], f[:63], f[:63], plan, lr=1e-2), lambda: T.muon_step(f, f, f[:60], plan, lr=1e-2),
+                lambda: T.muon_step(f, f, f.half(), plan, lr=1e-2), lambda: T.muon_step(f, f, f, plan, lr=1e-2, lr_scale='x'),
+                lambda: T.muon_step(f, f, f, plan, lr=1e-2, momentum=1.0), lambda: T.muon_step(f, f, f, plan, lr=-1.0),
+                lambda: T.muon_step(f, f, f, plan, lr=1e-2, max_norm=1.0), lambda: T.adamw_step(f, f, f, f, lr=1e-2, step=0),
+                lambda: T.adamw_step(f, f, f, f, lr=1e-2, step=1, beta1=1.0), lambda: T.adamw_step(f, f, f, f, lr=float('nan'), step=1),
+                lambda: T.adamw_step(f, f, f, f, lr=1e-2, step=1, max_norm=1.0),
+                lambda: T.adamw_step(f, f, f, f.cpu(), lr=1e-2, step=1), lambda: T.adamw_step(f[::2], f[::2], f[::2], f[::2], lr=1e-2, step=1)):
+        with pytest.raises(DasHipError):
+            bad()
+    assert (f == 1).all() and (u == 1).all()
