@@ -76,7 +76,7 @@ class DasNsShape(C.Structure):
 
 class DasNsPlan(C.Structure):
     _fields_ = [('n_groups', i32), ('n_matrices', i32), ('n_chunks', i32), ('n_gram', i32), ('n_update', i32), ('steps', i32),
-                ('x_elems', i64), ('a_elems', i64), ('extent', i64),
+                ('gram_tile', i32), ('update_tile', i32), ('x_elems', i64), ('a_elems', i64), ('extent', i64),
                 ('mat_at', i64), ('chunk_at', i64), ('gram_at', i64), ('update_at', i64), ('table_bytes', i64),
                 ('coef', f32 * (3 * DAS_NS_MAX_STEPS)), ('eps', f32)]
 
@@ -181,7 +181,7 @@ SIGNATURES = {
     'das_grad_sumsq': (i32, [vp, i64, vp, i32, vp]),
     'das_sgd_momentum_step': (i32, [vp, vp, vp, i64, f32, f32, f32, f32, f32, vp, i32, vp]),
     'das_ns_plan': (i32, [C.POINTER(DasNsShape), i32, i32, C.POINTER(f32), f32, C.POINTER(DasNsPlan), vp, i64]),
-    'das_ns_ws_bytes': (i64, [C.POINTER(DasNsPlan)]),
+    'das_ns_ws_bytes': (i64, [C.POINTER(DasNsPlan), i32]),
     'das_orthogonalize': (i32, [C.POINTER(DasNsPlan), vp, C.POINTER(DasNsSource), i32, i32, vp, i32, vp, vp]),
     'das_muon_step': (i32, [C.POINTER(DasNsPlan), vp, vp, vp, vp, f32, f32, f32, i32, i32, f32, f32, vp, vp, vp]),
     'das_adamw_step': (i32, [vp, vp, vp, vp, i64, f64, f64, f64, f64, f64, i64, f32, f32, vp, vp]),

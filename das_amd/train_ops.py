@@ -178,6 +178,7 @@ def adamw_step(p, g, m, v, lr, step, beta1=0.9, beta2=0.999, eps=1e-8, weight_de
                                               _ptr(sumsq), _stream()), 'das_adamw_step')
 
 
+_NS_DT = {torch.float32: _lib.DAS_F32, torch.bfloat16: _lib.DAS_BF16, torch.float16: _lib.DAS_F16}
 NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)   # quintic of the published Muon optimizer: singular values of [1e-3, 1] -> [0.7, 1.2]
 
 
@@ -223,7 +224,7 @@ class NewtonSchulzPlan:
                 self._build([(o, s) for o, s, n in zip(self._out_offsets, self.shapes, sizes) if n], co)
 
     def _build(self, entries, co):
-        """-> (DasNsPlan, device tables, workspace bytes), None for no entries"""
+        """-> (DasNsPlan, device tables), None for no entries"""
         if not entries:
             return None
         lib = _lib.load()
@@ -235,24 +236,26 @@ class NewtonSchulzPlan:
         _lib.check(lib.das_ns_plan(arr, len(entries), self.steps, cf, self.eps, C.byref(plan), None, 0), 'das_ns_plan')
         host = torch.empty(plan.table_bytes, dtype=torch.uint8)
         _lib.check(lib.das_ns_plan(arr, len(entries), self.steps, cf, self.eps, C.byref(plan), _ptr(host), plan.table_bytes), 'das_ns_plan')
-        return plan, host.to(self.device), lib.das_ns_ws_bytes(C.byref(plan))
+        return plan, host.to(self.device)
 
 
 def orthogonalize(mats, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, out_dtype=torch.bfloat16, plan=None):
     """The orthogonal factor of every matrix of a list (or of one tensor) by `steps` Newton-Schulz products: for U = mats[i],
     X = U / (|U| + eps), then X <- (a I + b X X^T + c (X X^T)^2) X. 2-D tensors are one matrix, 3-D ones a stack; f32, bf16 or f16 (one
-    type a call), any row / stack stride, unit column stride. Returns tensors of the same shapes, bf16 (default) or f16.
+    type a call), any row / stack stride, unit column stride. Returns tensors of the same shapes.
+    out_dtype sets the precision too: bf16 (default) and f16 results come from products of f16 operands, 1e-3 off exact arithmetic for the
+    gradients of a training run (2-norm) and up to 5e-2 where the singular values span many orders of magnitude; f32 ones from
+    pairs of f16, 2e-4 off at most.
     plan: a NewtonSchulzPlan of these shapes (built here if None, which copies its tables to the device: keep one where the call
-    repeats; inside a hipGraph capture it is required). Products take f16 operands: a few 1e-3 off exact arithmetic, up to
-    5e-2 for matrices whose singular values span many orders of magnitude. Inf or NaN in a matrix makes that matrix NaN, no other."""
+    repeats; inside a hipGraph capture it is required). Inf or NaN in a matrix makes that matrix NaN, no other."""
     one = torch.is_tensor(mats)
     mats = [mats] if one else list(mats)
     _need_gpu(*mats)
-    if out_dtype not in (torch.bfloat16, torch.float16):
-        raise _lib.DasHipError('orthogonalize: out_dtype is bfloat16 or float16')
+    if out_dtype not in _NS_DT:
+        raise _lib.DasHipError('orthogonalize: out_dtype is bfloat16, float16 or float32')
     if not mats:
         return []
-    dt = {torch.float32: _lib.DAS_F32, torch.bfloat16: _lib.DAS_BF16, torch.float16: _lib.DAS_F16}.get(mats[0].dtype)
+    dt = _NS_DT.get(mats[0].dtype)
     if dt is None or any(t.dtype != mats[0].dtype or t.device != mats[0].device or t.dim() not in (2, 3) for t in mats):
         raise _lib.DasHipError('orthogonalize: 2-D or 3-D tensors of one type (float32, bfloat16, float16) on one device')
     shapes = [tuple(t.shape) if t.dim() == 3 else (1,) + tuple(t.shape) for t in mats]
@@ -266,16 +269,16 @@ def orthogonalize(mats, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, out_dty
         raise _lib.DasHipError('orthogonalize: a plan with offsets of its own is for muon_step')
     out = torch.empty(plan._out_size, dtype=out_dtype, device=dev)
     if plan._out is not None:
-        p, tables, ws_bytes = plan._out
+        p, tables = plan._out
         live = [t for t in mats if t.numel()]
         src = (_lib.DasNsSource * len(live))()
         for s, t in zip(src, live):
             s.base, s.row_stride, s.batch_stride = t.data_ptr(), t.stride(-2), t.stride(0) if t.dim() == 3 else 0
         with torch.cuda.device(dev):
-            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-            _lib.check(_lib.load().das_orthogonalize(C.byref(p), _ptr(tables), src, len(live), dt, _ptr(out),
-                                                     _lib.DAS_BF16 if out_dtype == torch.bfloat16 else _lib.DAS_F16, _ptr(ws),
-                                                     _stream()), 'das_orthogonalize')
+            lib = _lib.load()
+            ws = torch.empty(lib.das_ns_ws_bytes(C.byref(p), int(out_dtype == torch.float32)), dtype=torch.uint8, device=dev)
+            _lib.check(lib.das_orthogonalize(C.byref(p), _ptr(tables), src, len(live), dt, _ptr(out), _NS_DT[out_dtype], _ptr(ws),
+                                             _stream()), 'das_orthogonalize')
     res = [out[o:o + t.numel()].view(t.shape) for o, t in zip(plan._out_offsets, mats)]
     return res[0] if one else res
 
@@ -294,14 +297,15 @@ def muon_step(p, g, buf, plan, lr, momentum=0.95, weight_decay=0.0, nesterov=Tru
         raise _lib.DasHipError(f'muon_step: the plan is on {plan.device}, the buffers on {p.device}')
     if plan._flat is None:
         return
-    c_plan, tables, ws_bytes = plan._flat
+    c_plan, tables = plan._flat
     if c_plan.extent > p.numel():
         raise _lib.DasHipError(f'muon_step: the plan reaches element {c_plan.extent} of buffers of {p.numel()}')
     with torch.cuda.device(p.device):
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=p.device)
-        _lib.check(_lib.load().das_muon_step(C.byref(c_plan), _ptr(tables), _ptr(p), _ptr(g), _ptr(buf), float(lr), float(momentum),
-                                             float(weight_decay), int(bool(nesterov)), int(lr_scale != 'original'), float(grad_scale),
-                                             float(max_norm), _ptr(sumsq), _ptr(ws), _stream()), 'das_muon_step')
+        lib = _lib.load()
+        ws = torch.empty(lib.das_ns_ws_bytes(C.byref(c_plan), 1), dtype=torch.uint8, device=p.device)
+        _lib.check(lib.das_muon_step(C.byref(c_plan), _ptr(tables), _ptr(p), _ptr(g), _ptr(buf), float(lr), float(momentum),
+                                     float(weight_decay), int(bool(nesterov)), int(lr_scale != 'original'), float(grad_scale),
+                                     float(max_norm), _ptr(sumsq), _ptr(ws), _stream()), 'das_muon_step')
 
 
 # ------------------------------------------------------------------ RealNVP log-density (RLE pose loss)

@@ -611,11 +611,10 @@ int das_sgd_momentum_step(float* p, const float* g, float* buf, long long n, flo
  * Newton-Schulz orthogonalisation of a ragged set of matrices. For each matrix U (rows x cols, m = min, n = max of the two,
  * transposed if rows > cols so that X is m x n):
  *   X = U / (|U|_F + eps);   steps times:  A = X X^T,  B = a I + b A + c A^2,  X = B X.
- * Products take f16 operands and sum in f32; X, A and B are rounded to f16 between products (X carries a power-of-two scale that
- * keeps its entries in f16's normal range), so a result is a few 1e-3 off a 64-bit evaluation for the gradients of a
- * training run, and up to 5e-2 (2-norm) for matrices whose singular values span many orders of magnitude. The sum of squares and
- * the joint scale of each 64 x 64 block are held in f32 / f64. Results do not depend on what else is in the set, and are the
- * same bits from run to run.
+ * The precision follows the result's type. f16 / bf16 results: products of f16 operands summed in f32, X, A and B rounded to f16 in between
+ * (1e-3 off a 64-bit evaluation, in the 2-norm, for the gradients of a training run, up to 5e-2 for matrices whose singular values span
+ * many orders of magnitude). f32 results and parameters: operands are pairs of f16 (22 bits), 2e-4 off at most. Sums of squares are
+ * held in f32 by 64 x 64 blocks and added in f64. Results are the same bits from run to run.
  *
  * A plan lists the set once: das_ns_plan() checks the shapes and the polynomial and writes the tables (host memory) that the
  * kernels walk; the caller copies them to the device and hands both to every call. Plans hold no pointers and no results. */
@@ -627,7 +626,7 @@ typedef struct {
   int reserved;
 } DasNsShape;
 typedef struct {
-  int n_groups, n_matrices, n_chunks, n_gram, n_update, steps;
+  int n_groups, n_matrices, n_chunks, n_gram, n_update, steps, gram_tile, update_tile;
   long long x_elems, a_elems, extent;            /* work areas (f16 elements); one past the last element of the flat buffers used */
   long long mat_at, chunk_at, gram_at, update_at, table_bytes;   /* byte offsets of the tables */
   float coef[3 * DAS_NS_MAX_STEPS];              /* a, b, c of each step */
@@ -639,12 +638,13 @@ typedef struct {
   long long batch_stride, row_stride;
 } DasNsSource;
 /* Fills *plan; with tables != NULL (plan->table_bytes host bytes) also the tables. DAS_ERR_ARG: n < 1, a shape without elements or
- * with a side over 1 << 20, overlapping matrices, steps outside 1 ... DAS_NS_MAX_STEPS, a polynomial that takes [0, 1] out of
- * [-16, 16] within `steps` steps (f16 would overflow), eps < 0, or tables too small. */
+ * with a side over 1 << 20 or both over 1 << 15, overlapping matrices, steps outside 1 ... DAS_NS_MAX_STEPS, a polynomial that takes [0, 1] out of
+ * [-16, 16] within `steps` steps or has |a + b s^2 + c s^4| > 64 there (f16 could overflow), eps < 0, or tables too small. */
 int das_ns_plan(const DasNsShape* shapes, int n, int steps, const float* coef, float eps, DasNsPlan* plan, void* tables,
                 long long table_bytes);
-long long das_ns_ws_bytes(const DasNsPlan* plan);
-/* out (flat, out_dtype DAS_BF16 or DAS_F16, plan offsets): the orthogonalised matrices; srcs: one per group of the plan, in_dtype
+/* f32_result: for das_muon_step, and for das_orthogonalize with out_dtype DAS_F32. */
+long long das_ns_ws_bytes(const DasNsPlan* plan, int f32_result);
+/* out (flat, out_dtype DAS_F32 / DAS_BF16 / DAS_F16, plan offsets): the orthogonalised matrices; srcs: one per group of the plan, in_dtype
  * DAS_F32 / DAS_BF16 / DAS_F16. `ws`: das_ns_ws_bytes() of device memory, 16-byte aligned, in use until the call's kernels end. */
 int das_orthogonalize(const DasNsPlan* plan, const void* tables_dev, const DasNsSource* srcs, int n_srcs, int in_dtype, void* out,
                       int out_dtype, void* ws, void* stream);

@@ -8,7 +8,7 @@ pytestmark = pytest.mark.gpu
 DEV = 'cuda'
 COEF = (3.4445, -4.7750, 2.0315)
 U16 = 2.0 ** -11     # half a step of f16
-HALF = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+HALF = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}
 
 
 def gradient(r, c, seed, k=None):
@@ -24,37 +24,60 @@ def gradient(r, c, seed, k=None):
     return g if k else g[0]
 
 
-def ns64(u, coef, eps=1e-7):
-    """(result in f64, bound on the 2-norm of a f16 evaluation's error). The bound follows the roundings: f16 holds X, A and B (relative
-    U16 each, and 2^-25 absolute below its normal range; X is scaled by about sqrt(n)); an error of X grows by at most L = max |p'|
-    over the singular values' range in a step (the derivative of an odd function of a matrix is bounded, in the 2-norm over all
-    entries, by its divided differences); f32 sums over K products add K 2^-23."""
+def norm2(x):
+    return float(torch.linalg.matrix_norm(x, 2))
+
+
+def ns64(u, coef, eps=1e-7, pairs=False):
+    """(result in f64, bound on the 2-norm of the kernels' error). The bounds follow the roundings to first order. An error of X grows by at
+    most L = max |p'| over the singular values' range in a step (the derivative of an odd function of a matrix is bounded, in the
+    2-norm over all entries, by its divided differences). f32 sums: K inner elements are at most 3 K / 32 + 5 additions one after the other.
+    f16 operands: X, G and Z are rounded by U16 (2^-25 absolute below the normal range; X is stored times about sqrt(n)).
+    Pairs of f16: 2^-22 a rounding and 2^-22 for the dropped product of the low parts; steps are taken on G in phases, and what
+    G and Q lose meanwhile is followed through G' = Z G Z and Q' = Z Q."""
     x = u.double()
     x = x / (x.norm() + eps)
     if x.shape[0] > x.shape[1]:
-        y, e = ns64(u.t(), coef, eps)
+        y, e = ns64(u.t(), coef, eps, pairs)
         return y.t(), e
     m, n = x.shape
-    tiny = 2.0 ** -25 * math.sqrt(m * n) / math.sqrt(n) * 2
+    rnd = 2.0 ** -22 if pairs else U16
+    tiny = 2.0 ** -25 * math.sqrt(m) * 2
     eye = torch.eye(m, dtype=torch.float64, device=x.device)
-    err = 2 * U16 * float(x.norm()) + 2 * tiny
-    for a, b, c in coef:
-        s2 = min(float(torch.linalg.matrix_norm(x, 2)) if m <= 512 else 1.25, float(x.norm()))
-        s = torch.linspace(0, max(s2, 1e-30) * 1.01, 2048, dtype=torch.float64)
-        lip = float((a + 3 * b * s ** 2 + 5 * c * s ** 4).abs().max())
-        g = x @ x.T
-        q = a * eye + b * g + c * (g @ g)
-        y = q @ x
-        acc = (n + 2 * m) * 2.0 ** -23
-        da = (U16 + acc) * float(g.norm()) + 2.0 ** -25 * m
-        db = abs(b) * da + abs(c) * 2 * s2 * s2 * da + (U16 + acc) * (float(q.norm())) + 2.0 ** -25 * m
-        err = lip * err + db * s2 + (U16 + acc) * float(y.norm()) + tiny
-        x = y
+
+    def acc(k):
+        return (3 * k / 32 + 5) * 2.0 ** -23 + (2.0 ** -22 if pairs else 0)
+
+    err = 2 * rnd * float(x.norm()) + 2 * tiny
+    k = 0
+    while k < len(coef):
+        x0, g = x, x @ x.T
+        eg = (rnd + acc(n)) * float(x.norm()) ** 2 + 2.0 ** -25 * m
+        q, eq, grow = eye, 0.0, 1.0
+        while True:
+            a, b, c = coef[k]
+            top = norm2(x)
+            s = torch.linspace(0, max(top, 1e-30) * 1.01, 2048, dtype=torch.float64)
+            err *= float((a + 3 * b * s ** 2 + 5 * c * s ** 4).abs().max())
+            g2 = top * top
+            z = a * eye + b * g + c * (g @ g)
+            ez = (abs(b) + 2 * abs(c) * g2) * eg + abs(c) * acc(m) * float(g.norm()) ** 2 + \
+                (rnd + 2.0 ** -22) * (float(z.norm()) + abs(b) * float(g.norm())) + 2.0 ** -25 * m
+            zn, r = norm2(z), z @ g
+            eq = zn * eq + norm2(q) * ez + (rnd + acc(m)) * float(z.norm()) * norm2(q)
+            er = zn * eg + g2 * ez + (rnd + acc(m)) * float(z.norm()) * g2 + 2.0 ** -25 * m
+            eg = zn * er + norm2(r) * ez + (rnd + acc(m)) * float(r.norm()) * zn + 2.0 ** -25 * m
+            q, x, g = z @ q, z @ x, r @ z
+            grow *= max(abs(a), zn) ** 2
+            k += 1
+            if k == len(coef) or not pairs or grow > 256:
+                break
+        err += eq * norm2(x0) + (rnd + acc(m)) * norm2(q) * float(x0.norm()) + tiny
     return x, err
 
 
 def check(got, u, coef, eps=1e-7, what=''):
-    ref, err = ns64(u, coef, eps)
+    ref, err = ns64(u, coef, eps, pairs=got.dtype == torch.float32)
     d = float((got.double() - ref).norm())
     tol = 1.1 * err + HALF[got.dtype] * float(ref.norm())
     assert torch.isfinite(got).all(), what
@@ -65,16 +88,17 @@ SHAPES = [(1, 1), (1, 64), (64, 1), (2, 3), (45, 256), (27, 2304), (64, 64), (64
           (256, 64), (333, 77), (512, 128), (500, 513), (700, 513), (256, 2304)]
 
 
+@pytest.mark.parametrize('out_dtype', [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize('steps', [1, 2, 5])
 @pytest.mark.parametrize('shape', SHAPES, ids=lambda s: '%dx%d' % s)
-def test_orthogonalize_one_matrix(shape, steps):
+def test_orthogonalize_one_matrix(shape, steps, out_dtype):
     from das_amd import train_ops as T
     u = gradient(*shape, seed=shape[0] * 7 + shape[1])
-    check(T.orthogonalize(u, steps=steps), u, [COEF] * steps)
+    check(T.orthogonalize(u, steps=steps, out_dtype=out_dtype), u, [COEF] * steps)
 
 
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16])
-@pytest.mark.parametrize('out_dtype', [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('out_dtype', [torch.bfloat16, torch.float16, torch.float32])
 def test_orthogonalize_set(dtype, out_dtype):
     """every matrix of a ragged set comes out as it does alone, bit for bit, and a second call gives the same bits"""
     from das_amd import train_ops as T
@@ -119,9 +143,10 @@ def test_orthogonalize_hard_spectra():
     from das_amd import train_ops as T
     gen = torch.Generator().manual_seed(1)
     a = (torch.randn(96, 8, generator=gen) @ torch.randn(8, 300, generator=gen)).to(DEV)
-    check(T.orthogonalize(a), a, [COEF] * 5)
     one = torch.outer(torch.randn(70, generator=gen), torch.randn(200, generator=gen)).to(DEV)
-    check(T.orthogonalize(one), one, [COEF] * 5)
+    for dt in (torch.bfloat16, torch.float32):
+        check(T.orthogonalize(a, out_dtype=dt), a, [COEF] * 5)
+        check(T.orthogonalize(one, out_dtype=dt), one, [COEF] * 5)
     assert not T.orthogonalize(torch.zeros(40, 70, device=DEV)).any()
     spike = 1e-6 * torch.randn(65, 130, generator=gen)
     spike[64, 129] = 1e6
@@ -148,6 +173,8 @@ def test_orthogonalize_other_polynomials_and_empty():
     check(T.orthogonalize(u, steps=3, coefficients=cubic), u, [cubic] * 3)
     per_step = [(4.0, -6.0, 2.5), (3.0, -4.0, 1.8), (2.0, -1.5, 0.5)]
     check(T.orthogonalize(u, steps=3, coefficients=per_step), u, per_step)
+    check(T.orthogonalize(u, steps=3, coefficients=per_step, out_dtype=torch.float32), u, per_step)
+    check(T.orthogonalize(u, steps=12, coefficients=cubic, out_dtype=torch.float32), u, [cubic] * 12)
     assert T.orthogonalize([]) == []
     e = T.orthogonalize([torch.zeros(0, 5, device=DEV), u, torch.zeros(3, 4, 0, device=DEV)])
     assert e[0].shape == (0, 5) and e[2].shape == (3, 4, 0) and torch.equal(e[1], T.orthogonalize(u))
@@ -159,6 +186,16 @@ def test_orthogonalize_many_tensors():
     mats = [gradient(3 + i % 7, 5 + i % 11, 100 + i) for i in range(150)]
     for t, y in zip(mats, T.orthogonalize(mats)):
         check(y, t, [COEF] * 5)
+
+
+def test_orthogonalize_large_tiles():
+    """sets of enough tiles for the 128 x 128 form, ragged at its edges"""
+    from das_amd import train_ops as T
+    mats = [gradient(300, 411, 1, k=40), gradient(257, 130, 2, k=30), gradient(129, 1025, 3, k=20)]
+    for dt in (torch.bfloat16, torch.float32):
+        for t, y in zip(mats, T.orthogonalize(mats, out_dtype=dt)):
+            for i in (0, 7, t.shape[0] - 1):
+                check(y[i], t[i], [COEF] * 5, what=(tuple(t.shape), i))
 
 
 def test_plan_serves_two_streams_and_a_graph():
@@ -200,7 +237,7 @@ def muon64(p, g, m, shapes, offsets, lr, momentum, wd, nesterov, lr_scale, coef)
             s = slice(o + i * r * c, o + (i + 1) * r * c)
             m[s] = momentum * m[s] + (1 - momentum) * g[s] * coef
             u = (1 - momentum) * g[s] * coef + momentum * m[s] if nesterov else m[s]
-            x, err = ns64(u.view(r, c), [COEF] * 5)
+            x, err = ns64(u.view(r, c), [COEF] * 5, pairs=True)
             f = math.sqrt(max(1.0, r / c)) if lr_scale == 'original' else 0.2 * math.sqrt(max(r, c))
             p[s] = p[s] * (1 - lr * wd) - lr * f * x.reshape(-1)
             tol[s] = 1.1 * lr * f * err      # (2-norm over the matrix)
@@ -299,7 +336,7 @@ def test_refusals():
     u = torch.ones(8, 8, device=DEV)
     f = torch.ones(64, device=DEV)
     plan = T.NewtonSchulzPlan([(8, 8)], DEV)
-    for bad in (lambda: T.orthogonalize(u, out_dtype=torch.float32), lambda: T.orthogonalize(u.double()),
+    for bad in (lambda: T.orthogonalize(u, out_dtype=torch.float64), lambda: T.orthogonalize(u.double()),
                 lambda: T.orthogonalize([u, u.half()]), lambda: T.orthogonalize(u[0]), lambda: T.orthogonalize(u.cpu()),
                 lambda: T.orthogonalize([u, u], plan=plan), lambda: T.orthogonalize(u, steps=0), lambda: T.orthogonalize(u, steps=17),
                 lambda: T.orthogonalize(u, coefficients=(float('nan'), 0, 0)), lambda: T.orthogonalize(u, coefficients=(40., 0, 0)),
