@@ -33,6 +33,7 @@ typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int TPB = 256;
+constexpr int N_AREAS = 5;   // m x m work matrices: G, R, Z, two of Q (the f16 form uses G and Z)
 constexpr int CHUNK = 64;   // side of the blocks that ingest_kernel / normalise_kernel work on
 
 struct NsMatrix {           // one matrix, as the kernels see it
@@ -104,6 +105,22 @@ __device__ __forceinline__ float block_reduce(float v, bool is_max, float* red) 
   return is_max ? fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])) : (red[0] + red[1]) + (red[2] + red[3]);
 }
 
+// g's factor: the scale times min(1, max_norm / (norm + 1e-6)); a NaN norm stays NaN
+__device__ __forceinline__ float grad_factor(const MuonIn& mu) {
+  float f = mu.grad_scale;
+  if (mu.max_norm > 0.f) {
+    const float k = mu.max_norm / (sqrtf(*mu.sumsq) * mu.grad_scale + 1e-6f);
+    f *= k > 1.f ? 1.f : k;
+  }
+  return f;
+}
+// the momentum's new value in b, returns U
+__device__ __forceinline__ float muon_in(const MuonIn& mu, float f, float g, float& b) {
+  g *= f;
+  b = mu.momentum * b + (1.f - mu.momentum) * g;
+  return mu.nesterov ? (1.f - mu.momentum) * g + mu.momentum * b : b;
+}
+
 template <typename T>
 __device__ __forceinline__ float load_as_f32(const void* base, long long i) {
   const T v = reinterpret_cast<const T*>(base)[i];
@@ -125,13 +142,7 @@ __global__ __launch_bounds__(TPB) void ingest_kernel(const NsMatrix* __restrict_
   const int r0 = ch.y * CHUNK, c0 = ch.z * CHUNK;
   const int c4 = (threadIdx.x & 15) * 4, rr = threadIdx.x >> 4;
   float coef = 1.f;
-  if constexpr (MUON) {
-    coef = mu.grad_scale;
-    if (mu.max_norm > 0.f) {
-      const float k = mu.max_norm / (sqrtf(*mu.sumsq) * mu.grad_scale + 1e-6f);
-      coef *= k > 1.f ? 1.f : k;   // (a NaN norm stays NaN)
-    }
-  }
+  if constexpr (MUON) coef = grad_factor(mu);
   float u[4][4], big = 0.f;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
@@ -143,10 +154,7 @@ __global__ __launch_bounds__(TPB) void ingest_kernel(const NsMatrix* __restrict_
       if (r < M.rows && c < M.cols) {
         if constexpr (MUON) {
           const long long i = M.src + (long long)r * M.cols + c;
-          const float g = mu.g[i] * coef;
-          const float b = mu.momentum * mu.buf[i] + (1.f - mu.momentum) * g;
-          mu.buf[i] = b;
-          v = mu.nesterov ? (1.f - mu.momentum) * g + mu.momentum * b : b;
+          v = muon_in(mu, coef, mu.g[i], mu.buf[i]);
         } else {
           const DasNsSource& s = src.s[M.group - src.first];
           v = load_as_f32<T>(s.base, M.index * s.batch_stride + r * s.row_stride + c);
@@ -447,6 +455,14 @@ struct Result {             // where the last product goes
   float keep, lr;
   int lr_scale;
 };
+__device__ __forceinline__ float result_factor(const NsMatrix& M, const Result& res) {
+  float f = 1.f / M.scale;
+  if (res.p) {
+    const float r = (float)M.rows, c = (float)M.cols;
+    f *= res.lr * (res.lr_scale ? 0.2f * sqrtf(fmaxf(r, c)) : sqrtf(fmaxf(1.f, r / c)));
+  }
+  return f;
+}
 
 // X' = Q X: Q's rows by X's columns. LAST: the result leaves the work area (and its scale S), transposed back where needed.
 template <int T, bool SPLIT, bool LAST>
@@ -469,11 +485,7 @@ __global__ __launch_bounds__(TPB, 2) void update_kernel(const NsMatrix* __restri
       if (i0 + r < M.m) put<SPLIT>(Y + W * M.x, M.ldx, i0 + r, j0 + c, v);   // (columns n ... ldx: zero, as X's are)
     });
   } else {
-    float f = 1.f / M.scale;
-    if (res.p) {
-      const float r = (float)M.rows, c = (float)M.cols;
-      f *= res.lr * (res.lr_scale ? 0.2f * sqrtf(fmaxf(r, c)) : sqrtf(fmaxf(1.f, r / c)));
-    }
+    const float f = result_factor(M, res);
     const bool vec = M.cols % 8 == 0 && M.src % 8 == 0 && !((uintptr_t)(res.p ? (const void*)res.p : res.out) & 15);
     auto emit = [&](int r, int c, float (&v)[8]) {   // in the caller's rows and columns
       if (r >= M.rows || c >= M.cols) return;
@@ -520,10 +532,239 @@ __global__ __launch_bounds__(TPB, 2) void update_kernel(const NsMatrix* __restri
   }
 }
 
+// ------------------------------------------------------------------ small matrices
+// m <= 64, n <= 256: the whole of it in one workgroup, everything between the caller's reads and writes in LDS (pairs of f16 whatever the
+// result's type: the products are a microsecond). A launch for every product would cost 4 us each; 64 x 64: 67 us as 17 launches.
+// X is 64 x NMAX, G, R, Z and two Q are 64 x 64, rows and columns past the matrix are zero, row pitches are 16 bytes past a multiple of the
+// banks' width. 32 columns of X take 128 bytes as f16 pairs and as floats: U and the result use the same place.
+constexpr int SMALL_M = 64, SMALL_N = 256;
+constexpr int PA = 2 * SMALL_M + 8;   // row pitch of the m x m matrices, f16 elements
+struct Steps {
+  float coef[3 * DAS_NS_MAX_STEPS];
+  int end[DAS_NS_MAX_STEPS];          // of the phase that starts at this step
+  int steps;
+  float eps;
+};
+
+__device__ __forceinline__ f16x8_t row_frag(const _Float16* p, int pitch, int row0, int k, int part) {
+  const int lane = threadIdx.x & 63;
+  return *reinterpret_cast<const f16x8_t*>(p + (row0 + (lane & 15)) * pitch + k * 64 + part * 32 + (lane >> 4) * 8);
+}
+__device__ __forceinline__ f16x8_t col_frag(const _Float16* x, int pitch, int col0, int k, int part) {
+  const int lane = threadIdx.x & 63, q = lane & 15, c = col0 + (q & 3) * 4;
+  f16x8_t f;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int r = k * 32 + (lane >> 4) * 8 + h * 4 + (q >> 2);
+    const f16x4_t v = __builtin_bit_cast(
+        f16x4_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4_t*)(x + r * pitch + (c >> 5) * 64 + part * 32 + (c & 31))));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[h * 4 + e] = v[e];
+  }
+  return f;
+}
+// the wave's 32 x 32 of P rows x (Q rows, or columns of Q): k32 inner steps of 32
+template <bool COLS>
+__device__ __forceinline__ void small_product(const _Float16* p, int pp, const _Float16* q, int qp, int col0, int k32, f32x4_t (&acc)[2][2]) {
+  const int wave = threadIdx.x >> 6, wr = (wave >> 1) * 32, wc = (wave & 1) * 32;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  for (int k = 0; k < k32; ++k) {
+    f16x8_t fa[2][2], fb[2][2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        fa[u][t] = row_frag(p, pp, wr + t * 16, k, u);
+        fb[u][t] = COLS ? col_frag(q, qp, col0 + wc + t * 16, k, u) : row_frag(q, qp, wc + t * 16, k, u);
+      }
+#pragma unroll
+    for (int z = 0; z < 3; ++z)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa[z == 0][i], fb[z == 1][j], acc[i][j], 0, 0, 0);
+  }
+}
+// a symmetric result, stored transposed (four values of a lane are neighbours then): f(row, col, four values) may change them
+template <typename F>
+__device__ __forceinline__ void small_store(const f32x4_t (&acc)[2][2], _Float16* out, F f) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int r = (wave & 1) * 32 + j * 16 + (lane & 15), c = (wave >> 1) * 32 + i * 16 + (lane >> 4) * 4;
+      float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+      f(r, c, v);
+      f16x4_t h, l;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        h[e] = (_Float16)v[e];
+        l[e] = (_Float16)(v[e] - (float)h[e]);
+      }
+      _Float16* p = out + r * PA + (c >> 5) * 64 + (c & 31);
+      *reinterpret_cast<f16x4_t*>(p) = h;
+      *reinterpret_cast<f16x4_t*>(p + 32) = l;
+    }
+}
+
+template <typename T, bool MUON, int NMAX>
+__global__ __launch_bounds__(TPB) void small_kernel(const NsMatrix* __restrict__ mats, Sources src, MuonIn mu, Steps st, Result res) {
+  extern __shared__ __align__(16) char smem[];
+  __shared__ float red[4];
+  __shared__ double redd[4];
+  constexpr int PX = 2 * NMAX + 8, PF = NMAX + 4;   // X's row pitch in f16 elements and in floats
+  const NsMatrix M = mats[blockIdx.x];
+  if (!MUON && (unsigned)(M.group - src.first) >= (unsigned)src.count) return;   // (whole workgroups)
+  _Float16* X = reinterpret_cast<_Float16*>(smem);
+  float* U = reinterpret_cast<float*>(smem);
+  _Float16* A[N_AREAS];
+#pragma unroll
+  for (int i = 0; i < N_AREAS; ++i) A[i] = X + SMALL_M * PX + i * SMALL_M * PA;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+
+  // U, zeros around it
+  for (int i = threadIdx.x; i < SMALL_M * PF / 4; i += TPB) reinterpret_cast<float4*>(U)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  __syncthreads();
+  float coef = 1.f, big = 0.f;
+  if constexpr (MUON) coef = grad_factor(mu);
+  for (int c = lane; c < M.cols; c += 64)
+#pragma unroll 4
+    for (int r = wave; r < M.rows; r += 4) {
+      float v;
+      if constexpr (MUON) {
+        const long long i = M.src + r * M.cols + c;
+        v = muon_in(mu, coef, mu.g[i], mu.buf[i]);
+      } else {
+        const DasNsSource& s = src.s[M.group - src.first];
+        v = load_as_f32<T>(s.base, M.index * s.batch_stride + r * s.row_stride + c);
+      }
+      U[M.tall ? c * PF + r : r * PF + c] = v;
+      big = fmaxf(big, fabsf(v));
+    }
+  big = block_reduce(big, true, red);   // (its barriers order U's writes too)
+  int e = 0;
+  if (big > 0.f && big <= 3.4028235e38f) (void)frexpf(big, &e);
+  float v[NMAX / 32][8], ss = 0.f;
+  const int row = threadIdx.x >> 2, c8 = (threadIdx.x & 3) * 8;
+#pragma unroll
+  for (int b = 0; b < NMAX / 32; ++b)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      v[b][k] = ldexpf(U[row * PF + b * 32 + c8 + k], -e);
+      ss += v[b][k] * v[b][k];
+    }
+  double sum = ss;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+  if (lane == 0) redd[wave] = sum;
+  __syncthreads();                       // (every read of U is done, too)
+  const float f = (float)ldexp((double)M.scale / (ldexp(sqrt((redd[0] + redd[1]) + (redd[2] + redd[3])), e) + (double)st.eps), e);
+#pragma unroll
+  for (int b = 0; b < NMAX / 32; ++b) {
+    f16x8_t h, l;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float x = v[b][k] * f;
+      h[k] = (_Float16)x;
+      l[k] = (_Float16)(x - (float)h[k]);
+    }
+    *reinterpret_cast<f16x8_t*>(X + row * PX + b * 64 + c8) = h;
+    *reinterpret_cast<f16x8_t*>(X + row * PX + b * 64 + 32 + c8) = l;
+  }
+  __syncthreads();
+
+  // the phases of iterate<true>
+  const int n32 = (M.n + 31) / 32, tiles = (M.n + 63) / 64;
+  f32x4_t acc[2][2];
+  auto plain = [](int, int, float (&)[4]) {};
+  for (int k = 0; k < st.steps;) {
+    const int end = st.end[k];
+    const float gs = M.gscale / (M.scale * M.scale);
+    _Float16 *G = A[0], *R = A[1], *Z = A[2], *q = nullptr, *spare = A[3], *other = A[4];
+    small_product<false>(X, PX, X, PX, 0, n32, acc);
+    small_store(acc, G, [&](int, int, float (&w)[4]) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) w[t] *= gs;
+    });
+    __syncthreads();
+    for (int j = k; j < end; ++j) {
+      const float ca = st.coef[3 * j], cb = st.coef[3 * j + 1] / M.gscale, cc = st.coef[3 * j + 2] / (M.gscale * M.gscale);
+      _Float16* z = q ? Z : spare;
+      small_product<false>(G, PA, G, PA, 0, 2, acc);
+      small_store(acc, z, [&](int r, int c, float (&w)[4]) {
+        const _Float16* g = G + r * PA + (c >> 5) * 64 + (c & 31);
+        const f16x4_t h = *reinterpret_cast<const f16x4_t*>(g), l = *reinterpret_cast<const f16x4_t*>(g + 32);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) w[t] = cc * w[t] + cb * ((float)h[t] + (float)l[t]) + (r == c + t ? ca : 0.f);
+      });
+      __syncthreads();
+      if (q) {
+        small_product<false>(z, PA, q, PA, 0, 2, acc);
+        small_store(acc, other, plain);
+      }
+      if (j + 1 < end) {
+        small_product<false>(z, PA, G, PA, 0, 2, acc);
+        small_store(acc, R, plain);
+      }
+      __syncthreads();
+      if (q) {
+        _Float16* t = q;
+        q = other;
+        other = t;
+      } else {
+        q = z;
+      }
+      if (j + 1 < end) {
+        small_product<false>(R, PA, z, PA, 0, 2, acc);
+        small_store(acc, G, plain);       // (nobody reads G any more)
+        __syncthreads();
+      }
+    }
+    const bool last = end == st.steps;
+    for (int t = 0; t < tiles; ++t) {
+      small_product<true>(q, PA, X, PX, t * 64, 2, acc);
+      __syncthreads();                    // (the 64 columns of X have been read; nobody else needs them)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const int r = (wave >> 1) * 32 + i * 16 + (lane >> 4) * 4 + w, c = t * 64 + (wave & 1) * 32 + j * 16 + (lane & 15);
+            const float x = acc[i][j][w];
+            if (last) {
+              U[r * PF + c] = x;
+            } else {
+              _Float16* p = X + r * PX + (c >> 5) * 64 + (c & 31);
+              p[0] = (_Float16)x;
+              p[32] = (_Float16)(x - (float)p[0]);
+            }
+          }
+    }
+    __syncthreads();
+    k = end;
+  }
+
+  const float g = result_factor(M, res);
+  for (int c = lane; c < M.cols; c += 64)
+#pragma unroll 4
+    for (int r = wave; r < M.rows; r += 4) {
+      const float x = g * U[M.tall ? c * PF + r : r * PF + c];
+      const long long o = M.src + r * M.cols + c;
+      if constexpr (MUON) res.p[o] = res.keep * res.p[o] - x;
+      else if (res.out_dtype == DAS_F32) reinterpret_cast<float*>(res.out)[o] = x;
+      else reinterpret_cast<uint16_t*>(res.out)[o] = res.out_dtype == DAS_BF16 ? f32_to_bf16(x) : __builtin_bit_cast(uint16_t, (_Float16)x);
+    }
+}
+
 // ------------------------------------------------------------------ host side
 inline long long up256(long long v) { return (v + 255) / 256 * 256; }
 
-constexpr int N_AREAS = 5;   // m x m work matrices: G, R, Z, two of Q (the f16 form uses G and Z)
 struct Work {
   _Float16 *x[2], *a[N_AREAS];
   Partial* part;
@@ -542,7 +783,7 @@ Work carve(const DasNsPlan* p, bool split, void* ws) {
 }
 
 bool plan_valid(const DasNsPlan* p, const void* tables, const void* ws) {
-  return p && tables && ws && p->n_matrices > 0 && p->n_chunks > 0 && p->n_gram > 0 && p->n_update > 0 && p->steps > 0 &&
+  return p && tables && ws && p->n_matrices > 0 && p->n_small >= 0 && p->n_small <= p->n_matrices && p->steps > 0 &&
          p->steps <= DAS_NS_MAX_STEPS && (p->gram_tile == 64 || p->gram_tile == 128) && (p->update_tile == 64 || p->update_tile == 128) &&
          !(((uintptr_t)tables | (uintptr_t)ws) & 15);
 }
@@ -570,16 +811,50 @@ bool polynomial_bounds(const float* coef, int steps, Bounds* out) {
   return true;
 }
 
+// where the phase that starts at step k ends (f32 results)
+int phase_end(const Bounds* bound, int steps, int k) {
+  double growth = bound[k].factor * bound[k].factor;
+  int end = k + 1;
+  while (end < steps && growth <= 256.0) {
+    growth *= bound[end].factor * bound[end].factor;
+    ++end;
+  }
+  return end;
+}
+
+template <typename T, bool MUON>
+int launch_small(const DasNsPlan* p, const char* tab, const Sources& src, const MuonIn& mu, const Result& res, hipStream_t s) {
+  if (p->n_small == 0) return DAS_OK;
+  Steps st = {};
+  Bounds bound[DAS_NS_MAX_STEPS];
+  if (!polynomial_bounds(p->coef, p->steps, bound)) return DAS_ERR_ARG;
+  memcpy(st.coef, p->coef, sizeof(st.coef));
+  st.steps = p->steps;
+  st.eps = p->eps;
+  for (int k = 0; k < p->steps; ++k) st.end[k] = phase_end(bound, p->steps, k);
+  const NsMatrix* mats = (const NsMatrix*)(tab + p->mat_at);
+  auto launch = [&](auto kernel, int nmax) {
+    const int lds = 2 * (SMALL_M * (2 * nmax + 8) + N_AREAS * SMALL_M * PA);
+    (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    hipLaunchKernelGGL(kernel, dim3(p->n_small), dim3(TPB), lds, s, mats, src, mu, st, res);
+  };
+  if (p->small_n <= 64) launch(small_kernel<T, MUON, 64>, 64);
+  else launch(small_kernel<T, MUON, 256>, 256);
+  DAS_CHECK_LAUNCH();
+  return DAS_OK;
+}
+
 template <bool SPLIT>
 int iterate(const DasNsPlan* p, const char* tab, Work w, const Result& res, hipStream_t s) {
   const NsMatrix* mats = (const NsMatrix*)(tab + p->mat_at);
-  const int4 *chunks = (const int4*)(tab + p->chunk_at), *gram = (const int4*)(tab + p->gram_at), *upd = (const int4*)(tab + p->update_at);
+  const int4 *chunks = (const int4*)(tab + p->chunk_at), *gram = (const int4*)(tab + p->gram_at), *upd = (const int4*)(tab + p->update_at),
+             *prod = (const int4*)(tab + p->product_at);
   auto sym = [&](auto kind, int products, const SymArgs& a) {
     constexpr SymKind K = decltype(kind)::value;
     if (p->gram_tile == 128)
-      hipLaunchKernelGGL((sym_kernel<128, SPLIT, K>), dim3(p->n_gram, products), dim3(TPB), 0, s, mats, gram, a);
+      hipLaunchKernelGGL((sym_kernel<128, SPLIT, K>), dim3(p->n_gram, products), dim3(TPB), 0, s, mats, K == GRAM ? gram : prod, a);
     else
-      hipLaunchKernelGGL((sym_kernel<64, SPLIT, K>), dim3(p->n_gram, products), dim3(TPB), 0, s, mats, gram, a);
+      hipLaunchKernelGGL((sym_kernel<64, SPLIT, K>), dim3(p->n_gram, products), dim3(TPB), 0, s, mats, K == GRAM ? gram : prod, a);
   };
   auto update = [&](auto last, const _Float16* q, const _Float16* x, _Float16* y) {
     constexpr bool L = decltype(last)::value;
@@ -598,14 +873,7 @@ int iterate(const DasNsPlan* p, const char* tab, Work w, const Result& res, hipS
   _Float16 *X = w.x[0], *Y = w.x[1], *G = w.a[0], *R = w.a[1], *Z = w.a[SPLIT ? 2 : 1];
   for (int k = 0; k < p->steps;) {
     // steps k ... end - 1 are one phase
-    int end = k + 1;
-    if (SPLIT) {
-      double growth = bound[k].factor * bound[k].factor;
-      while (end < p->steps && growth <= 256.0) {
-        growth *= bound[end].factor * bound[end].factor;
-        ++end;
-      }
-    }
+    const int end = SPLIT ? phase_end(bound, p->steps, k) : k + 1;
     sym(gram_k, 1, SymArgs{{X}, {X}, {G}, 0.f, 0.f, 0.f});
     _Float16 *q = nullptr, *spare = w.a[SPLIT ? 3 : 1], *other = SPLIT ? w.a[4] : nullptr;   // (q: the phase's product so far)
     for (int j = k; j < end; ++j) {
@@ -642,9 +910,13 @@ extern "C" int das_ns_plan(const DasNsShape* shapes, int n, int steps, const flo
       !polynomial_bounds(coef, steps, bound))
     return DAS_ERR_ARG;
   memset(plan, 0, sizeof(*plan));
+  auto is_small = [&](int g) {
+    return std::min(shapes[g].rows, shapes[g].cols) <= SMALL_M && std::max(shapes[g].rows, shapes[g].cols) <= SMALL_N;
+  };
   auto tiles = [&](int t, bool sym) {
     long long c = 0;
     for (int g = 0; g < n; ++g) {
+      if (is_small(g)) continue;
       const long long m = std::min(shapes[g].rows, shapes[g].cols), nn = std::max(shapes[g].rows, shapes[g].cols);
       const long long tm = (m + t - 1) / t, tn = (nn + 127) / 128 * (128 / t);
       c += shapes[g].count * (sym ? tm * (tm + 1) / 2 : tm * tn);
@@ -661,9 +933,14 @@ extern "C" int das_ns_plan(const DasNsShape* shapes, int n, int steps, const flo
     const long long m = std::min(s.rows, s.cols), nn = std::max(s.rows, s.cols);
     const long long ldx = (nn + 127) / 128 * 128, lda = (m + 63) / 64 * 64;
     n_mat += s.count;
-    n_chunks += s.count * (lda / 64) * (ldx / 64);
-    plan->x_elems += s.count * m * ldx;
-    plan->a_elems += s.count * m * lda;
+    if (is_small(g)) {
+      plan->n_small += s.count;
+      plan->small_n = std::max(plan->small_n, (int)nn);
+    } else {
+      n_chunks += s.count * (lda / 64) * (ldx / 64);
+      plan->x_elems += s.count * m * ldx;
+      plan->a_elems += s.count * m * lda;
+    }
     if (n_mat > (1 << 24) || n_chunks > (1 << 26) || m > (1 << 15)) return DAS_ERR_ARG;
     spans.push_back({s.off, s.off + (long long)s.count * s.rows * s.cols});
   }
@@ -680,28 +957,33 @@ extern "C" int das_ns_plan(const DasNsShape* shapes, int n, int steps, const flo
   plan->mat_at = 0;
   plan->chunk_at = up256(n_mat * (long long)sizeof(NsMatrix));
   plan->gram_at = plan->chunk_at + up256(16 * n_chunks);
-  plan->update_at = plan->gram_at + up256(16 * n_gram);
+  plan->product_at = plan->gram_at + up256(16 * n_gram);
+  plan->update_at = plan->product_at + up256(16 * n_gram);
   plan->table_bytes = plan->update_at + up256(16 * n_upd);
   if (!tables) return DAS_OK;
   if (table_bytes < plan->table_bytes) return DAS_ERR_ARG;
   memset(tables, 0, plan->table_bytes);
   char* tab = (char*)tables;
   NsMatrix* mats = (NsMatrix*)(tab + plan->mat_at);
-  int4 *chunk = (int4*)(tab + plan->chunk_at), *gram = (int4*)(tab + plan->gram_at), *upd = (int4*)(tab + plan->update_at);
+  int4 *chunk = (int4*)(tab + plan->chunk_at), *gram = (int4*)(tab + plan->gram_at), *upd = (int4*)(tab + plan->update_at),
+       *prod = (int4*)(tab + plan->product_at);
   long long x = 0, a = 0;
-  int q = 0, c = 0;
+  int small = 0, big = plan->n_small, c = 0;   // (the small matrices come first in the table)
   for (int g = 0; g < n; ++g) {
     const DasNsShape& s = shapes[g];
-    for (int i = 0; i < s.count; ++i, ++q) {
+    for (int i = 0; i < s.count; ++i) {
+      const int q = is_small(g) ? small++ : big++;
       NsMatrix& M = mats[q];
       M.rows = s.rows; M.cols = s.cols; M.m = std::min(s.rows, s.cols); M.n = std::max(s.rows, s.cols);
       M.tall = s.rows > s.cols;
       M.ldx = (M.n + 127) / 128 * 128; M.lda = (M.m + 63) / 64 * 64;
       M.src = s.off + (long long)i * s.rows * s.cols;
-      M.x = x; M.a = a; M.group = g; M.index = i; M.chunk0 = c;
+      M.group = g; M.index = i;
       M.scale = (float)std::ldexp(1.0, (int)std::lround(0.5 * std::log2((double)M.n)));
       // about m, and top^2 gscale within f16
       M.gscale = (float)std::ldexp(1.0, std::min((int)std::lround(std::log2((double)M.m)), (int)std::floor(std::log2(32768.0 / (top * top)))));
+      if (is_small(g)) continue;
+      M.x = x; M.a = a; M.chunk0 = c;
       x += (long long)M.m * M.ldx; a += (long long)M.m * M.lda;
       int k = 0;
       for (int r = 0; r < (M.tall ? M.ldx : M.lda) / CHUNK; ++r)
@@ -710,25 +992,28 @@ extern "C" int das_ns_plan(const DasNsShape* shapes, int n, int steps, const flo
     }
   }
   // longest inner axis first: the last workgroups to start are the shortest ones
-  std::vector<int> order(n_mat);
-  for (int i = 0; i < (int)n_mat; ++i) order[i] = i;
-  std::stable_sort(order.begin(), order.end(), [&](int u, int v) { return mats[u].n > mats[v].n; });
+  std::vector<int> by_n, by_m;
+  for (int i = plan->n_small; i < (int)n_mat; ++i) by_n.push_back(i);
+  by_m = by_n;
+  std::stable_sort(by_n.begin(), by_n.end(), [&](int u, int v) { return mats[u].n > mats[v].n; });
+  std::stable_sort(by_m.begin(), by_m.end(), [&](int u, int v) { return mats[u].m > mats[v].m; });
   auto across = [](int v, int t) { return (v + t - 1) / t; };
-  int t = 0;
-  for (int i : order)
-    for (int r = 0; r < across(mats[i].m, plan->gram_tile); ++r)
-      for (int j = 0; j <= r; ++j) gram[t++] = make_int4(i, r, j, 0);
-  std::stable_sort(order.begin(), order.end(), [&](int u, int v) { return mats[u].m > mats[v].m; });
-  t = 0;
-  for (int i : order)
+  auto lower = [&](const std::vector<int>& order, int4* t) {
+    for (int i : order)
+      for (int r = 0; r < across(mats[i].m, plan->gram_tile); ++r)
+        for (int j = 0; j <= r; ++j) *t++ = make_int4(i, r, j, 0);
+  };
+  lower(by_n, gram);
+  lower(by_m, prod);
+  for (int i : by_m)
     for (int j = 0; j < mats[i].ldx / plan->update_tile; ++j)
-      for (int r = 0; r < across(mats[i].m, plan->update_tile); ++r) upd[t++] = make_int4(i, r, j, 0);
+      for (int r = 0; r < across(mats[i].m, plan->update_tile); ++r) *upd++ = make_int4(i, r, j, 0);
   return DAS_OK;
 }
 
 extern "C" long long das_ns_ws_bytes(const DasNsPlan* p, int f32_result) {
   if (!p) return -1;
-  return carve(p, f32_result != 0, nullptr).bytes;
+  return std::max(256LL, carve(p, f32_result != 0, nullptr).bytes);
 }
 
 extern "C" int das_orthogonalize(const DasNsPlan* plan, const void* tables_dev, const DasNsSource* srcs, int n_srcs, int in_dtype,
@@ -746,12 +1031,19 @@ extern "C" int das_orthogonalize(const DasNsPlan* plan, const void* tables_dev, 
   const NsMatrix* mats = (const NsMatrix*)(tab + plan->mat_at);
   const int4* chunks = (const int4*)(tab + plan->chunk_at);
   const MuonIn none = {};
+  const Result res = {out, out_dtype, nullptr, 1.f, 0.f, 0};
   // one launch for every 64 source tensors (one in all but unusual sets): its workgroups of other tensors' blocks end at once
   for (int first = 0; first < n_srcs; first += Sources::MAX) {
     Sources a;
     a.first = first;
     a.count = std::min(Sources::MAX, n_srcs - first);
     for (int i = 0; i < Sources::MAX; ++i) a.s[i] = srcs[first + std::min(i, a.count - 1)];
+    int st = DAS_OK;
+    if (in_dtype == DAS_F32) st = launch_small<float, false>(plan, tab, a, none, res, s);
+    else if (in_dtype == DAS_BF16) st = launch_small<bf16_t, false>(plan, tab, a, none, res, s);
+    else st = launch_small<_Float16, false>(plan, tab, a, none, res, s);
+    if (st != DAS_OK) return st;
+    if (plan->n_chunks == 0) continue;
     auto launch = [&](auto kernel) {
       hipLaunchKernelGGL(kernel, dim3(plan->n_chunks), dim3(TPB), 0, s, mats, chunks, a, none, w.x[0], w.part);
     };
@@ -760,7 +1052,7 @@ extern "C" int das_orthogonalize(const DasNsPlan* plan, const void* tables_dev, 
     else split ? launch(ingest_kernel<_Float16, false, true>) : launch(ingest_kernel<_Float16, false, false>);
     DAS_CHECK_LAUNCH();
   }
-  const Result res = {out, out_dtype, nullptr, 1.f, 0.f, 0};
+  if (plan->n_chunks == 0) return DAS_OK;
   return split ? iterate<true>(plan, tab, w, res, s) : iterate<false>(plan, tab, w, res, s);
 }
 
@@ -776,9 +1068,11 @@ extern "C" int das_muon_step(const DasNsPlan* plan, const void* tables_dev, floa
   const char* tab = (const char*)tables_dev;
   const Work w = carve(plan, true, ws);
   const MuonIn mu = {g, buf, momentum, grad_scale, max_norm, nesterov, grad_sumsq};
+  const Result res = {nullptr, 0, p, (float)(1.0 - (double)lr * (double)weight_decay), lr, lr_scale};
+  const int st = launch_small<float, true>(plan, tab, Sources{}, mu, res, s);
+  if (st != DAS_OK || plan->n_chunks == 0) return st;
   hipLaunchKernelGGL((ingest_kernel<float, true, true>), dim3(plan->n_chunks), dim3(TPB), 0, s, (const NsMatrix*)(tab + plan->mat_at),
                      (const int4*)(tab + plan->chunk_at), Sources{}, mu, w.x[0], w.part);
   DAS_CHECK_LAUNCH();
-  const Result res = {nullptr, 0, p, (float)(1.0 - (double)lr * (double)weight_decay), lr, lr_scale};
   return iterate<true>(plan, tab, w, res, s);
 }

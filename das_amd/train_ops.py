@@ -1,4 +1,5 @@
 """ctypes wrappers of the loss / target / optimizer entry points (train_loss.hip, adamw.hip, muon.hip)."""
+import contextlib
 import ctypes as C
 
 import torch
@@ -155,6 +156,14 @@ def _flat_buffers(what, *ts):
             raise _lib.DasHipError(f'{what}: parameters, gradients and state are contiguous float32 tensors of one size on one device')
 
 
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def _on(device):
+    """Launches go to the tensors' device, whichever is current (entering torch's guard costs microseconds: only where needed)"""
+    return _SAME_DEVICE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
 def _clip_sum(what, max_norm, grad_sumsq_t, device):
     if not max_norm > 0:
         return None
@@ -172,7 +181,7 @@ def adamw_step(p, g, m, v, lr, step, beta1=0.9, beta2=0.999, eps=1e-8, weight_de
     sumsq = _clip_sum('adamw_step', max_norm, grad_sumsq_t, p.device)
     if p.numel() == 0:
         return
-    with torch.cuda.device(p.device):
+    with _on(p.device):
         _lib.check(_lib.load().das_adamw_step(_ptr(p), _ptr(g), _ptr(m), _ptr(v), p.numel(), float(lr), float(beta1), float(beta2),
                                               float(eps), float(weight_decay), int(step), float(grad_scale), float(max_norm),
                                               _ptr(sumsq), _stream()), 'das_adamw_step')
@@ -274,7 +283,7 @@ def orthogonalize(mats, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, out_dty
         src = (_lib.DasNsSource * len(live))()
         for s, t in zip(src, live):
             s.base, s.row_stride, s.batch_stride = t.data_ptr(), t.stride(-2), t.stride(0) if t.dim() == 3 else 0
-        with torch.cuda.device(dev):
+        with _on(dev):
             lib = _lib.load()
             ws = torch.empty(lib.das_ns_ws_bytes(C.byref(p), int(out_dtype == torch.float32)), dtype=torch.uint8, device=dev)
             _lib.check(lib.das_orthogonalize(C.byref(p), _ptr(tables), src, len(live), dt, _ptr(out), _NS_DT[out_dtype], _ptr(ws),
@@ -300,7 +309,7 @@ def muon_step(p, g, buf, plan, lr, momentum=0.95, weight_decay=0.0, nesterov=Tru
     c_plan, tables = plan._flat
     if c_plan.extent > p.numel():
         raise _lib.DasHipError(f'muon_step: the plan reaches element {c_plan.extent} of buffers of {p.numel()}')
-    with torch.cuda.device(p.device):
+    with _on(p.device):
         lib = _lib.load()
         ws = torch.empty(lib.das_ns_ws_bytes(C.byref(c_plan), 1), dtype=torch.uint8, device=p.device)
         _lib.check(lib.das_muon_step(C.byref(c_plan), _ptr(tables), _ptr(p), _ptr(g), _ptr(buf), float(lr), float(momentum),

@@ -626,9 +626,9 @@ typedef struct {
   int reserved;
 } DasNsShape;
 typedef struct {
-  int n_groups, n_matrices, n_chunks, n_gram, n_update, steps, gram_tile, update_tile;
+  int n_groups, n_matrices, n_chunks, n_gram, n_update, steps, gram_tile, update_tile, n_small, small_n;
   long long x_elems, a_elems, extent;            /* work areas (f16 elements); one past the last element of the flat buffers used */
-  long long mat_at, chunk_at, gram_at, update_at, table_bytes;   /* byte offsets of the tables */
+  long long mat_at, chunk_at, gram_at, product_at, update_at, table_bytes;   /* byte offsets of the tables */
   float coef[3 * DAS_NS_MAX_STEPS];              /* a, b, c of each step */
   float eps;
 } DasNsPlan;
