@@ -242,6 +242,8 @@ __global__ __launch_bounds__(TPB) void normalise_kernel(const NsMatrix* __restri
 // one of two buffers while the other is multiplied; the fragments are read before the next copies are issued, so no LDS read waits for them.
 //   plain:  acc += A0 B0 + A1 B1   (two halves of the inner axis)
 //   SPLIT:  acc += Ah Bh + Ah Bl + Al Bh   (the low x low part is 2^-22 of the product)
+// KG groups of four waves divide the inner axis between them (KG = 4 where a launch has fewer tiles than CUs and latency is all: every
+// group has its own buffers and copies in flight) and join their sums through LDS, in order.
 // LDS images. Rows by rows (gram, product, and B of the update): two panels of T rows x 64 bytes, 16-byte slot s of row r holds source
 // slot s ^ (r / 2 % 4): eight neighbouring rows cover all banks. Columns of X (update): inner rows as they are in memory, 32-byte units
 // swizzled by row, read with ds_read_tr16_b64 (four inner rows x 16 columns a 16-lane group, one column a lane).
@@ -255,16 +257,16 @@ __device__ __forceinline__ void copy16(const void* src, char* lds_wave_base) {
 template <int T>
 struct RowsOperand {        // T rows of a matrix whose rows run along the inner axis
   const char* src[T / 32];
-  __device__ __forceinline__ void init(const _Float16* base, int pitch, int row0, int rows) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  __device__ __forceinline__ void init(const _Float16* base, int pitch, int row0, int rows, int stage0) {
+    const int lane = threadIdx.x & 63, wave = (threadIdx.x >> 6) & 3;
 #pragma unroll
     for (int i = 0; i < T / 32; ++i) {
       const int q = wave * (T / 32) + i, r = (q >> 1) * 16 + (lane >> 2), kg = (lane & 3) ^ ((r >> 1) & 3);
-      src[i] = (const char*)(base + (long long)min(row0 + r, rows - 1) * pitch + (q & 1) * 32 + kg * 8);   // (rows past the end: stand-ins)
+      src[i] = (const char*)(base + (long long)min(row0 + r, rows - 1) * pitch + stage0 * 64 + (q & 1) * 32 + kg * 8);   // (rows past the end: stand-ins)
     }
   }
   __device__ __forceinline__ void issue(char* lds) {
-    const int wave = threadIdx.x >> 6;
+    const int wave = (threadIdx.x >> 6) & 3;
 #pragma unroll
     for (int i = 0; i < T / 32; ++i) {
       const int q = wave * (T / 32) + i;
@@ -283,19 +285,18 @@ template <int T, bool SPLIT>
 struct ColsOperand {        // T columns of a matrix whose rows run across the inner axis
   static constexpr int ROWB = SPLIT ? T * 4 : T * 2, LPR = ROWB / 16, ROWS = SPLIT ? 32 : 64;   // bytes and lanes of a row, rows of a stage
   const char* base;
-  int pitch, rows, row;     // bytes; rows of the matrix; this lane's row in the first copy
-  int slot;
+  int pitch, rows, row;     // bytes; rows of the matrix; the stage's first row
   static __device__ __forceinline__ int swz(int r) {
     return ROWB >= 256 ? ((r & 3) | ((r >> 1) & 4)) : (((r >> 1) & 1) | ((r >> 2) & 2));
   }
-  __device__ __forceinline__ void init(const _Float16* x, int pitch_elems, int col0, int rows_) {
+  __device__ __forceinline__ void init(const _Float16* x, int pitch_elems, int col0, int rows_, int stage0) {
     base = (const char*)(x + col0 * (SPLIT ? 2 : 1));
     pitch = pitch_elems * 2;
     rows = rows_;
-    row = 0;
+    row = stage0 * ROWS;
   }
   __device__ __forceinline__ void issue(char* lds) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = (threadIdx.x >> 6) & 3;
 #pragma unroll
     for (int i = 0; i < T / 32; ++i) {
       const int q = wave * (T / 32) + i, r = q * (64 / LPR) + lane / LPR, s = lane % LPR;
@@ -328,55 +329,86 @@ struct ColsOperand {        // T columns of a matrix whose rows run across the i
 template <int T>
 using Acc = f32x4_t[T / 32][T / 32];
 
-template <int T, bool SPLIT, typename OB>
+template <int T, int KG>
+constexpr int lds_bytes() { return KG * 4 * T * 128; }
+
+// `stages`: of the whole inner axis; the group's first one is group * ceil(stages / KG)
+template <int T, bool SPLIT, int KG, typename OB>
 __device__ __forceinline__ void multiply(RowsOperand<T>& a, OB& b, int stages, char* smem, Acc<T>& acc) {
   constexpr int HALF = T * 128, N = T / 32;   // bytes of one operand's stage; fragments a wave has of each operand
-  const int wave = threadIdx.x >> 6, wr = (wave >> 1) * (T / 2), wc = (wave & 1) * (T / 2);
+  const int wave = (threadIdx.x >> 6) & 3, wr = (wave >> 1) * (T / 2), wc = (wave & 1) * (T / 2);
+  const int group = KG == 1 ? 0 : threadIdx.x >> 8, per = (stages + KG - 1) / KG, mine = KG == 1 ? stages : min(per, stages - group * per);
+  char* base = smem + group * 4 * HALF;
 #pragma unroll
   for (int i = 0; i < N; ++i)
 #pragma unroll
     for (int j = 0; j < N; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  a.issue(smem);
-  b.issue(smem + HALF);
+  if (KG == 1 || mine > 0) {
+    a.issue(base);
+    b.issue(base + HALF);
+  }
   __syncthreads();
-  for (int k = 0; k < stages; ++k) {
-    const char* cur = smem + (k & 1) * 2 * HALF;
-    char* nxt = smem + ((k & 1) ^ 1) * 2 * HALF;
-    f16x8_t fa[2][N], fb[2][N];
+  for (int k = 0; k < per; ++k) {
+    if (KG == 1 || k < mine) {
+      const char* cur = base + (k & 1) * 2 * HALF;
+      char* nxt = base + ((k & 1) ^ 1) * 2 * HALF;
+      f16x8_t fa[2][N], fb[2][N];
 #pragma unroll
-    for (int p = 0; p < 2; ++p)
+      for (int p = 0; p < 2; ++p)
 #pragma unroll
-      for (int t = 0; t < N; ++t) {
-        fa[p][t] = RowsOperand<T>::frag(cur, wr, t, p);
-        fb[p][t] = OB::frag(cur + HALF, wc, t, p);
+        for (int t = 0; t < N; ++t) {
+          fa[p][t] = RowsOperand<T>::frag(cur, wr, t, p);
+          fb[p][t] = OB::frag(cur + HALF, wc, t, p);
+        }
+      if (k + 1 < mine) {
+        a.issue(nxt);
+        b.issue(nxt + HALF);
       }
-    if (k + 1 < stages) {
-      a.issue(nxt);
-      b.issue(nxt + HALF);
-    }
 #pragma unroll
-    for (int q = 0; q < (SPLIT ? 3 : 2); ++q)   // plain: 00 11; split: low parts first (10, 01), then 00
+      for (int q = 0; q < (SPLIT ? 3 : 2); ++q)   // plain: 00 11; split: low parts first (10, 01), then 00
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+          for (int j = 0; j < N; ++j) {
+            const int pa = SPLIT ? q == 0 : q, pb = SPLIT ? q == 1 : q;
+            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa[pa][i], fb[pb][j], acc[i][j], 0, 0, 0);
+          }
+    }
+    __syncthreads();
+  }
+  if constexpr (KG > 1) {
+    f32x4_t* sums = reinterpret_cast<f32x4_t*>(smem);   // [group - 1][fragment][thread of the group]
+    const int t = threadIdx.x & 255;
+    if (group > 0) {
 #pragma unroll
       for (int i = 0; i < N; ++i)
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-          const int pa = SPLIT ? q == 0 : q, pb = SPLIT ? q == 1 : q;
-          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa[pa][i], fb[pb][j], acc[i][j], 0, 0, 0);
-        }
+        for (int j = 0; j < N; ++j) sums[((group - 1) * N * N + i * N + j) * 256 + t] = acc[i][j];
+    }
     __syncthreads();
+    if (group == 0) {
+#pragma unroll
+      for (int g = 0; g < KG - 1; ++g)
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+          for (int j = 0; j < N; ++j) acc[i][j] += sums[(g * N * N + i * N + j) * 256 + t];
+    }
   }
 }
+template <int KG>
+__device__ __forceinline__ int first_stage(int stages) { return KG == 1 ? 0 : (int)(threadIdx.x >> 8) * ((stages + KG - 1) / KG); }
 
-// The tile through LDS, row by row: f(row, col, eight values of the row). TRANSPOSED: rows and columns of the tile exchanged.
-template <int T, bool TRANSPOSED, typename F>
+// The tile (of the first group) through LDS, row by row: f(row, col, eight values of the row). TRANSPOSED: rows and columns exchanged.
+template <int T, int KG, bool TRANSPOSED, typename F>
 __device__ __forceinline__ void store_tile(const Acc<T>& acc, char* smem, F f) {
   constexpr int P = T + 4;   // floats of a row: the four row groups of a fragment start 16 banks apart
   float* buf = reinterpret_cast<float*>(smem);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int major = (TRANSPOSED ? wave & 1 : wave >> 1) * (T / 2), minor = (TRANSPOSED ? wave >> 1 : wave & 1) * (T / 2);
+  const int major = (TRANSPOSED ? wave & 1 : (wave >> 1) & 1) * (T / 2), minor = (TRANSPOSED ? (wave >> 1) & 1 : wave & 1) * (T / 2);
   for (int r0 = 0; r0 < T; r0 += 64) {
     __syncthreads();
-    if (T == 64 || major == r0) {
+    if ((KG == 1 || wave < 4) && (T == 64 || major == r0)) {
 #pragma unroll
       for (int i = 0; i < T / 32; ++i)
 #pragma unroll
@@ -390,10 +422,11 @@ __device__ __forceinline__ void store_tile(const Acc<T>& acc, char* smem, F f) {
         }
     }
     __syncthreads();
-    constexpr int TPR = T / 8, RPS = TPB / TPR;
+    constexpr int TPR = T / 8, RPS = KG * TPB / TPR;
 #pragma unroll
-    for (int s = 0; s < 64 / RPS; ++s) {
+    for (int s = 0; s < (64 + RPS - 1) / RPS; ++s) {
       const int r = s * RPS + threadIdx.x / TPR, c = (threadIdx.x % TPR) * 8;
+      if (RPS > 64 && r >= 64) continue;
       float v[8];
       *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(buf + r * P + c);
       *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(buf + r * P + c + 4);
@@ -412,9 +445,9 @@ struct SymArgs {            // two independent products a launch (blockIdx.y)
 // Symmetric m x m results, tiles on and below the diagonal, each stored as it is and transposed.
 //   GRAM:     G = X X^T times (gscale / S^2)      POLY: Z = a I + b G + c G G      PRODUCT: P Q of symmetric P, Q that commute
 // Columns m ... lda are stored as zeros: the inner axis of the next product.
-template <int T, bool SPLIT, SymKind KIND>
-__global__ __launch_bounds__(TPB, 2) void sym_kernel(const NsMatrix* __restrict__ mats, const int4* __restrict__ tiles, SymArgs s) {
-  __shared__ __align__(16) char smem[4 * T * 128];
+template <int T, bool SPLIT, int KG, SymKind KIND>
+__global__ __launch_bounds__(KG * TPB, KG == 1 ? 2 : 4) void sym_kernel(const NsMatrix* __restrict__ mats, const int4* __restrict__ tiles, SymArgs s) {
+  extern __shared__ __align__(16) char smem[];
   const int4 t = tiles[blockIdx.x];
   const NsMatrix M = mats[t.x];
   const int z = blockIdx.y, i0 = t.y * T, j0 = t.z * T;
@@ -422,10 +455,11 @@ __global__ __launch_bounds__(TPB, 2) void sym_kernel(const NsMatrix* __restrict_
   const _Float16* P = s.p[z] + (SPLIT ? 2 : 1) * (KIND == GRAM ? M.x : M.a);
   const _Float16* Q = s.q[z] + (SPLIT ? 2 : 1) * (KIND == GRAM ? M.x : M.a);
   RowsOperand<T> a, b;
-  a.init(P, pitch, i0, M.m);
-  b.init(Q, pitch, j0, M.m);
+  const int stages = pitch / 64, first = first_stage<KG>(stages);
+  a.init(P, pitch, i0, M.m, first);
+  b.init(Q, pitch, j0, M.m, first);
   Acc<T> acc;
-  multiply<T, SPLIT>(a, b, pitch / 64, smem, acc);
+  multiply<T, SPLIT, KG>(a, b, stages, smem, acc);
   _Float16* out = s.out[z] + (SPLIT ? 2 : 1) * M.a;
   const float f = KIND == GRAM ? M.gscale / (M.scale * M.scale) : 1.f, cb = s.b / M.gscale, cc = s.c / (M.gscale * M.gscale);
   auto store = [&](int r, int c, float (&v)[8]) {
@@ -444,8 +478,8 @@ __global__ __launch_bounds__(TPB, 2) void sym_kernel(const NsMatrix* __restrict_
       if (c + e >= M.m) v[e] = 0.f;
     put<SPLIT>(out, M.lda, r, c, v);
   };
-  store_tile<T, false>(acc, smem, [&](int r, int c, float (&v)[8]) { store(i0 + r, j0 + c, v); });
-  if (i0 != j0) store_tile<T, true>(acc, smem, [&](int r, int c, float (&v)[8]) { store(j0 + r, i0 + c, v); });
+  store_tile<T, KG, false>(acc, smem, [&](int r, int c, float (&v)[8]) { store(i0 + r, j0 + c, v); });
+  if (i0 != j0) store_tile<T, KG, true>(acc, smem, [&](int r, int c, float (&v)[8]) { store(j0 + r, i0 + c, v); });
 }
 
 struct Result {             // where the last product goes
@@ -465,23 +499,24 @@ __device__ __forceinline__ float result_factor(const NsMatrix& M, const Result& 
 }
 
 // X' = Q X: Q's rows by X's columns. LAST: the result leaves the work area (and its scale S), transposed back where needed.
-template <int T, bool SPLIT, bool LAST>
-__global__ __launch_bounds__(TPB, 2) void update_kernel(const NsMatrix* __restrict__ mats, const int4* __restrict__ tiles,
+template <int T, bool SPLIT, int KG, bool LAST>
+__global__ __launch_bounds__(KG * TPB, KG == 1 ? 2 : 4) void update_kernel(const NsMatrix* __restrict__ mats, const int4* __restrict__ tiles,
                                                         const _Float16* __restrict__ Q, const _Float16* __restrict__ X,
                                                         _Float16* __restrict__ Y, Result res) {
-  __shared__ __align__(16) char smem[4 * T * 128];
+  extern __shared__ __align__(16) char smem[];
   const int4 t = tiles[blockIdx.x];
   const NsMatrix M = mats[t.x];
   const int i0 = t.y * T, j0 = t.z * T;
   constexpr int W = SPLIT ? 2 : 1;
   RowsOperand<T> a;
   ColsOperand<T, SPLIT> b;
-  a.init(Q + W * M.a, W * M.lda, i0, M.m);
-  b.init(X + W * M.x, W * M.ldx, j0, M.m);
+  const int stages = W * M.lda / 64, first = first_stage<KG>(stages);
+  a.init(Q + W * M.a, W * M.lda, i0, M.m, first);
+  b.init(X + W * M.x, W * M.ldx, j0, M.m, first);
   Acc<T> acc;
-  multiply<T, SPLIT>(a, b, W * M.lda / 64, smem, acc);
+  multiply<T, SPLIT, KG>(a, b, stages, smem, acc);
   if constexpr (!LAST) {
-    store_tile<T, false>(acc, smem, [&](int r, int c, float (&v)[8]) {
+    store_tile<T, KG, false>(acc, smem, [&](int r, int c, float (&v)[8]) {
       if (i0 + r < M.m) put<SPLIT>(Y + W * M.x, M.ldx, i0 + r, j0 + c, v);   // (columns n ... ldx: zero, as X's are)
     });
   } else {
@@ -527,8 +562,8 @@ __global__ __launch_bounds__(TPB, 2) void update_kernel(const NsMatrix* __restri
         }
       }
     };
-    if (M.tall) store_tile<T, true>(acc, smem, [&](int r, int c, float (&v)[8]) { emit(j0 + r, i0 + c, v); });
-    else store_tile<T, false>(acc, smem, [&](int r, int c, float (&v)[8]) { emit(i0 + r, j0 + c, v); });
+    if (M.tall) store_tile<T, KG, true>(acc, smem, [&](int r, int c, float (&v)[8]) { emit(j0 + r, i0 + c, v); });
+    else store_tile<T, KG, false>(acc, smem, [&](int r, int c, float (&v)[8]) { emit(i0 + r, j0 + c, v); });
   }
 }
 
@@ -632,20 +667,37 @@ __global__ __launch_bounds__(TPB) void small_kernel(const NsMatrix* __restrict__
   __syncthreads();
   float coef = 1.f, big = 0.f;
   if constexpr (MUON) coef = grad_factor(mu);
-  for (int c = lane; c < M.cols; c += 64)
-#pragma unroll 4
-    for (int r = wave; r < M.rows; r += 4) {
-      float v;
-      if constexpr (MUON) {
-        const long long i = M.src + r * M.cols + c;
-        v = muon_in(mu, coef, mu.g[i], mu.buf[i]);
-      } else {
-        const DasNsSource& s = src.s[M.group - src.first];
-        v = load_as_f32<T>(s.base, M.index * s.batch_stride + r * s.row_stride + c);
+  const int count = M.rows * M.cols;
+  const float per_row = 1.f / (float)M.cols;   // (index + 1/2) / cols is exact enough to truncate for indices under 2^14
+  constexpr int BATCH = 8;                     // loads in flight per thread: a load a time is a memory latency each
+  for (int i0 = threadIdx.x; i0 < count; i0 += BATCH * TPB) {
+    float v[BATCH], b[BATCH];
+    const DasNsSource& s = src.s[MUON ? 0 : M.group - src.first];
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) {
+      const int i = i0 + k * TPB, r = (int)((i + 0.5f) * per_row), c = i - r * M.cols;
+      v[k] = 0.f;
+      if (i < count) {
+        if constexpr (MUON) {
+          v[k] = mu.g[M.src + i];
+          b[k] = mu.buf[M.src + i];
+        } else {
+          v[k] = load_as_f32<T>(s.base, M.index * s.batch_stride + r * s.row_stride + c);
+        }
       }
-      U[M.tall ? c * PF + r : r * PF + c] = v;
-      big = fmaxf(big, fabsf(v));
     }
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) {
+      const int i = i0 + k * TPB, r = (int)((i + 0.5f) * per_row), c = i - r * M.cols;
+      if (i >= count) continue;
+      if constexpr (MUON) {
+        v[k] = muon_in(mu, coef, v[k], b[k]);
+        mu.buf[M.src + i] = b[k];
+      }
+      U[M.tall ? c * PF + r : r * PF + c] = v[k];
+      big = fmaxf(big, fabsf(v[k]));
+    }
+  }
   big = block_reduce(big, true, red);   // (its barriers order U's writes too)
   int e = 0;
   if (big > 0.f && big <= 3.4028235e38f) (void)frexpf(big, &e);
@@ -654,9 +706,11 @@ __global__ __launch_bounds__(TPB) void small_kernel(const NsMatrix* __restrict__
 #pragma unroll
   for (int b = 0; b < NMAX / 32; ++b)
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      v[b][k] = ldexpf(U[row * PF + b * 32 + c8 + k], -e);
-      ss += v[b][k] * v[b][k];
+    for (int k = 0; k < 8; k += 4) {
+      const float4 w = *reinterpret_cast<const float4*>(U + row * PF + b * 32 + c8 + k);
+      v[b][k] = ldexpf(w.x, -e); v[b][k + 1] = ldexpf(w.y, -e); v[b][k + 2] = ldexpf(w.z, -e); v[b][k + 3] = ldexpf(w.w, -e);
+#pragma unroll
+      for (int q = k; q < k + 4; ++q) ss += v[b][q] * v[b][q];
     }
   double sum = ss;
 #pragma unroll
@@ -751,15 +805,22 @@ __global__ __launch_bounds__(TPB) void small_kernel(const NsMatrix* __restrict__
   }
 
   const float g = result_factor(M, res);
-  for (int c = lane; c < M.cols; c += 64)
-#pragma unroll 4
-    for (int r = wave; r < M.rows; r += 4) {
-      const float x = g * U[M.tall ? c * PF + r : r * PF + c];
-      const long long o = M.src + r * M.cols + c;
-      if constexpr (MUON) res.p[o] = res.keep * res.p[o] - x;
-      else if (res.out_dtype == DAS_F32) reinterpret_cast<float*>(res.out)[o] = x;
-      else reinterpret_cast<uint16_t*>(res.out)[o] = res.out_dtype == DAS_BF16 ? f32_to_bf16(x) : __builtin_bit_cast(uint16_t, (_Float16)x);
+  for (int i0 = threadIdx.x; i0 < count; i0 += BATCH * TPB) {
+    float w[BATCH];
+    if constexpr (MUON) {
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k) w[k] = i0 + k * TPB < count ? res.p[M.src + i0 + k * TPB] : 0.f;
     }
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) {
+      const int i = i0 + k * TPB, r = (int)((i + 0.5f) * per_row), c = i - r * M.cols;
+      if (i >= count) continue;
+      const float x = g * U[M.tall ? c * PF + r : r * PF + c];
+      if constexpr (MUON) res.p[M.src + i] = res.keep * w[k] - x;
+      else if (res.out_dtype == DAS_F32) reinterpret_cast<float*>(res.out)[M.src + i] = x;
+      else reinterpret_cast<uint16_t*>(res.out)[M.src + i] = res.out_dtype == DAS_BF16 ? f32_to_bf16(x) : __builtin_bit_cast(uint16_t, (_Float16)x);
+    }
+  }
 }
 
 // ------------------------------------------------------------------ host side
@@ -851,17 +912,23 @@ int iterate(const DasNsPlan* p, const char* tab, Work w, const Result& res, hipS
              *prod = (const int4*)(tab + p->product_at);
   auto sym = [&](auto kind, int products, const SymArgs& a) {
     constexpr SymKind K = decltype(kind)::value;
-    if (p->gram_tile == 128)
-      hipLaunchKernelGGL((sym_kernel<128, SPLIT, K>), dim3(p->n_gram, products), dim3(TPB), 0, s, mats, K == GRAM ? gram : prod, a);
-    else
-      hipLaunchKernelGGL((sym_kernel<64, SPLIT, K>), dim3(p->n_gram, products), dim3(TPB), 0, s, mats, K == GRAM ? gram : prod, a);
+    auto launch = [&](auto kernel, int tile, int kg) {
+      const int lds = kg * 4 * tile * 128;
+      (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+      hipLaunchKernelGGL(kernel, dim3(p->n_gram, products), dim3(kg * TPB), lds, s, mats, K == GRAM ? gram : prod, a);
+    };
+    if (p->gram_tile == 128) launch(sym_kernel<128, SPLIT, 1, K>, 128, 1);
+    else launch(sym_kernel<64, SPLIT, 4, K>, 64, 4);
   };
   auto update = [&](auto last, const _Float16* q, const _Float16* x, _Float16* y) {
     constexpr bool L = decltype(last)::value;
-    if (p->update_tile == 128)
-      hipLaunchKernelGGL((update_kernel<128, SPLIT, L>), dim3(p->n_update), dim3(TPB), 0, s, mats, upd, q, x, y, res);
-    else
-      hipLaunchKernelGGL((update_kernel<64, SPLIT, L>), dim3(p->n_update), dim3(TPB), 0, s, mats, upd, q, x, y, res);
+    auto launch = [&](auto kernel, int tile, int kg) {
+      const int lds = kg * 4 * tile * 128;
+      (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+      hipLaunchKernelGGL(kernel, dim3(p->n_update), dim3(kg * TPB), lds, s, mats, upd, q, x, y, res);
+    };
+    if (p->update_tile == 128) launch(update_kernel<128, SPLIT, 1, L>, 128, 1);
+    else launch(update_kernel<64, SPLIT, 4, L>, 64, 4);
   };
   const std::integral_constant<SymKind, GRAM> gram_k;
   const std::integral_constant<SymKind, POLY> poly_k;
