@@ -75,11 +75,11 @@ class DasNsShape(C.Structure):
 
 
 class DasNsPlan(C.Structure):
-    _fields_ = [('n_groups', i32), ('n_matrices', i32), ('n_chunks', i32), ('n_gram', i32), ('n_update', i32), ('steps', i32),
-                ('gram_tile', i32), ('update_tile', i32), ('n_small', i32), ('small_n', i32),
-                ('x_elems', i64), ('a_elems', i64), ('extent', i64),
-                ('mat_at', i64), ('chunk_at', i64), ('gram_at', i64), ('product_at', i64), ('update_at', i64), ('table_bytes', i64),
-                ('coef', f32 * (3 * DAS_NS_MAX_STEPS)), ('eps', f32)]
+    _fields_ = [(k, i32) for k in ('n_groups', 'n_matrices', 'n_small', 'small_n', 'n_chunks', 'n_gram', 'n_join', 'n_product',
+                                   'n_update', 'steps', 'product_tile', 'update_tile', 'gram_kg', 'reserved')] + \
+               [(k, i64) for k in ('x_elems', 'a_elems', 'n_slots', 'extent', 'mat_at', 'chunk_at', 'gram_at', 'join_at', 'product_at',
+                                   'update_at', 'table_bytes')] + \
+               [('coef', f32 * (3 * DAS_NS_MAX_STEPS)), ('eps', f32)]
 
 
 class DasNsSource(C.Structure):

@@ -33,6 +33,7 @@ typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int TPB = 256;
+constexpr int GRAM_TILE = 128;
 constexpr int N_AREAS = 5;   // m x m work matrices: G, R, Z, two of Q (the f16 form uses G and Z)
 constexpr int CHUNK = 64;   // side of the blocks that ingest_kernel / normalise_kernel work on
 
@@ -44,6 +45,11 @@ struct NsMatrix {           // one matrix, as the kernels see it
   int chunk0, chunks;       // its blocks in the partial-sum table
   float scale, gscale;      // S; what G is kept times
   int tall;                 // rows > cols: X holds the transpose
+};
+struct NsItem {             // a workgroup's share: output tile (ti, tj) of a matrix, inner elements 64 k0 ... 64 (k0 + kn)
+  int matrix, ti, tj, k0, kn;
+  int slot;                 // >= 0: the sums go to this slot of the partial tiles; JOIN items: the first of `slots`
+  int slots, pad;
 };
 struct Partial {            // of one 64 x 64 block: sum of squares of (u 2^-e), and e
   float ss;
@@ -238,8 +244,8 @@ __global__ __launch_bounds__(TPB) void normalise_kernel(const NsMatrix* __restri
 // B), inner elements (l / 16) * 8 ... + 8, and gets column l % 16, rows (l / 16) * 4 ... + 4 of the result.
 //
 // A stage is 128 bytes of every row of both operands: 64 inner elements, or (SPLIT) 32 high parts and their 32 low parts, which lie next to
-// each other in memory so that both forms read whole 128-byte lines. It is copied global -> LDS without passing registers, into
-// one of two buffers while the other is multiplied; the fragments are read before the next copies are issued, so no LDS read waits for them.
+// each other in memory so that both forms read whole 128-byte lines. It is copied global -> LDS without passing registers into one of
+// two buffers.
 //   plain:  acc += A0 B0 + A1 B1   (two halves of the inner axis)
 //   SPLIT:  acc += Ah Bh + Ah Bl + Al Bh   (the low x low part is 2^-22 of the product)
 // KG groups of four waves divide the inner axis between them (KG = 4 where a launch has fewer tiles than CUs and latency is all: every
@@ -249,10 +255,18 @@ __global__ __launch_bounds__(TPB) void normalise_kernel(const NsMatrix* __restri
 // swizzled by row, read with ds_read_tr16_b64 (four inner rows x 16 columns a 16-lane group, one column a lane).
 typedef short i16x4_t __attribute__((ext_vector_type(4)));
 
-__device__ __forceinline__ void copy16(const void* src, char* lds_wave_base) {
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
-                                   (__attribute__((address_space(3))) void*)lds_wave_base, 16, 0, 0);
+// 16 bytes a lane, global -> LDS (lane 0's destination + 16 l). Issued from asm: for the builtin hipcc waits for every copy in flight in front
+// of the next LDS read. The waits are multiply()'s. M0 (the destination) is put back.
+__device__ __forceinline__ void copy16(const void* src, const char* lds_wave_base) {
+  unsigned keep;
+  const unsigned dst = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(const __attribute__((address_space(3))) char*)lds_wave_base);
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
+               : "=&s"(keep)
+               : "v"(src), "s"(dst)
+               : "memory");
 }
+// every copy of this wave has landed and every LDS read of it is done, then the same of every wave
+__device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 template <int T>
 struct RowsOperand {        // T rows of a matrix whose rows run along the inner axis
@@ -332,7 +346,7 @@ using Acc = f32x4_t[T / 32][T / 32];
 template <int T, int KG>
 constexpr int lds_bytes() { return KG * 4 * T * 128; }
 
-// `stages`: of the whole inner axis; the group's first one is group * ceil(stages / KG)
+// `stages`: of the workgroup's part of the inner axis; the group's first one is group * ceil(stages / KG)
 template <int T, bool SPLIT, int KG, typename OB>
 __device__ __forceinline__ void multiply(RowsOperand<T>& a, OB& b, int stages, char* smem, Acc<T>& acc) {
   constexpr int HALF = T * 128, N = T / 32;   // bytes of one operand's stage; fragments a wave has of each operand
@@ -343,27 +357,32 @@ __device__ __forceinline__ void multiply(RowsOperand<T>& a, OB& b, int stages, c
   for (int i = 0; i < N; ++i)
 #pragma unroll
     for (int j = 0; j < N; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  if (KG == 1 || mine > 0) {
-    a.issue(base);
-    b.issue(base + HALF);
-  }
-  __syncthreads();
-  for (int k = 0; k < per; ++k) {
-    if (KG == 1 || k < mine) {
-      const char* cur = base + (k & 1) * 2 * HALF;
-      char* nxt = base + ((k & 1) ^ 1) * 2 * HALF;
-      f16x8_t fa[2][N], fb[2][N];
+  f16x8_t fa[2][2][N], fb[2][2][N];   // [parity of the stage][part][fragment]
+  auto read = [&](int k, auto parity) {
+    constexpr int Z = decltype(parity)::value;
+    const char* cur = base + (k & 1) * 2 * HALF;
 #pragma unroll
-      for (int p = 0; p < 2; ++p)
+    for (int p = 0; p < 2; ++p)
 #pragma unroll
-        for (int t = 0; t < N; ++t) {
-          fa[p][t] = RowsOperand<T>::frag(cur, wr, t, p);
-          fb[p][t] = OB::frag(cur + HALF, wc, t, p);
-        }
-      if (k + 1 < mine) {
-        a.issue(nxt);
-        b.issue(nxt + HALF);
+      for (int t = 0; t < N; ++t) {
+        fa[Z][p][t] = RowsOperand<T>::frag(cur, wr, t, p);
+        fb[Z][p][t] = OB::frag(cur + HALF, wc, t, p);
       }
+  };
+  auto issue = [&](int k) {
+    if (k < mine) {
+      char* dst = base + (k & 1) * 2 * HALF;
+      a.issue(dst);
+      b.issue(dst + HALF);
+    }
+  };
+  // Stage k is multiplied from registers while stage k + 1 is read from LDS and stage k + 2 is copied into the buffer that k has left.
+  auto step = [&](int k, auto parity) {
+    constexpr int Z = decltype(parity)::value;
+    landed();                          // stage k + 1 is in LDS, stage k in registers, in every wave
+    issue(k + 2);
+    if (k + 1 < mine) read(k + 1, std::integral_constant<int, Z ^ 1>{});
+    if (k < mine) {
 #pragma unroll
       for (int q = 0; q < (SPLIT ? 3 : 2); ++q)   // plain: 00 11; split: low parts first (10, 01), then 00
 #pragma unroll
@@ -371,11 +390,19 @@ __device__ __forceinline__ void multiply(RowsOperand<T>& a, OB& b, int stages, c
 #pragma unroll
           for (int j = 0; j < N; ++j) {
             const int pa = SPLIT ? q == 0 : q, pb = SPLIT ? q == 1 : q;
-            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa[pa][i], fb[pb][j], acc[i][j], 0, 0, 0);
+            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa[Z][pa][i], fb[Z][pb][j], acc[i][j], 0, 0, 0);
           }
     }
-    __syncthreads();
+  };
+  issue(0);
+  landed();
+  issue(1);
+  if (mine > 0) read(0, std::integral_constant<int, 0>{});
+  for (int k = 0; k < per; k += 2) {
+    step(k, std::integral_constant<int, 0>{});
+    if (k + 1 < per) step(k + 1, std::integral_constant<int, 1>{});
   }
+  __syncthreads();
   if constexpr (KG > 1) {
     f32x4_t* sums = reinterpret_cast<f32x4_t*>(smem);   // [group - 1][fragment][thread of the group]
     const int t = threadIdx.x & 255;
@@ -446,20 +473,8 @@ struct SymArgs {            // two independent products a launch (blockIdx.y)
 //   GRAM:     G = X X^T times (gscale / S^2)      POLY: Z = a I + b G + c G G      PRODUCT: P Q of symmetric P, Q that commute
 // Columns m ... lda are stored as zeros: the inner axis of the next product.
 template <int T, bool SPLIT, int KG, SymKind KIND>
-__global__ __launch_bounds__(KG * TPB, KG == 1 ? 2 : 4) void sym_kernel(const NsMatrix* __restrict__ mats, const int4* __restrict__ tiles, SymArgs s) {
-  extern __shared__ __align__(16) char smem[];
-  const int4 t = tiles[blockIdx.x];
-  const NsMatrix M = mats[t.x];
-  const int z = blockIdx.y, i0 = t.y * T, j0 = t.z * T;
-  const int ld = KIND == GRAM ? M.ldx : M.lda, pitch = SPLIT ? 2 * ld : ld;
-  const _Float16* P = s.p[z] + (SPLIT ? 2 : 1) * (KIND == GRAM ? M.x : M.a);
-  const _Float16* Q = s.q[z] + (SPLIT ? 2 : 1) * (KIND == GRAM ? M.x : M.a);
-  RowsOperand<T> a, b;
-  const int stages = pitch / 64, first = first_stage<KG>(stages);
-  a.init(P, pitch, i0, M.m, first);
-  b.init(Q, pitch, j0, M.m, first);
-  Acc<T> acc;
-  multiply<T, SPLIT, KG>(a, b, stages, smem, acc);
+__device__ __forceinline__ void sym_store(const NsMatrix& M, const SymArgs& s, int z, int i0, int j0, const Acc<T>& acc, char* smem) {
+  const _Float16* P = s.p[z] + (SPLIT ? 2 : 1) * M.a;
   _Float16* out = s.out[z] + (SPLIT ? 2 : 1) * M.a;
   const float f = KIND == GRAM ? M.gscale / (M.scale * M.scale) : 1.f, cb = s.b / M.gscale, cc = s.c / (M.gscale * M.gscale);
   auto store = [&](int r, int c, float (&v)[8]) {
@@ -482,6 +497,71 @@ __global__ __launch_bounds__(KG * TPB, KG == 1 ? 2 : 4) void sym_kernel(const Ns
   if (i0 != j0) store_tile<T, KG, true>(acc, smem, [&](int r, int c, float (&v)[8]) { store(j0 + r, i0 + c, v); });
 }
 
+template <int T, bool SPLIT, int KG, SymKind KIND>
+__global__ __launch_bounds__(KG * TPB, KG == 1 ? 2 : KG) void sym_kernel(const NsMatrix* __restrict__ mats, const NsItem* __restrict__ items,
+                                                                         SymArgs s, f32x4_t* __restrict__ partial) {
+  extern __shared__ __align__(16) char smem[];
+  const NsItem t = items[blockIdx.x];
+  if (t.matrix < 0) return;   // (filling: an XCD's queue is shorter than the longest)
+  const NsMatrix M = mats[t.matrix];
+  const int z = blockIdx.y, i0 = t.ti * T, j0 = t.tj * T;
+  const int ld = KIND == GRAM ? M.ldx : M.lda, pitch = SPLIT ? 2 * ld : ld;
+  const _Float16* P = s.p[z] + (SPLIT ? 2 : 1) * (KIND == GRAM ? M.x : M.a);
+  const _Float16* Q = s.q[z] + (SPLIT ? 2 : 1) * (KIND == GRAM ? M.x : M.a);
+  RowsOperand<T> a, b;
+  const int stages = (SPLIT ? 2 : 1) * t.kn, first = (SPLIT ? 2 : 1) * t.k0 + first_stage<KG>(stages);
+  a.init(P, pitch, i0, M.m, first);
+  b.init(Q, pitch, j0, M.m, first);
+  Acc<T> acc;
+  multiply<T, SPLIT, KG>(a, b, stages, smem, acc);
+  if (KIND == GRAM && t.slot >= 0) {   // (a part of the inner axis: join_kernel goes on)
+    if (KG == 1 || threadIdx.x < TPB) {
+#pragma unroll
+      for (int i = 0; i < T / 32; ++i)
+#pragma unroll
+        for (int j = 0; j < T / 32; ++j) partial[((long long)t.slot * (T / 32) * (T / 32) + i * (T / 32) + j) * TPB + threadIdx.x] = acc[i][j];
+    }
+    return;
+  }
+  sym_store<T, SPLIT, KG, KIND>(M, s, z, i0, j0, acc, smem);
+}
+
+// The parts of a tile whose inner axis was split, added in order, and stored as sym_store does; 16 workgroups a tile, four rows of one
+// column a thread (one workgroup a tile: 12 us, most of them waiting for one load after the other).
+template <bool SPLIT>
+__global__ __launch_bounds__(TPB) void join_kernel(const NsMatrix* __restrict__ mats, const NsItem* __restrict__ items, _Float16* __restrict__ G,
+                                                   const f32x4_t* __restrict__ partial) {
+  constexpr int N = GRAM_TILE / 32, W = SPLIT ? 2 : 1;
+  const NsItem t = items[blockIdx.x / (N * N)];
+  const NsMatrix M = mats[t.matrix];
+  const int frag = blockIdx.x % (N * N), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
+  for (int k0 = 0; k0 < t.slots; k0 += 4) {
+    f32x4_t v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      v[k] = k0 + k < t.slots ? partial[((long long)(t.slot + k0 + k) * N * N + frag) * TPB + threadIdx.x] : f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) sum += v[k];
+  }
+  const float f = M.gscale / (M.scale * M.scale);
+  const int r = t.ti * GRAM_TILE + (wave >> 1) * (GRAM_TILE / 2) + (frag / N) * 16 + (lane >> 4) * 4;   // four rows of one column
+  const int c = t.tj * GRAM_TILE + (wave & 1) * (GRAM_TILE / 2) + (frag % N) * 16 + (lane & 15);
+  _Float16* out = G + W * M.a;
+  float v[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = r + e < M.m && c < M.m ? sum[e] * f : 0.f;
+  if (c < M.m && r < M.lda) put<SPLIT>(out, M.lda, c, r, v);
+  if (t.ti == t.tj) return;   // (a diagonal tile holds both halves)
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (r + e < M.m && c < M.lda) {
+      _Float16* p = out + at<SPLIT>(M.lda, r + e, c);
+      p[0] = (_Float16)v[e];
+      if constexpr (SPLIT) p[32] = (_Float16)(v[e] - (float)p[0]);
+    }
+}
+
 struct Result {             // where the last product goes
   void* out;                // das_orthogonalize
   int out_dtype;
@@ -500,17 +580,18 @@ __device__ __forceinline__ float result_factor(const NsMatrix& M, const Result& 
 
 // X' = Q X: Q's rows by X's columns. LAST: the result leaves the work area (and its scale S), transposed back where needed.
 template <int T, bool SPLIT, int KG, bool LAST>
-__global__ __launch_bounds__(KG * TPB, KG == 1 ? 2 : 4) void update_kernel(const NsMatrix* __restrict__ mats, const int4* __restrict__ tiles,
+__global__ __launch_bounds__(KG * TPB, KG == 1 ? 2 : KG) void update_kernel(const NsMatrix* __restrict__ mats, const NsItem* __restrict__ items,
                                                         const _Float16* __restrict__ Q, const _Float16* __restrict__ X,
                                                         _Float16* __restrict__ Y, Result res) {
   extern __shared__ __align__(16) char smem[];
-  const int4 t = tiles[blockIdx.x];
-  const NsMatrix M = mats[t.x];
-  const int i0 = t.y * T, j0 = t.z * T;
+  const NsItem t = items[blockIdx.x];
+  if (t.matrix < 0) return;
+  const NsMatrix M = mats[t.matrix];
+  const int i0 = t.ti * T, j0 = t.tj * T;
   constexpr int W = SPLIT ? 2 : 1;
   RowsOperand<T> a;
   ColsOperand<T, SPLIT> b;
-  const int stages = W * M.lda / 64, first = first_stage<KG>(stages);
+  const int stages = W * t.kn, first = first_stage<KG>(stages);
   a.init(Q + W * M.a, W * M.lda, i0, M.m, first);
   b.init(X + W * M.x, W * M.ldx, j0, M.m, first);
   Acc<T> acc;
@@ -829,6 +910,7 @@ inline long long up256(long long v) { return (v + 255) / 256 * 256; }
 struct Work {
   _Float16 *x[2], *a[N_AREAS];
   Partial* part;
+  f32x4_t* slots;            // partial tiles
   long long bytes;
 };
 Work carve(const DasNsPlan* p, bool split, void* ws) {
@@ -840,12 +922,13 @@ Work carve(const DasNsPlan* p, bool split, void* ws) {
   for (int i = 0; i < 2; ++i) w.x[i] = (_Float16*)take(xb);
   for (int i = 0; i < areas; ++i) w.a[i] = (_Float16*)take(ab);
   w.part = (Partial*)take(up256((long long)sizeof(Partial) * p->n_chunks));
+  w.slots = (f32x4_t*)take(4LL * GRAM_TILE * GRAM_TILE * p->n_slots);
   return w;
 }
 
 bool plan_valid(const DasNsPlan* p, const void* tables, const void* ws) {
   return p && tables && ws && p->n_matrices > 0 && p->n_small >= 0 && p->n_small <= p->n_matrices && p->steps > 0 &&
-         p->steps <= DAS_NS_MAX_STEPS && (p->gram_tile == 64 || p->gram_tile == 128) && (p->update_tile == 64 || p->update_tile == 128) &&
+         p->steps <= DAS_NS_MAX_STEPS && (p->product_tile == 64 || p->product_tile == 128) && (p->update_tile == 64 || p->update_tile == 128) &&
          !(((uintptr_t)tables | (uintptr_t)ws) & 15);
 }
 
@@ -908,17 +991,25 @@ int launch_small(const DasNsPlan* p, const char* tab, const Sources& src, const 
 template <bool SPLIT>
 int iterate(const DasNsPlan* p, const char* tab, Work w, const Result& res, hipStream_t s) {
   const NsMatrix* mats = (const NsMatrix*)(tab + p->mat_at);
-  const int4 *chunks = (const int4*)(tab + p->chunk_at), *gram = (const int4*)(tab + p->gram_at), *upd = (const int4*)(tab + p->update_at),
-             *prod = (const int4*)(tab + p->product_at);
+  const int4* chunks = (const int4*)(tab + p->chunk_at);
+  const NsItem *gram = (const NsItem*)(tab + p->gram_at), *prod = (const NsItem*)(tab + p->product_at),
+               *upd = (const NsItem*)(tab + p->update_at), *join = (const NsItem*)(tab + p->join_at);
+  auto launch_sym = [&](auto kernel, int tile, int kg, const NsItem* items, int n, int products, const SymArgs& a) {
+    const int lds = kg * 4 * tile * 128;
+    (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    hipLaunchKernelGGL(kernel, dim3(n, products), dim3(kg * TPB), lds, s, mats, items, a, w.slots);
+  };
+  auto gram_of = [&](const _Float16* x, _Float16* g) {
+    const SymArgs a = {{x}, {x}, {g}, 0.f, 0.f, 0.f};
+    if (p->gram_kg == 2) launch_sym(sym_kernel<GRAM_TILE, SPLIT, 2, GRAM>, GRAM_TILE, 2, gram, p->n_gram, 1, a);
+    else launch_sym(sym_kernel<GRAM_TILE, SPLIT, 1, GRAM>, GRAM_TILE, 1, gram, p->n_gram, 1, a);
+    if (p->n_join)
+      hipLaunchKernelGGL((join_kernel<SPLIT>), dim3(p->n_join * (GRAM_TILE / 32) * (GRAM_TILE / 32)), dim3(TPB), 0, s, mats, join, g, w.slots);
+  };
   auto sym = [&](auto kind, int products, const SymArgs& a) {
     constexpr SymKind K = decltype(kind)::value;
-    auto launch = [&](auto kernel, int tile, int kg) {
-      const int lds = kg * 4 * tile * 128;
-      (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-      hipLaunchKernelGGL(kernel, dim3(p->n_gram, products), dim3(kg * TPB), lds, s, mats, K == GRAM ? gram : prod, a);
-    };
-    if (p->gram_tile == 128) launch(sym_kernel<128, SPLIT, 1, K>, 128, 1);
-    else launch(sym_kernel<64, SPLIT, 4, K>, 64, 4);
+    if (p->product_tile == 128) launch_sym(sym_kernel<128, SPLIT, 1, K>, 128, 1, prod, p->n_product, products, a);
+    else launch_sym(sym_kernel<64, SPLIT, 4, K>, 64, 4, prod, p->n_product, products, a);
   };
   auto update = [&](auto last, const _Float16* q, const _Float16* x, _Float16* y) {
     constexpr bool L = decltype(last)::value;
@@ -930,7 +1021,6 @@ int iterate(const DasNsPlan* p, const char* tab, Work w, const Result& res, hipS
     if (p->update_tile == 128) launch(update_kernel<128, SPLIT, 1, L>, 128, 1);
     else launch(update_kernel<64, SPLIT, 4, L>, 64, 4);
   };
-  const std::integral_constant<SymKind, GRAM> gram_k;
   const std::integral_constant<SymKind, POLY> poly_k;
   const std::integral_constant<SymKind, PRODUCT> product_k;
   hipLaunchKernelGGL(normalise_kernel<SPLIT>, dim3(p->n_chunks), dim3(TPB), 0, s, mats, chunks, p->eps, w.x[0], w.part);
@@ -941,7 +1031,7 @@ int iterate(const DasNsPlan* p, const char* tab, Work w, const Result& res, hipS
   for (int k = 0; k < p->steps;) {
     // steps k ... end - 1 are one phase
     const int end = SPLIT ? phase_end(bound, p->steps, k) : k + 1;
-    sym(gram_k, 1, SymArgs{{X}, {X}, {G}, 0.f, 0.f, 0.f});
+    gram_of(X, G);
     _Float16 *q = nullptr, *spare = w.a[SPLIT ? 3 : 1], *other = SPLIT ? w.a[4] : nullptr;   // (q: the phase's product so far)
     for (int j = k; j < end; ++j) {
       const float* c = p->coef + 3 * j;
@@ -968,6 +1058,178 @@ int iterate(const DasNsPlan* p, const char* tab, Work w, const Result& res, hipS
   return DAS_OK;
 }
 
+
+// Items of one launch. The hardware deals workgroups to the 8 XCDs in turn, and every XCD has its own 4 MiB L2: tiles that share rows
+// or columns are kept together in a group, groups go to the XCD with the least work so far, longest inner axis first, and the queues
+// are interleaved (item i runs on XCD i % 8). (Tiles in table order: each XCD read nearly every panel itself, 512 x 4608: 47 us
+// for X X^T at the Infinity Cache's rate.)
+struct Launch {
+  struct Group {
+    std::vector<NsItem> items;
+    long long cost = 0;
+    int longest = 0;
+  };
+  std::vector<Group> groups;
+  std::vector<NsItem> order;
+
+  void add(bool fresh, const NsItem& t) {
+    if (fresh || groups.empty()) groups.emplace_back();
+    Group& g = groups.back();
+    g.items.push_back(t);
+    g.cost += t.kn + 2;        // (a tile's start and end cost about two steps of its inner axis)
+    g.longest = std::max(g.longest, t.kn);
+  }
+  void place() {
+    std::stable_sort(groups.begin(), groups.end(), [](const Group& u, const Group& v) {
+      return u.longest != v.longest ? u.longest > v.longest : u.cost > v.cost;
+    });
+    std::vector<NsItem> queue[8];
+    long long load[8] = {};
+    for (const Group& g : groups) {
+      const int x = (int)(std::min_element(load, load + 8) - load);
+      queue[x].insert(queue[x].end(), g.items.begin(), g.items.end());
+      load[x] += g.cost;
+    }
+    size_t depth = 0;
+    for (const auto& q : queue) depth = std::max(depth, q.size());
+    NsItem none = {};
+    none.matrix = -1;
+    for (size_t i = 0; i < depth; ++i)
+      for (const auto& q : queue) order.push_back(i < q.size() ? q[i] : none);
+    while (!order.empty() && order.back().matrix < 0) order.pop_back();
+  }
+};
+
+struct Tables {
+  std::vector<NsMatrix> mats;
+  std::vector<int4> chunks;
+  Launch gram, product, update;
+  std::vector<NsItem> join;
+};
+
+inline int over(long long v, int t) { return (int)((v + t - 1) / t); }
+
+// tiles on and below the diagonal of an m x m matrix, in blocks of `side` x `side` tiles: f(first of a block, row, column)
+template <typename F>
+void lower_blocks(int tiles, int side, F f) {
+  for (int bi = 0; bi < tiles; bi += side)
+    for (int bj = 0; bj <= bi; bj += side) {
+      bool fresh = true;
+      for (int i = bi; i < std::min(tiles, bi + side); ++i)
+        for (int j = bj; j <= std::min(i, bj + side - 1); ++j, fresh = false) f(fresh, i, j);
+    }
+}
+
+// The whole schedule of a set; false for shapes that it does not take.
+bool build(const DasNsShape* shapes, int n, double top, DasNsPlan* plan, Tables& t) {
+  std::vector<std::pair<long long, long long>> spans;
+  long long n_mat = 0, n_chunks = 0;
+  auto is_small = [&](const DasNsShape& s) { return std::min(s.rows, s.cols) <= SMALL_M && std::max(s.rows, s.cols) <= SMALL_N; };
+  for (int g = 0; g < n; ++g) {
+    const DasNsShape& s = shapes[g];
+    if (s.off < 0 || s.count < 1 || s.rows < 1 || s.cols < 1 || s.rows > (1 << 20) || s.cols > (1 << 20)) return false;
+    const long long m = std::min(s.rows, s.cols), nn = std::max(s.rows, s.cols);
+    n_mat += s.count;
+    if (is_small(s)) {
+      plan->n_small += s.count;
+      plan->small_n = std::max(plan->small_n, (int)nn);
+    } else {
+      n_chunks += (long long)s.count * over(m, 64) * over(nn, 128) * 2;
+    }
+    if (n_mat > (1 << 22) || n_chunks > (1 << 24) || m > (1 << 15)) return false;
+    spans.push_back({s.off, s.off + (long long)s.count * s.rows * s.cols});
+  }
+  std::sort(spans.begin(), spans.end());
+  for (size_t i = 1; i < spans.size(); ++i)
+    if (spans[i].first < spans[i - 1].second) return false;   // two workgroups would write the same elements
+  plan->extent = spans.back().second;
+
+  t.mats.resize(n_mat);
+  int small = 0, big = plan->n_small;   // (the small matrices come first in the table)
+  long long lower128 = 0, all128 = 0, gram_steps = 0;
+  for (int g = 0; g < n; ++g) {
+    const DasNsShape& s = shapes[g];
+    for (int i = 0; i < s.count; ++i) {
+      const int q = is_small(s) ? small++ : big++;
+      NsMatrix& M = t.mats[q];
+      M = NsMatrix{};
+      M.rows = s.rows; M.cols = s.cols; M.m = std::min(s.rows, s.cols); M.n = std::max(s.rows, s.cols);
+      M.tall = s.rows > s.cols;
+      M.ldx = over(M.n, 128) * 128; M.lda = over(M.m, 64) * 64;
+      M.src = s.off + (long long)i * s.rows * s.cols;
+      M.group = g; M.index = i;
+      M.scale = (float)std::ldexp(1.0, (int)std::lround(0.5 * std::log2((double)M.n)));
+      // about m, and top^2 gscale within f16
+      M.gscale = (float)std::ldexp(1.0, std::min((int)std::lround(std::log2((double)M.m)), (int)std::floor(std::log2(32768.0 / (top * top)))));
+      if (is_small(s)) continue;
+      M.x = plan->x_elems; M.a = plan->a_elems; M.chunk0 = (int)t.chunks.size();
+      plan->x_elems += (long long)M.m * M.ldx;
+      plan->a_elems += (long long)M.m * M.lda;
+      int k = 0;
+      for (int r = 0; r < (M.tall ? M.ldx : M.lda) / CHUNK; ++r)
+        for (int c = 0; c < (M.tall ? M.lda : M.ldx) / CHUNK; ++c) t.chunks.push_back(make_int4(q, r, c, k++));
+      M.chunks = k;
+      const long long tm = over(M.m, 128);
+      lower128 += tm * (tm + 1) / 2;
+      all128 += tm * (M.ldx / 128);
+      gram_steps += tm * (tm + 1) / 2 * (M.ldx / 64);
+    }
+  }
+  // Products and updates: 128 x 128 tiles where they fill the 256 CUs, else 64 x 64 ones whose inner axis four wave groups share.
+  plan->product_tile = lower128 >= 256 ? 128 : 64;
+  plan->update_tile = all128 >= 256 ? 128 : 64;
+  // X X^T: 128 x 128 tiles; where there are fewer than two for each CU, two wave groups share a tile's inner axis, and it is
+  // split further until about 256 workgroups have a share, of at least 256 elements. Long ones are split in larger sets too: the
+  // last tile to finish should not have more than its 512th of the work.
+  plan->gram_kg = lower128 >= 384 ? 1 : 2;
+  const long long share = std::max<long long>(4, (gram_steps + 255) / (plan->gram_kg == 1 ? 512 : 256));
+  // blocks of up to 8 x 8 tiles, smaller where one would be more than a 16th of the launch (half of an XCD's part)
+  auto side_for = [](long long launch, int steps) {
+    int side = 8;
+    while (side > 1 && (long long)side * side * (steps + 2) * 16 > launch) side /= 2;
+    return side;
+  };
+  long long product_cost = 0, update_cost = 0, gram_cost = 0;
+  for (int q = plan->n_small; q < (int)n_mat; ++q) {
+    const NsMatrix& M = t.mats[q];
+    const long long p = over(M.m, plan->product_tile), r = over(M.m, plan->update_tile), w = over(M.m, GRAM_TILE);
+    product_cost += p * (p + 1) / 2 * (M.lda / 64 + 2);
+    update_cost += r * (M.ldx / plan->update_tile) * (M.lda / 64 + 2);
+    gram_cost += w * (w + 1) / 2 * (M.ldx / 64 + 2);
+  }
+  for (int q = plan->n_small; q < (int)n_mat; ++q) {
+    const NsMatrix& M = t.mats[q];
+    const int steps = M.ldx / 64, parts = (int)std::min<long long>(16, std::max<long long>(1, (steps + share / 2) / share));
+    const int tm = over(M.m, GRAM_TILE);
+    if (parts > 1) {   // (one part of the inner axis = one group: it is read by one XCD alone)
+      for (int k = 0; k < parts; ++k) {
+        int tile = 0;
+        const int k0 = (int)((long long)steps * k / parts), k1 = (int)((long long)steps * (k + 1) / parts);
+        lower_blocks(tm, 1 << 16, [&](bool fresh, int i, int j) {
+          t.gram.add(fresh, NsItem{q, i, j, k0, k1 - k0, (int)plan->n_slots + tile++ * parts + k, 1, 0});
+        });
+      }
+      lower_blocks(tm, 1 << 16, [&](bool, int i, int j) {
+        t.join.push_back(NsItem{q, i, j, 0, steps, (int)plan->n_slots, parts, 0});
+        plan->n_slots += parts;
+      });
+    } else {
+      lower_blocks(tm, side_for(gram_cost, steps), [&](bool fresh, int i, int j) { t.gram.add(fresh, NsItem{q, i, j, 0, steps, -1, 1, 0}); });
+    }
+    lower_blocks(over(M.m, plan->product_tile), side_for(product_cost, M.lda / 64),
+                 [&](bool fresh, int i, int j) { t.product.add(fresh, NsItem{q, i, j, 0, M.lda / 64, -1, 1, 0}); });
+    const int rows = over(M.m, plan->update_tile), cols = M.ldx / plan->update_tile, side = side_for(update_cost, M.lda / 64);
+    for (int bj = 0; bj < cols; bj += side)
+      for (int bi = 0; bi < rows; bi += side)
+        for (int j = bj; j < std::min(cols, bj + side); ++j)
+          for (int i = bi; i < std::min(rows, bi + side); ++i) t.update.add(i == bi && j == bj, NsItem{q, i, j, 0, M.lda / 64, -1, 1, 0});
+  }
+  t.gram.place();
+  t.product.place();
+  t.update.place();
+  return t.gram.order.size() < (1u << 30) && t.update.order.size() < (1u << 30);
+}
+
 }  // namespace
 
 extern "C" int das_ns_plan(const DasNsShape* shapes, int n, int steps, const float* coef, float eps, DasNsPlan* plan, void* tables,
@@ -976,105 +1238,43 @@ extern "C" int das_ns_plan(const DasNsShape* shapes, int n, int steps, const flo
   if (!shapes || n < 1 || !coef || !plan || steps < 1 || steps > DAS_NS_MAX_STEPS || !(eps >= 0.f) || !std::isfinite(eps) ||
       !polynomial_bounds(coef, steps, bound))
     return DAS_ERR_ARG;
-  memset(plan, 0, sizeof(*plan));
-  auto is_small = [&](int g) {
-    return std::min(shapes[g].rows, shapes[g].cols) <= SMALL_M && std::max(shapes[g].rows, shapes[g].cols) <= SMALL_N;
-  };
-  auto tiles = [&](int t, bool sym) {
-    long long c = 0;
-    for (int g = 0; g < n; ++g) {
-      if (is_small(g)) continue;
-      const long long m = std::min(shapes[g].rows, shapes[g].cols), nn = std::max(shapes[g].rows, shapes[g].cols);
-      const long long tm = (m + t - 1) / t, tn = (nn + 127) / 128 * (128 / t);
-      c += shapes[g].count * (sym ? tm * (tm + 1) / 2 : tm * tn);
-    }
-    return c;
-  };
-  long long n_mat = 0, n_chunks = 0;
   double top = 1.0;
   for (int k = 0; k < steps; ++k) top = std::max(top, bound[k].top);
-  std::vector<std::pair<long long, long long>> spans;
-  for (int g = 0; g < n; ++g) {
-    const DasNsShape& s = shapes[g];
-    if (s.off < 0 || s.count < 1 || s.rows < 1 || s.cols < 1 || s.rows > (1 << 20) || s.cols > (1 << 20)) return DAS_ERR_ARG;
-    const long long m = std::min(s.rows, s.cols), nn = std::max(s.rows, s.cols);
-    const long long ldx = (nn + 127) / 128 * 128, lda = (m + 63) / 64 * 64;
-    n_mat += s.count;
-    if (is_small(g)) {
-      plan->n_small += s.count;
-      plan->small_n = std::max(plan->small_n, (int)nn);
-    } else {
-      n_chunks += s.count * (lda / 64) * (ldx / 64);
-      plan->x_elems += s.count * m * ldx;
-      plan->a_elems += s.count * m * lda;
+  try {
+    DasNsPlan p;
+    memset(&p, 0, sizeof(p));
+    Tables t;
+    if (!build(shapes, n, top, &p, t)) return DAS_ERR_ARG;
+    p.n_groups = n; p.n_matrices = (int)t.mats.size(); p.n_chunks = (int)t.chunks.size();
+    p.n_gram = (int)t.gram.order.size(); p.n_product = (int)t.product.order.size(); p.n_update = (int)t.update.order.size();
+    p.n_join = (int)t.join.size();
+    p.steps = steps; p.eps = eps;
+    memcpy(p.coef, coef, sizeof(float) * 3 * steps);
+    char* out = nullptr;
+    auto put_table = [&](const auto& v, long long& at) {
+      at = p.table_bytes;
+      const long long bytes = (long long)(v.size() * sizeof(v[0]));
+      if (out && bytes) memcpy(out + at, v.data(), bytes);
+      p.table_bytes += up256(bytes);
+    };
+    for (int pass = 0; pass < (tables ? 2 : 1); ++pass) {
+      if (pass) {
+        if (table_bytes < p.table_bytes) return DAS_ERR_ARG;
+        out = (char*)tables;
+        memset(tables, 0, p.table_bytes);
+      }
+      p.table_bytes = 0;
+      put_table(t.mats, p.mat_at);
+      put_table(t.chunks, p.chunk_at);
+      put_table(t.gram.order, p.gram_at);
+      put_table(t.join, p.join_at);
+      put_table(t.product.order, p.product_at);
+      put_table(t.update.order, p.update_at);
     }
-    if (n_mat > (1 << 24) || n_chunks > (1 << 26) || m > (1 << 15)) return DAS_ERR_ARG;
-    spans.push_back({s.off, s.off + (long long)s.count * s.rows * s.cols});
+    *plan = p;
+  } catch (...) {   // (no memory for the tables)
+    return DAS_ERR_ARG;
   }
-  std::sort(spans.begin(), spans.end());
-  for (size_t i = 1; i < spans.size(); ++i)
-    if (spans[i].first < spans[i - 1].second) return DAS_ERR_ARG;   // two workgroups would write the same elements
-  plan->gram_tile = tiles(128, true) >= 256 ? 128 : 64;
-  plan->update_tile = tiles(128, false) >= 256 ? 128 : 64;
-  const long long n_gram = tiles(plan->gram_tile, true), n_upd = tiles(plan->update_tile, false);
-  if (n_gram > (1 << 26) || n_upd > (1 << 26)) return DAS_ERR_ARG;
-  plan->n_groups = n; plan->n_matrices = (int)n_mat; plan->n_chunks = (int)n_chunks; plan->n_gram = (int)n_gram;
-  plan->n_update = (int)n_upd; plan->steps = steps; plan->eps = eps; plan->extent = spans.back().second;
-  memcpy(plan->coef, coef, sizeof(float) * 3 * steps);
-  plan->mat_at = 0;
-  plan->chunk_at = up256(n_mat * (long long)sizeof(NsMatrix));
-  plan->gram_at = plan->chunk_at + up256(16 * n_chunks);
-  plan->product_at = plan->gram_at + up256(16 * n_gram);
-  plan->update_at = plan->product_at + up256(16 * n_gram);
-  plan->table_bytes = plan->update_at + up256(16 * n_upd);
-  if (!tables) return DAS_OK;
-  if (table_bytes < plan->table_bytes) return DAS_ERR_ARG;
-  memset(tables, 0, plan->table_bytes);
-  char* tab = (char*)tables;
-  NsMatrix* mats = (NsMatrix*)(tab + plan->mat_at);
-  int4 *chunk = (int4*)(tab + plan->chunk_at), *gram = (int4*)(tab + plan->gram_at), *upd = (int4*)(tab + plan->update_at),
-       *prod = (int4*)(tab + plan->product_at);
-  long long x = 0, a = 0;
-  int small = 0, big = plan->n_small, c = 0;   // (the small matrices come first in the table)
-  for (int g = 0; g < n; ++g) {
-    const DasNsShape& s = shapes[g];
-    for (int i = 0; i < s.count; ++i) {
-      const int q = is_small(g) ? small++ : big++;
-      NsMatrix& M = mats[q];
-      M.rows = s.rows; M.cols = s.cols; M.m = std::min(s.rows, s.cols); M.n = std::max(s.rows, s.cols);
-      M.tall = s.rows > s.cols;
-      M.ldx = (M.n + 127) / 128 * 128; M.lda = (M.m + 63) / 64 * 64;
-      M.src = s.off + (long long)i * s.rows * s.cols;
-      M.group = g; M.index = i;
-      M.scale = (float)std::ldexp(1.0, (int)std::lround(0.5 * std::log2((double)M.n)));
-      // about m, and top^2 gscale within f16
-      M.gscale = (float)std::ldexp(1.0, std::min((int)std::lround(std::log2((double)M.m)), (int)std::floor(std::log2(32768.0 / (top * top)))));
-      if (is_small(g)) continue;
-      M.x = x; M.a = a; M.chunk0 = c;
-      x += (long long)M.m * M.ldx; a += (long long)M.m * M.lda;
-      int k = 0;
-      for (int r = 0; r < (M.tall ? M.ldx : M.lda) / CHUNK; ++r)
-        for (int cc = 0; cc < (M.tall ? M.lda : M.ldx) / CHUNK; ++cc) chunk[c++] = make_int4(q, r, cc, k++);
-      M.chunks = k;
-    }
-  }
-  // longest inner axis first: the last workgroups to start are the shortest ones
-  std::vector<int> by_n, by_m;
-  for (int i = plan->n_small; i < (int)n_mat; ++i) by_n.push_back(i);
-  by_m = by_n;
-  std::stable_sort(by_n.begin(), by_n.end(), [&](int u, int v) { return mats[u].n > mats[v].n; });
-  std::stable_sort(by_m.begin(), by_m.end(), [&](int u, int v) { return mats[u].m > mats[v].m; });
-  auto across = [](int v, int t) { return (v + t - 1) / t; };
-  auto lower = [&](const std::vector<int>& order, int4* t) {
-    for (int i : order)
-      for (int r = 0; r < across(mats[i].m, plan->gram_tile); ++r)
-        for (int j = 0; j <= r; ++j) *t++ = make_int4(i, r, j, 0);
-  };
-  lower(by_n, gram);
-  lower(by_m, prod);
-  for (int i : by_m)
-    for (int j = 0; j < mats[i].ldx / plan->update_tile; ++j)
-      for (int r = 0; r < across(mats[i].m, plan->update_tile); ++r) *upd++ = make_int4(i, r, j, 0);
   return DAS_OK;
 }
 

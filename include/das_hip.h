@@ -626,9 +626,10 @@ typedef struct {
   int reserved;
 } DasNsShape;
 typedef struct {
-  int n_groups, n_matrices, n_chunks, n_gram, n_update, steps, gram_tile, update_tile, n_small, small_n;
-  long long x_elems, a_elems, extent;            /* work areas (f16 elements); one past the last element of the flat buffers used */
-  long long mat_at, chunk_at, gram_at, product_at, update_at, table_bytes;   /* byte offsets of the tables */
+  int n_groups, n_matrices, n_small, small_n, n_chunks, n_gram, n_join, n_product, n_update, steps;
+  int product_tile, update_tile, gram_kg, reserved;
+  long long x_elems, a_elems, n_slots, extent;            /* work areas (f16 elements); one past the last element of the flat buffers used */
+  long long mat_at, chunk_at, gram_at, join_at, product_at, update_at, table_bytes;   /* byte offsets of the tables */
   float coef[3 * DAS_NS_MAX_STEPS];              /* a, b, c of each step */
   float eps;
 } DasNsPlan;
