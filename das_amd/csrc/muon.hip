@@ -21,6 +21,8 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <functional>
+#include <queue>
 #include <type_traits>
 #include <vector>
 
@@ -33,7 +35,7 @@ typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int TPB = 256;
-constexpr int GRAM_TILE = 128;
+constexpr int JOIN_TILE = 128;   // tiles whose inner axis may be split over workgroups
 constexpr int N_AREAS = 5;   // m x m work matrices: G, R, Z, two of Q (the f16 form uses G and Z)
 constexpr int CHUNK = 64;   // side of the blocks that ingest_kernel / normalise_kernel work on
 
@@ -138,8 +140,8 @@ __device__ __forceinline__ float load_as_f32(const void* base, long long i) {
 // squares, store u 2^-e in X's layout (transposed through LDS for tall matrices), zeros in the padding. The exponent keeps gradients
 // of any magnitude inside f16's range until the norm is known; normalise_kernel rounds a second time.
 template <typename T, bool MUON, bool SPLIT>
-__global__ __launch_bounds__(TPB) void ingest_kernel(const NsMatrix* __restrict__ mats, const int4* __restrict__ chunks,
-                                                     Sources src, MuonIn mu, _Float16* __restrict__ X, Partial* __restrict__ part) {
+__global__ __launch_bounds__(TPB) void ingest_kernel(const NsMatrix* __restrict__ mats, const int4* __restrict__ chunks, Sources src,
+                                                     MuonIn mu, _Float16* __restrict__ X, Partial* __restrict__ part) {
   __shared__ float tile[CHUNK][CHUNK + 1];
   __shared__ float red[4];
   const int4 ch = chunks[blockIdx.x];
@@ -147,29 +149,78 @@ __global__ __launch_bounds__(TPB) void ingest_kernel(const NsMatrix* __restrict_
   if (!MUON && (unsigned)(M.group - src.first) >= (unsigned)src.count) return;   // (whole workgroups)
   const int r0 = ch.y * CHUNK, c0 = ch.z * CHUNK;
   const int c4 = (threadIdx.x & 15) * 4, rr = threadIdx.x >> 4;
-  float coef = 1.f;
-  if constexpr (MUON) coef = grad_factor(mu);
-  float u[4][4], big = 0.f;
+  float u[4][4] = {}, big = 0.f;
+  // Four values a load where the matrix allows it: every row of four starts on 16 bytes (8 for two-byte types) of the source
+  const int c = c0 + c4, left = M.cols - c;
+  if constexpr (MUON) {
+    const float coef = grad_factor(mu);
+    const float* g = mu.g + M.src + c;
+    float* m = mu.buf + M.src + c;
+    float b[4][4];
+    if (!((M.cols | M.src) & 3) && !(((uintptr_t)mu.g | (uintptr_t)mu.buf) & 15)) {
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const int r = r0 + rr + k * 16;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int c = c0 + c4 + j;
-      float v = 0.f;
-      if (r < M.rows && c < M.cols) {
-        if constexpr (MUON) {
-          const long long i = M.src + (long long)r * M.cols + c;
-          v = muon_in(mu, coef, mu.g[i], mu.buf[i]);
-        } else {
-          const DasNsSource& s = src.s[M.group - src.first];
-          v = load_as_f32<T>(s.base, M.index * s.batch_stride + r * s.row_stride + c);
+      for (int k = 0; k < 4; ++k) {
+        const long long o = (long long)(r0 + rr + k * 16) * M.cols;
+        if (r0 + rr + k * 16 < M.rows && left > 0) {
+          *reinterpret_cast<float4*>(u[k]) = *reinterpret_cast<const float4*>(g + o);
+          *reinterpret_cast<float4*>(b[k]) = *reinterpret_cast<const float4*>(m + o);
         }
       }
-      u[k][j] = v;
-      big = fmaxf(big, fabsf(v));   // (NaN is passed over here and stays NaN in u)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const long long o = (long long)(r0 + rr + k * 16) * M.cols;
+        if (r0 + rr + k * 16 < M.rows && left > 0) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) u[k][j] = muon_in(mu, coef, u[k][j], b[k][j]);
+          *reinterpret_cast<float4*>(m + o) = *reinterpret_cast<const float4*>(b[k]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const long long o = (long long)(r0 + rr + k * 16) * M.cols;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (r0 + rr + k * 16 < M.rows && j < left) {
+            u[k][j] = g[o + j];
+            b[k][j] = m[o + j];
+          }
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const long long o = (long long)(r0 + rr + k * 16) * M.cols;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (r0 + rr + k * 16 < M.rows && j < left) {
+            u[k][j] = muon_in(mu, coef, u[k][j], b[k][j]);
+            m[o + j] = b[k][j];
+          }
+      }
+    }
+  } else {
+    const DasNsSource& s = src.s[M.group - src.first];
+    const T* from = reinterpret_cast<const T*>(s.base) + M.index * s.batch_stride + c;
+    const bool vec = !((s.row_stride | s.batch_stride) & 3) && !((uintptr_t)s.base & (4 * sizeof(T) - 1));
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const long long o = (r0 + rr + k * 16) * s.row_stride;
+      if (r0 + rr + k * 16 >= M.rows) continue;
+      if (vec && left >= 4) {
+        struct alignas(4 * sizeof(T)) Four { T v[4]; };
+        const Four f = *reinterpret_cast<const Four*>(from + o);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) u[k][j] = load_as_f32<T>(f.v, j);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (j < left) u[k][j] = load_as_f32<T>(from, o + j);
+      }
     }
   }
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) big = fmaxf(big, fabsf(u[k][j]));   // (NaN is passed over here and stays NaN in u)
   big = block_reduce(big, true, red);
   int e = 0;
   if (big > 0.f && big <= 3.4028235e38f) {
@@ -467,6 +518,7 @@ struct SymArgs {            // two independent products a launch (blockIdx.y)
   const _Float16 *p[2], *q[2];
   _Float16* out[2];
   float a, b, c;
+  long long slots;          // partial tiles of one product
 };
 
 // Symmetric m x m results, tiles on and below the diagonal, each stored as it is and transposed.
@@ -514,12 +566,12 @@ __global__ __launch_bounds__(KG * TPB, KG == 1 ? 2 : KG) void sym_kernel(const N
   b.init(Q, pitch, j0, M.m, first);
   Acc<T> acc;
   multiply<T, SPLIT, KG>(a, b, stages, smem, acc);
-  if (KIND == GRAM && t.slot >= 0) {   // (a part of the inner axis: join_kernel goes on)
+  if (T == JOIN_TILE && t.slot >= 0) {   // (a part of the inner axis: join_kernel goes on)
     if (KG == 1 || threadIdx.x < TPB) {
 #pragma unroll
       for (int i = 0; i < T / 32; ++i)
 #pragma unroll
-        for (int j = 0; j < T / 32; ++j) partial[((long long)t.slot * (T / 32) * (T / 32) + i * (T / 32) + j) * TPB + threadIdx.x] = acc[i][j];
+        for (int j = 0; j < T / 32; ++j) partial[(((long long)z * s.slots + t.slot) * (T / 32) * (T / 32) + i * (T / 32) + j) * TPB + threadIdx.x] = acc[i][j];
     }
     return;
   }
@@ -528,30 +580,43 @@ __global__ __launch_bounds__(KG * TPB, KG == 1 ? 2 : KG) void sym_kernel(const N
 
 // The parts of a tile whose inner axis was split, added in order, and stored as sym_store does; 16 workgroups a tile, four rows of one
 // column a thread (one workgroup a tile: 12 us, most of them waiting for one load after the other).
-template <bool SPLIT>
-__global__ __launch_bounds__(TPB) void join_kernel(const NsMatrix* __restrict__ mats, const NsItem* __restrict__ items, _Float16* __restrict__ G,
+template <bool SPLIT, SymKind KIND>
+__global__ __launch_bounds__(TPB) void join_kernel(const NsMatrix* __restrict__ mats, const NsItem* __restrict__ items, SymArgs s,
                                                    const f32x4_t* __restrict__ partial) {
-  constexpr int N = GRAM_TILE / 32, W = SPLIT ? 2 : 1;
+  constexpr int N = JOIN_TILE / 32, W = SPLIT ? 2 : 1;
   const NsItem t = items[blockIdx.x / (N * N)];
   const NsMatrix M = mats[t.matrix];
-  const int frag = blockIdx.x % (N * N), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int frag = blockIdx.x % (N * N), z = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const f32x4_t* from = partial + (((long long)z * s.slots + t.slot) * N * N + frag) * TPB + threadIdx.x;
   f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
   for (int k0 = 0; k0 < t.slots; k0 += 4) {
     f32x4_t v[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      v[k] = k0 + k < t.slots ? partial[((long long)(t.slot + k0 + k) * N * N + frag) * TPB + threadIdx.x] : f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int k = 0; k < 4; ++k) v[k] = k0 + k < t.slots ? from[(long long)(k0 + k) * N * N * TPB] : f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int k = 0; k < 4; ++k) sum += v[k];
   }
-  const float f = M.gscale / (M.scale * M.scale);
-  const int r = t.ti * GRAM_TILE + (wave >> 1) * (GRAM_TILE / 2) + (frag / N) * 16 + (lane >> 4) * 4;   // four rows of one column
-  const int c = t.tj * GRAM_TILE + (wave & 1) * (GRAM_TILE / 2) + (frag % N) * 16 + (lane & 15);
-  _Float16* out = G + W * M.a;
-  float v[4];
+  const int r = t.ti * JOIN_TILE + (wave >> 1) * (JOIN_TILE / 2) + (frag / N) * 16 + (lane >> 4) * 4;   // four rows of one column
+  const int c = t.tj * JOIN_TILE + (wave & 1) * (JOIN_TILE / 2) + (frag % N) * 16 + (lane & 15);
+  if (r >= M.lda) return;
+  _Float16* out = s.out[z] + W * M.a;
+  float v[4] = {sum[0], sum[1], sum[2], sum[3]};
+  if constexpr (KIND == GRAM) {
+    const float f = M.gscale / (M.scale * M.scale);
 #pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = r + e < M.m && c < M.m ? sum[e] * f : 0.f;
-  if (c < M.m && r < M.lda) put<SPLIT>(out, M.lda, c, r, v);
+    for (int e = 0; e < 4; ++e) v[e] *= f;
+  }
+  if constexpr (KIND == POLY) {
+    const float cb = s.b / M.gscale, cc = s.c / (M.gscale * M.gscale);
+    float g[4] = {0.f, 0.f, 0.f, 0.f};
+    if (c < M.m) get<SPLIT>(s.p[0] + W * M.a, M.lda, c, r, g);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = cc * v[e] + cb * g[e] + (r + e == c ? s.a : 0.f);
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (r + e >= M.m || c >= M.m) v[e] = 0.f;
+  if (c < M.m) put<SPLIT>(out, M.lda, c, r, v);
   if (t.ti == t.tj) return;   // (a diagonal tile holds both halves)
 #pragma unroll
   for (int e = 0; e < 4; ++e)
@@ -922,13 +987,18 @@ Work carve(const DasNsPlan* p, bool split, void* ws) {
   for (int i = 0; i < 2; ++i) w.x[i] = (_Float16*)take(xb);
   for (int i = 0; i < areas; ++i) w.a[i] = (_Float16*)take(ab);
   w.part = (Partial*)take(up256((long long)sizeof(Partial) * p->n_chunks));
-  w.slots = (f32x4_t*)take(4LL * GRAM_TILE * GRAM_TILE * p->n_slots);
+  w.slots = (f32x4_t*)take(4LL * JOIN_TILE * JOIN_TILE * std::max(p->gram_slots, 2 * p->product_slots));
   return w;
 }
 
+bool phases_valid(const DasNsPlan* p) {
+  for (int k = 0; k < p->steps; ++k)
+    if (p->phase_end[k] <= k || p->phase_end[k] > p->steps) return false;
+  return true;
+}
 bool plan_valid(const DasNsPlan* p, const void* tables, const void* ws) {
   return p && tables && ws && p->n_matrices > 0 && p->n_small >= 0 && p->n_small <= p->n_matrices && p->steps > 0 &&
-         p->steps <= DAS_NS_MAX_STEPS && (p->product_tile == 64 || p->product_tile == 128) && (p->update_tile == 64 || p->update_tile == 128) &&
+         p->steps <= DAS_NS_MAX_STEPS && phases_valid(p) && (p->product_tile == 64 || p->product_tile == 128) && (p->update_tile == 64 || p->update_tile == 128) &&
          !(((uintptr_t)tables | (uintptr_t)ws) & 15);
 }
 
@@ -969,13 +1039,11 @@ int phase_end(const Bounds* bound, int steps, int k) {
 template <typename T, bool MUON>
 int launch_small(const DasNsPlan* p, const char* tab, const Sources& src, const MuonIn& mu, const Result& res, hipStream_t s) {
   if (p->n_small == 0) return DAS_OK;
-  Steps st = {};
-  Bounds bound[DAS_NS_MAX_STEPS];
-  if (!polynomial_bounds(p->coef, p->steps, bound)) return DAS_ERR_ARG;
+  Steps st;
   memcpy(st.coef, p->coef, sizeof(st.coef));
+  memcpy(st.end, p->phase_end, sizeof(st.end));
   st.steps = p->steps;
   st.eps = p->eps;
-  for (int k = 0; k < p->steps; ++k) st.end[k] = phase_end(bound, p->steps, k);
   const NsMatrix* mats = (const NsMatrix*)(tab + p->mat_at);
   auto launch = [&](auto kernel, int nmax) {
     const int lds = 2 * (SMALL_M * (2 * nmax + 8) + N_AREAS * SMALL_M * PA);
@@ -993,23 +1061,28 @@ int iterate(const DasNsPlan* p, const char* tab, Work w, const Result& res, hipS
   const NsMatrix* mats = (const NsMatrix*)(tab + p->mat_at);
   const int4* chunks = (const int4*)(tab + p->chunk_at);
   const NsItem *gram = (const NsItem*)(tab + p->gram_at), *prod = (const NsItem*)(tab + p->product_at),
-               *upd = (const NsItem*)(tab + p->update_at), *join = (const NsItem*)(tab + p->join_at);
+               *upd = (const NsItem*)(tab + p->update_at), *gram_join = (const NsItem*)(tab + p->gram_join_at),
+               *prod_join = (const NsItem*)(tab + p->product_join_at);
   auto launch_sym = [&](auto kernel, int tile, int kg, const NsItem* items, int n, int products, const SymArgs& a) {
     const int lds = kg * 4 * tile * 128;
     (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     hipLaunchKernelGGL(kernel, dim3(n, products), dim3(kg * TPB), lds, s, mats, items, a, w.slots);
   };
+  constexpr int JOINERS = (JOIN_TILE / 32) * (JOIN_TILE / 32);
   auto gram_of = [&](const _Float16* x, _Float16* g) {
-    const SymArgs a = {{x}, {x}, {g}, 0.f, 0.f, 0.f};
-    if (p->gram_kg == 2) launch_sym(sym_kernel<GRAM_TILE, SPLIT, 2, GRAM>, GRAM_TILE, 2, gram, p->n_gram, 1, a);
-    else launch_sym(sym_kernel<GRAM_TILE, SPLIT, 1, GRAM>, GRAM_TILE, 1, gram, p->n_gram, 1, a);
-    if (p->n_join)
-      hipLaunchKernelGGL((join_kernel<SPLIT>), dim3(p->n_join * (GRAM_TILE / 32) * (GRAM_TILE / 32)), dim3(TPB), 0, s, mats, join, g, w.slots);
+    const SymArgs a = {{x}, {x}, {g}, 0.f, 0.f, 0.f, p->gram_slots};
+    if (p->gram_kg == 2) launch_sym(sym_kernel<JOIN_TILE, SPLIT, 2, GRAM>, JOIN_TILE, 2, gram, p->n_gram, 1, a);
+    else launch_sym(sym_kernel<JOIN_TILE, SPLIT, 1, GRAM>, JOIN_TILE, 1, gram, p->n_gram, 1, a);
+    if (p->n_gram_join)
+      hipLaunchKernelGGL((join_kernel<SPLIT, GRAM>), dim3(p->n_gram_join * JOINERS), dim3(TPB), 0, s, mats, gram_join, a, w.slots);
   };
-  auto sym = [&](auto kind, int products, const SymArgs& a) {
+  auto sym = [&](auto kind, int products, SymArgs a) {
     constexpr SymKind K = decltype(kind)::value;
+    a.slots = p->product_slots;
     if (p->product_tile == 128) launch_sym(sym_kernel<128, SPLIT, 1, K>, 128, 1, prod, p->n_product, products, a);
     else launch_sym(sym_kernel<64, SPLIT, 4, K>, 64, 4, prod, p->n_product, products, a);
+    if (p->n_product_join)
+      hipLaunchKernelGGL((join_kernel<SPLIT, K>), dim3(p->n_product_join * JOINERS, products), dim3(TPB), 0, s, mats, prod_join, a, w.slots);
   };
   auto update = [&](auto last, const _Float16* q, const _Float16* x, _Float16* y) {
     constexpr bool L = decltype(last)::value;
@@ -1025,12 +1098,10 @@ int iterate(const DasNsPlan* p, const char* tab, Work w, const Result& res, hipS
   const std::integral_constant<SymKind, PRODUCT> product_k;
   hipLaunchKernelGGL(normalise_kernel<SPLIT>, dim3(p->n_chunks), dim3(TPB), 0, s, mats, chunks, p->eps, w.x[0], w.part);
   DAS_CHECK_LAUNCH();
-  Bounds bound[DAS_NS_MAX_STEPS];
-  if (!polynomial_bounds(p->coef, p->steps, bound)) return DAS_ERR_ARG;
   _Float16 *X = w.x[0], *Y = w.x[1], *G = w.a[0], *R = w.a[1], *Z = w.a[SPLIT ? 2 : 1];
   for (int k = 0; k < p->steps;) {
     // steps k ... end - 1 are one phase
-    const int end = SPLIT ? phase_end(bound, p->steps, k) : k + 1;
+    const int end = SPLIT ? p->phase_end[k] : k + 1;
     gram_of(X, G);
     _Float16 *q = nullptr, *spare = w.a[SPLIT ? 3 : 1], *other = SPLIT ? w.a[4] : nullptr;   // (q: the phase's product so far)
     for (int j = k; j < end; ++j) {
@@ -1060,8 +1131,8 @@ int iterate(const DasNsPlan* p, const char* tab, Work w, const Result& res, hipS
 
 
 // Items of one launch. The hardware deals workgroups to the 8 XCDs in turn, and every XCD has its own 4 MiB L2: tiles that share rows
-// or columns are kept together in a group, groups go to the XCD with the least work so far, longest inner axis first, and the queues
-// are interleaved (item i runs on XCD i % 8). (Tiles in table order: each XCD read nearly every panel itself, 512 x 4608: 47 us
+// or columns are kept together in a group, the XCDs' queues are filled evenly, longest inner axis first, and then
+// interleaved (item i runs on XCD i % 8). (Tiles in table order: each XCD read nearly every panel itself, 512 x 4608: 47 us
 // for X X^T at the Infinity Cache's rate.)
 struct Launch {
   struct Group {
@@ -1085,10 +1156,26 @@ struct Launch {
     });
     std::vector<NsItem> queue[8];
     long long load[8] = {};
-    for (const Group& g : groups) {
-      const int x = (int)(std::min_element(load, load + 8) - load);
-      queue[x].insert(queue[x].end(), g.items.begin(), g.items.end());
-      load[x] += g.cost;
+    for (size_t i = 0; i < groups.size();) {
+      // groups of one length: the least loaded queues are filled up to the level that the whole class brings them to
+      size_t end = i;
+      long long cost = 0;
+      for (; end < groups.size() && groups[end].longest == groups[i].longest; ++end) cost += groups[end].cost;
+      int by_load[8] = {0, 1, 2, 3, 4, 5, 6, 7};
+      std::stable_sort(by_load, by_load + 8, [&](int u, int v) { return load[u] < load[v]; });
+      long long level = 0, sum = cost;
+      for (int k = 0; k < 8; ++k) {
+        sum += load[by_load[k]];
+        level = (sum + k) / (k + 1);
+        if (k == 7 || level <= load[by_load[k + 1]]) break;
+      }
+      int k = 0;
+      for (; i < end; ++i)
+        for (const NsItem& t : groups[i].items) {
+          while (k < 7 && load[by_load[k]] + (t.kn + 2) / 2 > level) ++k;
+          queue[by_load[k]].push_back(t);
+          load[by_load[k]] += t.kn + 2;
+        }
     }
     size_t depth = 0;
     for (const auto& q : queue) depth = std::max(depth, q.size());
@@ -1104,8 +1191,102 @@ struct Tables {
   std::vector<NsMatrix> mats;
   std::vector<int4> chunks;
   Launch gram, product, update;
-  std::vector<NsItem> join;
+  std::vector<NsItem> gram_join, product_join;
 };
+
+struct Tile {
+  bool fresh;                // first of its group
+  int matrix, ti, tj, steps;
+};
+
+// when the last of `slots` workers is done, longest pieces first; late (if given): the pieces that end after `limit`
+long long makespan(const std::vector<int>& pieces, int slots, long long limit, std::vector<int>* late) {
+  std::priority_queue<long long, std::vector<long long>, std::greater<long long>> free_at;
+  for (int i = 0; i < slots; ++i) free_at.push(0);
+  long long last = 0;
+  for (size_t i = 0; i < pieces.size(); ++i) {
+    const long long end = free_at.top() + pieces[i] + 2;
+    free_at.pop();
+    free_at.push(end);
+    last = std::max(last, end);
+    if (late && end > limit) late->push_back((int)i);
+  }
+  return last;
+}
+
+// Symmetric tiles of a launch for `slots` workgroups at a time. Tiles that would end after the others are split along the inner axis
+// where that pays: 1056 equal tiles in 512 slots are two rounds and a sixteenth, and took the time of nearly three. A part costs 128 KiB
+// of traffic, the join a launch (in steps of 64 inner elements, 1.3 us: 0.025 and 2.5); a part has at least 4 steps.
+void schedule(const std::vector<Tile>& tiles, int slots, Launch& launch, std::vector<NsItem>& join, long long& n_slots) {
+  std::vector<int> order(tiles.size()), parts(tiles.size(), 1), late;
+  for (size_t i = 0; i < tiles.size(); ++i) order[i] = (int)i;
+  std::stable_sort(order.begin(), order.end(), [&](int u, int v) { return tiles[u].steps > tiles[v].steps; });
+  long long total = 0;
+  std::vector<int> whole;
+  for (int i : order) {
+    total += tiles[i].steps + 2;
+    whole.push_back(tiles[i].steps);
+  }
+  const double even = (double)total / slots;
+  double best = (double)makespan(whole, slots, (long long)(1.05 * even), &late);
+  if (slots > 256) best = 0.5 * (best + even);   // (a workgroup whose neighbour on the CU has ended runs up to twice as fast)
+  if (tiles.size() < 16u * slots && best > 1.1 * even) {
+    std::vector<char> is_late(tiles.size(), 0);
+    for (int k : late) is_late[k] = 1;
+    int choice = 1;
+    for (int p : {2, 3, 4, 6, 8, 12, 16}) {
+      std::vector<int> pieces;
+      long long count = 0;
+      for (size_t k = 0; k < order.size(); ++k) {
+        const int steps = whole[k], q = is_late[k] ? std::max(1, std::min(p, steps / 4)) : 1;
+        for (int j = 0; j < q; ++j) pieces.push_back((int)((long long)steps * (j + 1) / q - (long long)steps * j / q));
+        if (q > 1) count += q;
+      }
+      std::sort(pieces.begin(), pieces.end(), std::greater<int>());
+      const double t = (double)makespan(pieces, slots, 0, nullptr) + (count ? 2.5 + 0.025 * (double)count : 0.0);
+      if (t < best) {
+        best = t;
+        choice = p;
+      }
+    }
+    for (size_t k = 0; k < order.size(); ++k)
+      if (is_late[k]) parts[order[k]] = std::max(1, std::min(choice, whole[k] / 4));
+  }
+  // whole tiles in their blocks; a part of the inner axis, of all the split tiles of a matrix, is a group: one XCD alone reads it
+  bool fresh = true;
+  for (size_t i = 0; i < tiles.size(); ++i) {
+    const Tile& t = tiles[i];
+    fresh |= t.fresh;
+    if (parts[i] > 1) continue;
+    launch.add(fresh, NsItem{t.matrix, t.ti, t.tj, 0, t.steps, -1, 1, 0});
+    fresh = false;
+  }
+  for (size_t i = 0; i < tiles.size();) {
+    size_t end = i;
+    while (end < tiles.size() && tiles[end].matrix == tiles[i].matrix) ++end;
+    int most = 1;
+    std::vector<int> slot(end - i, -1);
+    for (size_t k = i; k < end; ++k) {
+      if (parts[k] == 1) continue;
+      most = std::max(most, parts[k]);
+      slot[k - i] = (int)n_slots;
+      join.push_back(NsItem{tiles[k].matrix, tiles[k].ti, tiles[k].tj, 0, tiles[k].steps, (int)n_slots, parts[k], 0});
+      n_slots += parts[k];
+    }
+    for (int j = 0; j < most && most > 1; ++j) {
+      bool first = true;
+      for (size_t k = i; k < end; ++k) {
+        const int q = parts[k];
+        if (q == 1 || j >= q) continue;
+        const int k0 = (int)((long long)tiles[k].steps * j / q), k1 = (int)((long long)tiles[k].steps * (j + 1) / q);
+        launch.add(first, NsItem{tiles[k].matrix, tiles[k].ti, tiles[k].tj, k0, k1 - k0, slot[k - i] + j, 1, 0});
+        first = false;
+      }
+    }
+    i = end;
+  }
+  launch.place();
+}
 
 inline int over(long long v, int t) { return (int)((v + t - 1) / t); }
 
@@ -1146,7 +1327,7 @@ bool build(const DasNsShape* shapes, int n, double top, DasNsPlan* plan, Tables&
 
   t.mats.resize(n_mat);
   int small = 0, big = plan->n_small;   // (the small matrices come first in the table)
-  long long lower128 = 0, all128 = 0, gram_steps = 0;
+  long long lower128 = 0, all128 = 0;
   for (int g = 0; g < n; ++g) {
     const DasNsShape& s = shapes[g];
     for (int i = 0; i < s.count; ++i) {
@@ -1172,17 +1353,13 @@ bool build(const DasNsShape* shapes, int n, double top, DasNsPlan* plan, Tables&
       const long long tm = over(M.m, 128);
       lower128 += tm * (tm + 1) / 2;
       all128 += tm * (M.ldx / 128);
-      gram_steps += tm * (tm + 1) / 2 * (M.ldx / 64);
     }
   }
   // Products and updates: 128 x 128 tiles where they fill the 256 CUs, else 64 x 64 ones whose inner axis four wave groups share.
   plan->product_tile = lower128 >= 256 ? 128 : 64;
   plan->update_tile = all128 >= 256 ? 128 : 64;
-  // X X^T: 128 x 128 tiles; where there are fewer than two for each CU, two wave groups share a tile's inner axis, and it is
-  // split further until about 256 workgroups have a share, of at least 256 elements. Long ones are split in larger sets too: the
-  // last tile to finish should not have more than its 512th of the work.
+  // X X^T: 128 x 128 tiles; where there are fewer than 384, two wave groups share a tile's inner axis (one workgroup a CU, not two)
   plan->gram_kg = lower128 >= 384 ? 1 : 2;
-  const long long share = std::max<long long>(4, (gram_steps + 255) / (plan->gram_kg == 1 ? 512 : 256));
   // blocks of up to 8 x 8 tiles, smaller where one would be more than a 16th of the launch (half of an XCD's part)
   auto side_for = [](long long launch, int steps) {
     int side = 8;
@@ -1192,40 +1369,31 @@ bool build(const DasNsShape* shapes, int n, double top, DasNsPlan* plan, Tables&
   long long product_cost = 0, update_cost = 0, gram_cost = 0;
   for (int q = plan->n_small; q < (int)n_mat; ++q) {
     const NsMatrix& M = t.mats[q];
-    const long long p = over(M.m, plan->product_tile), r = over(M.m, plan->update_tile), w = over(M.m, GRAM_TILE);
+    const long long p = over(M.m, plan->product_tile), r = over(M.m, plan->update_tile), w = over(M.m, JOIN_TILE);
     product_cost += p * (p + 1) / 2 * (M.lda / 64 + 2);
     update_cost += r * (M.ldx / plan->update_tile) * (M.lda / 64 + 2);
     gram_cost += w * (w + 1) / 2 * (M.ldx / 64 + 2);
   }
+  std::vector<Tile> gram, product;
   for (int q = plan->n_small; q < (int)n_mat; ++q) {
     const NsMatrix& M = t.mats[q];
-    const int steps = M.ldx / 64, parts = (int)std::min<long long>(16, std::max<long long>(1, (steps + share / 2) / share));
-    const int tm = over(M.m, GRAM_TILE);
-    if (parts > 1) {   // (one part of the inner axis = one group: it is read by one XCD alone)
-      for (int k = 0; k < parts; ++k) {
-        int tile = 0;
-        const int k0 = (int)((long long)steps * k / parts), k1 = (int)((long long)steps * (k + 1) / parts);
-        lower_blocks(tm, 1 << 16, [&](bool fresh, int i, int j) {
-          t.gram.add(fresh, NsItem{q, i, j, k0, k1 - k0, (int)plan->n_slots + tile++ * parts + k, 1, 0});
-        });
-      }
-      lower_blocks(tm, 1 << 16, [&](bool, int i, int j) {
-        t.join.push_back(NsItem{q, i, j, 0, steps, (int)plan->n_slots, parts, 0});
-        plan->n_slots += parts;
-      });
-    } else {
-      lower_blocks(tm, side_for(gram_cost, steps), [&](bool fresh, int i, int j) { t.gram.add(fresh, NsItem{q, i, j, 0, steps, -1, 1, 0}); });
-    }
+    lower_blocks(over(M.m, JOIN_TILE), side_for(gram_cost, M.ldx / 64),
+                 [&](bool fresh, int i, int j) { gram.push_back(Tile{fresh, q, i, j, M.ldx / 64}); });
     lower_blocks(over(M.m, plan->product_tile), side_for(product_cost, M.lda / 64),
-                 [&](bool fresh, int i, int j) { t.product.add(fresh, NsItem{q, i, j, 0, M.lda / 64, -1, 1, 0}); });
+                 [&](bool fresh, int i, int j) { product.push_back(Tile{fresh, q, i, j, M.lda / 64}); });
     const int rows = over(M.m, plan->update_tile), cols = M.ldx / plan->update_tile, side = side_for(update_cost, M.lda / 64);
     for (int bj = 0; bj < cols; bj += side)
       for (int bi = 0; bi < rows; bi += side)
         for (int j = bj; j < std::min(cols, bj + side); ++j)
           for (int i = bi; i < std::min(rows, bi + side); ++i) t.update.add(i == bi && j == bj, NsItem{q, i, j, 0, M.lda / 64, -1, 1, 0});
   }
-  t.gram.place();
-  t.product.place();
+  schedule(gram, plan->gram_kg == 1 ? 512 : 256, t.gram, t.gram_join, plan->gram_slots);
+  if (plan->product_tile == JOIN_TILE) {
+    schedule(product, 512, t.product, t.product_join, plan->product_slots);
+  } else {
+    for (const Tile& p : product) t.product.add(p.fresh, NsItem{p.matrix, p.ti, p.tj, 0, p.steps, -1, 1, 0});
+    t.product.place();
+  }
   t.update.place();
   return t.gram.order.size() < (1u << 30) && t.update.order.size() < (1u << 30);
 }
@@ -1247,8 +1415,9 @@ extern "C" int das_ns_plan(const DasNsShape* shapes, int n, int steps, const flo
     if (!build(shapes, n, top, &p, t)) return DAS_ERR_ARG;
     p.n_groups = n; p.n_matrices = (int)t.mats.size(); p.n_chunks = (int)t.chunks.size();
     p.n_gram = (int)t.gram.order.size(); p.n_product = (int)t.product.order.size(); p.n_update = (int)t.update.order.size();
-    p.n_join = (int)t.join.size();
+    p.n_gram_join = (int)t.gram_join.size(); p.n_product_join = (int)t.product_join.size();
     p.steps = steps; p.eps = eps;
+    for (int k = 0; k < steps; ++k) p.phase_end[k] = phase_end(bound, steps, k);
     memcpy(p.coef, coef, sizeof(float) * 3 * steps);
     char* out = nullptr;
     auto put_table = [&](const auto& v, long long& at) {
@@ -1267,8 +1436,9 @@ extern "C" int das_ns_plan(const DasNsShape* shapes, int n, int steps, const flo
       put_table(t.mats, p.mat_at);
       put_table(t.chunks, p.chunk_at);
       put_table(t.gram.order, p.gram_at);
-      put_table(t.join, p.join_at);
+      put_table(t.gram_join, p.gram_join_at);
       put_table(t.product.order, p.product_at);
+      put_table(t.product_join, p.product_join_at);
       put_table(t.update.order, p.update_at);
     }
     *plan = p;

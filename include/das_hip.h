@@ -626,11 +626,12 @@ typedef struct {
   int reserved;
 } DasNsShape;
 typedef struct {
-  int n_groups, n_matrices, n_small, small_n, n_chunks, n_gram, n_join, n_product, n_update, steps;
-  int product_tile, update_tile, gram_kg, reserved;
-  long long x_elems, a_elems, n_slots, extent;            /* work areas (f16 elements); one past the last element of the flat buffers used */
-  long long mat_at, chunk_at, gram_at, join_at, product_at, update_at, table_bytes;   /* byte offsets of the tables */
+  int n_groups, n_matrices, n_small, small_n, n_chunks, n_gram, n_gram_join, n_product, n_product_join, n_update, steps;
+  int product_tile, update_tile, gram_kg;
+  long long x_elems, a_elems, gram_slots, product_slots, extent;            /* work areas (f16 elements); one past the last element of the flat buffers used */
+  long long mat_at, chunk_at, gram_at, gram_join_at, product_at, product_join_at, update_at, table_bytes;   /* byte offsets of the tables */
   float coef[3 * DAS_NS_MAX_STEPS];              /* a, b, c of each step */
+  int phase_end[DAS_NS_MAX_STEPS];               /* f32 results: where a run of steps on the m x m matrices that starts here ends */
   float eps;
 } DasNsPlan;
 /* One source tensor of das_orthogonalize: `count` matrices, element (i, r, c) at base[i * batch_stride + r * row_stride + c]. */
