@@ -727,6 +727,8 @@ struct Steps {
   float eps;
 };
 
+constexpr int SMALL_TPB = 1024;       // 16 waves, a 16 x 16 fragment of every 64 x 64 product each: latencies overlap (four waves: 19 us for 64 x 64)
+
 __device__ __forceinline__ f16x8_t row_frag(const _Float16* p, int pitch, int row0, int k, int part) {
   const int lane = threadIdx.x & 63;
   return *reinterpret_cast<const f16x8_t*>(p + (row0 + (lane & 15)) * pitch + k * 64 + part * 32 + (lane >> 4) * 8);
@@ -744,60 +746,49 @@ __device__ __forceinline__ f16x8_t col_frag(const _Float16* x, int pitch, int co
   }
   return f;
 }
-// the wave's 32 x 32 of P rows x (Q rows, or columns of Q): k32 inner steps of 32
+// the wave's 16 x 16 of P rows x (Q rows, or columns of Q from col0 on): k32 inner steps of 32
 template <bool COLS>
-__device__ __forceinline__ void small_product(const _Float16* p, int pp, const _Float16* q, int qp, int col0, int k32, f32x4_t (&acc)[2][2]) {
-  const int wave = threadIdx.x >> 6, wr = (wave >> 1) * 32, wc = (wave & 1) * 32;
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+__device__ __forceinline__ f32x4_t small_product(const _Float16* p, int pp, const _Float16* q, int qp, int col0, int k32) {
+  const int wave = threadIdx.x >> 6, wr = (wave >> 2) * 16, wc = (wave & 3) * 16;
+  f32x4_t high = {0.f, 0.f, 0.f, 0.f}, low = {0.f, 0.f, 0.f, 0.f};   // (two chains)
   for (int k = 0; k < k32; ++k) {
-    f16x8_t fa[2][2], fb[2][2];
+    f16x8_t fa[2], fb[2];
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        fa[u][t] = row_frag(p, pp, wr + t * 16, k, u);
-        fb[u][t] = COLS ? col_frag(q, qp, col0 + wc + t * 16, k, u) : row_frag(q, qp, wc + t * 16, k, u);
-      }
-#pragma unroll
-    for (int z = 0; z < 3; ++z)
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa[z == 0][i], fb[z == 1][j], acc[i][j], 0, 0, 0);
+    for (int u = 0; u < 2; ++u) {
+      fa[u] = row_frag(p, pp, wr, k, u);
+      fb[u] = COLS ? col_frag(q, qp, col0 + wc, k, u) : row_frag(q, qp, wc, k, u);
+    }
+    high = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa[0], fb[0], high, 0, 0, 0);
+    low = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa[1], fb[0], low, 0, 0, 0);
+    low = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa[0], fb[1], low, 0, 0, 0);
   }
+  return high + low;
+}
+__device__ __forceinline__ void put4(_Float16* p, const float (&v)[4]) {
+  f16x4_t h, l;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    h[e] = (_Float16)v[e];
+    l[e] = (_Float16)(v[e] - (float)h[e]);
+  }
+  *reinterpret_cast<f16x4_t*>(p) = h;
+  *reinterpret_cast<f16x4_t*>(p + 32) = l;
 }
 // a symmetric result, stored transposed (four values of a lane are neighbours then): f(row, col, four values) may change them
 template <typename F>
-__device__ __forceinline__ void small_store(const f32x4_t (&acc)[2][2], _Float16* out, F f) {
+__device__ __forceinline__ void small_store(f32x4_t acc, _Float16* out, F f) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int r = (wave & 1) * 32 + j * 16 + (lane & 15), c = (wave >> 1) * 32 + i * 16 + (lane >> 4) * 4;
-      float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-      f(r, c, v);
-      f16x4_t h, l;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        h[e] = (_Float16)v[e];
-        l[e] = (_Float16)(v[e] - (float)h[e]);
-      }
-      _Float16* p = out + r * PA + (c >> 5) * 64 + (c & 31);
-      *reinterpret_cast<f16x4_t*>(p) = h;
-      *reinterpret_cast<f16x4_t*>(p + 32) = l;
-    }
+  const int r = (wave & 3) * 16 + (lane & 15), c = (wave >> 2) * 16 + (lane >> 4) * 4;
+  float v[4] = {acc[0], acc[1], acc[2], acc[3]};
+  f(r, c, v);
+  put4(out + r * PA + (c >> 5) * 64 + (c & 31), v);
 }
 
 template <typename T, bool MUON, int NMAX>
-__global__ __launch_bounds__(TPB) void small_kernel(const NsMatrix* __restrict__ mats, Sources src, MuonIn mu, Steps st, Result res) {
+__global__ __launch_bounds__(SMALL_TPB) void small_kernel(const NsMatrix* __restrict__ mats, Sources src, MuonIn mu, Steps st, Result res) {
   extern __shared__ __align__(16) char smem[];
-  __shared__ float red[4];
-  __shared__ double redd[4];
+  __shared__ float red[SMALL_TPB / 64];
+  __shared__ double redd[SMALL_TPB / 64];
   constexpr int PX = 2 * NMAX + 8, PF = NMAX + 4;   // X's row pitch in f16 elements and in floats
   const NsMatrix M = mats[blockIdx.x];
   if (!MUON && (unsigned)(M.group - src.first) >= (unsigned)src.count) return;   // (whole workgroups)
@@ -808,20 +799,18 @@ __global__ __launch_bounds__(TPB) void small_kernel(const NsMatrix* __restrict__
   for (int i = 0; i < N_AREAS; ++i) A[i] = X + SMALL_M * PX + i * SMALL_M * PA;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 
-  // U, zeros around it
-  for (int i = threadIdx.x; i < SMALL_M * PF / 4; i += TPB) reinterpret_cast<float4*>(U)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-  __syncthreads();
-  float coef = 1.f, big = 0.f;
-  if constexpr (MUON) coef = grad_factor(mu);
+  // U, zeros around it. The loads go out first.
   const int count = M.rows * M.cols;
   const float per_row = 1.f / (float)M.cols;   // (index + 1/2) / cols is exact enough to truncate for indices under 2^14
-  constexpr int BATCH = 8;                     // loads in flight per thread: a load a time is a memory latency each
-  for (int i0 = threadIdx.x; i0 < count; i0 += BATCH * TPB) {
+  constexpr int BATCH = 4;                     // loads in flight per thread: a load a time is a memory latency each
+  float big = 0.f, coef = 1.f;
+  if constexpr (MUON) coef = grad_factor(mu);
+  for (int i0 = threadIdx.x; i0 < max(count, SMALL_TPB); i0 += BATCH * SMALL_TPB) {
     float v[BATCH], b[BATCH];
     const DasNsSource& s = src.s[MUON ? 0 : M.group - src.first];
 #pragma unroll
     for (int k = 0; k < BATCH; ++k) {
-      const int i = i0 + k * TPB, r = (int)((i + 0.5f) * per_row), c = i - r * M.cols;
+      const int i = i0 + k * SMALL_TPB, r = (int)((i + 0.5f) * per_row), c = i - r * M.cols;
       v[k] = 0.f;
       if (i < count) {
         if constexpr (MUON) {
@@ -832,9 +821,13 @@ __global__ __launch_bounds__(TPB) void small_kernel(const NsMatrix* __restrict__
         }
       }
     }
+    if (i0 < SMALL_TPB) {
+      for (int i = threadIdx.x; i < SMALL_M * PF / 4; i += SMALL_TPB) reinterpret_cast<float4*>(U)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      __syncthreads();
+    }
 #pragma unroll
     for (int k = 0; k < BATCH; ++k) {
-      const int i = i0 + k * TPB, r = (int)((i + 0.5f) * per_row), c = i - r * M.cols;
+      const int i = i0 + k * SMALL_TPB, r = (int)((i + 0.5f) * per_row), c = i - r * M.cols;
       if (i >= count) continue;
       if constexpr (MUON) {
         v[k] = muon_in(mu, coef, v[k], b[k]);
@@ -844,50 +837,48 @@ __global__ __launch_bounds__(TPB) void small_kernel(const NsMatrix* __restrict__
       big = fmaxf(big, fabsf(v[k]));
     }
   }
-  big = block_reduce(big, true, red);   // (its barriers order U's writes too)
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor(big, o, 64));
+  if (lane == 0) red[wave] = big;
+  __syncthreads();                             // (U is whole, too)
+#pragma unroll
+  for (int i = 0; i < SMALL_TPB / 64; ++i) big = fmaxf(big, red[i]);
   int e = 0;
   if (big > 0.f && big <= 3.4028235e38f) (void)frexpf(big, &e);
-  float v[NMAX / 32][8], ss = 0.f;
-  const int row = threadIdx.x >> 2, c8 = (threadIdx.x & 3) * 8;
+  float v[NMAX / 64][4], ss = 0.f;
+  const int row = threadIdx.x >> 4, c4 = (threadIdx.x & 15) * 4;
 #pragma unroll
-  for (int b = 0; b < NMAX / 32; ++b)
+  for (int b = 0; b < NMAX / 64; ++b) {
+    const float4 w = *reinterpret_cast<const float4*>(U + row * PF + b * 64 + c4);
+    v[b][0] = ldexpf(w.x, -e); v[b][1] = ldexpf(w.y, -e); v[b][2] = ldexpf(w.z, -e); v[b][3] = ldexpf(w.w, -e);
 #pragma unroll
-    for (int k = 0; k < 8; k += 4) {
-      const float4 w = *reinterpret_cast<const float4*>(U + row * PF + b * 32 + c8 + k);
-      v[b][k] = ldexpf(w.x, -e); v[b][k + 1] = ldexpf(w.y, -e); v[b][k + 2] = ldexpf(w.z, -e); v[b][k + 3] = ldexpf(w.w, -e);
-#pragma unroll
-      for (int q = k; q < k + 4; ++q) ss += v[b][q] * v[b][q];
-    }
+    for (int k = 0; k < 4; ++k) ss += v[b][k] * v[b][k];
+  }
   double sum = ss;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
   if (lane == 0) redd[wave] = sum;
-  __syncthreads();                       // (every read of U is done, too)
-  const float f = (float)ldexp((double)M.scale / (ldexp(sqrt((redd[0] + redd[1]) + (redd[2] + redd[3])), e) + (double)st.eps), e);
+  __syncthreads();                             // (every read of U is done, too)
+  sum = 0.0;
 #pragma unroll
-  for (int b = 0; b < NMAX / 32; ++b) {
-    f16x8_t h, l;
+  for (int i = 0; i < SMALL_TPB / 64; ++i) sum += redd[i];
+  const float f = (float)ldexp((double)M.scale / (ldexp(sqrt(sum), e) + (double)st.eps), e);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const float x = v[b][k] * f;
-      h[k] = (_Float16)x;
-      l[k] = (_Float16)(x - (float)h[k]);
-    }
-    *reinterpret_cast<f16x8_t*>(X + row * PX + b * 64 + c8) = h;
-    *reinterpret_cast<f16x8_t*>(X + row * PX + b * 64 + 32 + c8) = l;
+  for (int b = 0; b < NMAX / 64; ++b) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[b][k] *= f;
+    put4(X + row * PX + b * 128 + (c4 >> 5) * 64 + (c4 & 31), v[b]);
   }
   __syncthreads();
 
   // the phases of iterate<true>
   const int n32 = (M.n + 31) / 32, tiles = (M.n + 63) / 64;
-  f32x4_t acc[2][2];
   auto plain = [](int, int, float (&)[4]) {};
   for (int k = 0; k < st.steps;) {
     const int end = st.end[k];
     const float gs = M.gscale / (M.scale * M.scale);
     _Float16 *G = A[0], *R = A[1], *Z = A[2], *q = nullptr, *spare = A[3], *other = A[4];
-    small_product<false>(X, PX, X, PX, 0, n32, acc);
-    small_store(acc, G, [&](int, int, float (&w)[4]) {
+    small_store(small_product<false>(X, PX, X, PX, 0, n32), G, [&](int, int, float (&w)[4]) {
 #pragma unroll
       for (int t = 0; t < 4; ++t) w[t] *= gs;
     });
@@ -895,23 +886,16 @@ __global__ __launch_bounds__(TPB) void small_kernel(const NsMatrix* __restrict__
     for (int j = k; j < end; ++j) {
       const float ca = st.coef[3 * j], cb = st.coef[3 * j + 1] / M.gscale, cc = st.coef[3 * j + 2] / (M.gscale * M.gscale);
       _Float16* z = q ? Z : spare;
-      small_product<false>(G, PA, G, PA, 0, 2, acc);
-      small_store(acc, z, [&](int r, int c, float (&w)[4]) {
+      small_store(small_product<false>(G, PA, G, PA, 0, 2), z, [&](int r, int c, float (&w)[4]) {
         const _Float16* g = G + r * PA + (c >> 5) * 64 + (c & 31);
         const f16x4_t h = *reinterpret_cast<const f16x4_t*>(g), l = *reinterpret_cast<const f16x4_t*>(g + 32);
 #pragma unroll
         for (int t = 0; t < 4; ++t) w[t] = cc * w[t] + cb * ((float)h[t] + (float)l[t]) + (r == c + t ? ca : 0.f);
       });
       __syncthreads();
-      if (q) {
-        small_product<false>(z, PA, q, PA, 0, 2, acc);
-        small_store(acc, other, plain);
-      }
-      if (j + 1 < end) {
-        small_product<false>(z, PA, G, PA, 0, 2, acc);
-        small_store(acc, R, plain);
-      }
-      __syncthreads();
+      if (q) small_store(small_product<false>(z, PA, q, PA, 0, 2), other, plain);
+      if (j + 1 < end) small_store(small_product<false>(z, PA, G, PA, 0, 2), R, plain);
+      if (q || j + 1 < end) __syncthreads();
       if (q) {
         _Float16* t = q;
         q = other;
@@ -920,46 +904,47 @@ __global__ __launch_bounds__(TPB) void small_kernel(const NsMatrix* __restrict__
         q = z;
       }
       if (j + 1 < end) {
-        small_product<false>(R, PA, z, PA, 0, 2, acc);
-        small_store(acc, G, plain);       // (nobody reads G any more)
+        small_store(small_product<false>(R, PA, z, PA, 0, 2), G, plain);       // (nobody reads G any more)
         __syncthreads();
       }
     }
     const bool last = end == st.steps;
-    for (int t = 0; t < tiles; ++t) {
-      small_product<true>(q, PA, X, PX, t * 64, 2, acc);
-      __syncthreads();                    // (the 64 columns of X have been read; nobody else needs them)
+    f32x4_t acc[NMAX / 64];
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+    for (int t = 0; t < NMAX / 64; ++t)
+      if (t < tiles) acc[t] = small_product<true>(q, PA, X, PX, t * 64, 2);
+    __syncthreads();                    // (X has been read)
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+    for (int t = 0; t < NMAX / 64; ++t) {
+      if (t >= tiles) continue;
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const int r = (wave >> 1) * 32 + i * 16 + (lane >> 4) * 4 + w, c = t * 64 + (wave & 1) * 32 + j * 16 + (lane & 15);
-            const float x = acc[i][j][w];
-            if (last) {
-              U[r * PF + c] = x;
-            } else {
-              _Float16* p = X + r * PX + (c >> 5) * 64 + (c & 31);
-              p[0] = (_Float16)x;
-              p[32] = (_Float16)(x - (float)p[0]);
-            }
-          }
+      for (int w = 0; w < 4; ++w) {
+        const int r = (wave >> 2) * 16 + (lane >> 4) * 4 + w, c = t * 64 + (wave & 3) * 16 + (lane & 15);
+        const float x = acc[t][w];
+        if (last) {
+          U[r * PF + c] = x;
+        } else {
+          _Float16* p = X + r * PX + (c >> 5) * 64 + (c & 31);
+          const _Float16 h = (_Float16)x;
+          p[0] = h;
+          p[32] = (_Float16)(x - (float)h);
+        }
+      }
     }
     __syncthreads();
     k = end;
   }
 
   const float g = result_factor(M, res);
-  for (int i0 = threadIdx.x; i0 < count; i0 += BATCH * TPB) {
+  for (int i0 = threadIdx.x; i0 < count; i0 += BATCH * SMALL_TPB) {
     float w[BATCH];
     if constexpr (MUON) {
 #pragma unroll
-      for (int k = 0; k < BATCH; ++k) w[k] = i0 + k * TPB < count ? res.p[M.src + i0 + k * TPB] : 0.f;
+      for (int k = 0; k < BATCH; ++k) w[k] = i0 + k * SMALL_TPB < count ? res.p[M.src + i0 + k * SMALL_TPB] : 0.f;
     }
 #pragma unroll
     for (int k = 0; k < BATCH; ++k) {
-      const int i = i0 + k * TPB, r = (int)((i + 0.5f) * per_row), c = i - r * M.cols;
+      const int i = i0 + k * SMALL_TPB, r = (int)((i + 0.5f) * per_row), c = i - r * M.cols;
       if (i >= count) continue;
       const float x = g * U[M.tall ? c * PF + r : r * PF + c];
       if constexpr (MUON) res.p[M.src + i] = res.keep * w[k] - x;
@@ -1048,7 +1033,7 @@ int launch_small(const DasNsPlan* p, const char* tab, const Sources& src, const 
   auto launch = [&](auto kernel, int nmax) {
     const int lds = 2 * (SMALL_M * (2 * nmax + 8) + N_AREAS * SMALL_M * PA);
     (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    hipLaunchKernelGGL(kernel, dim3(p->n_small), dim3(TPB), lds, s, mats, src, mu, st, res);
+    hipLaunchKernelGGL(kernel, dim3(p->n_small), dim3(SMALL_TPB), lds, s, mats, src, mu, st, res);
   };
   if (p->small_n <= 64) launch(small_kernel<T, MUON, 64>, 64);
   else launch(small_kernel<T, MUON, 256>, 256);
@@ -1216,7 +1201,9 @@ long long makespan(const std::vector<int>& pieces, int slots, long long limit, s
 
 // Symmetric tiles of a launch for `slots` workgroups at a time. Tiles that would end after the others are split along the inner axis
 // where that pays: 1056 equal tiles in 512 slots are two rounds and a sixteenth, and took the time of nearly three. A part costs 128 KiB
-// of traffic, the join a launch (in steps of 64 inner elements, 1.3 us: 0.025 and 2.5); a part has at least 4 steps.
+// of traffic, the join a launch: 0.0125 and 1.2 steps of 64 inner elements (2.5 us with two workgroups on a CU; 13 us measured for 272
+// parts). A workgroup whose neighbour on the CU has ended runs up to twice as fast, so only half of what sticks out counts. A part has
+// at least 4 steps.
 void schedule(const std::vector<Tile>& tiles, int slots, Launch& launch, std::vector<NsItem>& join, long long& n_slots) {
   std::vector<int> order(tiles.size()), parts(tiles.size(), 1), late;
   for (size_t i = 0; i < tiles.size(); ++i) order[i] = (int)i;
@@ -1228,9 +1215,9 @@ void schedule(const std::vector<Tile>& tiles, int slots, Launch& launch, std::ve
     whole.push_back(tiles[i].steps);
   }
   const double even = (double)total / slots;
-  double best = (double)makespan(whole, slots, (long long)(1.05 * even), &late);
-  if (slots > 256) best = 0.5 * (best + even);   // (a workgroup whose neighbour on the CU has ended runs up to twice as fast)
-  if (tiles.size() < 16u * slots && best > 1.1 * even) {
+  auto seen = [&](long long t) { return slots > 256 ? 0.5 * ((double)t + even) : (double)t; };
+  double best = 0.95 * seen(makespan(whole, slots, (long long)(1.05 * even), &late));
+  if (tiles.size() < 16u * slots && best > even) {
     std::vector<char> is_late(tiles.size(), 0);
     for (int k : late) is_late[k] = 1;
     int choice = 1;
@@ -1243,7 +1230,7 @@ void schedule(const std::vector<Tile>& tiles, int slots, Launch& launch, std::ve
         if (q > 1) count += q;
       }
       std::sort(pieces.begin(), pieces.end(), std::greater<int>());
-      const double t = (double)makespan(pieces, slots, 0, nullptr) + (count ? 2.5 + 0.025 * (double)count : 0.0);
+      const double t = seen(makespan(pieces, slots, 0, nullptr)) + 1.2 + 0.0125 * (double)count;
       if (t < best) {
         best = t;
         choice = p;

@@ -150,9 +150,11 @@ def sgd_momentum_step(p, g, buf, lr, momentum, weight_decay, grad_scale=1.0, max
 # ------------------------------------------------------------------ AdamW, Newton-Schulz orthogonalisation, Muon
 def _flat_buffers(what, *ts):
     """Contiguous f32 tensors of one size on one GPU: what the flat-buffer optimizer steps take."""
-    _need_gpu(*ts)
+    n, dev = ts[0].numel(), ts[0].device
     for t in ts:
-        if t.dtype != torch.float32 or not t.is_contiguous() or t.numel() != ts[0].numel() or t.device != ts[0].device:
+        if not t.is_cuda:
+            _need_gpu(t)
+        if t.dtype is not torch.float32 or not t.is_contiguous() or t.numel() != n or t.device != dev:
             raise _lib.DasHipError(f'{what}: parameters, gradients and state are contiguous float32 tensors of one size on one device')
 
 
@@ -162,6 +164,11 @@ _SAME_DEVICE = contextlib.nullcontext()
 def _on(device):
     """Launches go to the tensors' device, whichever is current (entering torch's guard costs microseconds: only where needed)"""
     return _SAME_DEVICE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _stream_of(device):
+    """The device's current stream (torch.cuda.current_stream() builds an object around it: 3 us of a 10 us step)"""
+    return C.c_void_p(torch._C._cuda_getCurrentRawStream(device.index))
 
 
 def _clip_sum(what, max_norm, grad_sumsq_t, device):
@@ -184,7 +191,7 @@ def adamw_step(p, g, m, v, lr, step, beta1=0.9, beta2=0.999, eps=1e-8, weight_de
     with _on(p.device):
         _lib.check(_lib.load().das_adamw_step(_ptr(p), _ptr(g), _ptr(m), _ptr(v), p.numel(), float(lr), float(beta1), float(beta2),
                                               float(eps), float(weight_decay), int(step), float(grad_scale), float(max_norm),
-                                              _ptr(sumsq), _stream()), 'das_adamw_step')
+                                              _ptr(sumsq), _stream_of(p.device)), 'das_adamw_step')
 
 
 _NS_DT = {torch.float32: _lib.DAS_F32, torch.bfloat16: _lib.DAS_BF16, torch.float16: _lib.DAS_F16}
@@ -287,7 +294,7 @@ def orthogonalize(mats, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, out_dty
             lib = _lib.load()
             ws = torch.empty(lib.das_ns_ws_bytes(C.byref(p), int(out_dtype == torch.float32)), dtype=torch.uint8, device=dev)
             _lib.check(lib.das_orthogonalize(C.byref(p), _ptr(tables), src, len(live), dt, _ptr(out), _NS_DT[out_dtype], _ptr(ws),
-                                             _stream()), 'das_orthogonalize')
+                                             _stream_of(dev)), 'das_orthogonalize')
     res = [out[o:o + t.numel()].view(t.shape) for o, t in zip(plan._out_offsets, mats)]
     return res[0] if one else res
 
@@ -314,7 +321,7 @@ def muon_step(p, g, buf, plan, lr, momentum=0.95, weight_decay=0.0, nesterov=Tru
         ws = torch.empty(lib.das_ns_ws_bytes(C.byref(c_plan), 1), dtype=torch.uint8, device=p.device)
         _lib.check(lib.das_muon_step(C.byref(c_plan), _ptr(tables), _ptr(p), _ptr(g), _ptr(buf), float(lr), float(momentum),
                                      float(weight_decay), int(bool(nesterov)), int(lr_scale != 'original'), float(grad_scale),
-                                     float(max_norm), _ptr(sumsq), _ptr(ws), _stream()), 'das_muon_step')
+                                     float(max_norm), _ptr(sumsq), _ptr(ws), _stream_of(p.device)), 'das_muon_step')
 
 
 # ------------------------------------------------------------------ RealNVP log-density (RLE pose loss)
