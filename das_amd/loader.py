@@ -173,6 +173,7 @@ class _FrameRing:
         self._mm = mmap.mmap(self._fd, slots * slot_bytes)
         self.bytes = np.frombuffer(self._mm, dtype=np.uint8)
         self.registered = False
+        self._copy = None
 
     @classmethod
     def create(cls, slots, slot_bytes, pin, min_slots=8):
@@ -214,14 +215,33 @@ class _FrameRing:
         return ring
 
     def pin(self):
-        """Page-lock the ring for asynchronous uploads (needs a GPU context: called when the loader is bound to its device)."""
+        """Make uploads asynchronous: page-lock the ring (needs a GPU context: called when the loader is bound to its device) or, where the
+        system refuses to lock memory that exists already, allocate a page-locked copy of it that frames pass through."""
         if not self.registered:
             t = torch.from_numpy(self.bytes)
             self.registered = int(torch.cuda.cudart().cudaHostRegister(t.data_ptr(), t.numel(), 0)) == 0
             if not self.registered:
-                import warnings
-                warnings.warn('das_amd.loader: could not page-lock the frame ring; uploads fall back to staged copies')
+                # the refusal stays the runtime's last error, and the next launch check would report it as its own: take it here
+                try:
+                    torch.zeros(1, device='cuda')
+                except RuntimeError:
+                    pass
+                try:
+                    self._copy = torch.empty(t.numel(), dtype=torch.uint8, pin_memory=True)
+                    self.registered = True
+                except RuntimeError:
+                    import warnings
+                    warnings.warn('das_amd.loader: could not page-lock the frame ring; uploads fall back to staged copies')
         return self.registered
+
+    def frame(self, i, nbytes):
+        """Slot i's bytes as the trainer uploads them: the ring's own, or its page-locked copy, brought up to date (a slot goes back to the
+        worker when its upload is done, so both are reused together)."""
+        if self._copy is None:
+            return self.slot(i, nbytes)
+        s = i * self.slot_bytes
+        self._copy[s:s + nbytes].copy_(torch.from_numpy(self.slot(i, nbytes)))
+        return self._copy.numpy()[s:s + nbytes]
 
     def unlink(self):
         """Remove the backing file's name (both sides keep their mappings): it can no longer outlive the processes."""
@@ -238,7 +258,7 @@ class _FrameRing:
     def close(self):
         if self._mm is None:
             return
-        if self.registered:
+        if self.registered and self._copy is None:
             try:
                 torch.cuda.cudart().cudaHostUnregister(torch.from_numpy(self.bytes).data_ptr())
             except Exception:   # noqa: BLE001
@@ -420,7 +440,7 @@ class ProcessLoader:
             if kind == 'ring':
                 _, i, shape, dt, plan = s['img']
                 n = int(np.prod(shape)) * np.dtype(dt).itemsize
-                plans.append(plan.with_frame(ring.slot(i, n).view(np.dtype(dt)).reshape(shape)))
+                plans.append(plan.with_frame(ring.frame(i, n).view(np.dtype(dt)).reshape(shape)))
             elif kind == 'plan':
                 plans.append(s['img'][1])
             else:
