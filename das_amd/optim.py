@@ -75,6 +75,11 @@ class FlatSGD:
     end of the buffer = the layers backward reaches first), so the collective sequence is identical on all
     ranks whatever the timing."""
 
+    _LAYOUT = ('bias', 'main')      # parameter groups in buffer order
+
+    def _group_of(self, name, p, module_of):
+        return 'bias' if _is_bias_param(name, module_of) else 'main'
+
     def __init__(self, model, lr, momentum=0.9, weight_decay=1e-4, bias_lr_mult=1.0, bias_decay_mult=1.0,
                  max_grad_norm=0.0, bucket_mb=64, overlap=True, force_collectives=False, comm_reserved_cus=None,
                  grad_comm_dtype='f32'):
@@ -92,15 +97,15 @@ class FlatSGD:
             for pname, _ in mod.named_parameters(recurse=False):
                 module_of[(mname + '.' if mname else '') + pname] = mod
         named = [(n, p) for n, p in model.named_parameters() if p.requires_grad]
-        groups = {'main': [], 'bias': []}
+        groups = {k: [] for k in self._LAYOUT}
         for n, p in named:
-            groups['bias' if _is_bias_param(n, module_of) else 'main'].append((n, p))
+            groups[self._group_of(n, p, module_of)].append((n, p))
         dev = named[0][1].device
-        # layout: [bias group | main group]; 4-D tensors start on 64-element boundaries: whole 256-byte f32 /
+        # layout: [bias group | main group] (FlatMuon: | matrices]); 4-D tensors start on 64-element boundaries: whole 256-byte f32 /
         # 128-byte bf16 lines, so that the weight-gradient atomics and the operand loads never straddle lines
         plan, off = [], 0
         bounds = {}
-        for key in ('bias', 'main'):
+        for key in self._LAYOUT:
             start = off
             for n, p in groups[key]:
                 if p.dim() == 4:
@@ -151,6 +156,8 @@ class FlatSGD:
         self.groups = [dict(key='main', start=bounds['main'][0], end=bounds['main'][1], lr_mult=1.0, wd=weight_decay),
                        dict(key='bias', start=bounds['bias'][0], end=bounds['bias'][1], lr_mult=bias_lr_mult,
                             wd=weight_decay * bias_decay_mult)]
+        if 'matrix' in bounds:
+            self.groups.insert(0, dict(key='matrix', start=bounds['matrix'][0], end=bounds['matrix'][1], lr_mult=1.0, wd=weight_decay))
         self.sumsq = torch.zeros(1, dtype=torch.float32, device=dev)
         self.steps = 0
         self._sig = self._param_signature()
@@ -417,14 +424,15 @@ class FlatSGD:
                                   for g in self.groups]
         return self._param_groups
 
-    def step(self, lr=None):
+    def _before_step(self):
+        """-> (gradient scale, sum of squares of the whole gradient or None)"""
         from .autograd import finish_backward
         finish_backward()
         self._check_grad_aliasing()
-        scale = 1.0 / self.world
-        sumsq = None
-        if self.max_grad_norm > 0:
-            sumsq = T.grad_sumsq(self.flat_g, self.sumsq)
+        return 1.0 / self.world, T.grad_sumsq(self.flat_g, self.sumsq) if self.max_grad_norm > 0 else None
+
+    def step(self, lr=None):
+        scale, sumsq = self._before_step()
         for gi, g in enumerate(self.groups):
             if g['end'] == g['start']:
                 continue
@@ -438,11 +446,14 @@ class FlatSGD:
         bump_param_epoch()  # packed bf16 weight copies are rebuilt on the next forward
 
     # ------------------------------------------------------------------ checkpointing
-    def _dense_momentum(self):
-        """name -> momentum buffer as a dense tensor of the parameter's own (OIHW) shape, on the host"""
-        out = {}
+    def _dense_momentum(self, flat=None):
+        """name -> momentum buffer as a dense tensor of the parameter's own (OIHW) shape, on the host (flat: another state
+        buffer of the flat layout; parameters past its end have none)"""
+        out, flat = {}, self.flat_m if flat is None else flat
         for n, p, sl in zip(self._names, self._params, self.slots):
-            m = self.flat_m[sl.off:sl.off + sl.numel]
+            if sl.off + sl.numel > flat.numel():
+                continue
+            m = flat[sl.off:sl.off + sl.numel]
             if sl.cl_shape is not None:
                 O, KH, KW, I = sl.cl_shape
                 m = m.view(O, KH, KW, I).permute(0, 3, 1, 2)
@@ -515,6 +526,165 @@ class FlatSGD:
         return float(torch.sqrt(T.grad_sumsq(self.flat_g)).item()) / self.world
 
 
+def _state_entries(sd, model):
+    """An optimizer state dict in torch's layout -> name -> state entry: parameters are numbered in `named_parameters()` order"""
+    ids = [i for g in sd['param_groups'] for i in g['params']]
+    order = [n for n, _ in model.named_parameters()]
+    if len(ids) != len(order):
+        raise ValueError(f'optimizer state holds {len(ids)} parameters, the model has {len(order)}')
+    st = sd['state']
+    return {n: st.get(i, st.get(str(i))) or {} for n, i in zip(order, ids)}
+
+
+class FlatAdamW(FlatSGD):
+    """AdamW (decoupled weight decay) over the same flat buffers, buckets and hooks as FlatSGD: one fused launch per group and step
+    (das_adamw_step). flat_m holds the first moments, flat_v the second ones. `state_dict()` is torch.optim.AdamW's layout with one
+    param group per parameter, as FlatSGD's is torch.optim.SGD's. The padding of odd shapes stays zero (its gradient, moments and weight
+    are). The step counter is the host's: a step is not for capture into a hipGraph and refuses it."""
+
+    def __init__(self, model, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, bias_lr_mult=1.0, bias_decay_mult=1.0, **kw):
+        b1, b2 = float(betas[0]), float(betas[1])
+        if not (0 <= b1 < 1 and 0 <= b2 < 1 and eps > 0):
+            raise ValueError(f'AdamW: betas in [0, 1) and eps > 0, got {betas} and {eps}')
+        super().__init__(model, lr, momentum=0.0, weight_decay=weight_decay, bias_lr_mult=bias_lr_mult,
+                         bias_decay_mult=bias_decay_mult, **kw)
+        self.betas, self.eps = (b1, b2), float(eps)
+        self.flat_v = torch.zeros(self._adamw_end(), dtype=torch.float32, device=self.flat_p.device)
+
+    def _adamw_end(self):
+        return self.flat_p.numel()
+
+    @property
+    def param_groups(self):
+        if not hasattr(self, '_param_groups'):
+            self._param_groups = [self._group_options(g) for g in self.groups]
+        return self._param_groups
+
+    def _group_options(self, g):
+        lr = self.base_lr * g['lr_mult']
+        return dict(lr=lr, initial_lr=lr, betas=self.betas, eps=self.eps, weight_decay=g['wd'], lr_mult=g['lr_mult'])
+
+    def step(self, lr=None):
+        if self.flat_p.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f'{type(self).__name__}.step: the step count and learning rate live on the host, a replayed graph would '
+                               'repeat them; run the step outside the capture')
+        scale, sumsq = self._before_step()
+        for gi, g in enumerate(self.groups):
+            if g['end'] > g['start']:
+                self._step_group(g, lr * g['lr_mult'] if lr is not None else self.param_groups[gi]['lr'], scale, sumsq)
+        self.steps += 1
+        from .nn import bump_param_epoch
+        bump_param_epoch()
+
+    def _step_group(self, g, lr, scale, sumsq):
+        s, e = g['start'], g['end']
+        T.adamw_step(self.flat_p[s:e], self.flat_g[s:e], self.flat_m[s:e], self.flat_v[s:e], lr, self.steps + 1, beta1=self.betas[0],
+                     beta2=self.betas[1], eps=self.eps, weight_decay=g['wd'], grad_scale=scale, max_norm=self.max_grad_norm,
+                     grad_sumsq_t=sumsq)
+
+    def state_dict(self):
+        first, second = self._dense_momentum(), self._dense_momentum(self.flat_v)
+        main = next(g for g in self.groups if g['key'] == 'main')
+        group_of = {n: g for g in self.groups for n, sl in zip(self._names, self.slots) if g['start'] <= sl.off < g['end']}
+        order = [n for n, _ in self.model.named_parameters()]
+        state, pgs = {}, []
+        for i, n in enumerate(order):
+            g = group_of.get(n, main)      # (frozen: the plain defaults, no state)
+            if self.steps > 0 and n in first:
+                state[i] = dict(momentum_buffer=first[n]) if g['key'] == 'matrix' else \
+                    dict(step=torch.tensor(float(self.steps)), exp_avg=first[n], exp_avg_sq=second[n])
+            opts = self._group_options(g)
+            del opts['lr_mult']
+            pgs.append(dict(opts, params=[i]))
+        return dict(state=state, param_groups=pgs, das_steps=self.steps, das_base_lr=self.base_lr, das_names=order)
+
+    def load_state_dict(self, sd):
+        """This class's layout or torch.optim.AdamW's (one group per parameter or one for all, `named_parameters()` order)."""
+        entries = _state_entries(sd, self.model)
+        steps = {int(e['step']) for e in entries.values() if 'step' in e}
+        if len(steps) > 1:
+            raise ValueError(f'parameters at different steps ({sorted(steps)}): the flat optimizer keeps one step count')
+        matrix = next((g for g in self.groups if g['key'] == 'matrix'), None)
+        for n, p, sl in zip(self._names, self._params, self.slots):
+            e = entries[n]
+            is_matrix = matrix is not None and matrix['start'] <= sl.off < matrix['end']
+            for flat, key in ((self.flat_m, 'momentum_buffer' if is_matrix else 'exp_avg'), (self.flat_v, None if is_matrix else 'exp_avg_sq')):
+                if key is None:
+                    continue
+                if e and key not in e:
+                    raise ValueError(f'optimizer state of {n} has no {key}: written by another optimizer')
+                dst = flat[sl.off:sl.off + sl.numel]
+                if not e:              # (torch creates state at a parameter's first gradient: never stepped = none)
+                    dst.zero_()
+                elif sl.cl_shape is not None:
+                    O, KH, KW, I = sl.cl_shape
+                    dst.view(O, KH, KW, I).copy_(e[key].to(dst.device, torch.float32).permute(0, 2, 3, 1))
+                else:
+                    dst.copy_(e[key].to(dst.device, torch.float32).reshape(-1))
+        self.steps = int(sd.get('das_steps', max(steps) if steps else 0))
+
+
+class FlatMuon(FlatAdamW):
+    """Muon for the weight matrices, AdamW for everything else, over the same flat buffers, buckets and hooks as FlatSGD.
+
+    A matrix is a 2-D weight, or a conv weight as output channels x (taps * input channels): the flat storage holds it as exactly that,
+    dense, so one das_muon_step call updates them all in place (momentum average, Newton-Schulz orthogonalisation, decoupled decay).
+    To AdamW go 1-D parameters, matrices with fewer than `min_side` rows or columns (a row alone would only be normalised: the
+    1- to 3-channel predictors, the flows' coordinates) and names that contain one of `adamw_params`.
+    lr drives the matrices, adamw_lr (default: lr) the rest; a schedule that sets lr scales both. lr_scale: 'original' or
+    'match_rms_adamw' (train_ops.muon_step). `state_dict()`: momentum_buffer for matrices, AdamW's state for the rest.
+    Several ranks: every rank updates every matrix from the summed gradient, to the same bits."""
+
+    _LAYOUT = ('bias', 'main', 'matrix')
+
+    def __init__(self, model, lr, momentum=0.95, weight_decay=1e-2, nesterov=True, ns_steps=5, ns_coefficients=T.NS_COEFFICIENTS,
+                 ns_eps=1e-7, lr_scale='original', min_side=8, adamw_params=(), adamw_lr=None, betas=(0.9, 0.999), eps=1e-8,
+                 adamw_weight_decay=None, bias_lr_mult=1.0, bias_decay_mult=1.0, **kw):
+        if not 0 <= momentum < 1 or lr_scale not in ('original', 'match_rms_adamw') or not lr > 0:
+            raise ValueError(f"Muon: lr > 0, momentum in [0, 1), lr_scale 'original' or 'match_rms_adamw'; got {lr}, {momentum}, {lr_scale!r}")
+        self._min_side, self._adamw_names = int(min_side), tuple(adamw_params)
+        ratio = 1.0 if adamw_lr is None else adamw_lr / lr
+        rest_wd = weight_decay if adamw_weight_decay is None else adamw_weight_decay
+        super().__init__(model, lr, betas=betas, eps=eps, weight_decay=rest_wd, bias_lr_mult=ratio * bias_lr_mult,
+                         bias_decay_mult=bias_decay_mult, **kw)
+        self.momentum, self.nesterov, self.lr_scale = momentum, bool(nesterov), lr_scale
+        self._ns = dict(steps=ns_steps, coefficients=ns_coefficients, eps=ns_eps)
+        self._plan = None
+        for g in self.groups:
+            if g['key'] == 'matrix':
+                g['wd'] = weight_decay
+            elif g['key'] == 'main':
+                g['lr_mult'] = ratio
+
+    @staticmethod
+    def _matrix(p):
+        return (p.shape[0], p.numel() // p.shape[0]) if p.dim() in (2, 4) and p.numel() else None
+
+    def _group_of(self, name, p, module_of):
+        m = self._matrix(p)
+        if m is not None and min(m) >= max(1, self._min_side) and not any(a in name for a in self._adamw_names):
+            return 'matrix'
+        return super()._group_of(name, p, module_of)
+
+    def _adamw_end(self):
+        return next(g for g in self.groups if g['key'] == 'matrix')['start']
+
+    def _group_options(self, g):
+        if g['key'] != 'matrix':
+            return super()._group_options(g)
+        return dict(lr=self.base_lr, initial_lr=self.base_lr, momentum=self.momentum, nesterov=self.nesterov, weight_decay=g['wd'],
+                    lr_mult=1.0)
+
+    def _step_group(self, g, lr, scale, sumsq):
+        if g['key'] != 'matrix':
+            return super()._step_group(g, lr, scale, sumsq)
+        if self._plan is None:
+            mats = [(self._matrix(p), sl.off) for p, sl in zip(self._params, self.slots) if g['start'] <= sl.off < g['end']]
+            self._plan = T.NewtonSchulzPlan([m for m, _ in mats], self.flat_p.device, offsets=[o for _, o in mats], **self._ns)
+        T.muon_step(self.flat_p, self.flat_g, self.flat_m, self._plan, lr, momentum=self.momentum, weight_decay=g['wd'],
+                    nesterov=self.nesterov, lr_scale=self.lr_scale, grad_scale=scale, max_norm=self.max_grad_norm, grad_sumsq_t=sumsq)
+
+
 def step_lr(base_lr, epoch, it, steps=(16, 20), gamma=0.1, warmup_iters=250, warmup_ratio=1.0 / 3):
     """mmcv StepLrUpdaterHook with linear warm-up: lr_it = lr*(1 - (1 - it/warm)*(1 - ratio))."""
     lr = base_lr * (gamma ** sum(1 for s in steps if epoch >= s))
@@ -524,14 +694,28 @@ def step_lr(base_lr, epoch, it, steps=(16, 20), gamma=0.1, warmup_iters=250, war
 
 
 def build_optimizer(model, cfg, optimizer_config=None):
-    """build_optimizer(model, cfg) with the whole config, or — the reference's call shape (mmdet3d/apis/train.py
+    """cfg.optimizer type 'SGD' (FlatSGD), 'AdamW' (FlatAdamW) or 'Muon' (FlatMuon).
+    build_optimizer(model, cfg) with the whole config, or — the reference's call shape (mmdet3d/apis/train.py
     via mmcv `build_optimizer(model, cfg.optimizer)`) — build_optimizer(model, cfg.optimizer, cfg.optimizer_config)."""
     if 'optimizer' not in cfg and ('type' in cfg or 'lr' in cfg):
         cfg = dict(optimizer=cfg, optimizer_config=optimizer_config or {})
     opt = dict(cfg.get('optimizer', {}))
-    assert opt.get('type', 'SGD') == 'SGD'
+    kind = opt.pop('type', 'SGD')
     pw = opt.get('paramwise_cfg', {}) or {}
     clip = (cfg.get('optimizer_config', {}) or {}).get('grad_clip') or {}
+    if kind in ('AdamW', 'Muon'):
+        cls = FlatAdamW if kind == 'AdamW' else FlatMuon
+        opt.pop('paramwise_cfg', None)
+        names = {'lr', 'betas', 'eps', 'weight_decay'}
+        if kind == 'Muon':
+            names |= {'momentum', 'nesterov', 'ns_steps', 'ns_coefficients', 'ns_eps', 'lr_scale', 'min_side', 'adamw_params', 'adamw_lr',
+                      'adamw_weight_decay'}
+        odd = [k for k in opt if k not in names] + [k for k in pw if k not in ('bias_lr_mult', 'bias_decay_mult')]
+        if odd or 'lr' not in opt:
+            raise ValueError(f'optimizer {kind}: ' + (f'unknown options {odd}' if odd else 'lr is missing'))
+        return cls(model, bias_lr_mult=pw.get('bias_lr_mult', 1.0), bias_decay_mult=pw.get('bias_decay_mult', 1.0),
+                   max_grad_norm=clip.get('max_norm', 0.0), **opt)
+    assert kind == 'SGD', kind
     return FlatSGD(model, lr=opt.get('lr', 0.02), momentum=opt.get('momentum', 0.9),
                    weight_decay=opt.get('weight_decay', 1e-4), bias_lr_mult=pw.get('bias_lr_mult', 1.0),
                    bias_decay_mult=pw.get('bias_decay_mult', 1.0), max_grad_norm=clip.get('max_norm', 0.0))

@@ -25,7 +25,8 @@ def gradient(r, c, seed, k=None):
 
 
 def norm2(x):
-    return float(torch.linalg.matrix_norm(x, 2))
+    g = (x @ x.T if x.shape[0] <= x.shape[1] else x.T @ x).cpu()
+    return math.sqrt(max(0.0, float(torch.linalg.eigvalsh((g + g.T) / 2)[-1])))
 
 
 def ns64(u, coef, eps=1e-7, pairs=False):
@@ -357,3 +358,173 @@ def test_refusals():
         with pytest.raises(DasHipError):
             bad()
     assert (f == 1).all() and (u == 1).all()
+
+
+# ------------------------------------------------------------------ the optimizers in a training run
+def detector():
+    from test_train_step_gpu import make
+    return make('f32')
+
+
+@pytest.mark.parametrize('kind', ['AdamW', 'Muon'])
+def test_optimizer_steps_follow_the_formulas(kind):
+    """Two training steps of a small detector: every parameter against the 64-bit formula applied to the gradients the step saw, clipping
+    and the bias rules included; the flat storage's padding stays zero."""
+    from das_amd.optim import build_optimizer
+    model, data = detector()
+    cfg = dict(optimizer=dict(type=kind, lr=0.01, weight_decay=0.1, paramwise_cfg=dict(bias_lr_mult=2., bias_decay_mult=0.)),
+               optimizer_config=dict(grad_clip=dict(max_norm=35, norm_type=2)))
+    if kind == 'Muon':
+        cfg['optimizer'].update(momentum=0.9, adamw_lr=1e-3)
+    opt = build_optimizer(model, cfg)
+    names = dict(zip(opt._names, zip(opt._params, opt.slots)))
+    m64 = {n: torch.zeros(sl.numel, dtype=torch.float64, device=DEV) for n, (p, sl) in names.items()}
+    v64 = {n: torch.zeros(sl.numel, dtype=torch.float64, device=DEV) for n, (p, sl) in names.items()}
+    p_err = {n: 0.0 for n in names}
+    groups = {n: next(g for g in opt.groups if g['start'] <= sl.off < g['end']) for n, (p, sl) in names.items()}
+    if kind == 'Muon':
+        assert sum(g['key'] == 'matrix' for g in groups.values()) > 20
+        assert groups['bbox_head.conv_cls.weight']['key'] == 'main' and groups['backbone.top.top.0.conv.weight']['key'] == 'matrix'
+    u = 2.0 ** -24
+    for step in (1, 2):
+        opt.zero_grad()
+        model.train_step(data, None)['loss'].backward()
+        opt.all_reduce_grads()
+        norm = float(opt.flat_g.double().norm())
+        k = min(1.0, 35 / (norm + 1e-6))
+        before, g0 = opt.flat_p.clone(), opt.flat_g.clone()
+        opt.step(0.01)
+        for n, (p, sl) in names.items():
+            s, g = slice(sl.off, sl.off + sl.numel), groups[n]
+            lr, wd = 0.01 * g['lr_mult'], g['wd']
+            gd, pd, got = g0[s].double() * k, before[s].double(), opt.flat_p[s].double()
+            clip = 2.0 ** -17       # (the f32 sum of squares over the whole gradient)
+            if g['key'] == 'matrix':
+                m64[n] = 0.9 * m64[n] + 0.1 * gd
+                r, c = p.shape[0], p.numel() // p.shape[0]
+                w = 0.1 * gd + 0.9 * m64[n]
+                x, err = ns64(w.view(r, c), [COEF] * 5, pairs=True)
+                f = math.sqrt(max(1.0, r / c))
+                want = pd * (1 - lr * wd) - lr * f * x.reshape(-1)
+                # the input itself carries the clip factor's and the momentum's rounding: a relative error of U's norm, times L^5 <= 3.4445^5
+                lim = lr * f * (1.1 * err + 485 * 16 * u) + 4 * u * float(pd.norm())
+                assert float((got - want).norm()) <= lim, (n, step)
+            else:
+                m64[n] = 0.9 * m64[n] + 0.1 * gd
+                v64[n] = 0.999 * v64[n] + 0.001 * gd * gd
+                den = (v64[n] / (1 - 0.999 ** step)).sqrt() + 1e-8
+                upd = (m64[n] / (1 - 0.9 ** step)) / den
+                want = pd * (1 - lr * wd) - lr * upd
+                # moments carry `clip` relative errors of their terms (|m| terms up to 2 |g| / den); the division and the root a few u
+                lim = 8 * u * pd.abs() + lr * (64 * u + 4 * clip) * (upd.abs() + 2 * gd.abs() / den + 1)
+                assert ((got - want).abs() <= lim).all(), (n, step)
+        for n, (p, sl) in names.items():
+            assert not opt.flat_p[sl.off + sl.numel:sl.off + sl.span].any()
+    assert all(torch.isfinite(p).all() for p in model.parameters())
+
+
+@pytest.mark.parametrize('kind', ['AdamW', 'Muon'])
+def test_optimizer_resumes_bit_for_bit(kind):
+    """state dict -> a fresh optimizer: same state, and the next step from the same parameters and gradients gives the same bits"""
+    from das_amd.optim import build_optimizer, train_iteration
+    cfg = dict(type=kind, lr=2e-3, weight_decay=0.01)
+    model, data = detector()
+    opt = build_optimizer(model, cfg)
+    for _ in range(2):
+        train_iteration(model, opt, data, 2e-3)
+    other, _ = detector()
+    other.load_state_dict(model.state_dict())
+    opt2 = build_optimizer(other, cfg)
+    opt2.load_state_dict(opt.state_dict())
+    assert opt2.steps == 2 and torch.equal(opt2.flat_m, opt.flat_m) and torch.equal(opt2.flat_v, opt.flat_v)
+    assert torch.equal(opt2.flat_p, opt.flat_p)
+    opt2.flat_g.copy_(opt.flat_g)
+    opt.step()
+    opt2.step()
+    assert torch.equal(opt2.flat_p, opt.flat_p) and torch.equal(opt2.flat_m, opt.flat_m)
+    assert torch.isfinite(opt.flat_p).all()
+
+
+def test_optimizer_refuses_capture():
+    from das_amd.optim import FlatAdamW
+    net = torch.nn.Linear(16, 16).to(DEV)
+    opt = FlatAdamW(net, lr=1e-3)
+    before = opt.flat_p.clone()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        scratch = torch.zeros(4, device=DEV)
+        with pytest.raises(RuntimeError):
+            opt.step()
+    assert opt.steps == 0 and torch.equal(opt.flat_p, before) and scratch.numel() == 4
+    opt.step()
+    assert opt.steps == 1
+
+
+def test_steps_replay_in_a_graph():
+    """the functional steps captured, with their fixed scalars: every replay equals the eager call, with eager work in between"""
+    from das_amd import train_ops as T
+    shapes = [(2, 130, 200), (3, 20, 30)]
+    n = sum(k * r * c for k, r, c in shapes)
+    gen = torch.Generator().manual_seed(0)
+    p, g, m, v = (torch.randn(n, generator=gen).to(DEV) for _ in range(4))
+    v = v * v
+    plan = T.NewtonSchulzPlan(shapes, DEV)
+    a, b = [t.clone() for t in (p, g, m, v)], [t.clone() for t in (p, g, m, v)]
+
+    def both(p, g, m, v):
+        T.muon_step(p, g, m, plan, lr=1e-2, weight_decay=0.1)
+        T.adamw_step(p, g, m, v, lr=1e-3, step=3)
+    graph = torch.cuda.CUDAGraph()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        both(*[t.clone() for t in a])
+    torch.cuda.current_stream().wait_stream(s)
+    with torch.cuda.graph(graph):
+        both(*a)
+    for i in range(4):
+        graph.replay()
+        both(*b)
+        torch.cuda.synchronize()
+        for x, y in zip(a, b):
+            assert torch.equal(x, y), i
+        a[1].mul_(1.5)
+        b[1].mul_(1.5)
+
+
+def test_large_offsets():
+    """matrices past 2^31 bytes of a flat buffer"""
+    from das_amd import train_ops as T
+    far = (1 << 29) + 8 * 12345        # elements: 2 GiB and some
+    shapes, offsets = [(1, 100, 70), (1, 80, 300)], [far, far + 7000]
+    n = far + 7000 + 24000
+    p, g, m = (torch.zeros(n, device=DEV) for _ in range(3))
+    gen = torch.Generator().manual_seed(2)
+    tail = [torch.randn(31000, generator=gen).to(DEV) for _ in range(3)]
+    for t, x in zip((p, g, m), tail):
+        t[far:] = x
+    T.muon_step(p, g, m, T.NewtonSchulzPlan(shapes, DEV, offsets=offsets), lr=0.1)
+    near = [t.clone() for t in tail]
+    T.muon_step(*near, T.NewtonSchulzPlan(shapes, DEV), lr=0.1)
+    for t, x in zip((p, g, m), near):
+        assert torch.equal(t[far:], x) and not t[:far].any()
+
+
+def test_train_cli_with_muon(tmp_path):
+    """tools/train.py with optimizer.type=Muon: trains, checkpoints, resumes"""
+    import os
+    from test_cli_gpu import run
+    work = str(tmp_path / 'w')
+    args = ['model.backbone.num_stages=1', 'data.samples_per_gpu=2', 'data.train.type=SyntheticPoseDataset', 'data.train.length=4',
+            'data.train.img_shape=(128,192)', 'log_config.interval=1', 'optimizer.type=Muon', 'optimizer.adamw_lr=0.0005',
+            'optimizer.momentum=0.95']
+    run('tools/train.py', 'configs/das/exp_panoptic.py', '--work-dir', work, '--no-validate', '--cfg-options', *args, 'runner.max_epochs=1')
+    ck = os.path.join(work, 'epoch_1.pth')
+    sd = torch.load(ck, map_location='cpu', weights_only=False)['optimizer']
+    i = sd['das_names'].index('backbone.top.top.0.conv.weight')
+    assert sd['das_steps'] == 2 and sd['state'][i]['momentum_buffer'].shape == (64, 3, 7, 7)
+    out = run('tools/train.py', 'configs/das/exp_panoptic.py', '--work-dir', work, '--no-validate', '--resume-from', ck, '--cfg-options',
+              *args, 'runner.max_epochs=2')
+    assert 'Epoch [2]' in out and 'nan' not in out
+    sd = torch.load(os.path.join(work, 'epoch_2.pth'), map_location='cpu', weights_only=False)['optimizer']
+    assert sd['das_steps'] == 4
