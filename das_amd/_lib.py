@@ -75,10 +75,12 @@ class DasNsShape(C.Structure):
 
 
 class DasNsPlan(C.Structure):
-    _fields_ = [(k, i32) for k in ('n_groups', 'n_matrices', 'n_small', 'small_n', 'n_chunks', 'n_gram', 'n_gram_join',
-                                   'n_product', 'n_product_join', 'n_update', 'steps', 'product_tile', 'update_tile', 'gram_kg')] + \
-               [(k, i64) for k in ('x_elems', 'a_elems', 'gram_slots', 'product_slots', 'extent', 'mat_at', 'chunk_at', 'gram_at',
-                                   'gram_join_at', 'product_at', 'product_join_at', 'update_at', 'table_bytes')] + \
+    _fields_ = [(k, i32) for k in ('n_groups', 'n_matrices', 'n_small', 'small_lds', 'n_thin', 'n_slices', 'n_chunks', 'n_tile_chunks',
+                                   'n_gram', 'n_gram_join', 'n_product', 'n_product_join', 'n_update', 'steps', 'product_tile',
+                                   'update_tile', 'gram_kg')] + \
+               [(k, i64) for k in ('x_elems', 'a_elems', 'thin_x_elems', 'thin_a_elems', 'thin_slots', 'gram_slots', 'product_slots',
+                                   'extent', 'mat_at', 'chunk_at', 'gram_at', 'gram_join_at', 'product_at', 'product_join_at',
+                                   'update_at', 'slice_at', 'thin_at', 'table_bytes')] + \
                [('coef', f32 * (3 * DAS_NS_MAX_STEPS)), ('phase_end', i32 * DAS_NS_MAX_STEPS), ('eps', f32)]
 
 

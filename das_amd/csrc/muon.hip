@@ -47,6 +47,7 @@ struct NsMatrix {           // one matrix, as the kernels see it
   int chunk0, chunks;       // its blocks in the partial-sum table
   float scale, gscale;      // S; what G is kept times
   int tall;                 // rows > cols: X holds the transpose
+  int thin;                 // m <= 64, too long for one workgroup: X and Q are in areas of their own, as pairs
 };
 struct NsItem {             // a workgroup's share: output tile (ti, tj) of a matrix, inner elements 64 k0 ... 64 (k0 + kn)
   int matrix, ti, tj, k0, kn;
@@ -141,7 +142,7 @@ __device__ __forceinline__ float load_as_f32(const void* base, long long i) {
 // of any magnitude inside f16's range until the norm is known; normalise_kernel rounds a second time.
 template <typename T, bool MUON, bool SPLIT>
 __global__ __launch_bounds__(TPB) void ingest_kernel(const NsMatrix* __restrict__ mats, const int4* __restrict__ chunks, Sources src,
-                                                     MuonIn mu, _Float16* __restrict__ X, Partial* __restrict__ part) {
+                                                     MuonIn mu, _Float16* __restrict__ X, _Float16* __restrict__ XT, Partial* __restrict__ part) {
   __shared__ float tile[CHUNK][CHUNK + 1];
   __shared__ float red[4];
   const int4 ch = chunks[blockIdx.x];
@@ -253,7 +254,8 @@ __global__ __launch_bounds__(TPB) void ingest_kernel(const NsMatrix* __restrict_
   for (int k = 0; k < 4; ++k) {
     const int r = x_r0 + rr + k * 16;
     if (r >= M.m) continue;
-    put<SPLIT>(X + (SPLIT ? 2 : 1) * M.x, M.ldx, r, x_c0 + c4, u[k]);
+    if (SPLIT || M.thin) put<true>((M.thin ? XT : X) + 2 * M.x, M.ldx, r, x_c0 + c4, u[k]);
+    else put<false>(X + M.x, M.ldx, r, x_c0 + c4, u[k]);
   }
 }
 
@@ -713,32 +715,43 @@ __global__ __launch_bounds__(KG * TPB, KG == 1 ? 2 : KG) void update_kernel(cons
   }
 }
 
-// ------------------------------------------------------------------ small matrices
-// m <= 64, n <= 256: the whole of it in one workgroup, everything between the caller's reads and writes in LDS (pairs of f16 whatever the
-// result's type: the products are a microsecond). A launch for every product would cost 4 us each; 64 x 64: 67 us as 17 launches.
-// X is 64 x NMAX, G, R, Z and two Q are 64 x 64, rows and columns past the matrix are zero, row pitches are 16 bytes past a multiple of the
-// banks' width. 32 columns of X take 128 bytes as f16 pairs and as floats: U and the result use the same place.
-constexpr int SMALL_M = 64, SMALL_N = 256;
+// ------------------------------------------------------------------ small and thin matrices
+// Matrices with m <= 64 take the pairs of f16 of f32 results whatever the result's type: their products are a microsecond, and few rows
+// do not average the roundings of plain f16 (2 x 2000: 3.5e-3).
+//
+// small_kernel: the whole of a matrix in one workgroup, everything between the caller's reads and writes in LDS, where it fits (64 x 256,
+// 16 x 1856). A launch for every product would cost 4 us each; 64 x 64: 67 us as 17 launches.
+// thin_kernel / chain_kernel: longer ones, by slices of their columns. X X^T is summed over the slices' parts by chain_kernel, which takes
+// all steps of a phase on the m x m matrices in LDS and leaves Q; the pass over the slices that forms Q X also forms the parts of the next
+// X X^T: five launches after the first pass (16 x 1056 by tiles: 85 us).
+//
+// 16 waves, one 16 x 16 fragment of an m x m product each; where m <= 32 leaves waves over they divide long inner axes. LDS matrices: rows of
+// pairs (32 high parts, 32 low parts, ...), row pitch 16 bytes past a multiple of 256; 32 columns of X take 128 bytes as pairs and as floats:
+// U, X and the result use the same place. Rows and columns up to the next multiple of 16 are zero.
+constexpr int SMALL_M = 64, SMALL_TPB = 1024, SMALL_LDS = 155 * 1024;
 constexpr int PA = 2 * SMALL_M + 8;   // row pitch of the m x m matrices, f16 elements
+constexpr int SMALL_QUADS = 8;        // float4 of U, and 16 x 16 fragments of X, a thread / wave can have: m n <= 32 Ki
 struct Steps {
   float coef[3 * DAS_NS_MAX_STEPS];
   int end[DAS_NS_MAX_STEPS];          // of the phase that starts at this step
   int steps;
   float eps;
 };
-
-constexpr int SMALL_TPB = 1024;       // 16 waves, a 16 x 16 fragment of every 64 x 64 product each: latencies overlap (four waves: 19 us for 64 x 64)
+__host__ __device__ inline int up16(int m) { return (m + 15) & ~15; }
+__host__ __device__ inline int up64(int n) { return (n + 63) & ~63; }
+// X, the m x m matrices, and room for the shares of a sum (not over the m x m matrices: m <= 16 reads 32 columns of them, 16 of them zero)
+inline long long small_lds(int m, int n) { return 2LL * up16(m) * (2 * up64(n) + 8 + N_AREAS * PA) + (m <= 32 ? SMALL_TPB * 16 : 0); }
 
 __device__ __forceinline__ f16x8_t row_frag(const _Float16* p, int pitch, int row0, int k, int part) {
   const int lane = threadIdx.x & 63;
   return *reinterpret_cast<const f16x8_t*>(p + (row0 + (lane & 15)) * pitch + k * 64 + part * 32 + (lane >> 4) * 8);
 }
-__device__ __forceinline__ f16x8_t col_frag(const _Float16* x, int pitch, int col0, int k, int part) {
+__device__ __forceinline__ f16x8_t col_frag(const _Float16* x, int pitch, int rows, int col0, int k, int part) {
   const int lane = threadIdx.x & 63, q = lane & 15, c = col0 + (q & 3) * 4;
   f16x8_t f;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const int r = k * 32 + (lane >> 4) * 8 + h * 4 + (q >> 2);
+    const int r = min(k * 32 + (lane >> 4) * 8 + h * 4 + (q >> 2), rows - 1);   // (rows past the end meet zeros of the other operand)
     const f16x4_t v = __builtin_bit_cast(
         f16x4_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4_t*)(x + r * pitch + (c >> 5) * 64 + part * 32 + (c & 31))));
 #pragma unroll
@@ -746,17 +759,17 @@ __device__ __forceinline__ f16x8_t col_frag(const _Float16* x, int pitch, int co
   }
   return f;
 }
-// the wave's 16 x 16 of P rows x (Q rows, or columns of Q from col0 on): k32 inner steps of 32
+// 16 x 16 of P's rows from row0 by (Q's rows from q0, or its columns from q0), inner steps of 32: k0, k0 + stride, ... < k1
 template <bool COLS>
-__device__ __forceinline__ f32x4_t small_product(const _Float16* p, int pp, const _Float16* q, int qp, int col0, int k32) {
-  const int wave = threadIdx.x >> 6, wr = (wave >> 2) * 16, wc = (wave & 3) * 16;
+__device__ __forceinline__ f32x4_t frag_product(const _Float16* p, int pp, int row0, const _Float16* q, int qp, int q_rows, int q0, int k0, int k1,
+                                                int stride) {
   f32x4_t high = {0.f, 0.f, 0.f, 0.f}, low = {0.f, 0.f, 0.f, 0.f};   // (two chains)
-  for (int k = 0; k < k32; ++k) {
+  for (int k = k0; k < k1; k += stride) {
     f16x8_t fa[2], fb[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      fa[u] = row_frag(p, pp, wr, k, u);
-      fb[u] = COLS ? col_frag(q, qp, col0 + wc, k, u) : row_frag(q, qp, wc, k, u);
+      fa[u] = row_frag(p, pp, row0, k, u);
+      fb[u] = COLS ? col_frag(q, qp, q_rows, q0, k, u) : row_frag(q, qp, q0, k, u);
     }
     high = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa[0], fb[0], high, 0, 0, 0);
     low = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa[1], fb[0], low, 0, 0, 0);
@@ -774,34 +787,109 @@ __device__ __forceinline__ void put4(_Float16* p, const float (&v)[4]) {
   *reinterpret_cast<f16x4_t*>(p) = h;
   *reinterpret_cast<f16x4_t*>(p + 32) = l;
 }
+__device__ __forceinline__ int pair_at(int pitch, int r, int c) { return r * pitch + (c >> 5) * 64 + (c & 31); }
+
+// Which fragment of an m16 x m16 matrix a wave has, and which share of a long inner axis
+struct Share {
+  int i, j, part, parts;
+  bool on;
+  __device__ explicit Share(int m16) {
+    const int w = threadIdx.x >> 6, n = m16 >> 4, f = n * n;
+    parts = f <= 4 ? 16 / f : 1;
+    on = w < f * parts;
+    part = w / f;
+    i = (w % f) / n;
+    j = w % n;
+  }
+};
 // a symmetric result, stored transposed (four values of a lane are neighbours then): f(row, col, four values) may change them
 template <typename F>
-__device__ __forceinline__ void small_store(f32x4_t acc, _Float16* out, F f) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int r = (wave & 3) * 16 + (lane & 15), c = (wave >> 2) * 16 + (lane >> 4) * 4;
+__device__ __forceinline__ void frag_store(const Share& w, f32x4_t acc, _Float16* out, F f) {
+  const int lane = threadIdx.x & 63, r = w.j * 16 + (lane & 15), c = w.i * 16 + (lane >> 4) * 4;
   float v[4] = {acc[0], acc[1], acc[2], acc[3]};
   f(r, c, v);
-  put4(out + r * PA + (c >> 5) * 64 + (c & 31), v);
+  put4(out + pair_at(PA, r, c), v);
+}
+// The shares of a sum over a long inner axis, added in order and stored as G; scratch: 16 KiB of LDS outside G and the operands, and the
+// caller's barrier before its next use
+__device__ __forceinline__ void store_gram(const Share& w, f32x4_t acc, f32x4_t* scratch, _Float16* G, float scale) {
+  if (w.parts > 1) {
+    scratch[threadIdx.x] = acc;
+    __syncthreads();
+    if (w.part == 0)
+      for (int s = 1; s < w.parts; ++s) acc += scratch[s * (SMALL_TPB / w.parts) + threadIdx.x];
+  }
+  if (w.on && w.part == 0)
+    frag_store(w, acc, G, [&](int, int, float (&v)[4]) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) v[t] *= scale;
+    });
+  __syncthreads();
+}
+// Steps k ... end - 1 on the m x m matrices (the same products as iterate<true>), G in A[0]; -> Q
+__device__ __forceinline__ _Float16* phase_chain(const Share& w, _Float16* const (&A)[N_AREAS], const Steps& st, int k, int end, float gscale, int m16) {
+  const int k32 = (m16 + 31) >> 5;
+  const bool on = w.on && w.part == 0;
+  _Float16 *G = A[0], *R = A[1], *Z = A[2], *q = nullptr, *spare = A[3], *other = A[4];
+  auto plain = [](int, int, float (&)[4]) {};
+  auto product = [&](const _Float16* p, const _Float16* x) { return frag_product<false>(p, PA, w.i * 16, x, PA, 0, w.j * 16, 0, k32, 1); };
+  for (int j = k; j < end; ++j) {
+    const float ca = st.coef[3 * j], cb = st.coef[3 * j + 1] / gscale, cc = st.coef[3 * j + 2] / (gscale * gscale);
+    _Float16* z = q ? Z : spare;
+    if (on)
+      frag_store(w, product(G, G), z, [&](int r, int c, float (&v)[4]) {
+        const _Float16* g = G + pair_at(PA, r, c);
+        const f16x4_t h = *reinterpret_cast<const f16x4_t*>(g), l = *reinterpret_cast<const f16x4_t*>(g + 32);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) v[t] = cc * v[t] + cb * ((float)h[t] + (float)l[t]) + (r == c + t ? ca : 0.f);
+      });
+    __syncthreads();
+    if (on && q) frag_store(w, product(z, q), other, plain);
+    if (on && j + 1 < end) frag_store(w, product(z, G), R, plain);
+    __syncthreads();
+    if (q) {
+      _Float16* t = q;
+      q = other;
+      other = t;
+    } else {
+      q = z;
+    }
+    if (j + 1 < end) {
+      if (on) frag_store(w, product(R, z), G, plain);       // (nobody reads G any more)
+      __syncthreads();
+    }
+  }
+  return q;
+}
+__device__ __forceinline__ void zero_lds(void* p, int bytes, int threads) {
+  for (int i = threadIdx.x; i < bytes / 16; i += threads) reinterpret_cast<uint4*>(p)[i] = make_uint4(0, 0, 0, 0);
+}
+// result element o = old value of a parameter, x = f X
+template <bool MUON>
+__device__ __forceinline__ void emit_one(const Result& res, long long o, float x, float old) {
+  if constexpr (MUON) res.p[o] = res.keep * old - x;
+  else if (res.out_dtype == DAS_F32) reinterpret_cast<float*>(res.out)[o] = x;
+  else reinterpret_cast<uint16_t*>(res.out)[o] = res.out_dtype == DAS_BF16 ? f32_to_bf16(x) : __builtin_bit_cast(uint16_t, (_Float16)x);
 }
 
-template <typename T, bool MUON, int NMAX>
+template <typename T, bool MUON>
 __global__ __launch_bounds__(SMALL_TPB) void small_kernel(const NsMatrix* __restrict__ mats, Sources src, MuonIn mu, Steps st, Result res) {
   extern __shared__ __align__(16) char smem[];
   __shared__ float red[SMALL_TPB / 64];
   __shared__ double redd[SMALL_TPB / 64];
-  constexpr int PX = 2 * NMAX + 8, PF = NMAX + 4;   // X's row pitch in f16 elements and in floats
   const NsMatrix M = mats[blockIdx.x];
   if (!MUON && (unsigned)(M.group - src.first) >= (unsigned)src.count) return;   // (whole workgroups)
+  const int m16 = up16(M.m), n64 = up64(M.n), PX = 2 * n64 + 8, PF = n64 + 4;   // X's row pitch in f16 elements and in floats
   _Float16* X = reinterpret_cast<_Float16*>(smem);
   float* U = reinterpret_cast<float*>(smem);
   _Float16* A[N_AREAS];
 #pragma unroll
-  for (int i = 0; i < N_AREAS; ++i) A[i] = X + SMALL_M * PX + i * SMALL_M * PA;
+  for (int i = 0; i < N_AREAS; ++i) A[i] = X + m16 * (PX + i * PA);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 
-  // U, zeros around it. The loads go out first.
+  // U, zeros around it and in the m x m matrices. The first loads go out before.
   const int count = M.rows * M.cols;
-  const float per_row = 1.f / (float)M.cols;   // (index + 1/2) / cols is exact enough to truncate for indices under 2^14
+  const float per_row = 1.f / (float)M.cols;   // (index + 1/2) / cols is exact enough to truncate for indices under 2^20
   constexpr int BATCH = 4;                     // loads in flight per thread: a load a time is a memory latency each
   float big = 0.f, coef = 1.f;
   if constexpr (MUON) coef = grad_factor(mu);
@@ -822,7 +910,7 @@ __global__ __launch_bounds__(SMALL_TPB) void small_kernel(const NsMatrix* __rest
       }
     }
     if (i0 < SMALL_TPB) {
-      for (int i = threadIdx.x; i < SMALL_M * PF / 4; i += SMALL_TPB) reinterpret_cast<float4*>(U)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      zero_lds(smem, 2 * m16 * (PX + N_AREAS * PA), SMALL_TPB);
       __syncthreads();
     }
 #pragma unroll
@@ -845,11 +933,13 @@ __global__ __launch_bounds__(SMALL_TPB) void small_kernel(const NsMatrix* __rest
   for (int i = 0; i < SMALL_TPB / 64; ++i) big = fmaxf(big, red[i]);
   int e = 0;
   if (big > 0.f && big <= 3.4028235e38f) (void)frexpf(big, &e);
-  float v[NMAX / 64][4], ss = 0.f;
-  const int row = threadIdx.x >> 4, c4 = (threadIdx.x & 15) * 4;
+  float v[SMALL_QUADS][4], ss = 0.f;
+  const int quads = m16 * n64 / 4, per = n64 / 4;
 #pragma unroll
-  for (int b = 0; b < NMAX / 64; ++b) {
-    const float4 w = *reinterpret_cast<const float4*>(U + row * PF + b * 64 + c4);
+  for (int b = 0; b < SMALL_QUADS; ++b) {
+    const int i = threadIdx.x + b * SMALL_TPB, r = i / per;
+    if (i >= quads) continue;
+    const float4 w = *reinterpret_cast<const float4*>(U + r * PF + (i - r * per) * 4);
     v[b][0] = ldexpf(w.x, -e); v[b][1] = ldexpf(w.y, -e); v[b][2] = ldexpf(w.z, -e); v[b][3] = ldexpf(w.w, -e);
 #pragma unroll
     for (int k = 0; k < 4; ++k) ss += v[b][k] * v[b][k];
@@ -864,70 +954,47 @@ __global__ __launch_bounds__(SMALL_TPB) void small_kernel(const NsMatrix* __rest
   for (int i = 0; i < SMALL_TPB / 64; ++i) sum += redd[i];
   const float f = (float)ldexp((double)M.scale / (ldexp(sqrt(sum), e) + (double)st.eps), e);
 #pragma unroll
-  for (int b = 0; b < NMAX / 64; ++b) {
+  for (int b = 0; b < SMALL_QUADS; ++b) {
+    const int i = threadIdx.x + b * SMALL_TPB, r = i / per;
+    if (i >= quads) continue;
 #pragma unroll
     for (int k = 0; k < 4; ++k) v[b][k] *= f;
-    put4(X + row * PX + b * 128 + (c4 >> 5) * 64 + (c4 & 31), v[b]);
+    put4(X + pair_at(PX, r, (i - r * per) * 4), v[b]);
   }
   __syncthreads();
 
-  // the phases of iterate<true>
-  const int n32 = (M.n + 31) / 32, tiles = (M.n + 63) / 64;
-  auto plain = [](int, int, float (&)[4]) {};
+  const Share w(m16);
+  const int n = m16 >> 4, cols = n64 >> 4, k32 = (m16 + 31) >> 5;
+  const float gs = M.gscale / (M.scale * M.scale);
   for (int k = 0; k < st.steps;) {
     const int end = st.end[k];
-    const float gs = M.gscale / (M.scale * M.scale);
-    _Float16 *G = A[0], *R = A[1], *Z = A[2], *q = nullptr, *spare = A[3], *other = A[4];
-    small_store(small_product<false>(X, PX, X, PX, 0, n32), G, [&](int, int, float (&w)[4]) {
-#pragma unroll
-      for (int t = 0; t < 4; ++t) w[t] *= gs;
-    });
-    __syncthreads();
-    for (int j = k; j < end; ++j) {
-      const float ca = st.coef[3 * j], cb = st.coef[3 * j + 1] / M.gscale, cc = st.coef[3 * j + 2] / (M.gscale * M.gscale);
-      _Float16* z = q ? Z : spare;
-      small_store(small_product<false>(G, PA, G, PA, 0, 2), z, [&](int r, int c, float (&w)[4]) {
-        const _Float16* g = G + r * PA + (c >> 5) * 64 + (c & 31);
-        const f16x4_t h = *reinterpret_cast<const f16x4_t*>(g), l = *reinterpret_cast<const f16x4_t*>(g + 32);
-#pragma unroll
-        for (int t = 0; t < 4; ++t) w[t] = cc * w[t] + cb * ((float)h[t] + (float)l[t]) + (r == c + t ? ca : 0.f);
-      });
-      __syncthreads();
-      if (q) small_store(small_product<false>(z, PA, q, PA, 0, 2), other, plain);
-      if (j + 1 < end) small_store(small_product<false>(z, PA, G, PA, 0, 2), R, plain);
-      if (q || j + 1 < end) __syncthreads();
-      if (q) {
-        _Float16* t = q;
-        q = other;
-        other = t;
-      } else {
-        q = z;
-      }
-      if (j + 1 < end) {
-        small_store(small_product<false>(R, PA, z, PA, 0, 2), G, plain);       // (nobody reads G any more)
-        __syncthreads();
-      }
-    }
+    f32x4_t g = {0.f, 0.f, 0.f, 0.f};
+    if (w.on) g = frag_product<false>(X, PX, w.i * 16, X, PX, 0, w.j * 16, w.part, n64 >> 5, w.parts);
+    store_gram(w, g, reinterpret_cast<f32x4_t*>(X + m16 * (PX + N_AREAS * PA)), A[0], gs);
+    const _Float16* q = phase_chain(w, A, st, k, end, M.gscale, m16);
     const bool last = end == st.steps;
-    f32x4_t acc[NMAX / 64];
+    f32x4_t acc[SMALL_QUADS];
 #pragma unroll
-    for (int t = 0; t < NMAX / 64; ++t)
-      if (t < tiles) acc[t] = small_product<true>(q, PA, X, PX, t * 64, 2);
+    for (int t = 0; t < SMALL_QUADS; ++t) {
+      const int x = t * 16 + wave, j = x / n;
+      if (j < cols) acc[t] = frag_product<true>(q, PA, (x - j * n) * 16, X, PX, m16, j * 16, 0, k32, 1);
+    }
     __syncthreads();                    // (X has been read)
 #pragma unroll
-    for (int t = 0; t < NMAX / 64; ++t) {
-      if (t >= tiles) continue;
+    for (int t = 0; t < SMALL_QUADS; ++t) {
+      const int x = t * 16 + wave, j = x / n;
+      if (j >= cols) continue;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const int r = (wave >> 2) * 16 + (lane >> 4) * 4 + w, c = t * 64 + (wave & 3) * 16 + (lane & 15);
-        const float x = acc[t][w];
+      for (int i = 0; i < 4; ++i) {
+        const int r = (x - j * n) * 16 + (lane >> 4) * 4 + i, c = j * 16 + (lane & 15);
+        const float y = acc[t][i];
         if (last) {
-          U[r * PF + c] = x;
+          U[r * PF + c] = y;
         } else {
-          _Float16* p = X + r * PX + (c >> 5) * 64 + (c & 31);
-          const _Float16 h = (_Float16)x;
+          _Float16* p = X + pair_at(PX, r, c);
+          const _Float16 h = (_Float16)y;
           p[0] = h;
-          p[32] = (_Float16)(x - (float)h);
+          p[32] = (_Float16)(y - (float)h);
         }
       }
     }
@@ -935,22 +1002,185 @@ __global__ __launch_bounds__(SMALL_TPB) void small_kernel(const NsMatrix* __rest
     k = end;
   }
 
-  const float g = result_factor(M, res);
+  const float factor = result_factor(M, res);
   for (int i0 = threadIdx.x; i0 < count; i0 += BATCH * SMALL_TPB) {
-    float w[BATCH];
-    if constexpr (MUON) {
+    float old[BATCH];
 #pragma unroll
-      for (int k = 0; k < BATCH; ++k) w[k] = i0 + k * SMALL_TPB < count ? res.p[M.src + i0 + k * SMALL_TPB] : 0.f;
-    }
+    for (int k = 0; k < BATCH; ++k) old[k] = MUON && i0 + k * SMALL_TPB < count ? res.p[M.src + i0 + k * SMALL_TPB] : 0.f;
 #pragma unroll
     for (int k = 0; k < BATCH; ++k) {
       const int i = i0 + k * SMALL_TPB, r = (int)((i + 0.5f) * per_row), c = i - r * M.cols;
-      if (i >= count) continue;
-      const float x = g * U[M.tall ? c * PF + r : r * PF + c];
-      if constexpr (MUON) res.p[M.src + i] = res.keep * w[k] - x;
-      else if (res.out_dtype == DAS_F32) reinterpret_cast<float*>(res.out)[M.src + i] = x;
-      else reinterpret_cast<uint16_t*>(res.out)[M.src + i] = res.out_dtype == DAS_BF16 ? f32_to_bf16(x) : __builtin_bit_cast(uint16_t, (_Float16)x);
+      if (i < count) emit_one<MUON>(res, M.src + i, factor * U[M.tall ? c * PF + r : r * PF + c], old[k]);
     }
+  }
+}
+
+// A slice of a thin matrix: t.kn pieces of 128 columns from piece t.k0 on. FIRST: X = U's blocks times their exponents and 1 / norm (as
+// normalise_kernel), and the slice's part of X X^T. MIDDLE: X = Q X, and the part. LAST: Q X goes to the result.
+enum ThinKind { FIRST, MIDDLE, LAST };
+constexpr int THIN_COLS = 128, PT = 2 * THIN_COLS + 8, PTF = THIN_COLS + 4;
+template <ThinKind KIND, bool MUON>
+__global__ __launch_bounds__(TPB) void thin_kernel(const NsMatrix* __restrict__ mats, const NsItem* __restrict__ items, float eps,
+                                                   const Partial* __restrict__ norm_part, _Float16* __restrict__ X, const _Float16* __restrict__ Q,
+                                                   f32x4_t* __restrict__ part, Result res) {
+  __shared__ __align__(16) _Float16 xs[SMALL_M * PT], qs[SMALL_M * PA];
+  __shared__ double red[4];
+  const NsItem t = items[blockIdx.x];
+  const NsMatrix M = mats[t.matrix];
+  const int m16 = up16(M.m), n = m16 >> 4, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, k32 = (m16 + 31) >> 5;
+  float* us = reinterpret_cast<float*>(xs);
+  float factor = 1.f;
+  double scale = 1.0;
+  if constexpr (KIND == FIRST) {
+    double s = 0.0;
+    for (int i = threadIdx.x; i < M.chunks; i += TPB) {
+      const Partial p = norm_part[M.chunk0 + i];
+      s += ldexp((double)p.ss, 2 * p.e);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    if (lane == 0) red[wave] = s;
+    __syncthreads();
+    scale = (double)M.scale / (sqrt((red[0] + red[1]) + (red[2] + red[3])) + (double)eps);
+  } else {
+    if constexpr (KIND == LAST) factor = result_factor(M, res);
+    for (int i = threadIdx.x; i < m16 * 16; i += TPB) {   // Q: rows of 256 bytes
+      const int r = i >> 4, c = i & 15;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (r < M.m) v = *reinterpret_cast<const uint4*>(Q + 2 * M.a + r * 128 + c * 8);
+      *reinterpret_cast<uint4*>(qs + r * PA + c * 8) = v;
+    }
+  }
+  f32x4_t gram[4] = {};
+  for (int piece = t.k0; piece < t.k0 + t.kn; ++piece) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < m16 * 16; i += TPB) {   // 8 columns of a row a thread
+      const int r = i >> 4, c = (i & 15) * 8;
+      float v[8] = {};
+      uint4 h = make_uint4(0, 0, 0, 0), l = h;
+      _Float16* p = X + 2 * M.x + at<true>(M.ldx, r, piece * THIN_COLS + c);
+      if (r < M.m) {
+        if constexpr (KIND == FIRST) {
+          // (m <= 64: one row of blocks along the columns of X, whichever way the source lies)
+          const int blk = piece * 2 + (c >> 6);
+          const float f = (float)ldexp(scale, norm_part[M.chunk0 + blk].e);
+          get<true>(X + 2 * M.x, M.ldx, r, piece * THIN_COLS + c, v);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] *= f;
+          put<true>(X + 2 * M.x, M.ldx, r, piece * THIN_COLS + c, v);
+        } else {
+          h = *reinterpret_cast<const uint4*>(p);
+          l = *reinterpret_cast<const uint4*>(p + 32);
+        }
+      }
+      if constexpr (KIND == FIRST) {
+        f16x8_t a, b;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          a[e] = (_Float16)v[e];
+          b[e] = (_Float16)(v[e] - (float)a[e]);
+        }
+        h = __builtin_bit_cast(uint4, a);
+        l = __builtin_bit_cast(uint4, b);
+      }
+      _Float16* d = xs + pair_at(PT, r, c);
+      *reinterpret_cast<uint4*>(d) = h;
+      *reinterpret_cast<uint4*>(d + 32) = l;
+    }
+    __syncthreads();
+    if constexpr (KIND != FIRST) {
+      f32x4_t acc[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int x = u * 4 + wave, j = x / n;
+        if (j < 8) acc[u] = frag_product<true>(qs, PA, (x - j * n) * 16, xs, PT, m16, j * 16, 0, k32, 1);
+      }
+      __syncthreads();
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int x = u * 4 + wave, j = x / n;
+        if (j >= 8) continue;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = (x - j * n) * 16 + (lane >> 4) * 4 + i, c = j * 16 + (lane & 15);
+          const float y = acc[u][i];
+          if constexpr (KIND == LAST) {
+            us[r * PTF + c] = y;
+          } else {
+            _Float16* p = xs + pair_at(PT, r, c);
+            const _Float16 h = (_Float16)y;
+            p[0] = h;
+            p[32] = (_Float16)(y - (float)h);
+          }
+        }
+      }
+      __syncthreads();
+      if constexpr (KIND == MIDDLE) {
+        for (int i = threadIdx.x; i < M.m * 32; i += TPB) {
+          const int r = i >> 5, c = (i & 31) * 8;    // 16 bytes of a row of 512
+          *reinterpret_cast<uint4*>(X + 2 * M.x + (long long)r * (2 * M.ldx) + piece * (2 * THIN_COLS) + c) =
+              *reinterpret_cast<const uint4*>(xs + r * PT + c);
+        }
+      }
+    }
+    if constexpr (KIND == LAST) {
+      const int c0 = piece * THIN_COLS, width = min(THIN_COLS, M.n - c0);
+      const long long base = M.tall ? M.src + (long long)c0 * M.cols : M.src + c0;
+      for (int i = threadIdx.x; i < M.m * THIN_COLS; i += TPB) {
+        // tall: the piece is `width` whole rows of the source, one after the other; else THIN_COLS of each of its m rows
+        const int r = M.tall ? i % M.m : i / THIN_COLS, c = M.tall ? i / M.m : i % THIN_COLS;
+        if (c >= width) continue;
+        const long long o = M.tall ? base + i : base + (long long)r * M.cols + c;
+        emit_one<MUON>(res, o, factor * us[r * PTF + c], MUON ? res.p[o] : 0.f);
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int x = u * 4 + wave, i = x / n;
+        if (i < n) gram[u] += frag_product<false>(xs, PT, i * 16, xs, PT, 0, (x - i * n) * 16, 0, THIN_COLS / 32, 1);
+      }
+    }
+  }
+  if constexpr (KIND != LAST) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int x = u * 4 + wave;
+      if (x < n * n) part[((long long)t.slot + x) * 64 + lane] = gram[u];
+    }
+  }
+}
+
+// One workgroup a thin matrix: X X^T from its slices' parts, the phase's steps, Q out
+__global__ __launch_bounds__(SMALL_TPB) void chain_kernel(const NsMatrix* __restrict__ mats, const NsItem* __restrict__ slices, const int2* __restrict__ thin,
+                                                          const f32x4_t* __restrict__ part, _Float16* __restrict__ Q, Steps st, int k) {
+  extern __shared__ __align__(16) char smem[];
+  const int2 range = thin[blockIdx.x];    // its slices
+  const NsItem first = slices[range.x];
+  const NsMatrix M = mats[first.matrix];
+  const int m16 = up16(M.m), lane = threadIdx.x & 63, f = (m16 >> 4) * (m16 >> 4);
+  _Float16* A[N_AREAS];
+#pragma unroll
+  for (int i = 0; i < N_AREAS; ++i) A[i] = reinterpret_cast<_Float16*>(smem) + i * m16 * PA;
+  f32x4_t* scratch = reinterpret_cast<f32x4_t*>(smem + 2 * N_AREAS * SMALL_M * PA);
+  zero_lds(smem, 2 * N_AREAS * m16 * PA, SMALL_TPB);
+  const Share w(m16);
+  f32x4_t g = {0.f, 0.f, 0.f, 0.f};
+  if (w.on) {
+    const f32x4_t* from = part + ((long long)first.slot + w.i * (m16 >> 4) + w.j) * 64 + lane;
+    for (int s0 = w.part; s0 < range.y; s0 += 4 * w.parts) {
+      f32x4_t v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v[u] = s0 + u * w.parts < range.y ? from[(long long)(s0 + u * w.parts) * f * 64] : f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int u = 0; u < 4; ++u) g += v[u];
+    }
+  }
+  __syncthreads();
+  store_gram(w, g, scratch, A[0], M.gscale / (M.scale * M.scale));
+  const _Float16* q = phase_chain(w, A, st, k, st.end[k], M.gscale, m16);
+  for (int i = threadIdx.x; i < M.m * 16; i += SMALL_TPB) {
+    const int r = i >> 4, c = i & 15;
+    *reinterpret_cast<uint4*>(Q + 2 * M.a + r * 128 + c * 8) = *reinterpret_cast<const uint4*>(q + r * PA + c * 8);
   }
 }
 
@@ -959,6 +1189,8 @@ inline long long up256(long long v) { return (v + 255) / 256 * 256; }
 
 struct Work {
   _Float16 *x[2], *a[N_AREAS];
+  _Float16 *xt, *qt;         // thin matrices: X, Q (pairs)
+  f32x4_t* thin_part;        // parts of X X^T
   Partial* part;
   f32x4_t* slots;            // partial tiles
   long long bytes;
@@ -971,6 +1203,9 @@ Work carve(const DasNsPlan* p, bool split, void* ws) {
   auto take = [&](long long n) { char* r = c; if (c) c += n; w.bytes += n; return r; };
   for (int i = 0; i < 2; ++i) w.x[i] = (_Float16*)take(xb);
   for (int i = 0; i < areas; ++i) w.a[i] = (_Float16*)take(ab);
+  w.xt = (_Float16*)take(up256(4 * p->thin_x_elems));
+  w.qt = (_Float16*)take(up256(4 * p->thin_a_elems));
+  w.thin_part = (f32x4_t*)take(1024 * p->thin_slots);
   w.part = (Partial*)take(up256((long long)sizeof(Partial) * p->n_chunks));
   w.slots = (f32x4_t*)take(4LL * JOIN_TILE * JOIN_TILE * std::max(p->gram_slots, 2 * p->product_slots));
   return w;
@@ -1021,23 +1256,47 @@ int phase_end(const Bounds* bound, int steps, int k) {
   return end;
 }
 
-template <typename T, bool MUON>
-int launch_small(const DasNsPlan* p, const char* tab, const Sources& src, const MuonIn& mu, const Result& res, hipStream_t s) {
-  if (p->n_small == 0) return DAS_OK;
+Steps steps_of(const DasNsPlan* p) {
   Steps st;
   memcpy(st.coef, p->coef, sizeof(st.coef));
   memcpy(st.end, p->phase_end, sizeof(st.end));
   st.steps = p->steps;
   st.eps = p->eps;
-  const NsMatrix* mats = (const NsMatrix*)(tab + p->mat_at);
-  auto launch = [&](auto kernel, int nmax) {
-    const int lds = 2 * (SMALL_M * (2 * nmax + 8) + N_AREAS * SMALL_M * PA);
-    (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    hipLaunchKernelGGL(kernel, dim3(p->n_small), dim3(SMALL_TPB), lds, s, mats, src, mu, st, res);
-  };
-  if (p->small_n <= 64) launch(small_kernel<T, MUON, 64>, 64);
-  else launch(small_kernel<T, MUON, 256>, 256);
+  return st;
+}
+
+template <typename T, bool MUON>
+int launch_small(const DasNsPlan* p, const char* tab, const Sources& src, const MuonIn& mu, const Result& res, hipStream_t s) {
+  if (p->n_small == 0) return DAS_OK;
+  (void)hipFuncSetAttribute((const void*)small_kernel<T, MUON>, hipFuncAttributeMaxDynamicSharedMemorySize, p->small_lds);
+  hipLaunchKernelGGL((small_kernel<T, MUON>), dim3(p->n_small), dim3(SMALL_TPB), p->small_lds, s, (const NsMatrix*)(tab + p->mat_at), src, mu,
+                     steps_of(p), res);
   DAS_CHECK_LAUNCH();
+  return DAS_OK;
+}
+
+// thin matrices, after ingest_kernel
+template <bool MUON>
+int launch_thin(const DasNsPlan* p, const char* tab, const Work& w, const Result& res, hipStream_t s) {
+  if (p->n_thin == 0) return DAS_OK;
+  const NsMatrix* mats = (const NsMatrix*)(tab + p->mat_at);
+  const NsItem* slices = (const NsItem*)(tab + p->slice_at);
+  const int2* thin = (const int2*)(tab + p->thin_at);
+  const Steps st = steps_of(p);
+  constexpr int LDS = 2 * N_AREAS * SMALL_M * PA + SMALL_TPB * 16;
+  (void)hipFuncSetAttribute((const void*)chain_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+  auto pass = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(p->n_slices), dim3(TPB), 0, s, mats, slices, p->eps, w.part, w.xt, w.qt, w.thin_part, res);
+  };
+  pass(thin_kernel<FIRST, false>);
+  DAS_CHECK_LAUNCH();
+  for (int k = 0; k < p->steps; k = p->phase_end[k]) {
+    hipLaunchKernelGGL(chain_kernel, dim3(p->n_thin), dim3(SMALL_TPB), LDS, s, mats, slices, thin, w.thin_part, w.qt, st, k);
+    DAS_CHECK_LAUNCH();
+    if (p->phase_end[k] < p->steps) pass(thin_kernel<MIDDLE, false>);
+    else pass(thin_kernel<LAST, MUON>);
+    DAS_CHECK_LAUNCH();
+  }
   return DAS_OK;
 }
 
@@ -1081,7 +1340,8 @@ int iterate(const DasNsPlan* p, const char* tab, Work w, const Result& res, hipS
   };
   const std::integral_constant<SymKind, POLY> poly_k;
   const std::integral_constant<SymKind, PRODUCT> product_k;
-  hipLaunchKernelGGL(normalise_kernel<SPLIT>, dim3(p->n_chunks), dim3(TPB), 0, s, mats, chunks, p->eps, w.x[0], w.part);
+  if (p->n_tile_chunks == 0) return DAS_OK;
+  hipLaunchKernelGGL(normalise_kernel<SPLIT>, dim3(p->n_tile_chunks), dim3(TPB), 0, s, mats, chunks, p->eps, w.x[0], w.part);
   DAS_CHECK_LAUNCH();
   _Float16 *X = w.x[0], *Y = w.x[1], *G = w.a[0], *R = w.a[1], *Z = w.a[SPLIT ? 2 : 1];
   for (int k = 0; k < p->steps;) {
@@ -1176,7 +1436,8 @@ struct Tables {
   std::vector<NsMatrix> mats;
   std::vector<int4> chunks;
   Launch gram, product, update;
-  std::vector<NsItem> gram_join, product_join;
+  std::vector<NsItem> gram_join, product_join, slices;
+  std::vector<int2> thin;    // first slice and slices of each thin matrix
 };
 
 struct Tile {
@@ -1292,18 +1553,18 @@ void lower_blocks(int tiles, int side, F f) {
 bool build(const DasNsShape* shapes, int n, double top, DasNsPlan* plan, Tables& t) {
   std::vector<std::pair<long long, long long>> spans;
   long long n_mat = 0, n_chunks = 0;
-  auto is_small = [&](const DasNsShape& s) { return std::min(s.rows, s.cols) <= SMALL_M && std::max(s.rows, s.cols) <= SMALL_N; };
+  enum Class { SMALL, TILED, THIN };
+  auto class_of = [](const DasNsShape& s) {
+    const int m = std::min(s.rows, s.cols), nn = std::max(s.rows, s.cols);
+    if (m > SMALL_M) return TILED;
+    return small_lds(m, nn) <= SMALL_LDS && (long long)up16(m) * up64(nn) <= 4 * SMALL_QUADS * SMALL_TPB ? SMALL : THIN;
+  };
   for (int g = 0; g < n; ++g) {
     const DasNsShape& s = shapes[g];
     if (s.off < 0 || s.count < 1 || s.rows < 1 || s.cols < 1 || s.rows > (1 << 20) || s.cols > (1 << 20)) return false;
     const long long m = std::min(s.rows, s.cols), nn = std::max(s.rows, s.cols);
     n_mat += s.count;
-    if (is_small(s)) {
-      plan->n_small += s.count;
-      plan->small_n = std::max(plan->small_n, (int)nn);
-    } else {
-      n_chunks += (long long)s.count * over(m, 64) * over(nn, 128) * 2;
-    }
+    if (class_of(s) != SMALL) n_chunks += (long long)s.count * over(m, 64) * over(nn, 128) * 2;
     if (n_mat > (1 << 22) || n_chunks > (1 << 24) || m > (1 << 15)) return false;
     spans.push_back({s.off, s.off + (long long)s.count * s.rows * s.cols});
   }
@@ -1312,36 +1573,55 @@ bool build(const DasNsShape* shapes, int n, double top, DasNsPlan* plan, Tables&
     if (spans[i].first < spans[i - 1].second) return false;   // two workgroups would write the same elements
   plan->extent = spans.back().second;
 
-  t.mats.resize(n_mat);
-  int small = 0, big = plan->n_small;   // (the small matrices come first in the table)
   long long lower128 = 0, all128 = 0;
-  for (int g = 0; g < n; ++g) {
-    const DasNsShape& s = shapes[g];
-    for (int i = 0; i < s.count; ++i) {
-      const int q = is_small(s) ? small++ : big++;
-      NsMatrix& M = t.mats[q];
-      M = NsMatrix{};
-      M.rows = s.rows; M.cols = s.cols; M.m = std::min(s.rows, s.cols); M.n = std::max(s.rows, s.cols);
-      M.tall = s.rows > s.cols;
-      M.ldx = over(M.n, 128) * 128; M.lda = over(M.m, 64) * 64;
-      M.src = s.off + (long long)i * s.rows * s.cols;
-      M.group = g; M.index = i;
-      M.scale = (float)std::ldexp(1.0, (int)std::lround(0.5 * std::log2((double)M.n)));
-      // about m, and top^2 gscale within f16
-      M.gscale = (float)std::ldexp(1.0, std::min((int)std::lround(std::log2((double)M.m)), (int)std::floor(std::log2(32768.0 / (top * top)))));
-      if (is_small(s)) continue;
-      M.x = plan->x_elems; M.a = plan->a_elems; M.chunk0 = (int)t.chunks.size();
-      plan->x_elems += (long long)M.m * M.ldx;
-      plan->a_elems += (long long)M.m * M.lda;
-      int k = 0;
-      for (int r = 0; r < (M.tall ? M.ldx : M.lda) / CHUNK; ++r)
-        for (int c = 0; c < (M.tall ? M.lda : M.ldx) / CHUNK; ++c) t.chunks.push_back(make_int4(q, r, c, k++));
-      M.chunks = k;
-      const long long tm = over(M.m, 128);
-      lower128 += tm * (tm + 1) / 2;
-      all128 += tm * (M.ldx / 128);
+  for (const Class cls : {SMALL, TILED, THIN}) {   // the order of the matrix and block tables
+    for (int g = 0; g < n; ++g) {
+      const DasNsShape& s = shapes[g];
+      if (class_of(s) != cls) continue;
+      for (int i = 0; i < s.count; ++i) {
+        NsMatrix M = {};
+        M.rows = s.rows; M.cols = s.cols; M.m = std::min(s.rows, s.cols); M.n = std::max(s.rows, s.cols);
+        M.tall = s.rows > s.cols;
+        M.thin = cls == THIN;
+        M.ldx = over(M.n, 128) * 128; M.lda = over(M.m, 64) * 64;
+        M.src = s.off + (long long)i * s.rows * s.cols;
+        M.group = g; M.index = i;
+        M.scale = (float)std::ldexp(1.0, (int)std::lround(0.5 * std::log2((double)M.n)));
+        // about m, and top^2 gscale within f16
+        M.gscale = (float)std::ldexp(1.0, std::min((int)std::lround(std::log2((double)M.m)), (int)std::floor(std::log2(32768.0 / (top * top)))));
+        if (cls == SMALL) {
+          plan->n_small++;
+          plan->small_lds = std::max(plan->small_lds, (int)small_lds(M.m, M.n));
+        } else {
+          long long &x = cls == THIN ? plan->thin_x_elems : plan->x_elems, &a = cls == THIN ? plan->thin_a_elems : plan->a_elems;
+          M.x = x; M.a = a; M.chunk0 = (int)t.chunks.size();
+          x += (long long)M.m * M.ldx;
+          a += (long long)M.m * M.lda;
+          int k = 0;
+          const int q = (int)t.mats.size();
+          for (int r = 0; r < (M.tall ? M.ldx : M.lda) / CHUNK; ++r)
+            for (int c = 0; c < (M.tall ? M.lda : M.ldx) / CHUNK; ++c) t.chunks.push_back(make_int4(q, r, c, k++));
+          M.chunks = k;
+          if (cls == TILED) {
+            const long long tm = over(M.m, 128);
+            lower128 += tm * (tm + 1) / 2;
+            all128 += tm * (M.ldx / 128);
+          } else {
+            // at most 64 slices: the chain's workgroup reads all their parts
+            const int pieces = M.ldx / THIN_COLS, per = over(pieces, 64), frags = up16(M.m) * up16(M.m) / 256;
+            t.thin.push_back(make_int2((int)t.slices.size(), over(pieces, per)));
+            for (int p = 0; p < pieces; p += per) {
+              t.slices.push_back(NsItem{q, 0, 0, p, std::min(per, pieces - p), (int)plan->thin_slots, frags, 0});
+              plan->thin_slots += frags;
+            }
+          }
+        }
+        t.mats.push_back(M);
+      }
     }
+    if (cls == TILED) plan->n_tile_chunks = (int)t.chunks.size();
   }
+  const int tiled_end = (int)(t.mats.size() - t.thin.size());
   // Products and updates: 128 x 128 tiles where they fill the 256 CUs, else 64 x 64 ones whose inner axis four wave groups share.
   plan->product_tile = lower128 >= 256 ? 128 : 64;
   plan->update_tile = all128 >= 256 ? 128 : 64;
@@ -1354,7 +1634,7 @@ bool build(const DasNsShape* shapes, int n, double top, DasNsPlan* plan, Tables&
     return side;
   };
   long long product_cost = 0, update_cost = 0, gram_cost = 0;
-  for (int q = plan->n_small; q < (int)n_mat; ++q) {
+  for (int q = plan->n_small; q < tiled_end; ++q) {
     const NsMatrix& M = t.mats[q];
     const long long p = over(M.m, plan->product_tile), r = over(M.m, plan->update_tile), w = over(M.m, JOIN_TILE);
     product_cost += p * (p + 1) / 2 * (M.lda / 64 + 2);
@@ -1362,7 +1642,7 @@ bool build(const DasNsShape* shapes, int n, double top, DasNsPlan* plan, Tables&
     gram_cost += w * (w + 1) / 2 * (M.ldx / 64 + 2);
   }
   std::vector<Tile> gram, product;
-  for (int q = plan->n_small; q < (int)n_mat; ++q) {
+  for (int q = plan->n_small; q < tiled_end; ++q) {
     const NsMatrix& M = t.mats[q];
     lower_blocks(over(M.m, JOIN_TILE), side_for(gram_cost, M.ldx / 64),
                  [&](bool fresh, int i, int j) { gram.push_back(Tile{fresh, q, i, j, M.ldx / 64}); });
@@ -1402,6 +1682,7 @@ extern "C" int das_ns_plan(const DasNsShape* shapes, int n, int steps, const flo
     if (!build(shapes, n, top, &p, t)) return DAS_ERR_ARG;
     p.n_groups = n; p.n_matrices = (int)t.mats.size(); p.n_chunks = (int)t.chunks.size();
     p.n_gram = (int)t.gram.order.size(); p.n_product = (int)t.product.order.size(); p.n_update = (int)t.update.order.size();
+    p.n_thin = (int)t.thin.size(); p.n_slices = (int)t.slices.size();
     p.n_gram_join = (int)t.gram_join.size(); p.n_product_join = (int)t.product_join.size();
     p.steps = steps; p.eps = eps;
     for (int k = 0; k < steps; ++k) p.phase_end[k] = phase_end(bound, steps, k);
@@ -1427,6 +1708,8 @@ extern "C" int das_ns_plan(const DasNsShape* shapes, int n, int steps, const flo
       put_table(t.product.order, p.product_at);
       put_table(t.product_join, p.product_join_at);
       put_table(t.update.order, p.update_at);
+      put_table(t.slices, p.slice_at);
+      put_table(t.thin, p.thin_at);
     }
     *plan = p;
   } catch (...) {   // (no memory for the tables)
@@ -1469,7 +1752,7 @@ extern "C" int das_orthogonalize(const DasNsPlan* plan, const void* tables_dev, 
     if (st != DAS_OK) return st;
     if (plan->n_chunks == 0) continue;
     auto launch = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, dim3(plan->n_chunks), dim3(TPB), 0, s, mats, chunks, a, none, w.x[0], w.part);
+      hipLaunchKernelGGL(kernel, dim3(plan->n_chunks), dim3(TPB), 0, s, mats, chunks, a, none, w.x[0], w.xt, w.part);
     };
     if (in_dtype == DAS_F32) split ? launch(ingest_kernel<float, false, true>) : launch(ingest_kernel<float, false, false>);
     else if (in_dtype == DAS_BF16) split ? launch(ingest_kernel<bf16_t, false, true>) : launch(ingest_kernel<bf16_t, false, false>);
@@ -1477,6 +1760,8 @@ extern "C" int das_orthogonalize(const DasNsPlan* plan, const void* tables_dev, 
     DAS_CHECK_LAUNCH();
   }
   if (plan->n_chunks == 0) return DAS_OK;
+  const int st = launch_thin<false>(plan, tab, w, res, s);
+  if (st != DAS_OK) return st;
   return split ? iterate<true>(plan, tab, w, res, s) : iterate<false>(plan, tab, w, res, s);
 }
 
@@ -1496,7 +1781,8 @@ extern "C" int das_muon_step(const DasNsPlan* plan, const void* tables_dev, floa
   const int st = launch_small<float, true>(plan, tab, Sources{}, mu, res, s);
   if (st != DAS_OK || plan->n_chunks == 0) return st;
   hipLaunchKernelGGL((ingest_kernel<float, true, true>), dim3(plan->n_chunks), dim3(TPB), 0, s, (const NsMatrix*)(tab + plan->mat_at),
-                     (const int4*)(tab + plan->chunk_at), Sources{}, mu, w.x[0], w.part);
+                     (const int4*)(tab + plan->chunk_at), Sources{}, mu, w.x[0], w.xt, w.part);
   DAS_CHECK_LAUNCH();
-  return iterate<true>(plan, tab, w, res, s);
+  const int thin = launch_thin<true>(plan, tab, w, res, s);
+  return thin != DAS_OK ? thin : iterate<true>(plan, tab, w, res, s);
 }

@@ -11,7 +11,7 @@ import torch.nn as nn
 COEF = (3.4445, -4.7750, 2.0315)
 MAT = np.dtype([('src', '<i8'), ('x', '<i8'), ('a', '<i8'), ('rows', '<i4'), ('cols', '<i4'), ('m', '<i4'), ('n', '<i4'), ('ldx', '<i4'),
                 ('lda', '<i4'), ('group', '<i4'), ('index', '<i4'), ('chunk0', '<i4'), ('chunks', '<i4'), ('scale', '<f4'),
-                ('gscale', '<f4'), ('tall', '<i4'), ('pad', '<i4')])
+                ('gscale', '<f4'), ('tall', '<i4'), ('thin', '<i4')])
 ITEM = np.dtype([(k, '<i4') for k in ('matrix', 'ti', 'tj', 'k0', 'kn', 'slot', 'slots', 'pad')])
 
 
@@ -36,22 +36,30 @@ def table(buf, at, n, dt):
     return buf[at:at + n * dt.itemsize].view(dt)
 
 
-@pytest.mark.parametrize('shapes', [[(1, 64, 64)], [(3, 45, 256), (1, 65, 64), (2, 700, 513), (1, 1, 4096)], [(1, 257, 8192)],
+@pytest.mark.parametrize('shapes', [[(1, 64, 64)], [(3, 45, 256), (1, 65, 64), (2, 700, 513), (1, 1, 4096), (2, 9000, 33)], [(1, 257, 8192)],
                                     [(2, 2048, 2048), (28, 256, 2304), (6, 512, 4608), (50, 64, 64)], [(5, 1536, 1000)]])
 def test_schedule_covers_every_product_once(shapes):
     """every tile of every matrix, every part of its inner axis, exactly once; offsets inside the work areas"""
     st, plan, buf = make_plan(shapes)
     assert st == 0 and MAT.itemsize == 80
     mats = table(buf, plan.mat_at, plan.n_matrices, MAT)
-    small = (mats['m'] <= 64) & (mats['n'] <= 256)
-    assert small[:plan.n_small].all() and not small[plan.n_small:].any() and plan.n_matrices == sum(s[0] for s in shapes)
+    end = plan.n_matrices - plan.n_thin
+    assert (mats['m'][:plan.n_small] <= 64).all() and not mats['thin'][:end].any()
+    assert (mats['m'][plan.n_small:end] > 64).all() and (mats['m'][end:] <= 64).all() and mats['thin'][end:].all()
+    assert plan.n_matrices == sum(s[0] for s in shapes) and plan.small_lds <= 155 * 1024
     assert sorted(zip(mats['rows'], mats['cols'])) == sorted((r, c) for k, r, c in shapes for _ in range(k))
-    big = mats[plan.n_small:]
-    assert (big['x'] + big['m'].astype(np.int64) * big['ldx'] <= plan.x_elems).all()
-    assert (big['a'] + big['m'].astype(np.int64) * big['lda'] <= plan.a_elems).all()
-    for lead, area in (('x', 'ldx'), ('a', 'lda')):
-        spans = sorted((int(o), int(o) + int(m) * int(ld)) for o, m, ld in zip(big[lead], big['m'], big[area]))
-        assert all(e <= s for (_, e), (s, _) in zip(spans, spans[1:]))
+    for part, x_elems, a_elems in ((mats[plan.n_small:end], plan.x_elems, plan.a_elems), (mats[end:], plan.thin_x_elems, plan.thin_a_elems)):
+        for lead, area, size in (('x', 'ldx', x_elems), ('a', 'lda', a_elems)):
+            spans = sorted((int(o), int(o) + int(m) * int(ld)) for o, m, ld in zip(part[lead], part['m'], part[area]))
+            assert all(e <= s for (_, e), (s, _) in zip(spans, spans[1:])) and (not spans or spans[-1][1] <= size)
+    slices = table(buf, plan.slice_at, plan.n_slices, ITEM)
+    for q, (first, count) in enumerate(table(buf, plan.thin_at, 2 * plan.n_thin, np.dtype('<i4')).reshape(-1, 2)):
+        M, mine = mats[end + q], slices[first:first + count]
+        frags = (-(-M['m'] // 16)) ** 2
+        assert (mine['matrix'] == end + q).all() and count <= 64 and mine['k0'][0] == 0
+        assert (mine['k0'][1:] == mine['k0'][:-1] + mine['kn'][:-1]).all() and (mine['k0'][-1] + mine['kn'][-1]) * 128 == M['ldx']
+        assert (mine['slot'] == mine['slot'][0] + frags * np.arange(count)).all() and mine['slot'][-1] + frags <= plan.thin_slots
+    assert sum(table(buf, plan.thin_at, 2 * plan.n_thin, np.dtype('<i4')).reshape(-1, 2)[:, 1]) == plan.n_slices
     chunks = table(buf, plan.chunk_at, plan.n_chunks, np.dtype([(k, '<i4') for k in 'qrci']))
     assert len(set(map(tuple, chunks[['q', 'r', 'c']].tolist()))) == plan.n_chunks
     for at, n, join_at, n_join, slots, tile, inner in (
@@ -64,7 +72,7 @@ def test_schedule_covers_every_product_once(shapes):
             assert t['kn'] > 0 and t['ti'] >= t['tj']
             seen.setdefault((t['matrix'], t['ti'], t['tj']), []).append((t['k0'], t['kn'], t['slot']))
         joins = {(t['matrix'], t['ti'], t['tj']): t for t in table(buf, join_at, n_join, ITEM)}
-        want = {(q, i, j) for q in range(plan.n_small, plan.n_matrices) for i in range(-(-mats[q]['m'] // tile)) for j in range(i + 1)}
+        want = {(q, i, j) for q in range(plan.n_small, end) for i in range(-(-mats[q]['m'] // tile)) for j in range(i + 1)}
         assert set(seen) == want
         for key, parts in seen.items():
             parts.sort()
@@ -79,7 +87,7 @@ def test_schedule_covers_every_product_once(shapes):
         assert len(set(used)) == len(used) and (not used or max(used) < slots)
     seen = [(t['matrix'], t['ti'], t['tj']) for t in table(buf, plan.update_at, plan.n_update, ITEM) if t['matrix'] >= 0]
     T = plan.update_tile
-    want = {(q, i, j) for q in range(plan.n_small, plan.n_matrices) for i in range(-(-mats[q]['m'] // T)) for j in range(mats[q]['ldx'] // T)}
+    want = {(q, i, j) for q in range(plan.n_small, end) for i in range(-(-mats[q]['m'] // T)) for j in range(mats[q]['ldx'] // T)}
     assert len(seen) == len(set(seen)) and set(seen) == want
 
 

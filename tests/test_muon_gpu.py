@@ -86,7 +86,7 @@ def check(got, u, coef, eps=1e-7, what=''):
 
 
 SHAPES = [(1, 1), (1, 64), (64, 1), (2, 3), (45, 256), (27, 2304), (64, 64), (33, 200), (256, 64), (64, 257), (64, 147), (65, 63), (63, 65), (128, 1152), (129, 1023),
-          (257, 64), (333, 77), (512, 128), (500, 513), (700, 513), (256, 2304)]
+          (257, 64), (16, 1856), (16, 1857), (32, 769), (48, 480), (9, 5000), (3000, 33), (2, 20000), (333, 77), (512, 128), (500, 513), (700, 513), (256, 2304)]
 
 
 @pytest.mark.parametrize('out_dtype', [torch.bfloat16, torch.float32])
