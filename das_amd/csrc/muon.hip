@@ -725,12 +725,14 @@ __global__ __launch_bounds__(KG * TPB, KG == 1 ? 2 : KG) void update_kernel(cons
 // all steps of a phase on the m x m matrices in LDS and leaves Q; the pass over the slices that forms Q X also forms the parts of the next
 // X X^T: five launches after the first pass (16 x 1056 by tiles: 85 us).
 //
-// 16 waves, one 16 x 16 fragment of an m x m product each; where m <= 32 leaves waves over they divide long inner axes. LDS matrices: rows of
-// pairs (32 high parts, 32 low parts, ...), row pitch 16 bytes past a multiple of 256; 32 columns of X take 128 bytes as pairs and as floats:
-// U, X and the result use the same place. Rows and columns up to the next multiple of 16 are zero.
+// 16 waves. m <= 32: one 16 x 16 fragment of an m x m product a wave, all inner elements in one instruction; waves left over divide the long
+// inner axis of X X^T. m > 32: four waves with 2 x 2 fragments each (one a wave reads every operand four times from LDS: 0.9 us a
+// product instead of 0.5). LDS matrices: rows of pairs (32 high parts, 32 low parts, ...), row pitch 16 bytes past a multiple of 256;
+// 32 columns of X take 128 bytes as pairs and as floats: U, X and the result use the same place. Rows and columns up to the next
+// multiple of 16 are zero.
 constexpr int SMALL_M = 64, SMALL_TPB = 1024, SMALL_LDS = 155 * 1024;
 constexpr int PA = 2 * SMALL_M + 8;   // row pitch of the m x m matrices, f16 elements
-constexpr int SMALL_QUADS = 8;        // float4 of U, and 16 x 16 fragments of X, a thread / wave can have: m n <= 32 Ki
+constexpr int SMALL_QUADS = 8;        // float4 of U, and 16 x 16 fragments of X, a thread / wave can have: m n <= 32 Ki (fewer where a set allows it: no spills)
 struct Steps {
   float coef[3 * DAS_NS_MAX_STEPS];
   int end[DAS_NS_MAX_STEPS];          // of the phase that starts at this step
@@ -739,8 +741,11 @@ struct Steps {
 };
 __host__ __device__ inline int up16(int m) { return (m + 15) & ~15; }
 __host__ __device__ inline int up64(int n) { return (n + 63) & ~63; }
-// X, the m x m matrices, and room for the shares of a sum (not over the m x m matrices: m <= 16 reads 32 columns of them, 16 of them zero)
-inline long long small_lds(int m, int n) { return 2LL * up16(m) * (2 * up64(n) + 8 + N_AREAS * PA) + (m <= 32 ? SMALL_TPB * 16 : 0); }
+// X, the m x m matrices, and behind them room for the shares of a sum (W = 1; not over the m x m matrices: m <= 16 reads 32 columns of them,
+// 16 of them zero) or for the rows that a second fragment past m = 48 reads for nothing
+inline long long small_lds(int m, int n) {
+  return 2LL * up16(m) * (2 * up64(n) + 8 + N_AREAS * PA) + (m <= 32 ? SMALL_TPB * 16 : up16(m) == 48 ? 2 * 16 * PA : 0);
+}
 
 __device__ __forceinline__ f16x8_t row_frag(const _Float16* p, int pitch, int row0, int k, int part) {
   const int lane = threadIdx.x & 63;
@@ -759,23 +764,64 @@ __device__ __forceinline__ f16x8_t col_frag(const _Float16* x, int pitch, int ro
   }
   return f;
 }
-// 16 x 16 of P's rows from row0 by (Q's rows from q0, or its columns from q0), inner steps of 32: k0, k0 + stride, ... < k1
-template <bool COLS>
-__device__ __forceinline__ f32x4_t frag_product(const _Float16* p, int pp, int row0, const _Float16* q, int qp, int q_rows, int q0, int k0, int k1,
-                                                int stride) {
-  f32x4_t high = {0.f, 0.f, 0.f, 0.f}, low = {0.f, 0.f, 0.f, 0.f};   // (two chains)
-  for (int k = k0; k < k1; k += stride) {
-    f16x8_t fa[2], fb[2];
+// W x W fragments: P's rows from row0 by (Q's rows from q0, or its columns from q0), inner steps of 32: k0, k0 + stride, ... < k1
+template <int W>
+using Frags = f32x4_t[W][W];
+template <int W, bool COLS>
+__device__ __forceinline__ void frag_step(const _Float16* p, int pp, int row0, const _Float16* q, int qp, int q_rows, int q0, int k, Frags<W>& high,
+                                          Frags<W>& low) {
+  f16x8_t fa[W][2], fb[W][2];
+#pragma unroll
+  for (int t = 0; t < W; ++t)
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      fa[u] = row_frag(p, pp, row0, k, u);
-      fb[u] = COLS ? col_frag(q, qp, q_rows, q0, k, u) : row_frag(q, qp, q0, k, u);
+      fa[t][u] = row_frag(p, pp, row0 + t * 16, k, u);
+      fb[t][u] = COLS ? col_frag(q, qp, q_rows, q0 + t * 16, k, u) : row_frag(q, qp, q0 + t * 16, k, u);
     }
-    high = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa[0], fb[0], high, 0, 0, 0);
-    low = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa[1], fb[0], low, 0, 0, 0);
-    low = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa[0], fb[1], low, 0, 0, 0);
-  }
-  return high + low;
+#pragma unroll
+  for (int i = 0; i < W; ++i)
+#pragma unroll
+    for (int j = 0; j < W; ++j) {   // (two chains)
+      high[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa[i][0], fb[j][0], high[i][j], 0, 0, 0);
+      low[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa[i][1], fb[j][0], low[i][j], 0, 0, 0);
+      low[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa[i][0], fb[j][1], low[i][j], 0, 0, 0);
+    }
+}
+template <int W, int K>   // K inner steps, unrolled
+__device__ __forceinline__ void square_product(const _Float16* p, int row0, const _Float16* q, int q0, Frags<W>& acc) {
+  Frags<W> low = {};
+#pragma unroll
+  for (int i = 0; i < W; ++i)
+#pragma unroll
+    for (int j = 0; j < W; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int k = 0; k < K; ++k) frag_step<W, false>(p, PA, row0, q, PA, 0, q0, k, acc, low);
+#pragma unroll
+  for (int i = 0; i < W; ++i)
+#pragma unroll
+    for (int j = 0; j < W; ++j) acc[i][j] += low[i][j];
+}
+template <int W, bool COLS>
+__device__ __forceinline__ void long_product(const _Float16* p, int pp, int row0, const _Float16* q, int qp, int q_rows, int q0, int k0, int k1,
+                                             int stride, Frags<W>& acc) {
+  Frags<W> low = {};
+#pragma unroll
+  for (int i = 0; i < W; ++i)
+#pragma unroll
+    for (int j = 0; j < W; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  for (int k = k0; k < k1; k += stride) frag_step<W, COLS>(p, pp, row0, q, qp, q_rows, q0, k, acc, low);
+#pragma unroll
+  for (int i = 0; i < W; ++i)
+#pragma unroll
+    for (int j = 0; j < W; ++j) acc[i][j] += low[i][j];
+}
+// Q's rows from row0 (m x m) by X's columns from col0: one fragment
+template <int K>
+__device__ __forceinline__ f32x4_t update_fragment(const _Float16* q, int row0, const _Float16* x, int pitch, int rows, int col0) {
+  Frags<1> acc = {}, low = {};
+#pragma unroll
+  for (int k = 0; k < K; ++k) frag_step<1, true>(q, PA, row0, x, pitch, rows, col0, k, acc, low);
+  return acc[0][0] + low[0][0];
 }
 __device__ __forceinline__ void put4(_Float16* p, const float (&v)[4]) {
   f16x4_t h, l;
@@ -789,63 +835,92 @@ __device__ __forceinline__ void put4(_Float16* p, const float (&v)[4]) {
 }
 __device__ __forceinline__ int pair_at(int pitch, int r, int c) { return r * pitch + (c >> 5) * 64 + (c & 31); }
 
-// Which fragment of an m16 x m16 matrix a wave has, and which share of a long inner axis
+// Which W x W fragments of an m16 x m16 matrix a wave has (first row and column of elements), and which share of a long inner axis
 struct Share {
-  int i, j, part, parts;
+  int r0, c0, part, parts;
   bool on;
-  __device__ explicit Share(int m16) {
-    const int w = threadIdx.x >> 6, n = m16 >> 4, f = n * n;
-    parts = f <= 4 ? 16 / f : 1;
-    on = w < f * parts;
-    part = w / f;
-    i = (w % f) / n;
-    j = w % n;
+  template <int W>
+  __device__ static Share of(int m16) {
+    Share s;
+    const int w = threadIdx.x >> 6;
+    if (W == 2 || m16 > 16) {        // 2 x 2 places
+      s.parts = W == 2 ? 1 : 4;
+      s.r0 = ((w >> 1) & 1) * 16 * W;
+      s.c0 = (w & 1) * 16 * W;
+      s.part = w >> 2;
+    } else {
+      s.parts = 16;
+      s.r0 = s.c0 = 0;
+      s.part = w;
+    }
+    s.on = s.part < s.parts;
+    return s;
   }
 };
-// a symmetric result, stored transposed (four values of a lane are neighbours then): f(row, col, four values) may change them
-template <typename F>
-__device__ __forceinline__ void frag_store(const Share& w, f32x4_t acc, _Float16* out, F f) {
-  const int lane = threadIdx.x & 63, r = w.j * 16 + (lane & 15), c = w.i * 16 + (lane >> 4) * 4;
-  float v[4] = {acc[0], acc[1], acc[2], acc[3]};
-  f(r, c, v);
-  put4(out + pair_at(PA, r, c), v);
+// a symmetric result, stored transposed (four values of a lane are neighbours then): f(row, col, four values) may change them. For m16 = 48 the
+// second fragments of the last places are outside.
+template <int W, typename F>
+__device__ __forceinline__ void frag_store(const Share& w, int m16, const Frags<W>& acc, _Float16* out, F f) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int i = 0; i < W; ++i)
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      const int r = w.c0 + j * 16 + (lane & 15), c = w.r0 + i * 16 + (lane >> 4) * 4;
+      if (W == 2 && (w.c0 + j * 16 >= m16 || w.r0 + i * 16 >= m16)) continue;
+      float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+      f(r, c, v);
+      put4(out + pair_at(PA, r, c), v);
+    }
 }
-// The shares of a sum over a long inner axis, added in order and stored as G; scratch: 16 KiB of LDS outside G and the operands, and the
-// caller's barrier before its next use
-__device__ __forceinline__ void store_gram(const Share& w, f32x4_t acc, f32x4_t* scratch, _Float16* G, float scale) {
-  if (w.parts > 1) {
-    scratch[threadIdx.x] = acc;
+// The shares of a sum over a long inner axis, added in order and stored as G. scratch: 16 KiB of LDS of its own (W = 1)
+template <int W>
+__device__ __forceinline__ void store_gram(const Share& w, int m16, Frags<W>& acc, f32x4_t* scratch, _Float16* G, float scale) {
+  if constexpr (W == 1) {
+    scratch[threadIdx.x] = acc[0][0];
     __syncthreads();
     if (w.part == 0)
-      for (int s = 1; s < w.parts; ++s) acc += scratch[s * (SMALL_TPB / w.parts) + threadIdx.x];
+      for (int s = 1; s < w.parts; ++s) acc[0][0] += scratch[s * (SMALL_TPB / w.parts) + threadIdx.x];
   }
   if (w.on && w.part == 0)
-    frag_store(w, acc, G, [&](int, int, float (&v)[4]) {
+    frag_store<W>(w, m16, acc, G, [&](int, int, float (&v)[4]) {
 #pragma unroll
       for (int t = 0; t < 4; ++t) v[t] *= scale;
     });
   __syncthreads();
 }
 // Steps k ... end - 1 on the m x m matrices (the same products as iterate<true>), G in A[0]; -> Q
+template <int W>
 __device__ __forceinline__ _Float16* phase_chain(const Share& w, _Float16* const (&A)[N_AREAS], const Steps& st, int k, int end, float gscale, int m16) {
-  const int k32 = (m16 + 31) >> 5;
+  constexpr int K = W;               // inner steps of 32: m <= 32 W
   const bool on = w.on && w.part == 0;
   _Float16 *G = A[0], *R = A[1], *Z = A[2], *q = nullptr, *spare = A[3], *other = A[4];
   auto plain = [](int, int, float (&)[4]) {};
-  auto product = [&](const _Float16* p, const _Float16* x) { return frag_product<false>(p, PA, w.i * 16, x, PA, 0, w.j * 16, 0, k32, 1); };
+  const float inv = 1.f / gscale;    // (a power of two)
   for (int j = k; j < end; ++j) {
-    const float ca = st.coef[3 * j], cb = st.coef[3 * j + 1] / gscale, cc = st.coef[3 * j + 2] / (gscale * gscale);
+    const float ca = st.coef[3 * j], cb = st.coef[3 * j + 1] * inv, cc = st.coef[3 * j + 2] * inv * inv;
     _Float16* z = q ? Z : spare;
-    if (on)
-      frag_store(w, product(G, G), z, [&](int r, int c, float (&v)[4]) {
+    Frags<W> acc;
+    if (on) {
+      square_product<W, K>(G, w.r0, G, w.c0, acc);
+      frag_store<W>(w, m16, acc, z, [&](int r, int c, float (&v)[4]) {
         const _Float16* g = G + pair_at(PA, r, c);
         const f16x4_t h = *reinterpret_cast<const f16x4_t*>(g), l = *reinterpret_cast<const f16x4_t*>(g + 32);
 #pragma unroll
         for (int t = 0; t < 4; ++t) v[t] = cc * v[t] + cb * ((float)h[t] + (float)l[t]) + (r == c + t ? ca : 0.f);
       });
+    }
     __syncthreads();
-    if (on && q) frag_store(w, product(z, q), other, plain);
-    if (on && j + 1 < end) frag_store(w, product(z, G), R, plain);
+    // Q = Z Q and R = Z G by different waves (the second share of a W = 2 place is idle otherwise)
+    const bool second = W == 2 && w.part == 1;
+    if (on && q) {
+      square_product<W, K>(z, w.r0, q, w.c0, acc);
+      frag_store<W>(w, m16, acc, other, plain);
+    }
+    if ((W == 2 && q ? second : on) && j + 1 < end) {
+      square_product<W, K>(z, w.r0, G, w.c0, acc);
+      frag_store<W>(w, m16, acc, R, plain);
+    }
     __syncthreads();
     if (q) {
       _Float16* t = q;
@@ -855,7 +930,10 @@ __device__ __forceinline__ _Float16* phase_chain(const Share& w, _Float16* const
       q = z;
     }
     if (j + 1 < end) {
-      if (on) frag_store(w, product(R, z), G, plain);       // (nobody reads G any more)
+      if (on) {
+        square_product<W, K>(R, w.r0, z, w.c0, acc);
+        frag_store<W>(w, m16, acc, G, plain);       // (nobody reads G any more)
+      }
       __syncthreads();
     }
   }
@@ -872,13 +950,9 @@ __device__ __forceinline__ void emit_one(const Result& res, long long o, float x
   else reinterpret_cast<uint16_t*>(res.out)[o] = res.out_dtype == DAS_BF16 ? f32_to_bf16(x) : __builtin_bit_cast(uint16_t, (_Float16)x);
 }
 
-template <typename T, bool MUON>
-__global__ __launch_bounds__(SMALL_TPB) void small_kernel(const NsMatrix* __restrict__ mats, Sources src, MuonIn mu, Steps st, Result res) {
-  extern __shared__ __align__(16) char smem[];
-  __shared__ float red[SMALL_TPB / 64];
-  __shared__ double redd[SMALL_TPB / 64];
-  const NsMatrix M = mats[blockIdx.x];
-  if (!MUON && (unsigned)(M.group - src.first) >= (unsigned)src.count) return;   // (whole workgroups)
+template <typename T, bool MUON, int QUADS, int W>
+__device__ __forceinline__ void small_matrix(const NsMatrix& M, const DasNsSource& s, const MuonIn& mu, const Steps& st, const Result& res, char* smem,
+                                             float* red, double* redd) {
   const int m16 = up16(M.m), n64 = up64(M.n), PX = 2 * n64 + 8, PF = n64 + 4;   // X's row pitch in f16 elements and in floats
   _Float16* X = reinterpret_cast<_Float16*>(smem);
   float* U = reinterpret_cast<float*>(smem);
@@ -895,7 +969,6 @@ __global__ __launch_bounds__(SMALL_TPB) void small_kernel(const NsMatrix* __rest
   if constexpr (MUON) coef = grad_factor(mu);
   for (int i0 = threadIdx.x; i0 < max(count, SMALL_TPB); i0 += BATCH * SMALL_TPB) {
     float v[BATCH], b[BATCH];
-    const DasNsSource& s = src.s[MUON ? 0 : M.group - src.first];
 #pragma unroll
     for (int k = 0; k < BATCH; ++k) {
       const int i = i0 + k * SMALL_TPB, r = (int)((i + 0.5f) * per_row), c = i - r * M.cols;
@@ -933,10 +1006,10 @@ __global__ __launch_bounds__(SMALL_TPB) void small_kernel(const NsMatrix* __rest
   for (int i = 0; i < SMALL_TPB / 64; ++i) big = fmaxf(big, red[i]);
   int e = 0;
   if (big > 0.f && big <= 3.4028235e38f) (void)frexpf(big, &e);
-  float v[SMALL_QUADS][4], ss = 0.f;
+  float v[QUADS][4], ss = 0.f;
   const int quads = m16 * n64 / 4, per = n64 / 4;
 #pragma unroll
-  for (int b = 0; b < SMALL_QUADS; ++b) {
+  for (int b = 0; b < QUADS; ++b) {
     const int i = threadIdx.x + b * SMALL_TPB, r = i / per;
     if (i >= quads) continue;
     const float4 w = *reinterpret_cast<const float4*>(U + r * PF + (i - r * per) * 4);
@@ -954,7 +1027,7 @@ __global__ __launch_bounds__(SMALL_TPB) void small_kernel(const NsMatrix* __rest
   for (int i = 0; i < SMALL_TPB / 64; ++i) sum += redd[i];
   const float f = (float)ldexp((double)M.scale / (ldexp(sqrt(sum), e) + (double)st.eps), e);
 #pragma unroll
-  for (int b = 0; b < SMALL_QUADS; ++b) {
+  for (int b = 0; b < QUADS; ++b) {
     const int i = threadIdx.x + b * SMALL_TPB, r = i / per;
     if (i >= quads) continue;
 #pragma unroll
@@ -963,25 +1036,25 @@ __global__ __launch_bounds__(SMALL_TPB) void small_kernel(const NsMatrix* __rest
   }
   __syncthreads();
 
-  const Share w(m16);
-  const int n = m16 >> 4, cols = n64 >> 4, k32 = (m16 + 31) >> 5;
+  const Share w = Share::of<W>(m16);
+  const int n = m16 >> 4, cols = n64 >> 4;
   const float gs = M.gscale / (M.scale * M.scale);
   for (int k = 0; k < st.steps;) {
     const int end = st.end[k];
-    f32x4_t g = {0.f, 0.f, 0.f, 0.f};
-    if (w.on) g = frag_product<false>(X, PX, w.i * 16, X, PX, 0, w.j * 16, w.part, n64 >> 5, w.parts);
-    store_gram(w, g, reinterpret_cast<f32x4_t*>(X + m16 * (PX + N_AREAS * PA)), A[0], gs);
-    const _Float16* q = phase_chain(w, A, st, k, end, M.gscale, m16);
+    Frags<W> g;
+    if (w.on) long_product<W, false>(X, PX, w.r0, X, PX, 0, w.c0, w.part, n64 >> 5, w.parts, g);
+    store_gram<W>(w, m16, g, reinterpret_cast<f32x4_t*>(X + m16 * (PX + N_AREAS * PA)), A[0], gs);
+    const _Float16* q = phase_chain<W>(w, A, st, k, end, M.gscale, m16);
     const bool last = end == st.steps;
-    f32x4_t acc[SMALL_QUADS];
+    f32x4_t acc[QUADS];
 #pragma unroll
-    for (int t = 0; t < SMALL_QUADS; ++t) {
+    for (int t = 0; t < QUADS; ++t) {
       const int x = t * 16 + wave, j = x / n;
-      if (j < cols) acc[t] = frag_product<true>(q, PA, (x - j * n) * 16, X, PX, m16, j * 16, 0, k32, 1);
+      if (j < cols) acc[t] = update_fragment<W>(q, (x - j * n) * 16, X, PX, m16, j * 16);
     }
     __syncthreads();                    // (X has been read)
 #pragma unroll
-    for (int t = 0; t < SMALL_QUADS; ++t) {
+    for (int t = 0; t < QUADS; ++t) {
       const int x = t * 16 + wave, j = x / n;
       if (j >= cols) continue;
 #pragma unroll
@@ -1013,6 +1086,18 @@ __global__ __launch_bounds__(SMALL_TPB) void small_kernel(const NsMatrix* __rest
       if (i < count) emit_one<MUON>(res, M.src + i, factor * U[M.tall ? c * PF + r : r * PF + c], old[k]);
     }
   }
+}
+
+template <typename T, bool MUON, int QUADS>
+__global__ __launch_bounds__(SMALL_TPB) void small_kernel(const NsMatrix* __restrict__ mats, Sources src, MuonIn mu, Steps st, Result res) {
+  extern __shared__ __align__(16) char smem[];
+  __shared__ float red[SMALL_TPB / 64];
+  __shared__ double redd[SMALL_TPB / 64];
+  const NsMatrix M = mats[blockIdx.x];
+  if (!MUON && (unsigned)(M.group - src.first) >= (unsigned)src.count) return;   // (whole workgroups)
+  const DasNsSource& s = src.s[MUON ? 0 : M.group - src.first];
+  if (M.m <= 32) small_matrix<T, MUON, QUADS, 1>(M, s, mu, st, res, smem, red, redd);
+  else small_matrix<T, MUON, QUADS, 2>(M, s, mu, st, res, smem, red, redd);
 }
 
 // A slice of a thin matrix: t.kn pieces of 128 columns from piece t.k0 on. FIRST: X = U's blocks times their exponents and 1 / norm (as
@@ -1093,7 +1178,8 @@ __global__ __launch_bounds__(TPB) void thin_kernel(const NsMatrix* __restrict__ 
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
         const int x = u * 4 + wave, j = x / n;
-        if (j < 8) acc[u] = frag_product<true>(qs, PA, (x - j * n) * 16, xs, PT, m16, j * 16, 0, k32, 1);
+        if (j < 8)
+          acc[u] = k32 == 1 ? update_fragment<1>(qs, (x - j * n) * 16, xs, PT, m16, j * 16) : update_fragment<2>(qs, (x - j * n) * 16, xs, PT, m16, j * 16);
       }
       __syncthreads();
 #pragma unroll
@@ -1137,7 +1223,11 @@ __global__ __launch_bounds__(TPB) void thin_kernel(const NsMatrix* __restrict__ 
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const int x = u * 4 + wave, i = x / n;
-        if (i < n) gram[u] += frag_product<false>(xs, PT, i * 16, xs, PT, 0, (x - i * n) * 16, 0, THIN_COLS / 32, 1);
+        if (i < n) {
+          Frags<1> g;
+          long_product<1, false>(xs, PT, i * 16, xs, PT, 0, (x - i * n) * 16, 0, THIN_COLS / 32, 1, g);
+          gram[u] += g[0][0];
+        }
       }
     }
   }
@@ -1151,37 +1241,50 @@ __global__ __launch_bounds__(TPB) void thin_kernel(const NsMatrix* __restrict__ 
 }
 
 // One workgroup a thin matrix: X X^T from its slices' parts, the phase's steps, Q out
+template <int W>
+__device__ __forceinline__ void chain_matrix(const NsMatrix& M, const f32x4_t* part, int slices, _Float16* Q, const Steps& st, int k, char* smem) {
+  const int m16 = up16(M.m), n = m16 >> 4, lane = threadIdx.x & 63;
+  _Float16* A[N_AREAS];
+#pragma unroll
+  for (int i = 0; i < N_AREAS; ++i) A[i] = reinterpret_cast<_Float16*>(smem) + i * m16 * PA;
+  f32x4_t* scratch = reinterpret_cast<f32x4_t*>(smem + 2 * N_AREAS * SMALL_M * PA);
+  zero_lds(smem, 2 * N_AREAS * m16 * PA, SMALL_TPB);
+  const Share w = Share::of<W>(m16);
+  Frags<W> g = {};
+  if (w.on) {
+#pragma unroll
+    for (int i = 0; i < W; ++i)
+#pragma unroll
+      for (int j = 0; j < W; ++j) {
+        const int fi = (w.r0 >> 4) + i, fj = (w.c0 >> 4) + j;
+        if (fi >= n || fj >= n) continue;
+        const f32x4_t* from = part + (fi * n + fj) * 64 + lane;
+        for (int s0 = w.part; s0 < slices; s0 += 4 * w.parts) {
+          f32x4_t v[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            v[u] = s0 + u * w.parts < slices ? from[(long long)(s0 + u * w.parts) * n * n * 64] : f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int u = 0; u < 4; ++u) g[i][j] += v[u];
+        }
+      }
+  }
+  __syncthreads();
+  store_gram<W>(w, m16, g, scratch, A[0], M.gscale / (M.scale * M.scale));
+  const _Float16* q = phase_chain<W>(w, A, st, k, st.end[k], M.gscale, m16);
+  for (int i = threadIdx.x; i < M.m * 16; i += SMALL_TPB) {
+    const int r = i >> 4, c = i & 15;
+    *reinterpret_cast<uint4*>(Q + 2 * M.a + r * 128 + c * 8) = *reinterpret_cast<const uint4*>(q + r * PA + c * 8);
+  }
+}
 __global__ __launch_bounds__(SMALL_TPB) void chain_kernel(const NsMatrix* __restrict__ mats, const NsItem* __restrict__ slices, const int2* __restrict__ thin,
                                                           const f32x4_t* __restrict__ part, _Float16* __restrict__ Q, Steps st, int k) {
   extern __shared__ __align__(16) char smem[];
   const int2 range = thin[blockIdx.x];    // its slices
   const NsItem first = slices[range.x];
   const NsMatrix M = mats[first.matrix];
-  const int m16 = up16(M.m), lane = threadIdx.x & 63, f = (m16 >> 4) * (m16 >> 4);
-  _Float16* A[N_AREAS];
-#pragma unroll
-  for (int i = 0; i < N_AREAS; ++i) A[i] = reinterpret_cast<_Float16*>(smem) + i * m16 * PA;
-  f32x4_t* scratch = reinterpret_cast<f32x4_t*>(smem + 2 * N_AREAS * SMALL_M * PA);
-  zero_lds(smem, 2 * N_AREAS * m16 * PA, SMALL_TPB);
-  const Share w(m16);
-  f32x4_t g = {0.f, 0.f, 0.f, 0.f};
-  if (w.on) {
-    const f32x4_t* from = part + ((long long)first.slot + w.i * (m16 >> 4) + w.j) * 64 + lane;
-    for (int s0 = w.part; s0 < range.y; s0 += 4 * w.parts) {
-      f32x4_t v[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) v[u] = s0 + u * w.parts < range.y ? from[(long long)(s0 + u * w.parts) * f * 64] : f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int u = 0; u < 4; ++u) g += v[u];
-    }
-  }
-  __syncthreads();
-  store_gram(w, g, scratch, A[0], M.gscale / (M.scale * M.scale));
-  const _Float16* q = phase_chain(w, A, st, k, st.end[k], M.gscale, m16);
-  for (int i = threadIdx.x; i < M.m * 16; i += SMALL_TPB) {
-    const int r = i >> 4, c = i & 15;
-    *reinterpret_cast<uint4*>(Q + 2 * M.a + r * 128 + c * 8) = *reinterpret_cast<const uint4*>(q + r * PA + c * 8);
-  }
+  if (M.m <= 32) chain_matrix<1>(M, part + (long long)first.slot * 64, range.y, Q, st, k, smem);
+  else chain_matrix<2>(M, part + (long long)first.slot * 64, range.y, Q, st, k, smem);
 }
 
 // ------------------------------------------------------------------ host side
@@ -1268,9 +1371,13 @@ Steps steps_of(const DasNsPlan* p) {
 template <typename T, bool MUON>
 int launch_small(const DasNsPlan* p, const char* tab, const Sources& src, const MuonIn& mu, const Result& res, hipStream_t s) {
   if (p->n_small == 0) return DAS_OK;
-  (void)hipFuncSetAttribute((const void*)small_kernel<T, MUON>, hipFuncAttributeMaxDynamicSharedMemorySize, p->small_lds);
-  hipLaunchKernelGGL((small_kernel<T, MUON>), dim3(p->n_small), dim3(SMALL_TPB), p->small_lds, s, (const NsMatrix*)(tab + p->mat_at), src, mu,
-                     steps_of(p), res);
+  auto launch = [&](auto kernel) {
+    (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, p->small_lds);
+    hipLaunchKernelGGL(kernel, dim3(p->n_small), dim3(SMALL_TPB), p->small_lds, s, (const NsMatrix*)(tab + p->mat_at), src, mu, steps_of(p), res);
+  };
+  if (p->small_quads <= 2) launch(small_kernel<T, MUON, 2>);
+  else if (p->small_quads <= 4) launch(small_kernel<T, MUON, 4>);
+  else launch(small_kernel<T, MUON, SMALL_QUADS>);
   DAS_CHECK_LAUNCH();
   return DAS_OK;
 }
@@ -1592,6 +1699,7 @@ bool build(const DasNsShape* shapes, int n, double top, DasNsPlan* plan, Tables&
         if (cls == SMALL) {
           plan->n_small++;
           plan->small_lds = std::max(plan->small_lds, (int)small_lds(M.m, M.n));
+          plan->small_quads = std::max(plan->small_quads, over((long long)up16(M.m) * up64(M.n), 4 * SMALL_TPB));
         } else {
           long long &x = cls == THIN ? plan->thin_x_elems : plan->x_elems, &a = cls == THIN ? plan->thin_a_elems : plan->a_elems;
           M.x = x; M.a = a; M.chunk0 = (int)t.chunks.size();
