@@ -952,7 +952,7 @@ __device__ __forceinline__ void emit_one(const Result& res, long long o, float x
 
 template <typename T, bool MUON, int QUADS, int W>
 __device__ __forceinline__ void small_matrix(const NsMatrix& M, const DasNsSource& s, const MuonIn& mu, const Steps& st, const Result& res, char* smem,
-                                             float* red, double* redd) {
+                                             double* redd) {
   const int m16 = up16(M.m), n64 = up64(M.n), PX = 2 * n64 + 8, PF = n64 + 4;   // X's row pitch in f16 elements and in floats
   _Float16* X = reinterpret_cast<_Float16*>(smem);
   float* U = reinterpret_cast<float*>(smem);
@@ -964,8 +964,9 @@ __device__ __forceinline__ void small_matrix(const NsMatrix& M, const DasNsSourc
   // U, zeros around it and in the m x m matrices. The first loads go out before.
   const int count = M.rows * M.cols;
   const float per_row = 1.f / (float)M.cols;   // (index + 1/2) / cols is exact enough to truncate for indices under 2^20
-  constexpr int BATCH = 4;                     // loads in flight per thread: a load a time is a memory latency each
-  float big = 0.f, coef = 1.f;
+  constexpr int BATCH = QUADS <= 2 ? 4 : 8;    // loads in flight per thread: a load a time is a memory latency each
+  float coef = 1.f;
+  double sum = 0.0;                            // (f64 holds the square of any f32: no scaling before the norm is known)
   if constexpr (MUON) coef = grad_factor(mu);
   for (int i0 = threadIdx.x; i0 < max(count, SMALL_TPB); i0 += BATCH * SMALL_TPB) {
     float v[BATCH], b[BATCH];
@@ -995,44 +996,31 @@ __device__ __forceinline__ void small_matrix(const NsMatrix& M, const DasNsSourc
         mu.buf[M.src + i] = b[k];
       }
       U[M.tall ? c * PF + r : r * PF + c] = v[k];
-      big = fmaxf(big, fabsf(v[k]));
+      sum += (double)v[k] * (double)v[k];
     }
   }
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor(big, o, 64));
-  if (lane == 0) red[wave] = big;
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+  if (lane == 0) redd[wave] = sum;
   __syncthreads();                             // (U is whole, too)
+  sum = 0.0;
 #pragma unroll
-  for (int i = 0; i < SMALL_TPB / 64; ++i) big = fmaxf(big, red[i]);
-  int e = 0;
-  if (big > 0.f && big <= 3.4028235e38f) (void)frexpf(big, &e);
-  float v[QUADS][4], ss = 0.f;
+  for (int i = 0; i < SMALL_TPB / 64; ++i) sum += redd[i];
+  const double f = (double)M.scale / (sqrt(sum) + (double)st.eps);
+  float v[QUADS][4];
   const int quads = m16 * n64 / 4, per = n64 / 4;
 #pragma unroll
   for (int b = 0; b < QUADS; ++b) {
     const int i = threadIdx.x + b * SMALL_TPB, r = i / per;
     if (i >= quads) continue;
     const float4 w = *reinterpret_cast<const float4*>(U + r * PF + (i - r * per) * 4);
-    v[b][0] = ldexpf(w.x, -e); v[b][1] = ldexpf(w.y, -e); v[b][2] = ldexpf(w.z, -e); v[b][3] = ldexpf(w.w, -e);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) ss += v[b][k] * v[b][k];
+    v[b][0] = (float)(w.x * f); v[b][1] = (float)(w.y * f); v[b][2] = (float)(w.z * f); v[b][3] = (float)(w.w * f);
   }
-  double sum = ss;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-  if (lane == 0) redd[wave] = sum;
-  __syncthreads();                             // (every read of U is done, too)
-  sum = 0.0;
-#pragma unroll
-  for (int i = 0; i < SMALL_TPB / 64; ++i) sum += redd[i];
-  const float f = (float)ldexp((double)M.scale / (ldexp(sqrt(sum), e) + (double)st.eps), e);
+  __syncthreads();                             // (every read of U is done)
 #pragma unroll
   for (int b = 0; b < QUADS; ++b) {
     const int i = threadIdx.x + b * SMALL_TPB, r = i / per;
-    if (i >= quads) continue;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) v[b][k] *= f;
-    put4(X + pair_at(PX, r, (i - r * per) * 4), v[b]);
+    if (i < quads) put4(X + pair_at(PX, r, (i - r * per) * 4), v[b]);
   }
   __syncthreads();
 
@@ -1091,13 +1079,12 @@ __device__ __forceinline__ void small_matrix(const NsMatrix& M, const DasNsSourc
 template <typename T, bool MUON, int QUADS>
 __global__ __launch_bounds__(SMALL_TPB) void small_kernel(const NsMatrix* __restrict__ mats, Sources src, MuonIn mu, Steps st, Result res) {
   extern __shared__ __align__(16) char smem[];
-  __shared__ float red[SMALL_TPB / 64];
   __shared__ double redd[SMALL_TPB / 64];
   const NsMatrix M = mats[blockIdx.x];
   if (!MUON && (unsigned)(M.group - src.first) >= (unsigned)src.count) return;   // (whole workgroups)
   const DasNsSource& s = src.s[MUON ? 0 : M.group - src.first];
-  if (M.m <= 32) small_matrix<T, MUON, QUADS, 1>(M, s, mu, st, res, smem, red, redd);
-  else small_matrix<T, MUON, QUADS, 2>(M, s, mu, st, res, smem, red, redd);
+  if (M.m <= 32) small_matrix<T, MUON, QUADS, 1>(M, s, mu, st, res, smem, redd);
+  else small_matrix<T, MUON, QUADS, 2>(M, s, mu, st, res, smem, redd);
 }
 
 // A slice of a thin matrix: t.kn pieces of 128 columns from piece t.k0 on. FIRST: X = U's blocks times their exponents and 1 / norm (as
@@ -1212,12 +1199,21 @@ __global__ __launch_bounds__(TPB) void thin_kernel(const NsMatrix* __restrict__ 
     if constexpr (KIND == LAST) {
       const int c0 = piece * THIN_COLS, width = min(THIN_COLS, M.n - c0);
       const long long base = M.tall ? M.src + (long long)c0 * M.cols : M.src + c0;
-      for (int i = threadIdx.x; i < M.m * THIN_COLS; i += TPB) {
+      constexpr int BATCH = 8;
+      for (int i0 = threadIdx.x; i0 < M.m * THIN_COLS; i0 += BATCH * TPB) {
         // tall: the piece is `width` whole rows of the source, one after the other; else THIN_COLS of each of its m rows
-        const int r = M.tall ? i % M.m : i / THIN_COLS, c = M.tall ? i / M.m : i % THIN_COLS;
-        if (c >= width) continue;
-        const long long o = M.tall ? base + i : base + (long long)r * M.cols + c;
-        emit_one<MUON>(res, o, factor * us[r * PTF + c], MUON ? res.p[o] : 0.f);
+        long long o[BATCH];
+        float x[BATCH], old[BATCH];
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+          const int i = i0 + k * TPB, r = M.tall ? i % M.m : i / THIN_COLS, c = M.tall ? i / M.m : i % THIN_COLS;
+          o[k] = i < M.m * THIN_COLS && c < width ? (M.tall ? base + i : base + (long long)r * M.cols + c) : -1;
+          x[k] = o[k] >= 0 ? factor * us[r * PTF + c] : 0.f;
+          old[k] = MUON && o[k] >= 0 ? res.p[o[k]] : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k)
+          if (o[k] >= 0) emit_one<MUON>(res, o[k], x[k], old[k]);
       }
     } else {
 #pragma unroll
@@ -1247,30 +1243,27 @@ __device__ __forceinline__ void chain_matrix(const NsMatrix& M, const f32x4_t* p
   _Float16* A[N_AREAS];
 #pragma unroll
   for (int i = 0; i < N_AREAS; ++i) A[i] = reinterpret_cast<_Float16*>(smem) + i * m16 * PA;
-  f32x4_t* scratch = reinterpret_cast<f32x4_t*>(smem + 2 * N_AREAS * SMALL_M * PA);
   zero_lds(smem, 2 * N_AREAS * m16 * PA, SMALL_TPB);
-  const Share w = Share::of<W>(m16);
-  Frags<W> g = {};
-  if (w.on) {
+  // thread = four values of a fragment; every one adds the slices' parts, eight loads in flight
+  const int frags = n * n;
+  f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
+  if ((int)threadIdx.x < frags * 64) {
+    for (int s0 = 0; s0 < slices; s0 += 8) {
+      f32x4_t v[8];
 #pragma unroll
-    for (int i = 0; i < W; ++i)
+      for (int u = 0; u < 8; ++u) v[u] = s0 + u < slices ? part[(long long)(s0 + u) * frags * 64 + threadIdx.x] : f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int j = 0; j < W; ++j) {
-        const int fi = (w.r0 >> 4) + i, fj = (w.c0 >> 4) + j;
-        if (fi >= n || fj >= n) continue;
-        const f32x4_t* from = part + (fi * n + fj) * 64 + lane;
-        for (int s0 = w.part; s0 < slices; s0 += 4 * w.parts) {
-          f32x4_t v[4];
-#pragma unroll
-          for (int u = 0; u < 4; ++u)
-            v[u] = s0 + u * w.parts < slices ? from[(long long)(s0 + u * w.parts) * n * n * 64] : f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int u = 0; u < 4; ++u) g[i][j] += v[u];
-        }
-      }
+      for (int u = 0; u < 8; ++u) sum += v[u];
+    }
   }
   __syncthreads();
-  store_gram<W>(w, m16, g, scratch, A[0], M.gscale / (M.scale * M.scale));
+  if ((int)threadIdx.x < frags * 64) {
+    const int f = threadIdx.x >> 6, r = (f % n) * 16 + (lane & 15), c = (f / n) * 16 + (lane >> 4) * 4;   // (stored transposed, as frag_store)
+    const float gs = M.gscale / (M.scale * M.scale), v[4] = {sum[0] * gs, sum[1] * gs, sum[2] * gs, sum[3] * gs};
+    put4(A[0] + pair_at(PA, r, c), v);
+  }
+  __syncthreads();
+  const Share w = Share::of<W>(m16);
   const _Float16* q = phase_chain<W>(w, A, st, k, st.end[k], M.gscale, m16);
   for (int i = threadIdx.x; i < M.m * 16; i += SMALL_TPB) {
     const int r = i >> 4, c = i & 15;
@@ -1390,7 +1383,7 @@ int launch_thin(const DasNsPlan* p, const char* tab, const Work& w, const Result
   const NsItem* slices = (const NsItem*)(tab + p->slice_at);
   const int2* thin = (const int2*)(tab + p->thin_at);
   const Steps st = steps_of(p);
-  constexpr int LDS = 2 * N_AREAS * SMALL_M * PA + SMALL_TPB * 16;
+  constexpr int LDS = 2 * N_AREAS * SMALL_M * PA;   // (m = 48: what a second fragment reads past its matrix is inside, too)
   (void)hipFuncSetAttribute((const void*)chain_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
   auto pass = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3(p->n_slices), dim3(TPB), 0, s, mats, slices, p->eps, w.part, w.xt, w.qt, w.thin_part, res);
