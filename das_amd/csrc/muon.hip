@@ -52,7 +52,10 @@ struct NsMatrix {           // one matrix, as the kernels see it
 struct NsItem {             // a workgroup's share: output tile (ti, tj) of a matrix, inner elements 64 k0 ... 64 (k0 + kn)
   int matrix, ti, tj, k0, kn;
   int slot;                 // >= 0: the sums go to this slot of the partial tiles; JOIN items: the first of `slots`
-  int slots, pad;
+  int slots;
+  int m, ldx, lda;          // of the matrix (copied here: a launch starts one load latency earlier than through its index)
+  float scale, gscale;
+  long long x, a;
 };
 struct Partial {            // of one 64 x 64 block: sum of squares of (u 2^-e), and e
   float ss;
@@ -527,7 +530,7 @@ struct SymArgs {            // two independent products a launch (blockIdx.y)
 //   GRAM:     G = X X^T times (gscale / S^2)      POLY: Z = a I + b G + c G G      PRODUCT: P Q of symmetric P, Q that commute
 // Columns m ... lda are stored as zeros: the inner axis of the next product.
 template <int T, bool SPLIT, int KG, SymKind KIND>
-__device__ __forceinline__ void sym_store(const NsMatrix& M, const SymArgs& s, int z, int i0, int j0, const Acc<T>& acc, char* smem) {
+__device__ __forceinline__ void sym_store(const NsItem& M, const SymArgs& s, int z, int i0, int j0, const Acc<T>& acc, char* smem) {
   const _Float16* P = s.p[z] + (SPLIT ? 2 : 1) * M.a;
   _Float16* out = s.out[z] + (SPLIT ? 2 : 1) * M.a;
   const float f = KIND == GRAM ? M.gscale / (M.scale * M.scale) : 1.f, cb = s.b / M.gscale, cc = s.c / (M.gscale * M.gscale);
@@ -552,20 +555,18 @@ __device__ __forceinline__ void sym_store(const NsMatrix& M, const SymArgs& s, i
 }
 
 template <int T, bool SPLIT, int KG, SymKind KIND>
-__global__ __launch_bounds__(KG * TPB, KG == 1 ? 2 : KG) void sym_kernel(const NsMatrix* __restrict__ mats, const NsItem* __restrict__ items,
-                                                                         SymArgs s, f32x4_t* __restrict__ partial) {
+__global__ __launch_bounds__(KG * TPB, KG == 1 ? 2 : KG) void sym_kernel(const NsItem* __restrict__ items, SymArgs s, f32x4_t* __restrict__ partial) {
   extern __shared__ __align__(16) char smem[];
   const NsItem t = items[blockIdx.x];
   if (t.matrix < 0) return;   // (filling: an XCD's queue is shorter than the longest)
-  const NsMatrix M = mats[t.matrix];
   const int z = blockIdx.y, i0 = t.ti * T, j0 = t.tj * T;
-  const int ld = KIND == GRAM ? M.ldx : M.lda, pitch = SPLIT ? 2 * ld : ld;
-  const _Float16* P = s.p[z] + (SPLIT ? 2 : 1) * (KIND == GRAM ? M.x : M.a);
-  const _Float16* Q = s.q[z] + (SPLIT ? 2 : 1) * (KIND == GRAM ? M.x : M.a);
+  const int ld = KIND == GRAM ? t.ldx : t.lda, pitch = SPLIT ? 2 * ld : ld;
+  const _Float16* P = s.p[z] + (SPLIT ? 2 : 1) * (KIND == GRAM ? t.x : t.a);
+  const _Float16* Q = s.q[z] + (SPLIT ? 2 : 1) * (KIND == GRAM ? t.x : t.a);
   RowsOperand<T> a, b;
   const int stages = (SPLIT ? 2 : 1) * t.kn, first = (SPLIT ? 2 : 1) * t.k0 + first_stage<KG>(stages);
-  a.init(P, pitch, i0, M.m, first);
-  b.init(Q, pitch, j0, M.m, first);
+  a.init(P, pitch, i0, t.m, first);
+  b.init(Q, pitch, j0, t.m, first);
   Acc<T> acc;
   multiply<T, SPLIT, KG>(a, b, stages, smem, acc);
   if (T == JOIN_TILE && t.slot >= 0) {   // (a part of the inner axis: join_kernel goes on)
@@ -577,17 +578,16 @@ __global__ __launch_bounds__(KG * TPB, KG == 1 ? 2 : KG) void sym_kernel(const N
     }
     return;
   }
-  sym_store<T, SPLIT, KG, KIND>(M, s, z, i0, j0, acc, smem);
+  sym_store<T, SPLIT, KG, KIND>(t, s, z, i0, j0, acc, smem);
 }
 
 // The parts of a tile whose inner axis was split, added in order, and stored as sym_store does; 16 workgroups a tile, four rows of one
 // column a thread (one workgroup a tile: 12 us, most of them waiting for one load after the other).
 template <bool SPLIT, SymKind KIND>
-__global__ __launch_bounds__(TPB) void join_kernel(const NsMatrix* __restrict__ mats, const NsItem* __restrict__ items, SymArgs s,
+__global__ __launch_bounds__(TPB) void join_kernel(const NsItem* __restrict__ items, SymArgs s,
                                                    const f32x4_t* __restrict__ partial) {
   constexpr int N = JOIN_TILE / 32, W = SPLIT ? 2 : 1;
   const NsItem t = items[blockIdx.x / (N * N)];
-  const NsMatrix M = mats[t.matrix];
   const int frag = blockIdx.x % (N * N), z = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const f32x4_t* from = partial + (((long long)z * s.slots + t.slot) * N * N + frag) * TPB + threadIdx.x;
   f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
@@ -600,30 +600,30 @@ __global__ __launch_bounds__(TPB) void join_kernel(const NsMatrix* __restrict__ 
   }
   const int r = t.ti * JOIN_TILE + (wave >> 1) * (JOIN_TILE / 2) + (frag / N) * 16 + (lane >> 4) * 4;   // four rows of one column
   const int c = t.tj * JOIN_TILE + (wave & 1) * (JOIN_TILE / 2) + (frag % N) * 16 + (lane & 15);
-  if (r >= M.lda) return;
-  _Float16* out = s.out[z] + W * M.a;
+  if (r >= t.lda) return;
+  _Float16* out = s.out[z] + W * t.a;
   float v[4] = {sum[0], sum[1], sum[2], sum[3]};
   if constexpr (KIND == GRAM) {
-    const float f = M.gscale / (M.scale * M.scale);
+    const float f = t.gscale / (t.scale * t.scale);
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] *= f;
   }
   if constexpr (KIND == POLY) {
-    const float cb = s.b / M.gscale, cc = s.c / (M.gscale * M.gscale);
+    const float cb = s.b / t.gscale, cc = s.c / (t.gscale * t.gscale);
     float g[4] = {0.f, 0.f, 0.f, 0.f};
-    if (c < M.m) get<SPLIT>(s.p[0] + W * M.a, M.lda, c, r, g);
+    if (c < t.m) get<SPLIT>(s.p[0] + W * t.a, t.lda, c, r, g);
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = cc * v[e] + cb * g[e] + (r + e == c ? s.a : 0.f);
   }
 #pragma unroll
   for (int e = 0; e < 4; ++e)
-    if (r + e >= M.m || c >= M.m) v[e] = 0.f;
-  if (c < M.m) put<SPLIT>(out, M.lda, c, r, v);
+    if (r + e >= t.m || c >= t.m) v[e] = 0.f;
+  if (c < t.m) put<SPLIT>(out, t.lda, c, r, v);
   if (t.ti == t.tj) return;   // (a diagonal tile holds both halves)
 #pragma unroll
   for (int e = 0; e < 4; ++e)
-    if (r + e < M.m && c < M.lda) {
-      _Float16* p = out + at<SPLIT>(M.lda, r + e, c);
+    if (r + e < t.m && c < t.lda) {
+      _Float16* p = out + at<SPLIT>(t.lda, r + e, c);
       p[0] = (_Float16)v[e];
       if constexpr (SPLIT) p[32] = (_Float16)(v[e] - (float)p[0]);
     }
@@ -653,21 +653,21 @@ __global__ __launch_bounds__(KG * TPB, KG == 1 ? 2 : KG) void update_kernel(cons
   extern __shared__ __align__(16) char smem[];
   const NsItem t = items[blockIdx.x];
   if (t.matrix < 0) return;
-  const NsMatrix M = mats[t.matrix];
   const int i0 = t.ti * T, j0 = t.tj * T;
   constexpr int W = SPLIT ? 2 : 1;
   RowsOperand<T> a;
   ColsOperand<T, SPLIT> b;
   const int stages = W * t.kn, first = first_stage<KG>(stages);
-  a.init(Q + W * M.a, W * M.lda, i0, M.m, first);
-  b.init(X + W * M.x, W * M.ldx, j0, M.m, first);
+  a.init(Q + W * t.a, W * t.lda, i0, t.m, first);
+  b.init(X + W * t.x, W * t.ldx, j0, t.m, first);
   Acc<T> acc;
   multiply<T, SPLIT, KG>(a, b, stages, smem, acc);
   if constexpr (!LAST) {
     store_tile<T, KG, false>(acc, smem, [&](int r, int c, float (&v)[8]) {
-      if (i0 + r < M.m) put<SPLIT>(Y + W * M.x, M.ldx, i0 + r, j0 + c, v);   // (columns n ... ldx: zero, as X's are)
+      if (i0 + r < t.m) put<SPLIT>(Y + W * t.x, t.ldx, i0 + r, j0 + c, v);   // (columns n ... ldx: zero, as X's are)
     });
   } else {
+    const NsMatrix M = mats[t.matrix];
     const float f = result_factor(M, res);
     const bool vec = M.cols % 8 == 0 && M.src % 8 == 0 && !((uintptr_t)(res.p ? (const void*)res.p : res.out) & 15);
     auto emit = [&](int r, int c, float (&v)[8]) {   // in the caller's rows and columns
@@ -1410,7 +1410,7 @@ int iterate(const DasNsPlan* p, const char* tab, Work w, const Result& res, hipS
   auto launch_sym = [&](auto kernel, int tile, int kg, const NsItem* items, int n, int products, const SymArgs& a) {
     const int lds = kg * 4 * tile * 128;
     (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    hipLaunchKernelGGL(kernel, dim3(n, products), dim3(kg * TPB), lds, s, mats, items, a, w.slots);
+    hipLaunchKernelGGL(kernel, dim3(n, products), dim3(kg * TPB), lds, s, items, a, w.slots);
   };
   constexpr int JOINERS = (JOIN_TILE / 32) * (JOIN_TILE / 32);
   auto gram_of = [&](const _Float16* x, _Float16* g) {
@@ -1418,7 +1418,7 @@ int iterate(const DasNsPlan* p, const char* tab, Work w, const Result& res, hipS
     if (p->gram_kg == 2) launch_sym(sym_kernel<JOIN_TILE, SPLIT, 2, GRAM>, JOIN_TILE, 2, gram, p->n_gram, 1, a);
     else launch_sym(sym_kernel<JOIN_TILE, SPLIT, 1, GRAM>, JOIN_TILE, 1, gram, p->n_gram, 1, a);
     if (p->n_gram_join)
-      hipLaunchKernelGGL((join_kernel<SPLIT, GRAM>), dim3(p->n_gram_join * JOINERS), dim3(TPB), 0, s, mats, gram_join, a, w.slots);
+      hipLaunchKernelGGL((join_kernel<SPLIT, GRAM>), dim3(p->n_gram_join * JOINERS), dim3(TPB), 0, s, gram_join, a, w.slots);
   };
   auto sym = [&](auto kind, int products, SymArgs a) {
     constexpr SymKind K = decltype(kind)::value;
@@ -1426,7 +1426,7 @@ int iterate(const DasNsPlan* p, const char* tab, Work w, const Result& res, hipS
     if (p->product_tile == 128) launch_sym(sym_kernel<128, SPLIT, 1, K>, 128, 1, prod, p->n_product, products, a);
     else launch_sym(sym_kernel<64, SPLIT, 4, K>, 64, 4, prod, p->n_product, products, a);
     if (p->n_product_join)
-      hipLaunchKernelGGL((join_kernel<SPLIT, K>), dim3(p->n_product_join * JOINERS, products), dim3(TPB), 0, s, mats, prod_join, a, w.slots);
+      hipLaunchKernelGGL((join_kernel<SPLIT, K>), dim3(p->n_product_join * JOINERS, products), dim3(TPB), 0, s, prod_join, a, w.slots);
   };
   auto update = [&](auto last, const _Float16* q, const _Float16* x, _Float16* y) {
     constexpr bool L = decltype(last)::value;
@@ -1538,6 +1538,10 @@ struct Tables {
   Launch gram, product, update;
   std::vector<NsItem> gram_join, product_join, slices;
   std::vector<int2> thin;    // first slice and slices of each thin matrix
+  NsItem item(int q, int ti, int tj, int k0, int kn, int slot, int slots) const {
+    const NsMatrix& M = mats[q];
+    return NsItem{q, ti, tj, k0, kn, slot, slots, M.m, M.ldx, M.lda, M.scale, M.gscale, M.x, M.a};
+  }
 };
 
 struct Tile {
@@ -1565,7 +1569,8 @@ long long makespan(const std::vector<int>& pieces, int slots, long long limit, s
 // of traffic, the join a launch: 0.0125 and 1.2 steps of 64 inner elements (2.5 us with two workgroups on a CU; 13 us measured for 272
 // parts). A workgroup whose neighbour on the CU has ended runs up to twice as fast, so only half of what sticks out counts. A part has
 // at least 4 steps.
-void schedule(const std::vector<Tile>& tiles, int slots, Launch& launch, std::vector<NsItem>& join, long long& n_slots) {
+void schedule(const Tables& tab, const std::vector<Tile>& tiles, int slots, Launch& launch, std::vector<NsItem>& join, long long& n_slots) {
+  auto item = [&](auto... v) { return tab.item(v...); };
   std::vector<int> order(tiles.size()), parts(tiles.size(), 1), late;
   for (size_t i = 0; i < tiles.size(); ++i) order[i] = (int)i;
   std::stable_sort(order.begin(), order.end(), [&](int u, int v) { return tiles[u].steps > tiles[v].steps; });
@@ -1582,7 +1587,7 @@ void schedule(const std::vector<Tile>& tiles, int slots, Launch& launch, std::ve
     std::vector<char> is_late(tiles.size(), 0);
     for (int k : late) is_late[k] = 1;
     int choice = 1;
-    for (int p : {2, 3, 4, 6, 8, 12, 16}) {
+    for (int p : {2, 3, 4, 5, 6, 7, 8, 10, 12, 14, 16}) {
       std::vector<int> pieces;
       long long count = 0;
       for (size_t k = 0; k < order.size(); ++k) {
@@ -1606,7 +1611,7 @@ void schedule(const std::vector<Tile>& tiles, int slots, Launch& launch, std::ve
     const Tile& t = tiles[i];
     fresh |= t.fresh;
     if (parts[i] > 1) continue;
-    launch.add(fresh, NsItem{t.matrix, t.ti, t.tj, 0, t.steps, -1, 1, 0});
+    launch.add(fresh, item(t.matrix, t.ti, t.tj, 0, t.steps, -1, 1));
     fresh = false;
   }
   for (size_t i = 0; i < tiles.size();) {
@@ -1618,7 +1623,7 @@ void schedule(const std::vector<Tile>& tiles, int slots, Launch& launch, std::ve
       if (parts[k] == 1) continue;
       most = std::max(most, parts[k]);
       slot[k - i] = (int)n_slots;
-      join.push_back(NsItem{tiles[k].matrix, tiles[k].ti, tiles[k].tj, 0, tiles[k].steps, (int)n_slots, parts[k], 0});
+      join.push_back(item(tiles[k].matrix, tiles[k].ti, tiles[k].tj, 0, tiles[k].steps, (int)n_slots, parts[k]));
       n_slots += parts[k];
     }
     for (int j = 0; j < most && most > 1; ++j) {
@@ -1627,7 +1632,7 @@ void schedule(const std::vector<Tile>& tiles, int slots, Launch& launch, std::ve
         const int q = parts[k];
         if (q == 1 || j >= q) continue;
         const int k0 = (int)((long long)tiles[k].steps * j / q), k1 = (int)((long long)tiles[k].steps * (j + 1) / q);
-        launch.add(first, NsItem{tiles[k].matrix, tiles[k].ti, tiles[k].tj, k0, k1 - k0, slot[k - i] + j, 1, 0});
+        launch.add(first, item(tiles[k].matrix, tiles[k].ti, tiles[k].tj, k0, k1 - k0, slot[k - i] + j, 1));
         first = false;
       }
     }
@@ -1712,7 +1717,9 @@ bool build(const DasNsShape* shapes, int n, double top, DasNsPlan* plan, Tables&
             const int pieces = M.ldx / THIN_COLS, per = over(pieces, 64), frags = up16(M.m) * up16(M.m) / 256;
             t.thin.push_back(make_int2((int)t.slices.size(), over(pieces, per)));
             for (int p = 0; p < pieces; p += per) {
-              t.slices.push_back(NsItem{q, 0, 0, p, std::min(per, pieces - p), (int)plan->thin_slots, frags, 0});
+              NsItem piece = {};
+              piece.matrix = q; piece.k0 = p; piece.kn = std::min(per, pieces - p); piece.slot = (int)plan->thin_slots; piece.slots = frags;
+              t.slices.push_back(piece);
               plan->thin_slots += frags;
             }
           }
@@ -1753,13 +1760,13 @@ bool build(const DasNsShape* shapes, int n, double top, DasNsPlan* plan, Tables&
     for (int bj = 0; bj < cols; bj += side)
       for (int bi = 0; bi < rows; bi += side)
         for (int j = bj; j < std::min(cols, bj + side); ++j)
-          for (int i = bi; i < std::min(rows, bi + side); ++i) t.update.add(i == bi && j == bj, NsItem{q, i, j, 0, M.lda / 64, -1, 1, 0});
+          for (int i = bi; i < std::min(rows, bi + side); ++i) t.update.add(i == bi && j == bj, t.item(q, i, j, 0, M.lda / 64, -1, 1));
   }
-  schedule(gram, plan->gram_kg == 1 ? 512 : 256, t.gram, t.gram_join, plan->gram_slots);
+  schedule(t, gram, plan->gram_kg == 1 ? 512 : 256, t.gram, t.gram_join, plan->gram_slots);
   if (plan->product_tile == JOIN_TILE) {
-    schedule(product, 512, t.product, t.product_join, plan->product_slots);
+    schedule(t, product, 512, t.product, t.product_join, plan->product_slots);
   } else {
-    for (const Tile& p : product) t.product.add(p.fresh, NsItem{p.matrix, p.ti, p.tj, 0, p.steps, -1, 1, 0});
+    for (const Tile& p : product) t.product.add(p.fresh, t.item(p.matrix, p.ti, p.tj, 0, p.steps, -1, 1));
     t.product.place();
   }
   t.update.place();

@@ -12,7 +12,8 @@ COEF = (3.4445, -4.7750, 2.0315)
 MAT = np.dtype([('src', '<i8'), ('x', '<i8'), ('a', '<i8'), ('rows', '<i4'), ('cols', '<i4'), ('m', '<i4'), ('n', '<i4'), ('ldx', '<i4'),
                 ('lda', '<i4'), ('group', '<i4'), ('index', '<i4'), ('chunk0', '<i4'), ('chunks', '<i4'), ('scale', '<f4'),
                 ('gscale', '<f4'), ('tall', '<i4'), ('thin', '<i4')])
-ITEM = np.dtype([(k, '<i4') for k in ('matrix', 'ti', 'tj', 'k0', 'kn', 'slot', 'slots', 'pad')])
+ITEM = np.dtype([(k, '<i4') for k in ('matrix', 'ti', 'tj', 'k0', 'kn', 'slot', 'slots', 'm', 'ldx', 'lda')] +
+                [('scale', '<f4'), ('gscale', '<f4'), ('x', '<i8'), ('a', '<i8')])
 
 
 def make_plan(shapes, steps=5, coef=COEF, offsets=None, eps=1e-7):
@@ -70,6 +71,7 @@ def test_schedule_covers_every_product_once(shapes):
             if t['matrix'] < 0:
                 continue
             assert t['kn'] > 0 and t['ti'] >= t['tj']
+            assert all(t[k] == mats[t['matrix']][k] for k in ('m', 'ldx', 'lda', 'scale', 'gscale', 'x', 'a'))
             seen.setdefault((t['matrix'], t['ti'], t['tj']), []).append((t['k0'], t['kn'], t['slot']))
         joins = {(t['matrix'], t['ti'], t['tj']): t for t in table(buf, join_at, n_join, ITEM)}
         want = {(q, i, j) for q in range(plan.n_small, end) for i in range(-(-mats[q]['m'] // tile)) for j in range(i + 1)}
