@@ -22,6 +22,8 @@
 #include <cmath>
 #include <cstring>
 #include <functional>
+#include <mutex>
+#include <new>
 #include <queue>
 #include <type_traits>
 #include <vector>
@@ -1352,6 +1354,92 @@ int phase_end(const Bounds* bound, int steps, int k) {
   return end;
 }
 
+// A second stream for the small and thin matrices of a set that holds others too: a chain of short launches that leaves the GPU nearly empty,
+// beside the tiles' launches instead of before them (fork and join by events; the caller's stream waits for the end). Streams of
+// default priority, from a pool: one call has one for itself. A call that is being captured stays on its stream.
+struct Side {
+  int dev = 0;
+  hipStream_t stream = nullptr;
+  hipEvent_t fork = nullptr, ready = nullptr, join = nullptr;
+};
+class Fork {
+ public:
+  Fork(hipStream_t main, bool wanted) : main_(main) {
+    if (!wanted) return;
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(main, &st) != hipSuccess) {
+      (void)hipGetLastError();
+      return;
+    }
+    if (st != hipStreamCaptureStatusNone) return;
+    side_ = take();
+    if (side_ && (hipEventRecord(side_->fork, main) != hipSuccess || hipStreamWaitEvent(side_->stream, side_->fork, 0) != hipSuccess)) {
+      (void)hipGetLastError();
+      give(side_);
+      side_ = nullptr;
+    }
+  }
+  ~Fork() { (void)finish(); }
+  hipStream_t stream() const { return side_ ? side_->stream : main_; }
+  // what the main stream has done so far comes before what the side stream does next
+  bool follow() {
+    return !side_ || (hipEventRecord(side_->ready, main_) == hipSuccess && hipStreamWaitEvent(side_->stream, side_->ready, 0) == hipSuccess);
+  }
+  int finish() {
+    if (!side_) return DAS_OK;
+    const bool ok = hipEventRecord(side_->join, side_->stream) == hipSuccess && hipStreamWaitEvent(main_, side_->join, 0) == hipSuccess;
+    if (!ok) (void)hipStreamSynchronize(side_->stream);   // (nothing of this call may run on after it is reported done)
+    give(side_);
+    side_ = nullptr;
+    return ok ? DAS_OK : DAS_ERR_LAUNCH;
+  }
+
+ private:
+  static std::mutex& mutex() {
+    static std::mutex m;
+    return m;
+  }
+  static std::vector<Side*>& pool() {
+    static std::vector<Side*>* p = new std::vector<Side*>;   // (lives as long as the process: streams outlast static destructors)
+    return *p;
+  }
+  static Side* take() {
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess) return nullptr;
+    {
+      std::lock_guard<std::mutex> lock(mutex());
+      auto& p = pool();
+      for (size_t i = 0; i < p.size(); ++i)
+        if (p[i]->dev == dev) {
+          Side* s = p[i];
+          p.erase(p.begin() + i);
+          return s;
+        }
+    }
+    Side* s = new (std::nothrow) Side;
+    if (!s) return nullptr;
+    s->dev = dev;
+    if (hipStreamCreateWithFlags(&s->stream, hipStreamNonBlocking) != hipSuccess ||
+        hipEventCreateWithFlags(&s->fork, hipEventDisableTiming) != hipSuccess ||
+        hipEventCreateWithFlags(&s->ready, hipEventDisableTiming) != hipSuccess ||
+        hipEventCreateWithFlags(&s->join, hipEventDisableTiming) != hipSuccess) {
+      (void)hipGetLastError();
+      delete s;          // (a device that gives no stream: the call goes on without)
+      return nullptr;
+    }
+    return s;
+  }
+  static void give(Side* s) {
+    std::lock_guard<std::mutex> lock(mutex());
+    pool().push_back(s);
+  }
+  hipStream_t main_;
+  Side* side_ = nullptr;
+};
+// Beside tiles it pays (seven small and thin matrices with two of 129 x 1023 and 700 x 513: 204 -> 177 us), beside thin matrices alone the
+// fork costs more than it hides (60 -> 85 us for five small and thin ones).
+bool worth_a_fork(const DasNsPlan* p) { return p->n_tile_chunks > 0 && p->n_small + p->n_thin > 0; }
+
 Steps steps_of(const DasNsPlan* p) {
   Steps st;
   memcpy(st.coef, p->coef, sizeof(st.coef));
@@ -1440,7 +1528,6 @@ int iterate(const DasNsPlan* p, const char* tab, Work w, const Result& res, hipS
   };
   const std::integral_constant<SymKind, POLY> poly_k;
   const std::integral_constant<SymKind, PRODUCT> product_k;
-  if (p->n_tile_chunks == 0) return DAS_OK;
   hipLaunchKernelGGL(normalise_kernel<SPLIT>, dim3(p->n_tile_chunks), dim3(TPB), 0, s, mats, chunks, p->eps, w.x[0], w.part);
   DAS_CHECK_LAUNCH();
   _Float16 *X = w.x[0], *Y = w.x[1], *G = w.a[0], *R = w.a[1], *Z = w.a[SPLIT ? 2 : 1];
@@ -1474,6 +1561,20 @@ int iterate(const DasNsPlan* p, const char* tab, Work w, const Result& res, hipS
   return DAS_OK;
 }
 
+
+// thin and tiled matrices after ingest_kernel, and the join with the small ones
+template <bool SPLIT, bool MUON>
+int the_rest(const DasNsPlan* p, const char* tab, const Work& w, const Result& res, hipStream_t s, Fork& fork) {
+  int st = DAS_OK;
+  if (p->n_thin) {
+    const bool beside = p->n_tile_chunks > 0;   // (else they have the caller's stream to themselves)
+    if (beside && !fork.follow()) return DAS_ERR_LAUNCH;
+    st = launch_thin<MUON>(p, tab, w, res, beside ? fork.stream() : s);
+  }
+  if (st == DAS_OK && p->n_tile_chunks) st = iterate<SPLIT>(p, tab, w, res, s);
+  const int joined = fork.finish();
+  return st != DAS_OK ? st : joined;
+}
 
 // Items of one launch. The hardware deals workgroups to the 8 XCDs in turn, and every XCD has its own 4 MiB L2: tiles that share rows
 // or columns are kept together in a group, the XCDs' queues are filled evenly, longest inner axis first, and then
@@ -1847,6 +1948,7 @@ extern "C" int das_orthogonalize(const DasNsPlan* plan, const void* tables_dev, 
   const int4* chunks = (const int4*)(tab + plan->chunk_at);
   const MuonIn none = {};
   const Result res = {out, out_dtype, nullptr, 1.f, 0.f, 0};
+  Fork fork(s, worth_a_fork(plan));
   // one launch for every 64 source tensors (one in all but unusual sets): its workgroups of other tensors' blocks end at once
   for (int first = 0; first < n_srcs; first += Sources::MAX) {
     Sources a;
@@ -1854,9 +1956,9 @@ extern "C" int das_orthogonalize(const DasNsPlan* plan, const void* tables_dev, 
     a.count = std::min(Sources::MAX, n_srcs - first);
     for (int i = 0; i < Sources::MAX; ++i) a.s[i] = srcs[first + std::min(i, a.count - 1)];
     int st = DAS_OK;
-    if (in_dtype == DAS_F32) st = launch_small<float, false>(plan, tab, a, none, res, s);
-    else if (in_dtype == DAS_BF16) st = launch_small<bf16_t, false>(plan, tab, a, none, res, s);
-    else st = launch_small<_Float16, false>(plan, tab, a, none, res, s);
+    if (in_dtype == DAS_F32) st = launch_small<float, false>(plan, tab, a, none, res, fork.stream());
+    else if (in_dtype == DAS_BF16) st = launch_small<bf16_t, false>(plan, tab, a, none, res, fork.stream());
+    else st = launch_small<_Float16, false>(plan, tab, a, none, res, fork.stream());
     if (st != DAS_OK) return st;
     if (plan->n_chunks == 0) continue;
     auto launch = [&](auto kernel) {
@@ -1867,10 +1969,7 @@ extern "C" int das_orthogonalize(const DasNsPlan* plan, const void* tables_dev, 
     else split ? launch(ingest_kernel<_Float16, false, true>) : launch(ingest_kernel<_Float16, false, false>);
     DAS_CHECK_LAUNCH();
   }
-  if (plan->n_chunks == 0) return DAS_OK;
-  const int st = launch_thin<false>(plan, tab, w, res, s);
-  if (st != DAS_OK) return st;
-  return split ? iterate<true>(plan, tab, w, res, s) : iterate<false>(plan, tab, w, res, s);
+  return split ? the_rest<true, false>(plan, tab, w, res, s, fork) : the_rest<false, false>(plan, tab, w, res, s, fork);
 }
 
 extern "C" int das_muon_step(const DasNsPlan* plan, const void* tables_dev, float* p, const float* g, float* buf, float lr,
@@ -1886,11 +1985,13 @@ extern "C" int das_muon_step(const DasNsPlan* plan, const void* tables_dev, floa
   const Work w = carve(plan, true, ws);
   const MuonIn mu = {g, buf, momentum, grad_scale, max_norm, nesterov, grad_sumsq};
   const Result res = {nullptr, 0, p, (float)(1.0 - (double)lr * (double)weight_decay), lr, lr_scale};
-  const int st = launch_small<float, true>(plan, tab, Sources{}, mu, res, s);
-  if (st != DAS_OK || plan->n_chunks == 0) return st;
-  hipLaunchKernelGGL((ingest_kernel<float, true, true>), dim3(plan->n_chunks), dim3(TPB), 0, s, (const NsMatrix*)(tab + plan->mat_at),
-                     (const int4*)(tab + plan->chunk_at), Sources{}, mu, w.x[0], w.xt, w.part);
-  DAS_CHECK_LAUNCH();
-  const int thin = launch_thin<true>(plan, tab, w, res, s);
-  return thin != DAS_OK ? thin : iterate<true>(plan, tab, w, res, s);
+  Fork fork(s, worth_a_fork(plan));
+  const int st = launch_small<float, true>(plan, tab, Sources{}, mu, res, fork.stream());
+  if (st != DAS_OK) return st;
+  if (plan->n_chunks) {
+    hipLaunchKernelGGL((ingest_kernel<float, true, true>), dim3(plan->n_chunks), dim3(TPB), 0, s, (const NsMatrix*)(tab + plan->mat_at),
+                       (const int4*)(tab + plan->chunk_at), Sources{}, mu, w.x[0], w.xt, w.part);
+    DAS_CHECK_LAUNCH();
+  }
+  return the_rest<true, true>(plan, tab, w, res, s, fork);
 }

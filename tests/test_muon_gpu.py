@@ -201,6 +201,54 @@ def test_orthogonalize_large_tiles():
                 check(y[i], t[i], [COEF] * 5, what=(tuple(t.shape), i))
 
 
+def test_mixed_set_from_threads_streams_and_a_graph():
+    """a set of every class (one workgroup, slices, tiles): the same bits alone, from two host threads on streams of their own at once, back to
+    back on one stream with its input overwritten in between, and replayed"""
+    import threading
+    from das_amd import train_ops as T
+    mats = [gradient(64, 64, 1, k=3), gradient(30, 3000, 2, k=2), gradient(200, 333, 3, k=2), gradient(5000, 12, 4)]
+    plan = T.NewtonSchulzPlan([tuple(t.shape) for t in mats], DEV)
+    for dt in (torch.bfloat16, torch.float32):
+        want = T.orthogonalize(mats, plan=plan, out_dtype=dt)
+        twice = [t * 2 for t in mats]
+        want2 = T.orthogonalize(twice, plan=plan, out_dtype=dt)
+        for t, y in zip(mats, want):
+            for i in range(y.shape[0] if y.dim() == 3 else 1):
+                check(y[i] if y.dim() == 3 else y, t[i] if y.dim() == 3 else t, [COEF] * 5)
+        torch.cuda.synchronize()
+        wrong = []
+
+        def work(src, ref):
+            s = torch.cuda.Stream()
+            with torch.cuda.stream(s):
+                buf = [t.clone() for t in src]
+                got = []
+                for _ in range(20):
+                    got.append(T.orthogonalize(buf, plan=plan, out_dtype=dt))
+                    for b, t in zip(buf, src):      # (the call's own work is ordered before this)
+                        b.zero_()
+                        b.copy_(t)
+            s.synchronize()
+            wrong.extend(1 for g in got for a, b in zip(g, ref) if not torch.equal(a, b))
+        ts = [threading.Thread(target=work, args=a) for a in ((mats, want), (twice, want2))]
+        for t in ts:
+            t.start()
+        for t in ts:
+            t.join()
+        assert not wrong
+        static, g = [t.clone() for t in mats], torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = T.orthogonalize(static, plan=plan, out_dtype=dt)
+        for src, ref in ((twice, want2), (mats, want), (twice, want2)):
+            for a, b in zip(static, src):
+                a.copy_(b)
+            g.replay()
+            eager = T.orthogonalize(src, plan=plan, out_dtype=dt)
+            torch.cuda.synchronize()
+            for a, b, c in zip(out, eager, ref):
+                assert torch.equal(a, c) and torch.equal(b, c)
+
+
 def test_plan_serves_two_streams_and_a_graph():
     from das_amd import train_ops as T
     u, v = gradient(256, 300, 1), gradient(256, 300, 2)
