@@ -727,9 +727,9 @@ __global__ __launch_bounds__(KG * TPB, KG == 1 ? 2 : KG) void update_kernel(cons
 // all steps of a phase on the m x m matrices in LDS and leaves Q; the pass over the slices that forms Q X also forms the parts of the next
 // X X^T: five launches after the first pass (16 x 1056 by tiles: 85 us).
 //
-// 16 waves. m <= 32: one 16 x 16 fragment of an m x m product a wave, all inner elements in one instruction; waves left over divide the long
-// inner axis of X X^T. m > 32: four waves with 2 x 2 fragments each (one a wave reads every operand four times from LDS: 0.9 us a
-// product instead of 0.5). LDS matrices: rows of pairs (32 high parts, 32 low parts, ...), row pitch 16 bytes past a multiple of 256;
+// 16 waves, one 16 x 16 fragment of an m x m product a wave (2 x 2 fragments each on four waves: 20.4 us for 64 x 64 instead of 19.8,
+// the flows' and predictors' set, up to 64 x 256, 31.7 us instead of 25.0: one wave a SIMD hides no latency). m <= 32 leaves waves over: they divide the long inner axis of X X^T,
+// and Z Q and Z G are formed by different ones. LDS matrices: rows of pairs (32 high parts, 32 low parts, ...), row pitch 16 bytes past a multiple of 256;
 // 32 columns of X take 128 bytes as pairs and as floats: U, X and the result use the same place. Rows and columns up to the next
 // multiple of 16 are zero.
 constexpr int SMALL_M = 64, SMALL_TPB = 1024, SMALL_LDS = 155 * 1024;
@@ -743,11 +743,9 @@ struct Steps {
 };
 __host__ __device__ inline int up16(int m) { return (m + 15) & ~15; }
 __host__ __device__ inline int up64(int n) { return (n + 63) & ~63; }
-// X, the m x m matrices, and behind them room for the shares of a sum (W = 1; not over the m x m matrices: m <= 16 reads 32 columns of them,
-// 16 of them zero) or for the rows that a second fragment past m = 48 reads for nothing
-inline long long small_lds(int m, int n) {
-  return 2LL * up16(m) * (2 * up64(n) + 8 + N_AREAS * PA) + (m <= 32 ? SMALL_TPB * 16 : up16(m) == 48 ? 2 * 16 * PA : 0);
-}
+// X, the m x m matrices, and behind them room for the shares of a sum (not over the m x m matrices: m <= 16 reads 32 columns of them,
+// 16 of them zero)
+inline long long small_lds(int m, int n) { return 2LL * up16(m) * (2 * up64(n) + 8 + N_AREAS * PA) + (m <= 32 ? SMALL_TPB * 16 : 0); }
 
 __device__ __forceinline__ f16x8_t row_frag(const _Float16* p, int pitch, int row0, int k, int part) {
   const int lane = threadIdx.x & 63;
@@ -766,64 +764,40 @@ __device__ __forceinline__ f16x8_t col_frag(const _Float16* x, int pitch, int ro
   }
   return f;
 }
-// W x W fragments: P's rows from row0 by (Q's rows from q0, or its columns from q0), inner steps of 32: k0, k0 + stride, ... < k1
-template <int W>
-using Frags = f32x4_t[W][W];
-template <int W, bool COLS>
-__device__ __forceinline__ void frag_step(const _Float16* p, int pp, int row0, const _Float16* q, int qp, int q_rows, int q0, int k, Frags<W>& high,
-                                          Frags<W>& low) {
-  f16x8_t fa[W][2], fb[W][2];
+// One fragment: P's rows from row0 by (Q's rows from q0, or its columns from q0), an inner step of 32. Two chains of sums
+template <bool COLS>
+__device__ __forceinline__ void frag_step(const _Float16* p, int pp, int row0, const _Float16* q, int qp, int q_rows, int q0, int k, f32x4_t& high,
+                                          f32x4_t& low) {
+  f16x8_t a[2], b[2];
 #pragma unroll
-  for (int t = 0; t < W; ++t)
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      fa[t][u] = row_frag(p, pp, row0 + t * 16, k, u);
-      fb[t][u] = COLS ? col_frag(q, qp, q_rows, q0 + t * 16, k, u) : row_frag(q, qp, q0 + t * 16, k, u);
-    }
-#pragma unroll
-  for (int i = 0; i < W; ++i)
-#pragma unroll
-    for (int j = 0; j < W; ++j) {   // (two chains)
-      high[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa[i][0], fb[j][0], high[i][j], 0, 0, 0);
-      low[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa[i][1], fb[j][0], low[i][j], 0, 0, 0);
-      low[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa[i][0], fb[j][1], low[i][j], 0, 0, 0);
-    }
+  for (int u = 0; u < 2; ++u) {
+    a[u] = row_frag(p, pp, row0, k, u);
+    b[u] = COLS ? col_frag(q, qp, q_rows, q0, k, u) : row_frag(q, qp, q0, k, u);
+  }
+  high = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[0], b[0], high, 0, 0, 0);
+  low = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[1], b[0], low, 0, 0, 0);
+  low = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[0], b[1], low, 0, 0, 0);
 }
-template <int W, int K>   // K inner steps, unrolled
-__device__ __forceinline__ void square_product(const _Float16* p, int row0, const _Float16* q, int q0, Frags<W>& acc) {
-  Frags<W> low = {};
+template <int K>   // m x m matrices, K inner steps
+__device__ __forceinline__ f32x4_t square_product(const _Float16* p, int row0, const _Float16* q, int q0) {
+  f32x4_t acc = {}, low = {};
 #pragma unroll
-  for (int i = 0; i < W; ++i)
-#pragma unroll
-    for (int j = 0; j < W; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int k = 0; k < K; ++k) frag_step<W, false>(p, PA, row0, q, PA, 0, q0, k, acc, low);
-#pragma unroll
-  for (int i = 0; i < W; ++i)
-#pragma unroll
-    for (int j = 0; j < W; ++j) acc[i][j] += low[i][j];
+  for (int k = 0; k < K; ++k) frag_step<false>(p, PA, row0, q, PA, 0, q0, k, acc, low);
+  return acc + low;
 }
-template <int W, bool COLS>
-__device__ __forceinline__ void long_product(const _Float16* p, int pp, int row0, const _Float16* q, int qp, int q_rows, int q0, int k0, int k1,
-                                             int stride, Frags<W>& acc) {
-  Frags<W> low = {};
-#pragma unroll
-  for (int i = 0; i < W; ++i)
-#pragma unroll
-    for (int j = 0; j < W; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  for (int k = k0; k < k1; k += stride) frag_step<W, COLS>(p, pp, row0, q, qp, q_rows, q0, k, acc, low);
-#pragma unroll
-  for (int i = 0; i < W; ++i)
-#pragma unroll
-    for (int j = 0; j < W; ++j) acc[i][j] += low[i][j];
+// X X^T, inner steps k0, k0 + stride, ... < k1
+__device__ __forceinline__ f32x4_t long_product(const _Float16* x, int pitch, int row0, int col0, int k0, int k1, int stride) {
+  f32x4_t acc = {}, low = {};
+  for (int k = k0; k < k1; k += stride) frag_step<false>(x, pitch, row0, x, pitch, 0, col0, k, acc, low);
+  return acc + low;
 }
-// Q's rows from row0 (m x m) by X's columns from col0: one fragment
+// Q's rows from row0 (m x m) by X's columns from col0
 template <int K>
 __device__ __forceinline__ f32x4_t update_fragment(const _Float16* q, int row0, const _Float16* x, int pitch, int rows, int col0) {
-  Frags<1> acc = {}, low = {};
+  f32x4_t acc = {}, low = {};
 #pragma unroll
-  for (int k = 0; k < K; ++k) frag_step<1, true>(q, PA, row0, x, pitch, rows, col0, k, acc, low);
-  return acc[0][0] + low[0][0];
+  for (int k = 0; k < K; ++k) frag_step<true>(q, PA, row0, x, pitch, rows, col0, k, acc, low);
+  return acc + low;
 }
 __device__ __forceinline__ void put4(_Float16* p, const float (&v)[4]) {
   f16x4_t h, l;
@@ -837,92 +811,60 @@ __device__ __forceinline__ void put4(_Float16* p, const float (&v)[4]) {
 }
 __device__ __forceinline__ int pair_at(int pitch, int r, int c) { return r * pitch + (c >> 5) * 64 + (c & 31); }
 
-// Which W x W fragments of an m16 x m16 matrix a wave has (first row and column of elements), and which share of a long inner axis
+// Which fragment of an m16 x m16 matrix a wave has (first row and column), and which share of a long inner axis
 struct Share {
-  int r0, c0, part, parts;
-  bool on;
-  template <int W>
-  __device__ static Share of(int m16) {
-    Share s;
-    const int w = threadIdx.x >> 6;
-    if (W == 2 || m16 > 16) {        // 2 x 2 places
-      s.parts = W == 2 ? 1 : 4;
-      s.r0 = ((w >> 1) & 1) * 16 * W;
-      s.c0 = (w & 1) * 16 * W;
-      s.part = w >> 2;
-    } else {
-      s.parts = 16;
-      s.r0 = s.c0 = 0;
-      s.part = w;
-    }
-    s.on = s.part < s.parts;
-    return s;
+  int r0, c0, part, parts;     // part >= parts: a wave without work
+  __device__ explicit Share(int m16) {
+    const int w = threadIdx.x >> 6, n = m16 >> 4, frags = n * n, f = w % frags;
+    parts = (SMALL_TPB / 64) / frags;
+    part = w / frags;
+    r0 = (f / n) * 16;
+    c0 = (f % n) * 16;
   }
 };
-// a symmetric result, stored transposed (four values of a lane are neighbours then): f(row, col, four values) may change them. For m16 = 48 the
-// second fragments of the last places are outside.
-template <int W, typename F>
-__device__ __forceinline__ void frag_store(const Share& w, int m16, const Frags<W>& acc, _Float16* out, F f) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int i = 0; i < W; ++i)
-#pragma unroll
-    for (int j = 0; j < W; ++j) {
-      const int r = w.c0 + j * 16 + (lane & 15), c = w.r0 + i * 16 + (lane >> 4) * 4;
-      if (W == 2 && (w.c0 + j * 16 >= m16 || w.r0 + i * 16 >= m16)) continue;
-      float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-      f(r, c, v);
-      put4(out + pair_at(PA, r, c), v);
-    }
+// a symmetric result, stored transposed (four values of a lane are neighbours then): f(row, col, four values) may change them
+template <typename F>
+__device__ __forceinline__ void frag_store(const Share& w, const f32x4_t& acc, _Float16* out, F f) {
+  const int lane = threadIdx.x & 63, r = w.c0 + (lane & 15), c = w.r0 + (lane >> 4) * 4;
+  float v[4] = {acc[0], acc[1], acc[2], acc[3]};
+  f(r, c, v);
+  put4(out + pair_at(PA, r, c), v);
 }
-// The shares of a sum over a long inner axis, added in order and stored as G. scratch: 16 KiB of LDS of its own (W = 1)
-template <int W>
-__device__ __forceinline__ void store_gram(const Share& w, int m16, Frags<W>& acc, f32x4_t* scratch, _Float16* G, float scale) {
-  if constexpr (W == 1) {
-    scratch[threadIdx.x] = acc[0][0];
+// The shares of a sum over a long inner axis, added in order and stored as G. scratch: 16 KiB of LDS of its own where there are several
+__device__ __forceinline__ void store_gram(const Share& w, f32x4_t acc, f32x4_t* scratch, _Float16* G, float scale) {
+  if (w.parts > 1) {
+    scratch[threadIdx.x] = acc;
     __syncthreads();
     if (w.part == 0)
-      for (int s = 1; s < w.parts; ++s) acc[0][0] += scratch[s * (SMALL_TPB / w.parts) + threadIdx.x];
+      for (int s = 1; s < w.parts; ++s) acc += scratch[s * (SMALL_TPB / w.parts) + threadIdx.x];
   }
-  if (w.on && w.part == 0)
-    frag_store<W>(w, m16, acc, G, [&](int, int, float (&v)[4]) {
+  if (w.part == 0)
+    frag_store(w, acc, G, [&](int, int, float (&v)[4]) {
 #pragma unroll
       for (int t = 0; t < 4; ++t) v[t] *= scale;
     });
   __syncthreads();
 }
 // Steps k ... end - 1 on the m x m matrices (the same products as iterate<true>), G in A[0]; -> Q
-template <int W>
-__device__ __forceinline__ _Float16* phase_chain(const Share& w, _Float16* const (&A)[N_AREAS], const Steps& st, int k, int end, float gscale, int m16) {
-  constexpr int K = W;               // inner steps of 32: m <= 32 W
-  const bool on = w.on && w.part == 0;
+template <int K>   // K inner steps of 32: m <= 32 K
+__device__ __forceinline__ _Float16* phase_chain(const Share& w, _Float16* const (&A)[N_AREAS], const Steps& st, int k, int end, float gscale) {
+  const bool on = w.part == 0, second = w.part == (w.parts > 1 ? 1 : 0);
   _Float16 *G = A[0], *R = A[1], *Z = A[2], *q = nullptr, *spare = A[3], *other = A[4];
   auto plain = [](int, int, float (&)[4]) {};
   const float inv = 1.f / gscale;    // (a power of two)
   for (int j = k; j < end; ++j) {
     const float ca = st.coef[3 * j], cb = st.coef[3 * j + 1] * inv, cc = st.coef[3 * j + 2] * inv * inv;
     _Float16* z = q ? Z : spare;
-    Frags<W> acc;
-    if (on) {
-      square_product<W, K>(G, w.r0, G, w.c0, acc);
-      frag_store<W>(w, m16, acc, z, [&](int r, int c, float (&v)[4]) {
+    if (on)
+      frag_store(w, square_product<K>(G, w.r0, G, w.c0), z, [&](int r, int c, float (&v)[4]) {
         const _Float16* g = G + pair_at(PA, r, c);
         const f16x4_t h = *reinterpret_cast<const f16x4_t*>(g), l = *reinterpret_cast<const f16x4_t*>(g + 32);
 #pragma unroll
         for (int t = 0; t < 4; ++t) v[t] = cc * v[t] + cb * ((float)h[t] + (float)l[t]) + (r == c + t ? ca : 0.f);
       });
-    }
     __syncthreads();
-    // Q = Z Q and R = Z G by different waves (the second share of a W = 2 place is idle otherwise)
-    const bool second = W == 2 && w.part == 1;
-    if (on && q) {
-      square_product<W, K>(z, w.r0, q, w.c0, acc);
-      frag_store<W>(w, m16, acc, other, plain);
-    }
-    if ((W == 2 && q ? second : on) && j + 1 < end) {
-      square_product<W, K>(z, w.r0, G, w.c0, acc);
-      frag_store<W>(w, m16, acc, R, plain);
-    }
+    if (on && q) frag_store(w, square_product<K>(z, w.r0, q, w.c0), other, plain);
+    if (second && j + 1 < end) frag_store(w, square_product<K>(z, w.r0, G, w.c0), R, plain);
     __syncthreads();
     if (q) {
       _Float16* t = q;
@@ -932,10 +874,7 @@ __device__ __forceinline__ _Float16* phase_chain(const Share& w, _Float16* const
       q = z;
     }
     if (j + 1 < end) {
-      if (on) {
-        square_product<W, K>(R, w.r0, z, w.c0, acc);
-        frag_store<W>(w, m16, acc, G, plain);       // (nobody reads G any more)
-      }
+      if (on) frag_store(w, square_product<K>(R, w.r0, z, w.c0), G, plain);   // (nobody reads G any more)
       __syncthreads();
     }
   }
@@ -952,7 +891,7 @@ __device__ __forceinline__ void emit_one(const Result& res, long long o, float x
   else reinterpret_cast<uint16_t*>(res.out)[o] = res.out_dtype == DAS_BF16 ? f32_to_bf16(x) : __builtin_bit_cast(uint16_t, (_Float16)x);
 }
 
-template <typename T, bool MUON, int QUADS, int W>
+template <typename T, bool MUON, int QUADS, int K>
 __device__ __forceinline__ void small_matrix(const NsMatrix& M, const DasNsSource& s, const MuonIn& mu, const Steps& st, const Result& res, char* smem,
                                              double* redd) {
   const int m16 = up16(M.m), n64 = up64(M.n), PX = 2 * n64 + 8, PF = n64 + 4;   // X's row pitch in f16 elements and in floats
@@ -1026,21 +965,21 @@ __device__ __forceinline__ void small_matrix(const NsMatrix& M, const DasNsSourc
   }
   __syncthreads();
 
-  const Share w = Share::of<W>(m16);
+  const Share w(m16);
   const int n = m16 >> 4, cols = n64 >> 4;
   const float gs = M.gscale / (M.scale * M.scale);
   for (int k = 0; k < st.steps;) {
     const int end = st.end[k];
-    Frags<W> g;
-    if (w.on) long_product<W, false>(X, PX, w.r0, X, PX, 0, w.c0, w.part, n64 >> 5, w.parts, g);
-    store_gram<W>(w, m16, g, reinterpret_cast<f32x4_t*>(X + m16 * (PX + N_AREAS * PA)), A[0], gs);
-    const _Float16* q = phase_chain<W>(w, A, st, k, end, M.gscale, m16);
+    f32x4_t g = {};
+    if (w.part < w.parts) g = long_product(X, PX, w.r0, w.c0, w.part, n64 >> 5, w.parts);
+    store_gram(w, g, reinterpret_cast<f32x4_t*>(X + m16 * (PX + N_AREAS * PA)), A[0], gs);
+    const _Float16* q = phase_chain<K>(w, A, st, k, end, M.gscale);
     const bool last = end == st.steps;
     f32x4_t acc[QUADS];
 #pragma unroll
     for (int t = 0; t < QUADS; ++t) {
       const int x = t * 16 + wave, j = x / n;
-      if (j < cols) acc[t] = update_fragment<W>(q, (x - j * n) * 16, X, PX, m16, j * 16);
+      if (j < cols) acc[t] = update_fragment<K>(q, (x - j * n) * 16, X, PX, m16, j * 16);
     }
     __syncthreads();                    // (X has been read)
 #pragma unroll
@@ -1222,9 +1161,7 @@ __global__ __launch_bounds__(TPB) void thin_kernel(const NsMatrix* __restrict__ 
       for (int u = 0; u < 4; ++u) {
         const int x = u * 4 + wave, i = x / n;
         if (i < n) {
-          Frags<1> g;
-          long_product<1, false>(xs, PT, i * 16, xs, PT, 0, (x - i * n) * 16, 0, THIN_COLS / 32, 1, g);
-          gram[u] += g[0][0];
+          gram[u] += long_product(xs, PT, i * 16, (x - i * n) * 16, 0, THIN_COLS / 32, 1);
         }
       }
     }
@@ -1239,8 +1176,8 @@ __global__ __launch_bounds__(TPB) void thin_kernel(const NsMatrix* __restrict__ 
 }
 
 // One workgroup a thin matrix: X X^T from its slices' parts, the phase's steps, Q out
-template <int W>
-__device__ __forceinline__ void chain_matrix(const NsMatrix& M, const f32x4_t* part, int slices, _Float16* Q, const Steps& st, int k, char* smem) {
+template <int K>
+__device__ __forceinline__ void chain_matrix(const NsMatrix& M, const f32x4_t* part, int slices, _Float16* Q, const Steps& st, int k0, char* smem) {
   const int m16 = up16(M.m), n = m16 >> 4, lane = threadIdx.x & 63;
   _Float16* A[N_AREAS];
 #pragma unroll
@@ -1265,8 +1202,8 @@ __device__ __forceinline__ void chain_matrix(const NsMatrix& M, const f32x4_t* p
     put4(A[0] + pair_at(PA, r, c), v);
   }
   __syncthreads();
-  const Share w = Share::of<W>(m16);
-  const _Float16* q = phase_chain<W>(w, A, st, k, st.end[k], M.gscale, m16);
+  const Share w(m16);
+  const _Float16* q = phase_chain<K>(w, A, st, k0, st.end[k0], M.gscale);
   for (int i = threadIdx.x; i < M.m * 16; i += SMALL_TPB) {
     const int r = i >> 4, c = i & 15;
     *reinterpret_cast<uint4*>(Q + 2 * M.a + r * 128 + c * 8) = *reinterpret_cast<const uint4*>(q + r * PA + c * 8);
@@ -1471,7 +1408,7 @@ int launch_thin(const DasNsPlan* p, const char* tab, const Work& w, const Result
   const NsItem* slices = (const NsItem*)(tab + p->slice_at);
   const int2* thin = (const int2*)(tab + p->thin_at);
   const Steps st = steps_of(p);
-  constexpr int LDS = 2 * N_AREAS * SMALL_M * PA;   // (m = 48: what a second fragment reads past its matrix is inside, too)
+  constexpr int LDS = 2 * N_AREAS * SMALL_M * PA;
   (void)hipFuncSetAttribute((const void*)chain_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
   auto pass = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3(p->n_slices), dim3(TPB), 0, s, mats, slices, p->eps, w.part, w.xt, w.qt, w.thin_part, res);
