@@ -9,6 +9,7 @@
 
 namespace {
 constexpr int TPB = 256;
+constexpr long long MOST = 1LL << 31;   // elements of a launch (a grid has fewer than 2^32 threads; a multiple of 4: alignment stays)
 
 struct AdamW {
   float keep, step_size, beta1, omb1, beta2, omb2, inv_bc2, eps;   // 1 - lr wd, lr / (1 - beta1^t), ..., 1 / (1 - beta2^t)
@@ -60,15 +61,20 @@ extern "C" int das_adamw_step(float* p, const float* g, float* m, float* v, long
   if (!p || !g || !m || !v || n <= 0 || step < 1 || !(beta1 >= 0 && beta1 < 1) || !(beta2 >= 0 && beta2 < 1) || !(eps >= 0) ||
       !(lr >= 0) || !(weight_decay >= 0) || (max_norm > 0.f && !grad_sumsq))
     return DAS_ERR_ARG;
-  if (((uintptr_t)p | (uintptr_t)g | (uintptr_t)m | (uintptr_t)v) & 3) return DAS_ERR_ARG;
+  if ((((uintptr_t)p | (uintptr_t)g | (uintptr_t)m | (uintptr_t)v) & 3) || n > (1LL << 60)) return DAS_ERR_ARG;
+  const void* const buffers[4] = {p, g, m, v};
+  for (int i = 0; i < 4; ++i)
+    for (int j = 0; j < i; ++j)
+      if (buffers_overlap(buffers[i], buffers[j], 4 * n)) return DAS_ERR_ARG;
   const double bc1 = 1.0 - std::pow(beta1, (double)step), bc2 = 1.0 - std::pow(beta2, (double)step);
   const AdamW a = {(float)(1.0 - lr * weight_decay), (float)(lr / bc1), (float)beta1, (float)(1.0 - beta1), (float)beta2,
                    (float)(1.0 - beta2), (float)(1.0 / bc2), (float)eps, grad_scale, max_norm};
   const bool vec = !(((uintptr_t)p | (uintptr_t)g | (uintptr_t)m | (uintptr_t)v) & 15);
-  const long long threads = vec ? std::max(1LL, n / 4) : n, blocks = (threads + TPB - 1) / TPB;
-  if (blocks > 0x7fffffffLL) return DAS_ERR_ARG;
-  hipLaunchKernelGGL(vec ? adamw_kernel<true> : adamw_kernel<false>, dim3((unsigned)blocks), dim3(TPB), 0, (hipStream_t)stream, p, g, m, v,
-                     n, a, grad_sumsq);
-  DAS_CHECK_LAUNCH();
+  for (long long at = 0; at < n; at += MOST) {
+    const long long k = std::min(MOST, n - at), threads = vec ? std::max(1LL, k / 4) : k;
+    hipLaunchKernelGGL(vec ? adamw_kernel<true> : adamw_kernel<false>, dim3((unsigned)((threads + TPB - 1) / TPB)), dim3(TPB), 0,
+                       (hipStream_t)stream, p + at, g + at, m + at, v + at, k, a, grad_sumsq);
+    DAS_CHECK_LAUNCH();
+  }
   return DAS_OK;
 }

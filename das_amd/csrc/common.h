@@ -16,6 +16,12 @@ typedef uint16_t bf16_t;  // raw bfloat16 bits
     if (e__ != hipSuccess) return DAS_ERR_LAUNCH;             \
   } while (0)
 
+// two buffers of `bytes` bytes each that share some
+inline bool buffers_overlap(const void* a, const void* b, long long bytes) {
+  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+  return (x > y ? x - y : y - x) < (uintptr_t)bytes;
+}
+
 __device__ __forceinline__ float bf16_to_f32(bf16_t v) { return __uint_as_float(((uint32_t)v) << 16); }
 
 // f32 -> bf16, round-to-nearest-even, NaN kept quiet: gfx950's v_cvt_pk_bf16_f32 (one instruction per PAIR; the

@@ -694,9 +694,14 @@ __global__ __launch_bounds__(KG * TPB, KG == 1 ? 2 : KG) void update_kernel(cons
         }
       } else if (res.out_dtype == DAS_F32) {
         float* p = reinterpret_cast<float*>(res.out) + o;
+        if (vec) {
+          *reinterpret_cast<float4*>(p) = *reinterpret_cast<const float4*>(v);
+          *reinterpret_cast<float4*>(p + 4) = *reinterpret_cast<const float4*>(v + 4);
+        } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (e < n) p[e] = v[e];
+          for (int e = 0; e < 8; ++e)
+            if (e < n) p[e] = v[e];
+        }
       } else {
         uint16_t h[8];
 #pragma unroll
@@ -1340,6 +1345,10 @@ class Fork {
     static std::vector<Side*>* p = new std::vector<Side*>;   // (lives as long as the process: streams outlast static destructors)
     return *p;
   }
+  static size_t& made() {
+    static size_t n = 0;
+    return n;
+  }
   static Side* take() {
     int dev = 0;
     if (hipGetDevice(&dev) != hipSuccess) return nullptr;
@@ -1356,6 +1365,13 @@ class Fork {
     Side* s = new (std::nothrow) Side;
     if (!s) return nullptr;
     s->dev = dev;
+    try {                // (room for it: giving it back never allocates)
+      std::lock_guard<std::mutex> lock(mutex());
+      pool().reserve(++made());
+    } catch (...) {
+      delete s;
+      return nullptr;
+    }
     if (hipStreamCreateWithFlags(&s->stream, hipStreamNonBlocking) != hipSuccess ||
         hipEventCreateWithFlags(&s->fork, hipEventDisableTiming) != hipSuccess ||
         hipEventCreateWithFlags(&s->ready, hipEventDisableTiming) != hipSuccess ||
@@ -1497,7 +1513,6 @@ int iterate(const DasNsPlan* p, const char* tab, Work w, const Result& res, hipS
   }
   return DAS_OK;
 }
-
 
 // thin and tiled matrices after ingest_kernel, and the join with the small ones
 template <bool SPLIT, bool MUON>
@@ -1704,11 +1719,12 @@ bool build(const DasNsShape* shapes, int n, double top, DasNsPlan* plan, Tables&
   };
   for (int g = 0; g < n; ++g) {
     const DasNsShape& s = shapes[g];
-    if (s.off < 0 || s.count < 1 || s.rows < 1 || s.cols < 1 || s.rows > (1 << 20) || s.cols > (1 << 20)) return false;
+    if (s.off < 0 || s.off > (1LL << 60) || s.count < 1 || s.rows < 1 || s.cols < 1 || s.rows > (1 << 20) || s.cols > (1 << 20)) return false;
     const long long m = std::min(s.rows, s.cols), nn = std::max(s.rows, s.cols);
     n_mat += s.count;
     if (class_of(s) != SMALL) n_chunks += (long long)s.count * over(m, 64) * over(nn, 128) * 2;
-    if (n_mat > (1 << 22) || n_chunks > (1 << 24) || m > (1 << 15)) return false;
+    // (a launch has fewer than 2^32 threads: 1024 for a small matrix, 256 for a block)
+    if (n_mat >= (1 << 22) || n_chunks >= (1 << 24) || m > (1 << 15)) return false;
     spans.push_back({s.off, s.off + (long long)s.count * s.rows * s.cols});
   }
   std::sort(spans.begin(), spans.end());
@@ -1808,7 +1824,9 @@ bool build(const DasNsShape* shapes, int n, double top, DasNsPlan* plan, Tables&
     t.product.place();
   }
   t.update.place();
-  return t.gram.order.size() < (1u << 30) && t.update.order.size() < (1u << 30);
+  // (KG x 256 threads for an item, 16 x 256 for a joined tile)
+  return std::max({t.gram.order.size(), t.product.order.size(), t.update.order.size()}) < (1u << 22) &&
+         std::max(t.gram_join.size(), t.product_join.size()) < (1u << 20);
 }
 
 }  // namespace
@@ -1917,6 +1935,8 @@ extern "C" int das_muon_step(const DasNsPlan* plan, const void* tables_dev, floa
       !(weight_decay >= 0.f) || (max_norm > 0.f && !grad_sumsq) || lr_scale < 0 || lr_scale > 1)
     return DAS_ERR_ARG;
   if (((uintptr_t)p | (uintptr_t)g | (uintptr_t)buf) & 3) return DAS_ERR_ARG;
+  const long long bytes = 4 * plan->extent;
+  if (buffers_overlap(p, g, bytes) || buffers_overlap(p, buf, bytes) || buffers_overlap(g, buf, bytes)) return DAS_ERR_ARG;
   hipStream_t s = (hipStream_t)stream;
   const char* tab = (const char*)tables_dev;
   const Work w = carve(plan, true, ws);

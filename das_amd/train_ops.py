@@ -181,7 +181,7 @@ def _clip_sum(what, max_norm, grad_sumsq_t, device):
 
 def adamw_step(p, g, m, v, lr, step, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=1e-2, grad_scale=1.0, max_norm=0.0,
                grad_sumsq_t=None):
-    """One AdamW step (decoupled weight decay, bias-corrected moments) in place on flat f32 buffers, `step` counting from 1; the
+    """One AdamW step (decoupled weight decay, bias-corrected moments) in place on flat f32 buffers that do not overlap, `step` counting from 1; the
     gradient is used times grad_scale * min(1, max_norm / (sqrt(grad_sumsq_t) * grad_scale + 1e-6)) (max_norm <= 0: no clipping). A NaN
     norm makes every element NaN. Scalars are fixed when a call is captured into a hipGraph."""
     _flat_buffers('adamw_step', p, g, m, v)
@@ -204,7 +204,7 @@ class NewtonSchulzPlan:
 
     shapes: (rows, cols) or (count, rows, cols) of equal matrices, in storage order. offsets: element offset of each entry's first
     matrix in the flat buffers of muon_step (default: back to back; only such a plan serves orthogonalize). coefficients: (a, b, c) for every step or one triple
-    per step. Entries without elements are allowed and left alone."""
+    per step. Entries without elements are allowed and left alone. Sides up to 2^20, the smaller one up to 2^15."""
 
     def __init__(self, shapes, device, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, offsets=None):
         self.shapes = [(1,) + tuple(int(v) for v in s) if len(s) == 2 else tuple(int(v) for v in s) for s in shapes]
@@ -215,8 +215,7 @@ class NewtonSchulzPlan:
             self.device = torch.device('cuda', torch.cuda.current_device())
         if any(len(s) != 3 or min(s) < 0 for s in self.shapes) or not 1 <= int(steps) <= _lib.DAS_NS_MAX_STEPS:
             raise _lib.DasHipError(f'NewtonSchulzPlan: shapes are (rows, cols) or (count, rows, cols), steps 1 ... {_lib.DAS_NS_MAX_STEPS}')
-        co = [float(v) for v in coefficients] if isinstance(coefficients[0], (int, float)) else \
-            [float(v) for t in coefficients for v in t]
+        co = [float(v) for t in coefficients for v in (t if hasattr(t, '__len__') else (t,))]
         co = co * int(steps) if len(co) == 3 else co
         if len(co) != 3 * int(steps):
             raise _lib.DasHipError('NewtonSchulzPlan: one (a, b, c) triple, or one for every step')
@@ -263,7 +262,7 @@ def orthogonalize(mats, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, out_dty
     gradients of a training run (2-norm) and up to 5e-2 where the singular values span many orders of magnitude; f32 ones from
     pairs of f16, 2e-4 off at most.
     plan: a NewtonSchulzPlan of these shapes (built here if None, which copies its tables to the device: keep one where the call
-    repeats; inside a hipGraph capture it is required). Inf or NaN in a matrix makes that matrix NaN, no other."""
+    repeats; inside a hipGraph capture it is required). Inf or NaN in a matrix makes that matrix NaN, no other. No gradient is recorded."""
     one = torch.is_tensor(mats)
     mats = [mats] if one else list(mats)
     _need_gpu(*mats)
@@ -301,8 +300,8 @@ def orthogonalize(mats, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, out_dty
 
 def muon_step(p, g, buf, plan, lr, momentum=0.95, weight_decay=0.0, nesterov=True, lr_scale='original', grad_scale=1.0, max_norm=0.0,
               grad_sumsq_t=None):
-    """One Muon step in place on flat f32 buffers holding the plan's matrices (parameters, gradients, momentum; what lies between them
-    is not touched): momentum average, orthogonalised direction, decoupled weight decay. lr_scale: 'original' = the
+    """One Muon step in place on flat f32 buffers holding the plan's matrices (parameters, gradients, momentum; not overlapping; what lies between
+    the matrices is not touched): momentum average, orthogonalised direction, decoupled weight decay. lr_scale: 'original' = the
     update of a rows x cols matrix times sqrt(max(1, rows / cols)); 'match_rms_adamw' = times 0.2 sqrt(max(rows, cols)), the size
     of an AdamW update. Gradient scaling and clipping as in adamw_step."""
     _flat_buffers('muon_step', p, g, buf)

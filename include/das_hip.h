@@ -611,9 +611,9 @@ int das_sgd_momentum_step(float* p, const float* g, float* buf, long long n, flo
  * Newton-Schulz orthogonalisation of a ragged set of matrices. For each matrix U (rows x cols, m = min, n = max of the two,
  * transposed if rows > cols so that X is m x n):
  *   X = U / (|U|_F + eps);   steps times:  A = X X^T,  B = a I + b A + c A^2,  X = B X.
- * The precision follows the result's type. f16 / bf16 results: products of f16 operands summed in f32, X, A and B rounded to f16 in between
+ * The precision follows the result's type. f16 / bf16 results of matrices with m > 64: products of f16 operands summed in f32, X, A and B rounded to f16 in between
  * (1e-3 off a 64-bit evaluation, in the 2-norm, for the gradients of a training run, up to 5e-2 for matrices whose singular values span
- * many orders of magnitude). f32 results and parameters: operands are pairs of f16 (22 bits), 2e-4 off at most. Sums of squares are
+ * many orders of magnitude). f32 results, parameters and m <= 64: operands are pairs of f16 (22 bits), 2e-4 off at most. Sums of squares are
  * held in f32 by 64 x 64 blocks and added in f64. Results are the same bits from run to run.
  *
  * A plan lists the set once: das_ns_plan() checks the shapes and the polynomial and writes the tables (host memory) that the
@@ -640,26 +640,29 @@ typedef struct {
   long long batch_stride, row_stride;
 } DasNsSource;
 /* Fills *plan; with tables != NULL (plan->table_bytes host bytes) also the tables. DAS_ERR_ARG: n < 1, a shape without elements or
- * with a side over 1 << 20 or both over 1 << 15, overlapping matrices, steps outside 1 ... DAS_NS_MAX_STEPS, a polynomial that takes [0, 1] out of
+ * with a side over 1 << 20 or both over 1 << 15, an offset over 1 << 60, 1 << 22 matrices or 1 << 24 blocks of 64 x 64, overlapping matrices, steps outside 1 ... DAS_NS_MAX_STEPS, a polynomial that takes [0, 1] out of
  * [-16, 16] within `steps` steps or has |a + b s^2 + c s^4| > 64 there (f16 could overflow), eps < 0, or tables too small. */
 int das_ns_plan(const DasNsShape* shapes, int n, int steps, const float* coef, float eps, DasNsPlan* plan, void* tables,
                 long long table_bytes);
 /* f32_result: for das_muon_step, and for das_orthogonalize with out_dtype DAS_F32. */
 long long das_ns_ws_bytes(const DasNsPlan* plan, int f32_result);
 /* out (flat, out_dtype DAS_F32 / DAS_BF16 / DAS_F16, plan offsets): the orthogonalised matrices; srcs: one per group of the plan, in_dtype
- * DAS_F32 / DAS_BF16 / DAS_F16. `ws`: das_ns_ws_bytes() of device memory, 16-byte aligned, in use until the call's kernels end. */
+ * DAS_F32 / DAS_BF16 / DAS_F16. `ws`: das_ns_ws_bytes() of device memory, 16-byte aligned, in use until the call's kernels end. `out`, the
+ * sources and ws do not overlap. Small and thin matrices of a set that holds others too run on a stream of the library's own (default priority,
+ * created at first need, kept) beside `stream`, which waits for them; a call that is being captured uses `stream` alone. */
 int das_orthogonalize(const DasNsPlan* plan, const void* tables_dev, const DasNsSource* srcs, int n_srcs, int in_dtype, void* out,
                       int out_dtype, void* ws, void* stream);
 /* Muon: with g' = g * grad_scale * min(1, max_norm / (sqrt(*grad_sumsq) * grad_scale + 1e-6)) (no clipping for max_norm <= 0),
  *   buf = momentum * buf + (1 - momentum) * g';   U = nesterov ? (1 - momentum) * g' + momentum * buf : buf;
  *   p = p * (1 - lr * weight_decay) - lr * f * orthogonalised(U),   f = sqrt(max(1, rows / cols)) (lr_scale 0) or
- *   0.2 * sqrt(max(rows, cols)) (lr_scale 1). Elements of p, g, buf outside the plan's matrices are not touched. */
+ *   0.2 * sqrt(max(rows, cols)) (lr_scale 1). Elements of p, g, buf outside the plan's matrices are not touched.
+ * The three buffers (plan->extent elements each) do not overlap: DAS_ERR_ARG otherwise. */
 int das_muon_step(const DasNsPlan* plan, const void* tables_dev, float* p, const float* g, float* buf, float lr, float momentum,
                   float weight_decay, int nesterov, int lr_scale, float grad_scale, float max_norm, const float* grad_sumsq,
                   void* ws, void* stream);
 /* AdamW on flat f32 buffers, g' as above, t = step >= 1:
  *   m = beta1 m + (1 - beta1) g';  v = beta2 v + (1 - beta2) g'^2;
- *   p = p (1 - lr weight_decay) - lr (m / (1 - beta1^t)) / (sqrt(v / (1 - beta2^t)) + eps). */
+ *   p = p (1 - lr weight_decay) - lr (m / (1 - beta1^t)) / (sqrt(v / (1 - beta2^t)) + eps). The four buffers do not overlap: DAS_ERR_ARG otherwise. */
 int das_adamw_step(float* p, const float* g, float* m, float* v, long long n, double lr, double beta1, double beta2, double eps,
                    double weight_decay, long long step, float grad_scale, float max_norm, const float* grad_sumsq, void* stream);
 

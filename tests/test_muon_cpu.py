@@ -105,6 +105,27 @@ def test_plan_refusals():
     assert make_plan([(1, 8, 8), (1, 8, 8)], offsets=[64, 0])[0] == 0
 
 
+def test_plan_limits():
+    """what a launch's grid, the offsets' arithmetic and the polynomial's forms bear"""
+    assert make_plan([(1 << 22, 2, 2)])[0] == 1 and make_plan([(1 << 20, 2, 2)])[0] == 0
+    assert make_plan([(1, 8, 8)], offsets=[(1 << 60) + 1])[0] == 1
+    assert make_plan([(1, 8, 8)], offsets=[(1 << 63) - 8])[0] == 1
+    st, plan, _ = make_plan([(1, 8, 8)], offsets=[1 << 60])
+    assert st == 0 and plan.extent == (1 << 60) + 64
+
+
+def test_overlapping_buffers_are_refused():
+    """by the library, before any launch: a step would read elements that it has already written"""
+    from das_amd import _lib
+    lib = _lib.load()
+    _, plan, _ = make_plan([(1, 8, 8)])
+    base, far = 1 << 20, 1 << 24
+    for p, g, b in ((base, base, far), (base, far, base + 4), (far, base + 252, base), (base + 16, far, base)):
+        assert lib.das_muon_step(C.byref(plan), 4096, p, g, b, 1e-2, 0.9, 0.0, 1, 0, 1.0, 0.0, None, 8192, None) == _lib.DAS_ERR_ARG
+    for bufs in ((base, base, far, 2 * far), (base, far, 2 * far, base + 252), (base, far, far + 4, 2 * far), (base, base + 256, far, far + 128)):
+        assert lib.das_adamw_step(*bufs, 64, 1e-3, 0.9, 0.999, 1e-8, 0.0, 1, 1.0, 0.0, None, None) == _lib.DAS_ERR_ARG
+
+
 def test_phases_follow_the_polynomial():
     """steps on the Gram matrix end before an error of it can have grown 256-fold: three, then two of the default polynomial; a cubic
     whose slope at zero is 1.5 may go further"""

@@ -408,6 +408,24 @@ def test_refusals():
     assert (f == 1).all() and (u == 1).all()
 
 
+def test_overlap_is_refused_and_neighbours_are_not():
+    from das_amd import train_ops as T
+    from das_amd._lib import DasHipError
+    whole = torch.ones(4 * 64, device=DEV)
+    parts = whole.split(64)
+    plan = T.NewtonSchulzPlan([(8, 8)], DEV)
+    for bad in (lambda: T.muon_step(parts[0], parts[0], parts[1], plan, lr=1e-2), lambda: T.muon_step(parts[0], parts[1], whole[32:96], plan, lr=1e-2),
+                lambda: T.adamw_step(parts[0], parts[1], parts[2], parts[2], lr=1e-2, step=1),
+                lambda: T.adamw_step(parts[0], whole[127:191], parts[1], parts[3], lr=1e-2, step=1),
+                lambda: T.orthogonalize(whole.view(16, 16), coefficients=())):
+        with pytest.raises(DasHipError):
+            bad()
+    assert (whole == 1).all()
+    T.adamw_step(*parts, lr=1e-2, step=1)
+    T.muon_step(*parts[:3], plan, lr=1e-2)
+    assert torch.isfinite(whole).all() and (whole[64:128] == 1).all()
+
+
 # ------------------------------------------------------------------ the optimizers in a training run
 def detector():
     from test_train_step_gpu import make
