@@ -306,7 +306,7 @@ __global__ __launch_bounds__(TPB) void normalise_kernel(const NsMatrix* __restri
 // two buffers.
 //   plain:  acc += A0 B0 + A1 B1   (two halves of the inner axis)
 //   SPLIT:  acc += Ah Bh + Ah Bl + Al Bh   (the low x low part is 2^-22 of the product)
-// KG groups of four waves divide the inner axis between them (KG = 4 where a launch has fewer tiles than CUs and latency is all: every
+// KG groups of four waves divide the inner axis between them (KG = 4 or 2 where a launch has few tiles and latency is all: every
 // group has its own buffers and copies in flight) and join their sums through LDS, in order.
 // LDS images. Rows by rows (gram, product, and B of the update): two panels of T rows x 64 bytes, 16-byte slot s of row r holds source
 // slot s ^ (r / 2 % 4): eight neighbouring rows cover all banks. Columns of X (update): inner rows as they are in memory, 32-byte units
@@ -324,7 +324,14 @@ __device__ __forceinline__ void copy16(const void* src, const char* lds_wave_bas
                : "memory");
 }
 // every copy of this wave has landed and every LDS read of it is done, then the same of every wave
-__device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+// (the wait is the builtin's: after one in asm hipcc takes the reads for unfinished and waits again, for the next stage's too, before
+// the first matrix instruction)
+__device__ __forceinline__ void landed() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0070);   // vmcnt(0) lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
 
 template <int T>
 struct RowsOperand {        // T rows of a matrix whose rows run along the inner axis
@@ -1464,7 +1471,8 @@ int iterate(const DasNsPlan* p, const char* tab, Work w, const Result& res, hipS
   auto sym = [&](auto kind, int products, SymArgs a) {
     constexpr SymKind K = decltype(kind)::value;
     a.slots = p->product_slots;
-    if (p->product_tile == 128) launch_sym(sym_kernel<128, SPLIT, 1, K>, 128, 1, prod, p->n_product, products, a);
+    if (p->product_tile == 128 && p->product_kg == 2) launch_sym(sym_kernel<128, SPLIT, 2, K>, 128, 2, prod, p->n_product, products, a);
+    else if (p->product_tile == 128) launch_sym(sym_kernel<128, SPLIT, 1, K>, 128, 1, prod, p->n_product, products, a);
     else launch_sym(sym_kernel<64, SPLIT, 4, K>, 64, 4, prod, p->n_product, products, a);
     if (p->n_product_join)
       hipLaunchKernelGGL((join_kernel<SPLIT, K>), dim3(p->n_product_join * JOINERS, products), dim3(TPB), 0, s, prod_join, a, w.slots);
@@ -1476,7 +1484,8 @@ int iterate(const DasNsPlan* p, const char* tab, Work w, const Result& res, hipS
       (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
       hipLaunchKernelGGL(kernel, dim3(p->n_update), dim3(kg * TPB), lds, s, mats, upd, q, x, y, res);
     };
-    if (p->update_tile == 128) launch(update_kernel<128, SPLIT, 1, L>, 128, 1);
+    if (p->update_tile == 128 && p->update_kg == 2) launch(update_kernel<128, SPLIT, 2, L>, 128, 2);
+    else if (p->update_tile == 128) launch(update_kernel<128, SPLIT, 1, L>, 128, 1);
     else launch(update_kernel<64, SPLIT, 4, L>, 64, 4);
   };
   const std::integral_constant<SymKind, POLY> poly_k;
@@ -1732,7 +1741,7 @@ bool build(const DasNsShape* shapes, int n, double top, DasNsPlan* plan, Tables&
     if (spans[i].first < spans[i - 1].second) return false;   // two workgroups would write the same elements
   plan->extent = spans.back().second;
 
-  long long lower128 = 0, all128 = 0;
+  long long lower128 = 0, all128 = 0, lower64 = 0, all64 = 0;
   for (const Class cls : {SMALL, TILED, THIN}) {   // the order of the matrix and block tables
     for (int g = 0; g < n; ++g) {
       const DasNsShape& s = shapes[g];
@@ -1766,6 +1775,8 @@ bool build(const DasNsShape* shapes, int n, double top, DasNsPlan* plan, Tables&
             const long long tm = over(M.m, 128);
             lower128 += tm * (tm + 1) / 2;
             all128 += tm * (M.ldx / 128);
+            lower64 += (long long)(M.lda / 64) * (M.lda / 64 + 1) / 2;
+            all64 += (long long)(M.lda / 64) * (M.ldx / 64);
           } else {
             // at most 64 slices: the chain's workgroup reads all their parts
             const int pieces = M.ldx / THIN_COLS, per = over(pieces, 64), frags = up16(M.m) * up16(M.m) / 256;
@@ -1784,9 +1795,14 @@ bool build(const DasNsShape* shapes, int n, double top, DasNsPlan* plan, Tables&
     if (cls == TILED) plan->n_tile_chunks = (int)t.chunks.size();
   }
   const int tiled_end = (int)(t.mats.size() - t.thin.size());
-  // Products and updates: 128 x 128 tiles where they fill the 256 CUs, else 64 x 64 ones whose inner axis four wave groups share.
-  plan->product_tile = lower128 >= 256 ? 128 : 64;
-  plan->update_tile = all128 >= 256 ? 128 : 64;
+  // Products and updates: 64 x 64 tiles whose inner axis four wave groups share while the 256 CUs have them in two rounds (9x 512x512,
+  // Muon: 314 us, 372 with 128 x 128 ones), else 128 x 128 (24x 512x512: 435 us, 576 with 64 x 64 ones). Where a CU gets one of those,
+  // two wave groups share it: at most 256 of an update, which has no second round to fill (512-channel bottleneck, 272 tiles: 233 us, 254 with two
+  // groups), under 384 of a product, whose long ones are split (2048x2048, 136 tiles: 1084 -> 853 us).
+  plan->product_tile = lower64 > 512 ? 128 : 64;
+  plan->product_kg = plan->product_tile == 64 ? 4 : lower128 >= 384 ? 1 : 2;
+  plan->update_tile = all64 > 512 ? 128 : 64;
+  plan->update_kg = plan->update_tile == 64 ? 4 : all128 > 256 ? 1 : 2;
   // X X^T: 128 x 128 tiles; where there are fewer than 384, two wave groups share a tile's inner axis (one workgroup a CU, not two)
   plan->gram_kg = lower128 >= 384 ? 1 : 2;
   // blocks of up to 8 x 8 tiles, smaller where one would be more than a 16th of the launch (half of an XCD's part)
@@ -1818,7 +1834,7 @@ bool build(const DasNsShape* shapes, int n, double top, DasNsPlan* plan, Tables&
   }
   schedule(t, gram, plan->gram_kg == 1 ? 512 : 256, t.gram, t.gram_join, plan->gram_slots);
   if (plan->product_tile == JOIN_TILE) {
-    schedule(t, product, 512, t.product, t.product_join, plan->product_slots);
+    schedule(t, product, plan->product_kg == 1 ? 512 : 256, t.product, t.product_join, plan->product_slots);
   } else {
     for (const Tile& p : product) t.product.add(p.fresh, t.item(p.matrix, p.ti, p.tj, 0, p.steps, -1, 1));
     t.product.place();
