@@ -1304,12 +1304,12 @@ int phase_end(const Bounds* bound, int steps, int k) {
 }
 
 // A second stream for the small and thin matrices of a set that holds others too: a chain of short launches that leaves the GPU nearly empty,
-// beside the tiles' launches instead of before them (fork and join by events; the caller's stream waits for the end). Streams of
+// beside the tiles' launches instead of before them, from their own part of the first pass on (fork and join by events; the caller's stream waits for the end). Streams of
 // default priority, from a pool: one call has one for itself. A call that is being captured stays on its stream.
 struct Side {
   int dev = 0;
   hipStream_t stream = nullptr;
-  hipEvent_t fork = nullptr, ready = nullptr, join = nullptr;
+  hipEvent_t fork = nullptr, join = nullptr;
 };
 class Fork {
  public:
@@ -1330,10 +1330,7 @@ class Fork {
   }
   ~Fork() { (void)finish(); }
   hipStream_t stream() const { return side_ ? side_->stream : main_; }
-  // what the main stream has done so far comes before what the side stream does next
-  bool follow() {
-    return !side_ || (hipEventRecord(side_->ready, main_) == hipSuccess && hipStreamWaitEvent(side_->stream, side_->ready, 0) == hipSuccess);
-  }
+  bool apart() const { return side_ != nullptr; }
   int finish() {
     if (!side_) return DAS_OK;
     const bool ok = hipEventRecord(side_->join, side_->stream) == hipSuccess && hipStreamWaitEvent(main_, side_->join, 0) == hipSuccess;
@@ -1381,7 +1378,6 @@ class Fork {
     }
     if (hipStreamCreateWithFlags(&s->stream, hipStreamNonBlocking) != hipSuccess ||
         hipEventCreateWithFlags(&s->fork, hipEventDisableTiming) != hipSuccess ||
-        hipEventCreateWithFlags(&s->ready, hipEventDisableTiming) != hipSuccess ||
         hipEventCreateWithFlags(&s->join, hipEventDisableTiming) != hipSuccess) {
       (void)hipGetLastError();
       delete s;          // (a device that gives no stream: the call goes on without)
@@ -1396,8 +1392,8 @@ class Fork {
   hipStream_t main_;
   Side* side_ = nullptr;
 };
-// Beside tiles it pays (seven small and thin matrices with two of 129 x 1023 and 700 x 513: 204 -> 177 us), beside thin matrices alone the
-// fork costs more than it hides (60 -> 85 us for five small and thin ones).
+// Beside tiles it pays (the detector's set 2276 -> 2216 us; seven small and thin matrices with two of 129 x 1023 and one of 700 x 513: 197 ->
+// 188 us), beside thin matrices alone the fork costs more than it hides (60 -> 85 us for five small and thin ones).
 bool worth_a_fork(const DasNsPlan* p) { return p->n_tile_chunks > 0 && p->n_small + p->n_thin > 0; }
 
 Steps steps_of(const DasNsPlan* p) {
@@ -1523,15 +1519,19 @@ int iterate(const DasNsPlan* p, const char* tab, Work w, const Result& res, hipS
   return DAS_OK;
 }
 
+// the blocks of the first pass: those of thin matrices (behind the tiled ones' in the table) on the stream that goes on with them
+template <typename F>
+void launch_ingest(const DasNsPlan* p, const char* tab, const Fork& fork, hipStream_t s, F launch) {
+  const int4* chunks = (const int4*)(tab + p->chunk_at);
+  const int here = fork.apart() ? p->n_tile_chunks : p->n_chunks;
+  if (here) launch(chunks, here, s);
+  if (p->n_chunks > here) launch(chunks + here, p->n_chunks - here, fork.stream());
+}
+
 // thin and tiled matrices after ingest_kernel, and the join with the small ones
 template <bool SPLIT, bool MUON>
 int the_rest(const DasNsPlan* p, const char* tab, const Work& w, const Result& res, hipStream_t s, Fork& fork) {
-  int st = DAS_OK;
-  if (p->n_thin) {
-    const bool beside = p->n_tile_chunks > 0;   // (else they have the caller's stream to themselves)
-    if (beside && !fork.follow()) return DAS_ERR_LAUNCH;
-    st = launch_thin<MUON>(p, tab, w, res, beside ? fork.stream() : s);
-  }
+  int st = launch_thin<MUON>(p, tab, w, res, fork.stream());
   if (st == DAS_OK && p->n_tile_chunks) st = iterate<SPLIT>(p, tab, w, res, s);
   const int joined = fork.finish();
   return st != DAS_OK ? st : joined;
@@ -1916,7 +1916,6 @@ extern "C" int das_orthogonalize(const DasNsPlan* plan, const void* tables_dev, 
   const bool split = out_dtype == DAS_F32;
   const Work w = carve(plan, split, ws);
   const NsMatrix* mats = (const NsMatrix*)(tab + plan->mat_at);
-  const int4* chunks = (const int4*)(tab + plan->chunk_at);
   const MuonIn none = {};
   const Result res = {out, out_dtype, nullptr, 1.f, 0.f, 0};
   Fork fork(s, worth_a_fork(plan));
@@ -1931,9 +1930,10 @@ extern "C" int das_orthogonalize(const DasNsPlan* plan, const void* tables_dev, 
     else if (in_dtype == DAS_BF16) st = launch_small<bf16_t, false>(plan, tab, a, none, res, fork.stream());
     else st = launch_small<_Float16, false>(plan, tab, a, none, res, fork.stream());
     if (st != DAS_OK) return st;
-    if (plan->n_chunks == 0) continue;
     auto launch = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, dim3(plan->n_chunks), dim3(TPB), 0, s, mats, chunks, a, none, w.x[0], w.xt, w.part);
+      launch_ingest(plan, tab, fork, s, [&](const int4* chunks, int n, hipStream_t on) {
+        hipLaunchKernelGGL(kernel, dim3(n), dim3(TPB), 0, on, mats, chunks, a, none, w.x[0], w.xt, w.part);
+      });
     };
     if (in_dtype == DAS_F32) split ? launch(ingest_kernel<float, false, true>) : launch(ingest_kernel<float, false, false>);
     else if (in_dtype == DAS_BF16) split ? launch(ingest_kernel<bf16_t, false, true>) : launch(ingest_kernel<bf16_t, false, false>);
@@ -1961,10 +1961,10 @@ extern "C" int das_muon_step(const DasNsPlan* plan, const void* tables_dev, floa
   Fork fork(s, worth_a_fork(plan));
   const int st = launch_small<float, true>(plan, tab, Sources{}, mu, res, fork.stream());
   if (st != DAS_OK) return st;
-  if (plan->n_chunks) {
-    hipLaunchKernelGGL((ingest_kernel<float, true, true>), dim3(plan->n_chunks), dim3(TPB), 0, s, (const NsMatrix*)(tab + plan->mat_at),
-                       (const int4*)(tab + plan->chunk_at), Sources{}, mu, w.x[0], w.xt, w.part);
-    DAS_CHECK_LAUNCH();
-  }
+  launch_ingest(plan, tab, fork, s, [&](const int4* chunks, int n, hipStream_t on) {
+    hipLaunchKernelGGL((ingest_kernel<float, true, true>), dim3(n), dim3(TPB), 0, on, (const NsMatrix*)(tab + plan->mat_at), chunks, Sources{}, mu,
+                       w.x[0], w.xt, w.part);
+  });
+  DAS_CHECK_LAUNCH();
   return the_rest<true, true>(plan, tab, w, res, s, fork);
 }
