@@ -11,8 +11,8 @@
  * or write a channel slice of a wider tensor). dtype codes: DAS_F32 / DAS_BF16 storage,
  * arithmetic always accumulates in f32.
  *
- * Every function is asynchronous on `stream`, never allocates, never synchronises, and
- * returns DAS_OK or a DAS_ERR_* code (argument errors are detected before any launch).
+ * Every function is asynchronous on `stream`, never allocates, never synchronises (das_orthogonalize and das_muon_step may
+ * create a side stream and events once, see there), and returns DAS_OK or a DAS_ERR_* code (argument errors are detected before any launch).
  */
 #ifndef DAS_HIP_H
 #define DAS_HIP_H
