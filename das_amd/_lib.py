@@ -77,7 +77,7 @@ class DasNsShape(C.Structure):
 class DasNsPlan(C.Structure):
     _fields_ = [(k, i32) for k in ('n_groups', 'n_matrices', 'n_small', 'small_lds', 'small_quads', 'n_thin', 'n_slices', 'n_chunks', 'n_tile_chunks',
                                    'n_gram', 'n_gram_join', 'n_product', 'n_product_join', 'n_update', 'steps', 'product_tile',
-                                   'update_tile', 'product_kg', 'update_kg', 'gram_kg')] + \
+                                   'update_tile', 'product_kg', 'update_kg', 'gram_tile', 'gram_kg')] + \
                [(k, i64) for k in ('x_elems', 'a_elems', 'thin_x_elems', 'thin_a_elems', 'thin_slots', 'gram_slots', 'product_slots',
                                    'extent', 'mat_at', 'chunk_at', 'gram_at', 'gram_join_at', 'product_at', 'product_join_at',
                                    'update_at', 'slice_at', 'thin_at', 'table_bytes')] + \

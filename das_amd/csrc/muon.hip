@@ -37,7 +37,6 @@ typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int TPB = 256;
-constexpr int JOIN_TILE = 128;   // tiles whose inner axis may be split over workgroups
 constexpr int N_AREAS = 5;   // m x m work matrices: G, R, Z, two of Q (the f16 form uses G and Z)
 constexpr int CHUNK = 64;   // side of the blocks that ingest_kernel / normalise_kernel work on
 
@@ -578,7 +577,7 @@ __global__ __launch_bounds__(KG * TPB, KG == 1 ? 2 : KG) void sym_kernel(const N
   b.init(Q, pitch, j0, t.m, first);
   Acc<T> acc;
   multiply<T, SPLIT, KG>(a, b, stages, smem, acc);
-  if (T == JOIN_TILE && t.slot >= 0) {   // (a part of the inner axis: join_kernel goes on)
+  if (t.slot >= 0) {   // (a part of the inner axis: join_kernel goes on)
     if (KG == 1 || threadIdx.x < TPB) {
 #pragma unroll
       for (int i = 0; i < T / 32; ++i)
@@ -592,10 +591,10 @@ __global__ __launch_bounds__(KG * TPB, KG == 1 ? 2 : KG) void sym_kernel(const N
 
 // The parts of a tile whose inner axis was split, added in order, and stored as sym_store does; 16 workgroups a tile, four rows of one
 // column a thread (one workgroup a tile: 12 us, most of them waiting for one load after the other).
-template <bool SPLIT, SymKind KIND>
+template <int T, bool SPLIT, SymKind KIND>
 __global__ __launch_bounds__(TPB) void join_kernel(const NsItem* __restrict__ items, SymArgs s,
                                                    const f32x4_t* __restrict__ partial) {
-  constexpr int N = JOIN_TILE / 32, W = SPLIT ? 2 : 1;
+  constexpr int N = T / 32, W = SPLIT ? 2 : 1;
   const NsItem t = items[blockIdx.x / (N * N)];
   const int frag = blockIdx.x % (N * N), z = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const f32x4_t* from = partial + (((long long)z * s.slots + t.slot) * N * N + frag) * TPB + threadIdx.x;
@@ -607,8 +606,8 @@ __global__ __launch_bounds__(TPB) void join_kernel(const NsItem* __restrict__ it
 #pragma unroll
     for (int k = 0; k < 4; ++k) sum += v[k];
   }
-  const int r = t.ti * JOIN_TILE + (wave >> 1) * (JOIN_TILE / 2) + (frag / N) * 16 + (lane >> 4) * 4;   // four rows of one column
-  const int c = t.tj * JOIN_TILE + (wave & 1) * (JOIN_TILE / 2) + (frag % N) * 16 + (lane & 15);
+  const int r = t.ti * T + (wave >> 1) * (T / 2) + (frag / N) * 16 + (lane >> 4) * 4;   // four rows of one column
+  const int c = t.tj * T + (wave & 1) * (T / 2) + (frag % N) * 16 + (lane & 15);
   if (r >= t.lda) return;
   _Float16* out = s.out[z] + W * t.a;
   float v[4] = {sum[0], sum[1], sum[2], sum[3]};
@@ -1254,7 +1253,7 @@ Work carve(const DasNsPlan* p, bool split, void* ws) {
   w.qt = (_Float16*)take(up256(4 * p->thin_a_elems));
   w.thin_part = (f32x4_t*)take(1024 * p->thin_slots);
   w.part = (Partial*)take(up256((long long)sizeof(Partial) * p->n_chunks));
-  w.slots = (f32x4_t*)take(4LL * JOIN_TILE * JOIN_TILE * std::max(p->gram_slots, 2 * p->product_slots));
+  w.slots = (f32x4_t*)take(4 * std::max(p->gram_slots * p->gram_tile * p->gram_tile, 2 * p->product_slots * p->product_tile * p->product_tile));
   return w;
 }
 
@@ -1456,13 +1455,15 @@ int iterate(const DasNsPlan* p, const char* tab, Work w, const Result& res, hipS
     (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     hipLaunchKernelGGL(kernel, dim3(n, products), dim3(kg * TPB), lds, s, items, a, w.slots);
   };
-  constexpr int JOINERS = (JOIN_TILE / 32) * (JOIN_TILE / 32);
   auto gram_of = [&](const _Float16* x, _Float16* g) {
     const SymArgs a = {{x}, {x}, {g}, 0.f, 0.f, 0.f, p->gram_slots};
-    if (p->gram_kg == 2) launch_sym(sym_kernel<JOIN_TILE, SPLIT, 2, GRAM>, JOIN_TILE, 2, gram, p->n_gram, 1, a);
-    else launch_sym(sym_kernel<JOIN_TILE, SPLIT, 1, GRAM>, JOIN_TILE, 1, gram, p->n_gram, 1, a);
-    if (p->n_gram_join)
-      hipLaunchKernelGGL((join_kernel<SPLIT, GRAM>), dim3(p->n_gram_join * JOINERS), dim3(TPB), 0, s, gram_join, a, w.slots);
+    if (p->gram_kg == 4) launch_sym(sym_kernel<64, SPLIT, 4, GRAM>, 64, 4, gram, p->n_gram, 1, a);
+    else if (p->gram_kg == 2) launch_sym(sym_kernel<128, SPLIT, 2, GRAM>, 128, 2, gram, p->n_gram, 1, a);
+    else launch_sym(sym_kernel<128, SPLIT, 1, GRAM>, 128, 1, gram, p->n_gram, 1, a);
+    if (p->n_gram_join && p->gram_kg == 4)
+      hipLaunchKernelGGL((join_kernel<64, SPLIT, GRAM>), dim3(p->n_gram_join * 4), dim3(TPB), 0, s, gram_join, a, w.slots);
+    else if (p->n_gram_join)
+      hipLaunchKernelGGL((join_kernel<128, SPLIT, GRAM>), dim3(p->n_gram_join * 16), dim3(TPB), 0, s, gram_join, a, w.slots);
   };
   auto sym = [&](auto kind, int products, SymArgs a) {
     constexpr SymKind K = decltype(kind)::value;
@@ -1471,7 +1472,7 @@ int iterate(const DasNsPlan* p, const char* tab, Work w, const Result& res, hipS
     else if (p->product_tile == 128) launch_sym(sym_kernel<128, SPLIT, 1, K>, 128, 1, prod, p->n_product, products, a);
     else launch_sym(sym_kernel<64, SPLIT, 4, K>, 64, 4, prod, p->n_product, products, a);
     if (p->n_product_join)
-      hipLaunchKernelGGL((join_kernel<SPLIT, K>), dim3(p->n_product_join * JOINERS, products), dim3(TPB), 0, s, prod_join, a, w.slots);
+      hipLaunchKernelGGL((join_kernel<128, SPLIT, K>), dim3(p->n_product_join * 16, products), dim3(TPB), 0, s, prod_join, a, w.slots);
   };
   auto update = [&](auto last, const _Float16* q, const _Float16* x, _Float16* y) {
     constexpr bool L = decltype(last)::value;
@@ -1629,9 +1630,9 @@ long long makespan(const std::vector<int>& pieces, int slots, long long limit, s
 // Symmetric tiles of a launch for `slots` workgroups at a time. Tiles that would end after the others are split along the inner axis
 // where that pays: 1056 equal tiles in 512 slots are two rounds and a sixteenth, and took the time of nearly three. A part costs 128 KiB
 // of traffic, the join a launch: 0.0125 and 1.2 steps of 64 inner elements (2.5 us with two workgroups on a CU; 13 us measured for 272
-// parts). A workgroup whose neighbour on the CU has ended runs up to twice as fast, so only half of what sticks out counts. A part has
+// parts), six of the shorter steps of 64 x 64 tiles with four wave groups (4 ... 8 is level; 12: 8x 256 x 1024, Muon, 155 us instead of 150). A workgroup whose neighbour on the CU has ended runs up to twice as fast, so only half of what sticks out counts. A part has
 // at least 4 steps.
-void schedule(const Tables& tab, const std::vector<Tile>& tiles, int slots, Launch& launch, std::vector<NsItem>& join, long long& n_slots) {
+void schedule(const Tables& tab, const std::vector<Tile>& tiles, int slots, double join_cost, Launch& launch, std::vector<NsItem>& join, long long& n_slots) {
   auto item = [&](auto... v) { return tab.item(v...); };
   std::vector<int> order(tiles.size()), parts(tiles.size(), 1), late;
   for (size_t i = 0; i < tiles.size(); ++i) order[i] = (int)i;
@@ -1658,7 +1659,7 @@ void schedule(const Tables& tab, const std::vector<Tile>& tiles, int slots, Laun
         if (q > 1) count += q;
       }
       std::sort(pieces.begin(), pieces.end(), std::greater<int>());
-      const double t = seen(makespan(pieces, slots, 0, nullptr)) + 1.2 + 0.0125 * (double)count;
+      const double t = seen(makespan(pieces, slots, 0, nullptr)) + join_cost + 0.0125 * (double)count;
       if (t < best) {
         best = t;
         choice = p;
@@ -1803,8 +1804,11 @@ bool build(const DasNsShape* shapes, int n, double top, DasNsPlan* plan, Tables&
   plan->product_kg = plan->product_tile == 64 ? 4 : lower128 >= 384 ? 1 : 2;
   plan->update_tile = all64 > 512 ? 128 : 64;
   plan->update_kg = plan->update_tile == 64 ? 4 : all128 > 256 ? 1 : 2;
-  // X X^T: 128 x 128 tiles; where there are fewer than 384, two wave groups share a tile's inner axis (one workgroup a CU, not two)
-  plan->gram_kg = lower128 >= 384 ? 1 : 2;
+  // X X^T, whose inner axis is long and may be split: 64 x 64 tiles and four wave groups for one round of the CUs (256 x 2304 to bf16: 109 -> 99 us,
+  // 512 x 512 114 -> 99, 128 x 1152 Muon 109 -> 101; 12x 512 x 2048, 432 tiles: 470 us, 486 with 64 x 64 ones), then 128 x 128; where
+  // there are fewer than 384 of those, two wave groups share a tile (one workgroup a CU, not two)
+  plan->gram_tile = lower64 <= 256 ? 64 : 128;
+  plan->gram_kg = lower64 <= 256 ? 4 : lower128 >= 384 ? 1 : 2;
   // blocks of up to 8 x 8 tiles, smaller where one would be more than a 16th of the launch (half of an XCD's part)
   auto side_for = [](long long launch, int steps) {
     int side = 8;
@@ -1814,7 +1818,7 @@ bool build(const DasNsShape* shapes, int n, double top, DasNsPlan* plan, Tables&
   long long product_cost = 0, update_cost = 0, gram_cost = 0;
   for (int q = plan->n_small; q < tiled_end; ++q) {
     const NsMatrix& M = t.mats[q];
-    const long long p = over(M.m, plan->product_tile), r = over(M.m, plan->update_tile), w = over(M.m, JOIN_TILE);
+    const long long p = over(M.m, plan->product_tile), r = over(M.m, plan->update_tile), w = over(M.m, plan->gram_tile);
     product_cost += p * (p + 1) / 2 * (M.lda / 64 + 2);
     update_cost += r * (M.ldx / plan->update_tile) * (M.lda / 64 + 2);
     gram_cost += w * (w + 1) / 2 * (M.ldx / 64 + 2);
@@ -1822,7 +1826,7 @@ bool build(const DasNsShape* shapes, int n, double top, DasNsPlan* plan, Tables&
   std::vector<Tile> gram, product;
   for (int q = plan->n_small; q < tiled_end; ++q) {
     const NsMatrix& M = t.mats[q];
-    lower_blocks(over(M.m, JOIN_TILE), side_for(gram_cost, M.ldx / 64),
+    lower_blocks(over(M.m, plan->gram_tile), side_for(gram_cost, M.ldx / 64),
                  [&](bool fresh, int i, int j) { gram.push_back(Tile{fresh, q, i, j, M.ldx / 64}); });
     lower_blocks(over(M.m, plan->product_tile), side_for(product_cost, M.lda / 64),
                  [&](bool fresh, int i, int j) { product.push_back(Tile{fresh, q, i, j, M.lda / 64}); });
@@ -1832,9 +1836,9 @@ bool build(const DasNsShape* shapes, int n, double top, DasNsPlan* plan, Tables&
         for (int j = bj; j < std::min(cols, bj + side); ++j)
           for (int i = bi; i < std::min(rows, bi + side); ++i) t.update.add(i == bi && j == bj, t.item(q, i, j, 0, M.lda / 64, -1, 1));
   }
-  schedule(t, gram, plan->gram_kg == 1 ? 512 : 256, t.gram, t.gram_join, plan->gram_slots);
-  if (plan->product_tile == JOIN_TILE) {
-    schedule(t, product, plan->product_kg == 1 ? 512 : 256, t.product, t.product_join, plan->product_slots);
+  schedule(t, gram, plan->gram_kg == 1 ? 512 : 256, plan->gram_kg == 4 ? 6.0 : 1.2, t.gram, t.gram_join, plan->gram_slots);
+  if (plan->product_tile == 128) {
+    schedule(t, product, plan->product_kg == 1 ? 512 : 256, 1.2, t.product, t.product_join, plan->product_slots);
   } else {
     for (const Tile& p : product) t.product.add(p.fresh, t.item(p.matrix, p.ti, p.tj, 0, p.steps, -1, 1));
     t.product.place();

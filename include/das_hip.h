@@ -627,7 +627,7 @@ typedef struct {
 } DasNsShape;
 typedef struct {
   int n_groups, n_matrices, n_small, small_lds, small_quads, n_thin, n_slices, n_chunks, n_tile_chunks, n_gram, n_gram_join, n_product, n_product_join, n_update, steps;
-  int product_tile, update_tile, product_kg, update_kg, gram_kg;
+  int product_tile, update_tile, product_kg, update_kg, gram_tile, gram_kg;
   long long x_elems, a_elems, thin_x_elems, thin_a_elems, thin_slots, gram_slots, product_slots, extent;            /* work areas (f16 elements); one past the last element of the flat buffers used */
   long long mat_at, chunk_at, gram_at, gram_join_at, product_at, product_join_at, update_at, slice_at, thin_at, table_bytes;   /* byte offsets of the tables */
   float coef[3 * DAS_NS_MAX_STEPS];              /* a, b, c of each step */

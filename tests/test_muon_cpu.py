@@ -64,7 +64,7 @@ def test_schedule_covers_every_product_once(shapes):
     chunks = table(buf, plan.chunk_at, plan.n_chunks, np.dtype([(k, '<i4') for k in 'qrci']))
     assert len(set(map(tuple, chunks[['q', 'r', 'c']].tolist()))) == plan.n_chunks
     for at, n, join_at, n_join, slots, tile, inner in (
-            (plan.gram_at, plan.n_gram, plan.gram_join_at, plan.n_gram_join, plan.gram_slots, 128, 'ldx'),
+            (plan.gram_at, plan.n_gram, plan.gram_join_at, plan.n_gram_join, plan.gram_slots, plan.gram_tile, 'ldx'),
             (plan.product_at, plan.n_product, plan.product_join_at, plan.n_product_join, plan.product_slots, plan.product_tile, 'lda')):
         seen, used = {}, []
         for t in table(buf, at, n, ITEM):
