@@ -1257,6 +1257,20 @@ Work carve(const DasNsPlan* p, bool split, void* ws) {
   return w;
 }
 
+// Lets a kernel have a whole CU's dynamic LDS: asked of the runtime once a thread, device and kernel (a call in front of every launch: 0.0 us)
+void allow_lds(const void* kernel) {
+  constexpr int KERNELS = 64;
+  thread_local const void* seen[KERNELS];
+  thread_local int n = 0, of_dev = -1;
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess) return;
+  if (dev != of_dev) n = 0;
+  of_dev = dev;
+  for (int i = 0; i < n; ++i)
+    if (seen[i] == kernel) return;
+  if (hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, SMALL_LDS) == hipSuccess && n < KERNELS) seen[n++] = kernel;
+}
+
 bool phases_valid(const DasNsPlan* p) {
   for (int k = 0; k < p->steps; ++k)
     if (p->phase_end[k] <= k || p->phase_end[k] > p->steps) return false;
@@ -1408,7 +1422,7 @@ template <typename T, bool MUON>
 int launch_small(const DasNsPlan* p, const char* tab, const Sources& src, const MuonIn& mu, const Result& res, hipStream_t s) {
   if (p->n_small == 0) return DAS_OK;
   auto launch = [&](auto kernel) {
-    (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, p->small_lds);
+    allow_lds((const void*)kernel);
     hipLaunchKernelGGL(kernel, dim3(p->n_small), dim3(SMALL_TPB), p->small_lds, s, (const NsMatrix*)(tab + p->mat_at), src, mu, steps_of(p), res);
   };
   if (p->small_quads <= 2) launch(small_kernel<T, MUON, 2>);
@@ -1427,7 +1441,7 @@ int launch_thin(const DasNsPlan* p, const char* tab, const Work& w, const Result
   const int2* thin = (const int2*)(tab + p->thin_at);
   const Steps st = steps_of(p);
   constexpr int LDS = 2 * N_AREAS * SMALL_M * PA;
-  (void)hipFuncSetAttribute((const void*)chain_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+  allow_lds((const void*)chain_kernel);
   auto pass = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3(p->n_slices), dim3(TPB), 0, s, mats, slices, p->eps, w.part, w.xt, w.qt, w.thin_part, res);
   };
@@ -1452,7 +1466,7 @@ int iterate(const DasNsPlan* p, const char* tab, Work w, const Result& res, hipS
                *prod_join = (const NsItem*)(tab + p->product_join_at);
   auto launch_sym = [&](auto kernel, int tile, int kg, const NsItem* items, int n, int products, const SymArgs& a) {
     const int lds = kg * 4 * tile * 128;
-    (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    allow_lds((const void*)kernel);
     hipLaunchKernelGGL(kernel, dim3(n, products), dim3(kg * TPB), lds, s, items, a, w.slots);
   };
   auto gram_of = [&](const _Float16* x, _Float16* g) {
@@ -1478,7 +1492,7 @@ int iterate(const DasNsPlan* p, const char* tab, Work w, const Result& res, hipS
     constexpr bool L = decltype(last)::value;
     auto launch = [&](auto kernel, int tile, int kg) {
       const int lds = kg * 4 * tile * 128;
-      (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+      allow_lds((const void*)kernel);
       hipLaunchKernelGGL(kernel, dim3(p->n_update), dim3(kg * TPB), lds, s, mats, upd, q, x, y, res);
     };
     if (p->update_tile == 128 && p->update_kg == 2) launch(update_kernel<128, SPLIT, 2, L>, 128, 2);
