@@ -1405,9 +1405,10 @@ class Fork {
   hipStream_t main_;
   Side* side_ = nullptr;
 };
-// Beside tiles it pays (the detector's set 2276 -> 2216 us; seven small and thin matrices with two of 129 x 1023 and one of 700 x 513: 197 ->
-// 188 us), beside thin matrices alone the fork costs more than it hides (60 -> 85 us for five small and thin ones).
-bool worth_a_fork(const DasNsPlan* p) { return p->n_tile_chunks > 0 && p->n_small + p->n_thin > 0; }
+// It pays beside launches of tens of microseconds (the detector's set 2276 -> 2216 us), that is with 128 x 128 tiles of the products. Its
+// events cost the host 80 us a call: as much as it hides beside 64 x 64 ones (182 us either way for seven small and thin matrices with two of
+// 129 x 1023 and one of 700 x 513), more where there are no tiles (60 -> 85 us for five small and thin ones).
+bool worth_a_fork(const DasNsPlan* p) { return p->product_tile == 128 && p->n_tile_chunks > 0 && p->n_small + p->n_thin > 0; }
 
 Steps steps_of(const DasNsPlan* p) {
   Steps st;

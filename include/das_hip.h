@@ -648,7 +648,7 @@ int das_ns_plan(const DasNsShape* shapes, int n, int steps, const float* coef, f
 long long das_ns_ws_bytes(const DasNsPlan* plan, int f32_result);
 /* out (flat, out_dtype DAS_F32 / DAS_BF16 / DAS_F16, plan offsets): the orthogonalised matrices; srcs: one per group of the plan, in_dtype
  * DAS_F32 / DAS_BF16 / DAS_F16. `ws`: das_ns_ws_bytes() of device memory, 16-byte aligned, in use until the call's kernels end. `out`, the
- * sources and ws do not overlap. Small and thin matrices of a set that holds others too run on a stream of the library's own (default priority,
+ * sources and ws do not overlap. Small and thin matrices of a set that holds many or large others run on a stream of the library's own (default priority,
  * created at first need, kept) beside `stream`, which waits for them; a call that is being captured uses `stream` alone. */
 int das_orthogonalize(const DasNsPlan* plan, const void* tables_dev, const DasNsSource* srcs, int n_srcs, int in_dtype, void* out,
                       int out_dtype, void* ws, void* stream);

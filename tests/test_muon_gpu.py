@@ -201,12 +201,13 @@ def test_orthogonalize_large_tiles():
                 check(y[i], t[i], [COEF] * 5, what=(tuple(t.shape), i))
 
 
-def test_mixed_set_from_threads_streams_and_a_graph():
+@pytest.mark.parametrize('many', [False, True])     # True: launches long enough for the second stream
+def test_mixed_set_from_threads_streams_and_a_graph(many):
     """a set of every class (one workgroup, slices, tiles): the same bits alone, from two host threads on streams of their own at once, back to
     back on one stream with its input overwritten in between, and replayed"""
     import threading
     from das_amd import train_ops as T
-    mats = [gradient(64, 64, 1, k=3), gradient(30, 3000, 2, k=2), gradient(200, 333, 3, k=2), gradient(5000, 12, 4)]
+    mats = [gradient(64, 64, 1, k=3), gradient(30, 3000, 2, k=2), gradient(200, 333, 3, k=2), gradient(5000, 12, 4)] + [gradient(256, 200, 5, k=60)] * many
     plan = T.NewtonSchulzPlan([tuple(t.shape) for t in mats], DEV)
     for dt in (torch.bfloat16, torch.float32):
         want = T.orthogonalize(mats, plan=plan, out_dtype=dt)
