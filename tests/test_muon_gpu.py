@@ -191,6 +191,17 @@ def test_orthogonalize_many_tensors():
         check(y, t, [COEF] * 5)
 
 
+def test_orthogonalize_twenty_thousand_matrices():
+    """tables of more than a megabyte beside few elements"""
+    from das_amd import train_ops as T
+    t = gradient(2, 3, 8, k=20000)
+    plan = T.NewtonSchulzPlan([(20000, 2, 3)], DEV)
+    assert plan._flat[0].table_bytes > (1 << 20) + t.numel() // 16
+    y = T.orthogonalize(t, plan=plan)
+    for i in (0, 1, 9999, 19999):
+        check(y[i], t[i], [COEF] * 5, what=i)
+
+
 def test_orthogonalize_large_tiles():
     """sets of enough tiles for the 128 x 128 form, ragged at its edges"""
     from das_amd import train_ops as T
