@@ -248,11 +248,12 @@ class NewtonSchulzPlan:
             a.off, a.count, a.rows, a.cols = o, k, r, c
         plan = _lib.DasNsPlan()
         cf = (C.c_float * len(co))(*co)
-        # (room for the tables of all but odd sets at the first try: the schedule is worked out once; pages not written cost nothing)
-        host = torch.empty((1 << 20) + sum(k * r * c for _, (k, r, c) in entries) // 16, dtype=torch.uint8)
+        # (room for the tables of all but odd sets at the first try: the schedule is worked out once; pages not written cost nothing.
+        # The library writes them from the host: host memory whatever torch's default device is)
+        host = torch.empty((1 << 20) + sum(k * r * c for _, (k, r, c) in entries) // 16, dtype=torch.uint8, device='cpu')
         if lib.das_ns_plan(arr, len(entries), self.steps, cf, self.eps, C.byref(plan), _ptr(host), host.numel()) != _lib.DAS_OK:
             _lib.check(lib.das_ns_plan(arr, len(entries), self.steps, cf, self.eps, C.byref(plan), None, 0), 'das_ns_plan')
-            host = torch.empty(plan.table_bytes, dtype=torch.uint8)
+            host = torch.empty(plan.table_bytes, dtype=torch.uint8, device='cpu')
             _lib.check(lib.das_ns_plan(arr, len(entries), self.steps, cf, self.eps, C.byref(plan), _ptr(host), plan.table_bytes), 'das_ns_plan')
         return plan, host[:plan.table_bytes].to(self.device)
 
