@@ -200,7 +200,8 @@ NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)   # quintic of the published Muon op
 
 class NewtonSchulzPlan:
     """The tables of das_orthogonalize / das_muon_step for one set of matrices: built once, usable by any number of calls, on any
-    stream (a plan is read-only; workspaces come from torch's allocator call by call).
+    stream (a plan is read-only; workspaces come from torch's allocator call by call). It may be dropped while calls that it served are
+    still running; a plan that a call captured into a hipGraph used is kept as long as that graph is replayed.
 
     shapes: (rows, cols) or (count, rows, cols) of equal matrices, in storage order. offsets: element offset of each entry's first
     matrix in the flat buffers of muon_step (default: back to back; only such a plan serves orthogonalize). coefficients: (a, b, c) for every step or one triple
@@ -228,6 +229,7 @@ class NewtonSchulzPlan:
             if len(self.offsets) != len(sizes):
                 raise _lib.DasHipError('NewtonSchulzPlan: one offset for every entry of shapes')
         live = [(o, s) for o, s, n in zip(self.offsets, self.shapes, sizes) if n]
+        self._home = torch._C._cuda_getCurrentRawStream(self.device.index)     # the stream that the tables' memory belongs to
         self._flat = self._build(live, co)
         # orthogonalize()'s results: one flat output, every entry on a 16-byte boundary of it
         self._out, self._out_offsets, self._out_size = None, [], 0
@@ -256,6 +258,12 @@ class NewtonSchulzPlan:
             host = torch.empty(plan.table_bytes, dtype=torch.uint8, device='cpu')
             _lib.check(lib.das_ns_plan(arr, len(entries), self.steps, cf, self.eps, C.byref(plan), _ptr(host), plan.table_bytes), 'das_ns_plan')
         return plan, host[:plan.table_bytes].to(self.device)
+
+    def _used(self, tables):
+        """A call on the current stream reads `tables`: if it is not the stream that they were allocated on, their memory is not given
+        away before that call has ended, whenever the plan is dropped. (A captured call's reads come later: the plan is its owner's to keep.)"""
+        if torch._C._cuda_getCurrentRawStream(self.device.index) != self._home and not torch.cuda.is_current_stream_capturing():
+            tables.record_stream(torch.cuda.current_stream(self.device))
 
 
 def orthogonalize(mats, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, out_dtype=torch.bfloat16, plan=None):
@@ -296,6 +304,7 @@ def orthogonalize(mats, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, out_dty
         with _on(dev):
             lib = _lib.load()
             ws = torch.empty(lib.das_ns_ws_bytes(C.byref(p), int(out_dtype == torch.float32)), dtype=torch.uint8, device=dev)
+            plan._used(tables)
             _lib.check(lib.das_orthogonalize(C.byref(p), _ptr(tables), src, len(live), dt, _ptr(out), _NS_DT[out_dtype], _ptr(ws),
                                              _stream_of(dev)), 'das_orthogonalize')
     res = [out[o:o + t.numel()].view(t.shape) for o, t in zip(plan._out_offsets, mats)]
@@ -322,6 +331,7 @@ def muon_step(p, g, buf, plan, lr, momentum=0.95, weight_decay=0.0, nesterov=Tru
     with _on(p.device):
         lib = _lib.load()
         ws = torch.empty(lib.das_ns_ws_bytes(C.byref(c_plan), 1), dtype=torch.uint8, device=p.device)
+        plan._used(tables)
         _lib.check(lib.das_muon_step(C.byref(c_plan), _ptr(tables), _ptr(p), _ptr(g), _ptr(buf), float(lr), float(momentum),
                                      float(weight_decay), int(bool(nesterov)), int(lr_scale != 'original'), float(grad_scale),
                                      float(max_norm), _ptr(sumsq), _ptr(ws), _stream_of(p.device)), 'das_muon_step')
