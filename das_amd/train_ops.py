@@ -229,7 +229,6 @@ class NewtonSchulzPlan:
             if len(self.offsets) != len(sizes):
                 raise _lib.DasHipError('NewtonSchulzPlan: one offset for every entry of shapes')
         live = [(o, s) for o, s, n in zip(self.offsets, self.shapes, sizes) if n]
-        self._home = torch._C._cuda_getCurrentRawStream(self.device.index)     # the stream that the tables' memory belongs to
         self._flat = self._build(live, co)
         # orthogonalize()'s results: one flat output, every entry on a 16-byte boundary of it
         self._out, self._out_offsets, self._out_size = None, [], 0
@@ -257,7 +256,9 @@ class NewtonSchulzPlan:
             _lib.check(lib.das_ns_plan(arr, len(entries), self.steps, cf, self.eps, C.byref(plan), None, 0), 'das_ns_plan')
             host = torch.empty(plan.table_bytes, dtype=torch.uint8, device='cpu')
             _lib.check(lib.das_ns_plan(arr, len(entries), self.steps, cf, self.eps, C.byref(plan), _ptr(host), plan.table_bytes), 'das_ns_plan')
-        return plan, host[:plan.table_bytes].to(self.device)
+        tables = host[:plan.table_bytes].to(self.device)
+        self._home = torch._C._cuda_getCurrentRawStream(self.device.index)     # the stream that the tables' memory belongs to
+        return plan, tables
 
     def _used(self, tables):
         """A call on the current stream reads `tables`: if it is not the stream that they were allocated on, their memory is not given
