@@ -63,6 +63,18 @@ struct Partial {            // of one 64 x 64 block: sum of squares of (u 2^-e),
   int e;
 };
 
+// v as a pair of f16: v rounded, and what that leaves. Both parts come from one f32 value: the empty asm (no instruction) keeps hipcc from
+// fusing the multiplication that v comes from into one of two conversions of it. v_fma_mixlo_f16 rounds the product once, v_mul_f32 and
+// v_cvt_pk_f16_f32 round it twice: next to a tie they differ, and a high part with the low part of its neighbour is 2^-11 of v off.
+struct Pair {
+  _Float16 high, low;
+};
+__device__ __forceinline__ Pair pair_of(float v) {
+  asm("" : "+v"(v));
+  const _Float16 h = (_Float16)v;
+  return {h, (_Float16)(v - (float)h)};
+}
+
 // N (4 or 8) neighbouring values of a row of a work matrix (SPLIT: 32 high parts, then their 32 low parts, and so on along the row)
 template <bool SPLIT>
 __device__ __forceinline__ long long at(int ld, int r, int c) {
@@ -75,8 +87,9 @@ __device__ __forceinline__ void put(_Float16* base, int ld, int r, int c, const 
   vec_t h, l;
 #pragma unroll
   for (int e = 0; e < N; ++e) {
-    h[e] = (_Float16)v[e];
-    l[e] = (_Float16)(v[e] - (float)h[e]);
+    const Pair q = pair_of(v[e]);
+    h[e] = q.high;
+    l[e] = q.low;
   }
   *reinterpret_cast<vec_t*>(p) = h;
   if constexpr (SPLIT) *reinterpret_cast<vec_t*>(p + 32) = l;
@@ -632,8 +645,9 @@ __global__ __launch_bounds__(TPB) void join_kernel(const NsItem* __restrict__ it
   for (int e = 0; e < 4; ++e)
     if (r + e < t.m && c < t.lda) {
       _Float16* p = out + at<SPLIT>(t.lda, r + e, c);
-      p[0] = (_Float16)v[e];
-      if constexpr (SPLIT) p[32] = (_Float16)(v[e] - (float)p[0]);
+      const Pair q = pair_of(v[e]);
+      p[0] = q.high;
+      if constexpr (SPLIT) p[32] = q.low;
     }
 }
 
@@ -814,8 +828,9 @@ __device__ __forceinline__ void put4(_Float16* p, const float (&v)[4]) {
   f16x4_t h, l;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    h[e] = (_Float16)v[e];
-    l[e] = (_Float16)(v[e] - (float)h[e]);
+    const Pair q = pair_of(v[e]);
+    h[e] = q.high;
+    l[e] = q.low;
   }
   *reinterpret_cast<f16x4_t*>(p) = h;
   *reinterpret_cast<f16x4_t*>(p + 32) = l;
@@ -1005,9 +1020,9 @@ __device__ __forceinline__ void small_matrix(const NsMatrix& M, const DasNsSourc
           U[r * PF + c] = y;
         } else {
           _Float16* p = X + pair_at(PX, r, c);
-          const _Float16 h = (_Float16)y;
-          p[0] = h;
-          p[32] = (_Float16)(y - (float)h);
+          const Pair h = pair_of(y);
+          p[0] = h.high;
+          p[32] = h.low;
         }
       }
     }
@@ -1101,8 +1116,9 @@ __global__ __launch_bounds__(TPB) void thin_kernel(const NsMatrix* __restrict__ 
         f16x8_t a, b;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          a[e] = (_Float16)v[e];
-          b[e] = (_Float16)(v[e] - (float)a[e]);
+          const Pair q = pair_of(v[e]);
+          a[e] = q.high;
+          b[e] = q.low;
         }
         h = __builtin_bit_cast(uint4, a);
         l = __builtin_bit_cast(uint4, b);
@@ -1133,9 +1149,9 @@ __global__ __launch_bounds__(TPB) void thin_kernel(const NsMatrix* __restrict__ 
             us[r * PTF + c] = y;
           } else {
             _Float16* p = xs + pair_at(PT, r, c);
-            const _Float16 h = (_Float16)y;
-            p[0] = h;
-            p[32] = (_Float16)(y - (float)h);
+            const Pair h = pair_of(y);
+            p[0] = h.high;
+            p[32] = h.low;
           }
         }
       }

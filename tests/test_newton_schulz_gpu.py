@@ -45,3 +45,17 @@ def test_plan_dropped_while_another_stream_reads_its_tables(muon):
     early = any(f.data_ptr() <= at < f.data_ptr() + size for f in fresh) and not s.query()
     s.synchronize()
     assert not early and torch.equal(got, want)
+
+
+@pytest.mark.parametrize('shape', [(600, 700), (900, 500), (1, 64, 5000), (3000, 48), (16, 64, 256), (40, 30, 64)])
+def test_every_element_keeps_its_22_bits(shape):
+    """One step of the polynomial x -> x: an element leaves as it went in, but for its two roundings to a pair of f16 (2^-22 each of it, and the
+    2^-25 of f16's subnormal numbers over the scale, at least sqrt(n / 2)), the f32 factor, its product, the sum that it is alone in and the norm
+    (f32 sums of squares of 24 additions, under a root): 2^-19 = (2 * 4 + 24) 2^-24 covers them. A wrong low part is 2^-11."""
+    from das_amd import train_ops as T
+    u = torch.randn(shape, generator=torch.Generator().manual_seed(shape[-1])).to(DEV)
+    u = u * torch.exp(torch.randn(shape[:-1], generator=torch.Generator().manual_seed(5)))[..., None].to(DEV)
+    got = T.orthogonalize(u, steps=1, coefficients=(1.0, 0.0, 0.0), out_dtype=torch.float32).double()
+    x = u.double() / (torch.linalg.matrix_norm(u.double())[..., None, None] + 1e-7)
+    off = (got - x).abs()
+    assert (off <= 2.0 ** -19 * x.abs() + 2.0 ** -25 / (max(shape[-2:]) / 2) ** 0.5).all(), float((off / x.abs()).max())
