@@ -848,7 +848,8 @@ struct Share {
     c0 = (f % n) * 16;
   }
 };
-// a symmetric result, stored transposed (four values of a lane are neighbours then): f(row, col, four values) may change them
+// P Q^T's fragment stored transposed (four values of a lane are neighbours then), so that Q P^T is what lies there: f(row, col, four values)
+// may change them
 template <typename F>
 __device__ __forceinline__ void frag_store(const Share& w, const f32x4_t& acc, _Float16* out, F f) {
   const int lane = threadIdx.x & 63, r = w.c0 + (lane & 15), c = w.r0 + (lane >> 4) * 4;
@@ -872,6 +873,9 @@ __device__ __forceinline__ void store_gram(const Share& w, f32x4_t acc, f32x4_t*
   __syncthreads();
 }
 // Steps k ... end - 1 on the m x m matrices (the same products as iterate<true>), G in A[0]; -> Q
+// The factors' order matters to rounding errors alone. Between the null space of X X^T, where Z is near 3.4, and the rest, where it is near 1, those
+// of Z G Z and of Z Q (Q's columns in the rest) grow by the product of both a step, those of Z Z G or Q Z by the larger one squared
+// (64 x 64 of rank one: 4e-4 off instead of 2e-5). The tiles' form has no order: it computes one half and mirrors it.
 template <int K>   // K inner steps of 32: m <= 32 K
 __device__ __forceinline__ _Float16* phase_chain(const Share& w, _Float16* const (&A)[N_AREAS], const Steps& st, int k, int end, float gscale) {
   const bool on = w.part == 0, second = w.part == (w.parts > 1 ? 1 : 0);
@@ -889,8 +893,9 @@ __device__ __forceinline__ _Float16* phase_chain(const Share& w, _Float16* const
         for (int t = 0; t < 4; ++t) v[t] = cc * v[t] + cb * ((float)h[t] + (float)l[t]) + (r == c + t ? ca : 0.f);
       });
     __syncthreads();
-    if (on && q) frag_store(w, square_product<K>(z, w.r0, q, w.c0), other, plain);
-    if (second && j + 1 < end) frag_store(w, square_product<K>(z, w.r0, G, w.c0), R, plain);
+    // Q between the steps is kept transposed, Q^T Z; the last product is Z (Q^T)^T, the rows that meet X
+    if (on && q) frag_store(w, j + 1 < end ? square_product<K>(z, w.r0, q, w.c0) : square_product<K>(q, w.r0, z, w.c0), other, plain);
+    if (second && j + 1 < end) frag_store(w, square_product<K>(G, w.r0, z, w.c0), R, plain);   // Z G
     __syncthreads();
     if (q) {
       _Float16* t = q;
@@ -900,7 +905,8 @@ __device__ __forceinline__ _Float16* phase_chain(const Share& w, _Float16* const
       q = z;
     }
     if (j + 1 < end) {
-      if (on) frag_store(w, square_product<K>(R, w.r0, z, w.c0), G, plain);   // (nobody reads G any more)
+      // Z (Z G)^T (nobody reads G any more)
+      if (on) frag_store(w, square_product<K>(R, w.r0, z, w.c0), G, plain);
       __syncthreads();
     }
   }

@@ -59,3 +59,46 @@ def test_every_element_keeps_its_22_bits(shape):
     x = u.double() / (torch.linalg.matrix_norm(u.double())[..., None, None] + 1e-7)
     off = (got - x).abs()
     assert (off <= 2.0 ** -19 * x.abs() + 2.0 ** -25 / (max(shape[-2:]) / 2) ** 0.5).all(), float((off / x.abs()).max())
+
+
+def low_rank(r, c, k, seed):
+    """a weight's gradient out of k pixels: channels of very different size times rectified features; for k = 0 out of more than the sides"""
+    gen = torch.Generator().manual_seed(seed)
+    k = k or 2 * max(r, c)
+    d = torch.randn(k, r, generator=gen) * torch.exp(torch.randn(r, generator=gen))
+    x = (torch.randn(k, c, generator=gen) + torch.randn(k, 1, generator=gen)).relu()
+    return d.to(DEV).t() @ x.to(DEV)
+
+
+def polar64(u, coef=COEF, steps=5, eps=1e-7):
+    """the formula in 64 bits"""
+    x = u.double() / (u.double().norm() + eps)
+    x = x.t() if x.shape[0] > x.shape[1] else x
+    a, b, c = coef
+    for _ in range(steps):
+        g = x @ x.t()
+        x = a * x + (b * g + c * (g @ g)) @ x
+    return x.t() if u.shape[0] > u.shape[1] else x
+
+
+def off(got, u, **kw):
+    """distance from the formula over its norm (2-norm over all entries)"""
+    ref = polar64(u, **kw)
+    return float((got.double() - ref).norm() / ref.norm())
+
+
+def pairs_bound(m, rank):
+    """Error of an f32 result of five default steps over the result's norm. What X is off outside its row and column space grows by 3.4445 a
+    step: 485 in all; the result's `rank` singular values are 0.7 at least. X is rounded to a pair three times on its way (as it comes in, divided
+    by its norm, after the first phase), by at most 2^-23 of an element each time, uniform in that: 3^-1/2 of it on the average of a matrix,
+    2^-23 for the three. Each of the two products Q X adds 3 m / 32 partial sums of m inner elements one after the other, in f32, half a step
+    (2^-24) at most each, again uniform: 2^-24 (m / 32)^1/2 a product. Errors of Q and G stay in X's row space and do not grow."""
+    return 3.4445 ** 5 / 0.7 * (2.0 ** -46 + 2 * m / 32 * 2.0 ** -48) ** 0.5 / min(rank or 16, 16) ** 0.5
+
+
+@pytest.mark.parametrize('rank', [1, 2, 16, 0])
+@pytest.mark.parametrize('shape', [(64, 64), (60, 64), (30, 3000), (3000, 20)], ids=lambda s: '%dx%d' % s)
+def test_f32_result_of_any_rank(shape, rank):
+    from das_amd import train_ops as T
+    u = low_rank(*shape, rank, seed=sum(shape) + rank)
+    assert off(T.orthogonalize(u, out_dtype=torch.float32), u) <= pairs_bound(min(shape), rank)
