@@ -16,8 +16,9 @@
 //   in the direction of small singular values s while G's true entries there grow alike but start smaller, has grown 256-fold: with
 //   the default polynomial three steps, then two. 5e-5 ... 2e-4 off 64-bit arithmetic for any spectrum (f32 throughout: 1e-6 ... 5e-5).
 //
-// Scales keep entries among f16's normal numbers: X is kept times S = 2^round(log2 sqrt(n)) (an orthogonal X has entries of 1 /
-// sqrt(n)), G times gscale, about m (its trace starts at one). Row lengths are padded with zeros (ldx, lda) to whole stages of the inner axis.
+// Scales keep entries, and the low parts of pairs, among f16's normal numbers. X is kept times S, 2^15 over the bound of its norm: an entry of
+// a rank-one X is about (m n)^-1/2, and with S = sqrt(n) its low part was subnormal, 2^-25 off (4096 x 4096, f32 result: 8e-4 off instead of
+// 3e-4). G is kept times gscale, about m (its trace starts at one). Row lengths are padded with zeros (ldx, lda) to whole stages of the inner axis.
 #include <algorithm>
 #include <cmath>
 #include <cstring>
@@ -1792,7 +1793,8 @@ bool build(const DasNsShape* shapes, int n, double top, DasNsPlan* plan, Tables&
         M.ldx = over(M.n, 128) * 128; M.lda = over(M.m, 64) * 64;
         M.src = s.off + (long long)i * s.rows * s.cols;
         M.group = g; M.index = i;
-        M.scale = (float)std::ldexp(1.0, (int)std::lround(0.5 * std::log2((double)M.n)));
+        // X's largest entry is its norm's bound: as near to f16's end as a factor of two allows
+        M.scale = (float)std::ldexp(1.0, (int)std::floor(std::log2(32768.0 / top)));
         // about m, and top^2 gscale within f16
         M.gscale = (float)std::ldexp(1.0, std::min((int)std::lround(std::log2((double)M.m)), (int)std::floor(std::log2(32768.0 / (top * top)))));
         if (cls == SMALL) {

@@ -61,6 +61,19 @@ def test_every_element_keeps_its_22_bits(shape):
     assert (off <= 2.0 ** -19 * x.abs() + 2.0 ** -25 / (max(shape[-2:]) / 2) ** 0.5).all(), float((off / x.abs()).max())
 
 
+@pytest.mark.parametrize('shape', [(64, 200), (40, 7000), (1500, 1500), (600, 5000)])
+def test_small_elements_keep_their_bits_too(shape):
+    """As above, of a rank-one matrix, whose elements are about (m n)^-1/2. The polynomial x -> x keeps X's norm at one, so that X is stored times
+    2^15 and a subnormal number is 2^-25 2^-15 off; the first pass stores blocks with their largest element at 2^9 or more: 2^-34 of it."""
+    from das_amd import train_ops as T
+    gen = torch.Generator().manual_seed(shape[1])
+    u = torch.outer(torch.randn(shape[0], generator=gen), torch.randn(shape[1], generator=gen)).to(DEV)
+    got = T.orthogonalize(u, steps=1, coefficients=(1.0, 0.0, 0.0), out_dtype=torch.float32).double()
+    x = u.double() / (u.double().norm() + 1e-7)
+    off = (got - x).abs()
+    assert (off <= 2.0 ** -19 * x.abs() + 2.0 ** -40 + 2.0 ** -34 * x.abs().max()).all(), float((off / x.abs()).max())
+
+
 def low_rank(r, c, k, seed):
     """a weight's gradient out of k pixels: channels of very different size times rectified features; for k = 0 out of more than the sides"""
     gen = torch.Generator().manual_seed(seed)
@@ -97,7 +110,8 @@ def pairs_bound(m, rank):
 
 
 @pytest.mark.parametrize('rank', [1, 2, 16, 0])
-@pytest.mark.parametrize('shape', [(64, 64), (60, 64), (30, 3000), (3000, 20)], ids=lambda s: '%dx%d' % s)
+@pytest.mark.parametrize('shape', [(64, 64), (60, 64), (30, 3000), (3000, 20), (256, 2304), (700, 513), (1024, 1024), (4096, 4096), (2048, 8192)],
+                         ids=lambda s: '%dx%d' % s)
 def test_f32_result_of_any_rank(shape, rank):
     from das_amd import train_ops as T
     u = low_rank(*shape, rank, seed=sum(shape) + rank)
