@@ -4,17 +4,17 @@
 // X = (a I + b X X^T + c (X X^T)^2) X: in singular values s -> s (a + b s^2 + c s^4). All matrices of a set go through the same launches:
 // a table (built once on the host, das_ns_plan) lists every tile of every matrix, one workgroup per tile.
 //
-// Two precisions, by the type of the result.
-// f16 / bf16 results: X, G and Z are f16 (11 bits; bf16's 8 would make the error 8 times larger at the same matrix-pipe rate), sums f32.
-//   G = X X^T   Z = a I + b G + c G G   X = Z X                            15 m m n + 5 m^3 flops for five steps
-//   (a symmetric product is computed on and below its diagonal). 1e-3 off 64-bit arithmetic for a training run's gradients.
-// f32 results (parameters, whose last bits a learning rate of 1e-2 already reaches): every operand is a pair of f16, high + low part, 22
-//   bits, and a product is three (high high + high low + low high). To pay for it the m x n matrix is touched as seldom as possible: Z(G)
-//   commutes with G, so several steps can be taken on m x m matrices alone,
-//     Q = Z Q,  G' = X' X'^T = Z G Z      and X' = Q X at the end of such a phase:   18 m m n + 42 m^3 for five steps
-//   (plain steps with three products: 45 m m n + 15 m^3). A phase ends before an error of G, which grows by (a + b s^2 + c s^4)^2 a step
-//   in the direction of small singular values s while G's true entries there grow alike but start smaller, has grown 256-fold: with
-//   the default polynomial three steps, then two. 5e-5 ... 2e-4 off 64-bit arithmetic for any spectrum (f32 throughout: 1e-6 ... 5e-5).
+// Every operand is a pair of f16, high + low part, 22 bits, and a product is three (high high + high low + low high), whatever the result's type:
+// an error of X outside its row and column space grows by |a| a step, 485-fold in five default ones. Single f16 operands, 11 bits, would do for
+// gradients of full rank (2e-3 off 64-bit arithmetic in bf16 with its own rounding, and 1.4 to 2.1 times faster), but lose gradients out of few
+// pixels: rank 128 1e-2, rank 16 4e-2, rank one 0.2 off. Pairs, f32 result: full rank 2e-6 ... 5e-6, rank 16 2e-5 ... 6e-5, rank one 9e-5 (256 x 2304)
+// ... 3e-4 (4096 x 4096). More steps, or steeper ones, cost the product of the polynomial's slopes.
+// To pay for three products the m x n matrix is touched as seldom as possible: Z(G) commutes with G, so several steps can be taken on m x m
+// matrices alone,
+//   G = X X^T;  each step  Z = a I + b G + c G G,  Q = Z Q,  G = X' X'^T = Z G Z;  X' = Q X at the end of such a phase
+// 18 m m n + 42 m^3 flops for five steps (plain steps with three products: 45 m m n + 15 m^3; a symmetric product is computed on and below its
+// diagonal). A phase ends before an error of G, which grows by (a + b s^2 + c s^4)^2 a step in the direction of small singular values s while
+// G's true entries there grow alike but start smaller, has grown 256-fold: with the default polynomial three steps, then two.
 //
 // Scales keep entries, and the low parts of pairs, among f16's normal numbers. X is kept times S, 2^15 over the bound of its norm: an entry of
 // a rank-one X is about (m n)^-1/2, and with S = sqrt(n) its low part was subnormal, 2^-25 off (4096 x 4096, f32 result: 8e-4 off instead of
@@ -38,7 +38,7 @@ typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int TPB = 256;
-constexpr int N_AREAS = 5;   // m x m work matrices: G, R, Z, two of Q (the f16 form uses G and Z)
+constexpr int N_AREAS = 5;   // m x m work matrices: G, R, Z, two of Q
 constexpr int CHUNK = 64;   // side of the blocks that ingest_kernel / normalise_kernel work on
 
 struct NsMatrix {           // one matrix, as the kernels see it
@@ -49,7 +49,7 @@ struct NsMatrix {           // one matrix, as the kernels see it
   int chunk0, chunks;       // its blocks in the partial-sum table
   float scale, gscale;      // S; what G is kept times
   int tall;                 // rows > cols: X holds the transpose
-  int thin;                 // m <= 64, too long for one workgroup: X and Q are in areas of their own, as pairs
+  int thin;                 // m <= 64, too long for one workgroup: X and Q are in areas of their own
 };
 struct NsItem {             // a workgroup's share: output tile (ti, tj) of a matrix, inner elements 64 k0 ... 64 (k0 + kn)
   int matrix, ti, tj, k0, kn;
@@ -76,15 +76,14 @@ __device__ __forceinline__ Pair pair_of(float v) {
   return {h, (_Float16)(v - (float)h)};
 }
 
-// N (4 or 8) neighbouring values of a row of a work matrix (SPLIT: 32 high parts, then their 32 low parts, and so on along the row)
-template <bool SPLIT>
+// N (4 or 8) neighbouring values of a row of a work matrix: 32 high parts, then their 32 low parts, and so on along the row
 __device__ __forceinline__ long long at(int ld, int r, int c) {
-  return SPLIT ? (long long)r * (2 * ld) + (c >> 5) * 64 + (c & 31) : (long long)r * ld + c;
+  return (long long)r * (2 * ld) + (c >> 5) * 64 + (c & 31);
 }
-template <bool SPLIT, int N>
+template <int N>
 __device__ __forceinline__ void put(_Float16* base, int ld, int r, int c, const float (&v)[N]) {
   typedef _Float16 vec_t __attribute__((ext_vector_type(N)));
-  _Float16* p = base + at<SPLIT>(ld, r, c);
+  _Float16* p = base + at(ld, r, c);
   vec_t h, l;
 #pragma unroll
   for (int e = 0; e < N; ++e) {
@@ -93,15 +92,13 @@ __device__ __forceinline__ void put(_Float16* base, int ld, int r, int c, const 
     l[e] = q.low;
   }
   *reinterpret_cast<vec_t*>(p) = h;
-  if constexpr (SPLIT) *reinterpret_cast<vec_t*>(p + 32) = l;
+  *reinterpret_cast<vec_t*>(p + 32) = l;
 }
-template <bool SPLIT, int N>
+template <int N>
 __device__ __forceinline__ void get(const _Float16* base, int ld, int r, int c, float (&v)[N]) {
   typedef _Float16 vec_t __attribute__((ext_vector_type(N)));
-  const _Float16* p = base + at<SPLIT>(ld, r, c);
-  const vec_t h = *reinterpret_cast<const vec_t*>(p);
-  vec_t l = {};
-  if constexpr (SPLIT) l = *reinterpret_cast<const vec_t*>(p + 32);
+  const _Float16* p = base + at(ld, r, c);
+  const vec_t h = *reinterpret_cast<const vec_t*>(p), l = *reinterpret_cast<const vec_t*>(p + 32);
 #pragma unroll
   for (int e = 0; e < N; ++e) v[e] = (float)h[e] + (float)l[e];
 }
@@ -158,7 +155,7 @@ __device__ __forceinline__ float load_as_f32(const void* base, long long i) {
 // One 64 x 64 block of U: update the momentum (Muon), find the block's exponent e (largest entry in [1/2, 1) 2^(e + 10)) and sum of
 // squares, store u 2^-e in X's layout (transposed through LDS for tall matrices), zeros in the padding. The exponent keeps gradients
 // of any magnitude inside f16's range until the norm is known; normalise_kernel rounds a second time.
-template <typename T, bool MUON, bool SPLIT>
+template <typename T, bool MUON>
 __global__ __launch_bounds__(TPB) void ingest_kernel(const NsMatrix* __restrict__ mats, const int4* __restrict__ chunks, Sources src,
                                                      MuonIn mu, _Float16* __restrict__ X, _Float16* __restrict__ XT, Partial* __restrict__ part) {
   __shared__ float tile[CHUNK][CHUNK + 1];
@@ -272,13 +269,11 @@ __global__ __launch_bounds__(TPB) void ingest_kernel(const NsMatrix* __restrict_
   for (int k = 0; k < 4; ++k) {
     const int r = x_r0 + rr + k * 16;
     if (r >= M.m) continue;
-    if (SPLIT || M.thin) put<true>((M.thin ? XT : X) + 2 * M.x, M.ldx, r, x_c0 + c4, u[k]);
-    else put<false>(X + M.x, M.ldx, r, x_c0 + c4, u[k]);
+    put((M.thin ? XT : X) + 2 * M.x, M.ldx, r, x_c0 + c4, u[k]);
   }
 }
 
 // X <- X 2^e S / (|U|_F + eps), block by block. Every workgroup sums its matrix's partials itself, in one fixed order, in f64.
-template <bool SPLIT>
 __global__ __launch_bounds__(TPB) void normalise_kernel(const NsMatrix* __restrict__ mats, const int4* __restrict__ chunks, float eps,
                                                         _Float16* __restrict__ X, const Partial* __restrict__ part) {
   __shared__ double red[4];
@@ -301,12 +296,12 @@ __global__ __launch_bounds__(TPB) void normalise_kernel(const NsMatrix* __restri
   for (int k = 0; k < 4; ++k) {
     const int r = x_r0 + rr + k * 16;
     if (r >= M.m) continue;
-    _Float16* x = X + (SPLIT ? 2 : 1) * M.x;
+    _Float16* x = X + 2 * M.x;
     float v[4];
-    get<SPLIT>(x, M.ldx, r, x_c0 + c4, v);
+    get(x, M.ldx, r, x_c0 + c4, v);
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] *= f;
-    put<SPLIT>(x, M.ldx, r, x_c0 + c4, v);
+    put(x, M.ldx, r, x_c0 + c4, v);
   }
 }
 
@@ -314,11 +309,9 @@ __global__ __launch_bounds__(TPB) void normalise_kernel(const NsMatrix* __restri
 // T x T tile (T = 128 or 64) of one matrix by four waves of T/2 x T/2, v_mfma_f32_16x16x32_f16: lane l holds row l % 16 of A (column of
 // B), inner elements (l / 16) * 8 ... + 8, and gets column l % 16, rows (l / 16) * 4 ... + 4 of the result.
 //
-// A stage is 128 bytes of every row of both operands: 64 inner elements, or (SPLIT) 32 high parts and their 32 low parts, which lie next to
-// each other in memory so that both forms read whole 128-byte lines. It is copied global -> LDS without passing registers into one of
-// two buffers.
-//   plain:  acc += A0 B0 + A1 B1   (two halves of the inner axis)
-//   SPLIT:  acc += Ah Bh + Ah Bl + Al Bh   (the low x low part is 2^-22 of the product)
+// A stage is 128 bytes of every row of both operands, a whole line: 32 inner elements' high parts and their low parts, which lie next to
+// each other in memory. It is copied global -> LDS without passing registers into one of two buffers.
+//   acc += Al Bh + Ah Bl + Ah Bh   (the low x low part is 2^-22 of the product)
 // KG groups of four waves divide the inner axis between them (KG = 4 or 2 where a launch has few tiles and latency is all: every
 // group has its own buffers and copies in flight) and join their sums through LDS, in order.
 // LDS images. Rows by rows (gram, product, and B of the update): two panels of T rows x 64 bytes, 16-byte slot s of row r holds source
@@ -373,16 +366,16 @@ struct RowsOperand {        // T rows of a matrix whose rows run along the inner
   }
 };
 
-template <int T, bool SPLIT>
+template <int T>
 struct ColsOperand {        // T columns of a matrix whose rows run across the inner axis
-  static constexpr int ROWB = SPLIT ? T * 4 : T * 2, LPR = ROWB / 16, ROWS = SPLIT ? 32 : 64;   // bytes and lanes of a row, rows of a stage
+  static constexpr int ROWB = T * 4, LPR = ROWB / 16, ROWS = 32;   // bytes and lanes of a row, rows of a stage
   const char* base;
   int pitch, rows, row;     // bytes; rows of the matrix; the stage's first row
   static __device__ __forceinline__ int swz(int r) {
-    return ROWB >= 256 ? ((r & 3) | ((r >> 1) & 4)) : (((r >> 1) & 1) | ((r >> 2) & 2));
+    return (r & 3) | ((r >> 1) & 4);
   }
   __device__ __forceinline__ void init(const _Float16* x, int pitch_elems, int col0, int rows_, int stage0) {
-    base = (const char*)(x + col0 * (SPLIT ? 2 : 1));
+    base = (const char*)(x + col0 * 2);
     pitch = pitch_elems * 2;
     rows = rows_;
     row = stage0 * ROWS;
@@ -399,11 +392,11 @@ struct ColsOperand {        // T columns of a matrix whose rows run across the i
   }
   static __device__ __forceinline__ f16x8_t frag(const char* lds, int col0, int t, int p) {
     const int lane = threadIdx.x & 63, q = lane & 15, c = col0 + t * 16;
-    const int unit = SPLIT ? (c >> 5) * 4 + p * 2 + ((c >> 4) & 1) : c >> 4;
+    const int unit = (c >> 5) * 4 + p * 2 + ((c >> 4) & 1);
     i16x4_t v[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int r = (SPLIT ? 0 : p * 32) + (lane >> 4) * 8 + h * 4 + (q >> 2);
+      const int r = (lane >> 4) * 8 + h * 4 + (q >> 2);
       v[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
           (__attribute__((address_space(3))) i16x4_t*)(lds + r * ROWB + ((unit ^ swz(r)) * 32) + (q & 3) * 8));
     }
@@ -425,7 +418,7 @@ template <int T, int KG>
 constexpr int lds_bytes() { return KG * 4 * T * 128; }
 
 // `stages`: of the workgroup's part of the inner axis; the group's first one is group * ceil(stages / KG)
-template <int T, bool SPLIT, int KG, typename OB>
+template <int T, int KG, typename OB>
 __device__ __forceinline__ void multiply(RowsOperand<T>& a, OB& b, int stages, char* smem, Acc<T>& acc) {
   constexpr int HALF = T * 128, N = T / 32;   // bytes of one operand's stage; fragments a wave has of each operand
   const int wave = (threadIdx.x >> 6) & 3, wr = (wave >> 1) * (T / 2), wc = (wave & 1) * (T / 2);
@@ -462,13 +455,12 @@ __device__ __forceinline__ void multiply(RowsOperand<T>& a, OB& b, int stages, c
     if (k + 1 < mine) read(k + 1, std::integral_constant<int, Z ^ 1>{});
     if (k < mine) {
 #pragma unroll
-      for (int q = 0; q < (SPLIT ? 3 : 2); ++q)   // plain: 00 11; split: low parts first (10, 01), then 00
+      for (int q = 0; q < 3; ++q)   // low parts first
 #pragma unroll
         for (int i = 0; i < N; ++i)
 #pragma unroll
           for (int j = 0; j < N; ++j) {
-            const int pa = SPLIT ? q == 0 : q, pb = SPLIT ? q == 1 : q;
-            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa[Z][pa][i], fb[Z][pb][j], acc[i][j], 0, 0, 0);
+            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa[Z][q == 0][i], fb[Z][q == 1][j], acc[i][j], 0, 0, 0);
           }
     }
   };
@@ -551,16 +543,16 @@ struct SymArgs {            // two independent products a launch (blockIdx.y)
 // Symmetric m x m results, tiles on and below the diagonal, each stored as it is and transposed.
 //   GRAM:     G = X X^T times (gscale / S^2)      POLY: Z = a I + b G + c G G      PRODUCT: P Q of symmetric P, Q that commute
 // Columns m ... lda are stored as zeros: the inner axis of the next product.
-template <int T, bool SPLIT, int KG, SymKind KIND>
+template <int T, int KG, SymKind KIND>
 __device__ __forceinline__ void sym_store(const NsItem& M, const SymArgs& s, int z, int i0, int j0, const Acc<T>& acc, char* smem) {
-  const _Float16* P = s.p[z] + (SPLIT ? 2 : 1) * M.a;
-  _Float16* out = s.out[z] + (SPLIT ? 2 : 1) * M.a;
+  const _Float16* P = s.p[z] + 2 * M.a;
+  _Float16* out = s.out[z] + 2 * M.a;
   const float f = KIND == GRAM ? M.gscale / (M.scale * M.scale) : 1.f, cb = s.b / M.gscale, cc = s.c / (M.gscale * M.gscale);
   auto store = [&](int r, int c, float (&v)[8]) {
     if (r >= M.m || c >= M.lda) return;
     if constexpr (KIND == POLY) {
       float g[8];
-      get<SPLIT>(P, M.lda, r, c, g);
+      get(P, M.lda, r, c, g);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = cc * v[e] + cb * g[e] + (r == c + e ? s.a : 0.f);
     } else {
@@ -570,27 +562,27 @@ __device__ __forceinline__ void sym_store(const NsItem& M, const SymArgs& s, int
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       if (c + e >= M.m) v[e] = 0.f;
-    put<SPLIT>(out, M.lda, r, c, v);
+    put(out, M.lda, r, c, v);
   };
   store_tile<T, KG, false>(acc, smem, [&](int r, int c, float (&v)[8]) { store(i0 + r, j0 + c, v); });
   if (i0 != j0) store_tile<T, KG, true>(acc, smem, [&](int r, int c, float (&v)[8]) { store(j0 + r, i0 + c, v); });
 }
 
-template <int T, bool SPLIT, int KG, SymKind KIND>
+template <int T, int KG, SymKind KIND>
 __global__ __launch_bounds__(KG * TPB, KG == 1 ? 2 : KG) void sym_kernel(const NsItem* __restrict__ items, SymArgs s, f32x4_t* __restrict__ partial) {
   extern __shared__ __align__(16) char smem[];
   const NsItem t = items[blockIdx.x];
   if (t.matrix < 0) return;   // (filling: an XCD's queue is shorter than the longest)
   const int z = blockIdx.y, i0 = t.ti * T, j0 = t.tj * T;
-  const int ld = KIND == GRAM ? t.ldx : t.lda, pitch = SPLIT ? 2 * ld : ld;
-  const _Float16* P = s.p[z] + (SPLIT ? 2 : 1) * (KIND == GRAM ? t.x : t.a);
-  const _Float16* Q = s.q[z] + (SPLIT ? 2 : 1) * (KIND == GRAM ? t.x : t.a);
+  const int ld = KIND == GRAM ? t.ldx : t.lda, pitch = 2 * ld;
+  const _Float16* P = s.p[z] + 2 * (KIND == GRAM ? t.x : t.a);
+  const _Float16* Q = s.q[z] + 2 * (KIND == GRAM ? t.x : t.a);
   RowsOperand<T> a, b;
-  const int stages = (SPLIT ? 2 : 1) * t.kn, first = (SPLIT ? 2 : 1) * t.k0 + first_stage<KG>(stages);
+  const int stages = 2 * t.kn, first = 2 * t.k0 + first_stage<KG>(stages);
   a.init(P, pitch, i0, t.m, first);
   b.init(Q, pitch, j0, t.m, first);
   Acc<T> acc;
-  multiply<T, SPLIT, KG>(a, b, stages, smem, acc);
+  multiply<T, KG>(a, b, stages, smem, acc);
   if (t.slot >= 0) {   // (a part of the inner axis: join_kernel goes on)
     if (KG == 1 || threadIdx.x < TPB) {
 #pragma unroll
@@ -600,15 +592,15 @@ __global__ __launch_bounds__(KG * TPB, KG == 1 ? 2 : KG) void sym_kernel(const N
     }
     return;
   }
-  sym_store<T, SPLIT, KG, KIND>(t, s, z, i0, j0, acc, smem);
+  sym_store<T, KG, KIND>(t, s, z, i0, j0, acc, smem);
 }
 
 // The parts of a tile whose inner axis was split, added in order, and stored as sym_store does; 16 workgroups a tile, four rows of one
 // column a thread (one workgroup a tile: 12 us, most of them waiting for one load after the other).
-template <int T, bool SPLIT, SymKind KIND>
+template <int T, SymKind KIND>
 __global__ __launch_bounds__(TPB) void join_kernel(const NsItem* __restrict__ items, SymArgs s,
                                                    const f32x4_t* __restrict__ partial) {
-  constexpr int N = T / 32, W = SPLIT ? 2 : 1;
+  constexpr int N = T / 32;
   const NsItem t = items[blockIdx.x / (N * N)];
   const int frag = blockIdx.x % (N * N), z = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const f32x4_t* from = partial + (((long long)z * s.slots + t.slot) * N * N + frag) * TPB + threadIdx.x;
@@ -623,7 +615,7 @@ __global__ __launch_bounds__(TPB) void join_kernel(const NsItem* __restrict__ it
   const int r = t.ti * T + (wave >> 1) * (T / 2) + (frag / N) * 16 + (lane >> 4) * 4;   // four rows of one column
   const int c = t.tj * T + (wave & 1) * (T / 2) + (frag % N) * 16 + (lane & 15);
   if (r >= t.lda) return;
-  _Float16* out = s.out[z] + W * t.a;
+  _Float16* out = s.out[z] + 2 * t.a;
   float v[4] = {sum[0], sum[1], sum[2], sum[3]};
   if constexpr (KIND == GRAM) {
     const float f = t.gscale / (t.scale * t.scale);
@@ -633,22 +625,22 @@ __global__ __launch_bounds__(TPB) void join_kernel(const NsItem* __restrict__ it
   if constexpr (KIND == POLY) {
     const float cb = s.b / t.gscale, cc = s.c / (t.gscale * t.gscale);
     float g[4] = {0.f, 0.f, 0.f, 0.f};
-    if (c < t.m) get<SPLIT>(s.p[0] + W * t.a, t.lda, c, r, g);
+    if (c < t.m) get(s.p[0] + 2 * t.a, t.lda, c, r, g);
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = cc * v[e] + cb * g[e] + (r + e == c ? s.a : 0.f);
   }
 #pragma unroll
   for (int e = 0; e < 4; ++e)
     if (r + e >= t.m || c >= t.m) v[e] = 0.f;
-  if (c < t.m) put<SPLIT>(out, t.lda, c, r, v);
+  if (c < t.m) put(out, t.lda, c, r, v);
   if (t.ti == t.tj) return;   // (a diagonal tile holds both halves)
 #pragma unroll
   for (int e = 0; e < 4; ++e)
     if (r + e < t.m && c < t.lda) {
-      _Float16* p = out + at<SPLIT>(t.lda, r + e, c);
+      _Float16* p = out + at(t.lda, r + e, c);
       const Pair q = pair_of(v[e]);
       p[0] = q.high;
-      if constexpr (SPLIT) p[32] = q.low;
+      p[32] = q.low;
     }
 }
 
@@ -669,7 +661,7 @@ __device__ __forceinline__ float result_factor(const NsMatrix& M, const Result& 
 }
 
 // X' = Q X: Q's rows by X's columns. LAST: the result leaves the work area (and its scale S), transposed back where needed.
-template <int T, bool SPLIT, int KG, bool LAST>
+template <int T, int KG, bool LAST>
 __global__ __launch_bounds__(KG * TPB, KG == 1 ? 2 : KG) void update_kernel(const NsMatrix* __restrict__ mats, const NsItem* __restrict__ items,
                                                         const _Float16* __restrict__ Q, const _Float16* __restrict__ X,
                                                         _Float16* __restrict__ Y, Result res) {
@@ -677,17 +669,16 @@ __global__ __launch_bounds__(KG * TPB, KG == 1 ? 2 : KG) void update_kernel(cons
   const NsItem t = items[blockIdx.x];
   if (t.matrix < 0) return;
   const int i0 = t.ti * T, j0 = t.tj * T;
-  constexpr int W = SPLIT ? 2 : 1;
   RowsOperand<T> a;
-  ColsOperand<T, SPLIT> b;
-  const int stages = W * t.kn, first = first_stage<KG>(stages);
-  a.init(Q + W * t.a, W * t.lda, i0, t.m, first);
-  b.init(X + W * t.x, W * t.ldx, j0, t.m, first);
+  ColsOperand<T> b;
+  const int stages = 2 * t.kn, first = first_stage<KG>(stages);
+  a.init(Q + 2 * t.a, 2 * t.lda, i0, t.m, first);
+  b.init(X + 2 * t.x, 2 * t.ldx, j0, t.m, first);
   Acc<T> acc;
-  multiply<T, SPLIT, KG>(a, b, stages, smem, acc);
+  multiply<T, KG>(a, b, stages, smem, acc);
   if constexpr (!LAST) {
     store_tile<T, KG, false>(acc, smem, [&](int r, int c, float (&v)[8]) {
-      if (i0 + r < t.m) put<SPLIT>(Y + W * t.x, t.ldx, i0 + r, j0 + c, v);   // (columns n ... ldx: zero, as X's are)
+      if (i0 + r < t.m) put(Y + 2 * t.x, t.ldx, i0 + r, j0 + c, v);   // (columns n ... ldx: zero, as X's are)
     });
   } else {
     const NsMatrix M = mats[t.matrix];
@@ -744,9 +735,6 @@ __global__ __launch_bounds__(KG * TPB, KG == 1 ? 2 : KG) void update_kernel(cons
 }
 
 // ------------------------------------------------------------------ small and thin matrices
-// Matrices with m <= 64 take the pairs of f16 of f32 results whatever the result's type: their products are a microsecond, and few rows
-// do not average the roundings of plain f16 (2 x 2000: 3.5e-3).
-//
 // small_kernel: the whole of a matrix in one workgroup, everything between the caller's reads and writes in LDS, where it fits (64 x 256,
 // 16 x 1856). A launch for every product would cost 4 us each; 64 x 64: 67 us as 17 launches.
 // thin_kernel / chain_kernel: longer ones, by slices of their columns. X X^T is summed over the slices' parts by chain_kernel, which takes
@@ -873,7 +861,7 @@ __device__ __forceinline__ void store_gram(const Share& w, f32x4_t acc, f32x4_t*
     });
   __syncthreads();
 }
-// Steps k ... end - 1 on the m x m matrices (the same products as iterate<true>), G in A[0]; -> Q
+// Steps k ... end - 1 on the m x m matrices (the same products as iterate), G in A[0]; -> Q
 // The factors' order matters to rounding errors alone. Between the null space of X X^T, where Z is near 3.4, and the rest, where it is near 1, those
 // of Z G Z and of Z Q (Q's columns in the rest) grow by the product of both a step, those of Z Z G or Q Z by the larger one squared
 // (64 x 64 of rank one: 4e-4 off instead of 2e-5). The tiles' form has no order: it computes one half and mirrors it.
@@ -1104,16 +1092,16 @@ __global__ __launch_bounds__(TPB) void thin_kernel(const NsMatrix* __restrict__ 
       const int r = i >> 4, c = (i & 15) * 8;
       float v[8] = {};
       uint4 h = make_uint4(0, 0, 0, 0), l = h;
-      _Float16* p = X + 2 * M.x + at<true>(M.ldx, r, piece * THIN_COLS + c);
+      _Float16* p = X + 2 * M.x + at(M.ldx, r, piece * THIN_COLS + c);
       if (r < M.m) {
         if constexpr (KIND == FIRST) {
           // (m <= 64: one row of blocks along the columns of X, whichever way the source lies)
           const int blk = piece * 2 + (c >> 6);
           const float f = (float)ldexp(scale, norm_part[M.chunk0 + blk].e);
-          get<true>(X + 2 * M.x, M.ldx, r, piece * THIN_COLS + c, v);
+          get(X + 2 * M.x, M.ldx, r, piece * THIN_COLS + c, v);
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[e] *= f;
-          put<true>(X + 2 * M.x, M.ldx, r, piece * THIN_COLS + c, v);
+          put(X + 2 * M.x, M.ldx, r, piece * THIN_COLS + c, v);
         } else {
           h = *reinterpret_cast<const uint4*>(p);
           l = *reinterpret_cast<const uint4*>(p + 32);
@@ -1258,20 +1246,19 @@ inline long long up256(long long v) { return (v + 255) / 256 * 256; }
 
 struct Work {
   _Float16 *x[2], *a[N_AREAS];
-  _Float16 *xt, *qt;         // thin matrices: X, Q (pairs)
+  _Float16 *xt, *qt;         // thin matrices: X, Q
   f32x4_t* thin_part;        // parts of X X^T
   Partial* part;
   f32x4_t* slots;            // partial tiles
   long long bytes;
 };
-Work carve(const DasNsPlan* p, bool split, void* ws) {
-  const long long xb = up256((split ? 4 : 2) * p->x_elems), ab = up256((split ? 4 : 2) * p->a_elems);
-  const int areas = split ? N_AREAS : 2;
+Work carve(const DasNsPlan* p, void* ws) {
+  const long long xb = up256(4 * p->x_elems), ab = up256(4 * p->a_elems);
   char* c = (char*)ws;
   Work w = {};
   auto take = [&](long long n) { char* r = c; if (c) c += n; w.bytes += n; return r; };
   for (int i = 0; i < 2; ++i) w.x[i] = (_Float16*)take(xb);
-  for (int i = 0; i < areas; ++i) w.a[i] = (_Float16*)take(ab);
+  for (int i = 0; i < N_AREAS; ++i) w.a[i] = (_Float16*)take(ab);
   w.xt = (_Float16*)take(up256(4 * p->thin_x_elems));
   w.qt = (_Float16*)take(up256(4 * p->thin_a_elems));
   w.thin_part = (f32x4_t*)take(1024 * p->thin_slots);
@@ -1309,7 +1296,7 @@ struct Bounds {              // of step k over the singular values that can reac
   double top;                // |X| before the step
   double factor;             // max |a + b s^2 + c s^4|
 };
-// What f16 and the phases of f32 results have to hold: X's norm, Z's norm step by step. false: outside f16's range.
+// What f16 and the phases have to hold: X's norm, Z's norm step by step. false: outside f16's range.
 bool polynomial_bounds(const float* coef, int steps, Bounds* out) {
   double top = 1.0;
   for (int k = 0; k < steps; ++k) {
@@ -1328,7 +1315,7 @@ bool polynomial_bounds(const float* coef, int steps, Bounds* out) {
   return true;
 }
 
-// where the phase that starts at step k ends (f32 results)
+// where the phase that starts at step k ends
 int phase_end(const Bounds* bound, int steps, int k) {
   double growth = bound[k].factor * bound[k].factor;
   int end = k + 1;
@@ -1481,7 +1468,6 @@ int launch_thin(const DasNsPlan* p, const char* tab, const Work& w, const Result
   return DAS_OK;
 }
 
-template <bool SPLIT>
 int iterate(const DasNsPlan* p, const char* tab, Work w, const Result& res, hipStream_t s) {
   const NsMatrix* mats = (const NsMatrix*)(tab + p->mat_at);
   const int4* chunks = (const int4*)(tab + p->chunk_at);
@@ -1495,22 +1481,22 @@ int iterate(const DasNsPlan* p, const char* tab, Work w, const Result& res, hipS
   };
   auto gram_of = [&](const _Float16* x, _Float16* g) {
     const SymArgs a = {{x}, {x}, {g}, 0.f, 0.f, 0.f, p->gram_slots};
-    if (p->gram_kg == 4) launch_sym(sym_kernel<64, SPLIT, 4, GRAM>, 64, 4, gram, p->n_gram, 1, a);
-    else if (p->gram_kg == 2) launch_sym(sym_kernel<128, SPLIT, 2, GRAM>, 128, 2, gram, p->n_gram, 1, a);
-    else launch_sym(sym_kernel<128, SPLIT, 1, GRAM>, 128, 1, gram, p->n_gram, 1, a);
+    if (p->gram_kg == 4) launch_sym(sym_kernel<64, 4, GRAM>, 64, 4, gram, p->n_gram, 1, a);
+    else if (p->gram_kg == 2) launch_sym(sym_kernel<128, 2, GRAM>, 128, 2, gram, p->n_gram, 1, a);
+    else launch_sym(sym_kernel<128, 1, GRAM>, 128, 1, gram, p->n_gram, 1, a);
     if (p->n_gram_join && p->gram_kg == 4)
-      hipLaunchKernelGGL((join_kernel<64, SPLIT, GRAM>), dim3(p->n_gram_join * 4), dim3(TPB), 0, s, gram_join, a, w.slots);
+      hipLaunchKernelGGL((join_kernel<64, GRAM>), dim3(p->n_gram_join * 4), dim3(TPB), 0, s, gram_join, a, w.slots);
     else if (p->n_gram_join)
-      hipLaunchKernelGGL((join_kernel<128, SPLIT, GRAM>), dim3(p->n_gram_join * 16), dim3(TPB), 0, s, gram_join, a, w.slots);
+      hipLaunchKernelGGL((join_kernel<128, GRAM>), dim3(p->n_gram_join * 16), dim3(TPB), 0, s, gram_join, a, w.slots);
   };
   auto sym = [&](auto kind, int products, SymArgs a) {
     constexpr SymKind K = decltype(kind)::value;
     a.slots = p->product_slots;
-    if (p->product_tile == 128 && p->product_kg == 2) launch_sym(sym_kernel<128, SPLIT, 2, K>, 128, 2, prod, p->n_product, products, a);
-    else if (p->product_tile == 128) launch_sym(sym_kernel<128, SPLIT, 1, K>, 128, 1, prod, p->n_product, products, a);
-    else launch_sym(sym_kernel<64, SPLIT, 4, K>, 64, 4, prod, p->n_product, products, a);
+    if (p->product_tile == 128 && p->product_kg == 2) launch_sym(sym_kernel<128, 2, K>, 128, 2, prod, p->n_product, products, a);
+    else if (p->product_tile == 128) launch_sym(sym_kernel<128, 1, K>, 128, 1, prod, p->n_product, products, a);
+    else launch_sym(sym_kernel<64, 4, K>, 64, 4, prod, p->n_product, products, a);
     if (p->n_product_join)
-      hipLaunchKernelGGL((join_kernel<128, SPLIT, K>), dim3(p->n_product_join * 16, products), dim3(TPB), 0, s, prod_join, a, w.slots);
+      hipLaunchKernelGGL((join_kernel<128, K>), dim3(p->n_product_join * 16, products), dim3(TPB), 0, s, prod_join, a, w.slots);
   };
   auto update = [&](auto last, const _Float16* q, const _Float16* x, _Float16* y) {
     constexpr bool L = decltype(last)::value;
@@ -1519,20 +1505,20 @@ int iterate(const DasNsPlan* p, const char* tab, Work w, const Result& res, hipS
       allow_lds((const void*)kernel);
       hipLaunchKernelGGL(kernel, dim3(p->n_update), dim3(kg * TPB), lds, s, mats, upd, q, x, y, res);
     };
-    if (p->update_tile == 128 && p->update_kg == 2) launch(update_kernel<128, SPLIT, 2, L>, 128, 2);
-    else if (p->update_tile == 128) launch(update_kernel<128, SPLIT, 1, L>, 128, 1);
-    else launch(update_kernel<64, SPLIT, 4, L>, 64, 4);
+    if (p->update_tile == 128 && p->update_kg == 2) launch(update_kernel<128, 2, L>, 128, 2);
+    else if (p->update_tile == 128) launch(update_kernel<128, 1, L>, 128, 1);
+    else launch(update_kernel<64, 4, L>, 64, 4);
   };
   const std::integral_constant<SymKind, POLY> poly_k;
   const std::integral_constant<SymKind, PRODUCT> product_k;
-  hipLaunchKernelGGL(normalise_kernel<SPLIT>, dim3(p->n_tile_chunks), dim3(TPB), 0, s, mats, chunks, p->eps, w.x[0], w.part);
+  hipLaunchKernelGGL(normalise_kernel, dim3(p->n_tile_chunks), dim3(TPB), 0, s, mats, chunks, p->eps, w.x[0], w.part);
   DAS_CHECK_LAUNCH();
-  _Float16 *X = w.x[0], *Y = w.x[1], *G = w.a[0], *R = w.a[1], *Z = w.a[SPLIT ? 2 : 1];
+  _Float16 *X = w.x[0], *Y = w.x[1], *G = w.a[0], *R = w.a[1], *Z = w.a[2];
   for (int k = 0; k < p->steps;) {
     // steps k ... end - 1 are one phase
-    const int end = SPLIT ? p->phase_end[k] : k + 1;
+    const int end = p->phase_end[k];
     gram_of(X, G);
-    _Float16 *q = nullptr, *spare = w.a[SPLIT ? 3 : 1], *other = SPLIT ? w.a[4] : nullptr;   // (q: the phase's product so far)
+    _Float16 *q = nullptr, *spare = w.a[3], *other = w.a[4];   // (q: the phase's product so far)
     for (int j = k; j < end; ++j) {
       const float* c = p->coef + 3 * j;
       _Float16* z = q ? Z : spare;
@@ -1568,10 +1554,10 @@ void launch_ingest(const DasNsPlan* p, const char* tab, const Fork& fork, hipStr
 }
 
 // thin and tiled matrices after ingest_kernel, and the join with the small ones
-template <bool SPLIT, bool MUON>
+template <bool MUON>
 int the_rest(const DasNsPlan* p, const char* tab, const Work& w, const Result& res, hipStream_t s, Fork& fork) {
   int st = launch_thin<MUON>(p, tab, w, res, fork.stream());
-  if (st == DAS_OK && p->n_tile_chunks) st = iterate<SPLIT>(p, tab, w, res, s);
+  if (st == DAS_OK && p->n_tile_chunks) st = iterate(p, tab, w, res, s);
   const int joined = fork.finish();
   return st != DAS_OK ? st : joined;
 }
@@ -1941,9 +1927,9 @@ extern "C" int das_ns_plan(const DasNsShape* shapes, int n, int steps, const flo
   return DAS_OK;
 }
 
-extern "C" long long das_ns_ws_bytes(const DasNsPlan* p, int f32_result) {
+extern "C" long long das_ns_ws_bytes(const DasNsPlan* p) {
   if (!p) return -1;
-  return std::max(256LL, carve(p, f32_result != 0, nullptr).bytes);
+  return std::max(256LL, carve(p, nullptr).bytes);
 }
 
 extern "C" int das_orthogonalize(const DasNsPlan* plan, const void* tables_dev, const DasNsSource* srcs, int n_srcs, int in_dtype,
@@ -1956,8 +1942,7 @@ extern "C" int das_orthogonalize(const DasNsPlan* plan, const void* tables_dev, 
     if (!srcs[i].base) return DAS_ERR_ARG;
   hipStream_t s = (hipStream_t)stream;
   const char* tab = (const char*)tables_dev;
-  const bool split = out_dtype == DAS_F32;
-  const Work w = carve(plan, split, ws);
+  const Work w = carve(plan, ws);
   const NsMatrix* mats = (const NsMatrix*)(tab + plan->mat_at);
   const MuonIn none = {};
   const Result res = {out, out_dtype, nullptr, 1.f, 0.f, 0};
@@ -1978,12 +1963,12 @@ extern "C" int das_orthogonalize(const DasNsPlan* plan, const void* tables_dev, 
         hipLaunchKernelGGL(kernel, dim3(n), dim3(TPB), 0, on, mats, chunks, a, none, w.x[0], w.xt, w.part);
       });
     };
-    if (in_dtype == DAS_F32) split ? launch(ingest_kernel<float, false, true>) : launch(ingest_kernel<float, false, false>);
-    else if (in_dtype == DAS_BF16) split ? launch(ingest_kernel<bf16_t, false, true>) : launch(ingest_kernel<bf16_t, false, false>);
-    else split ? launch(ingest_kernel<_Float16, false, true>) : launch(ingest_kernel<_Float16, false, false>);
+    if (in_dtype == DAS_F32) launch(ingest_kernel<float, false>);
+    else if (in_dtype == DAS_BF16) launch(ingest_kernel<bf16_t, false>);
+    else launch(ingest_kernel<_Float16, false>);
     DAS_CHECK_LAUNCH();
   }
-  return split ? the_rest<true, false>(plan, tab, w, res, s, fork) : the_rest<false, false>(plan, tab, w, res, s, fork);
+  return the_rest<false>(plan, tab, w, res, s, fork);
 }
 
 extern "C" int das_muon_step(const DasNsPlan* plan, const void* tables_dev, float* p, const float* g, float* buf, float lr,
@@ -1998,16 +1983,16 @@ extern "C" int das_muon_step(const DasNsPlan* plan, const void* tables_dev, floa
   if (buffers_overlap(p, g, bytes) || buffers_overlap(p, buf, bytes) || buffers_overlap(g, buf, bytes)) return DAS_ERR_ARG;
   hipStream_t s = (hipStream_t)stream;
   const char* tab = (const char*)tables_dev;
-  const Work w = carve(plan, true, ws);
+  const Work w = carve(plan, ws);
   const MuonIn mu = {g, buf, momentum, grad_scale, max_norm, nesterov, grad_sumsq};
   const Result res = {nullptr, 0, p, (float)(1.0 - (double)lr * (double)weight_decay), lr, lr_scale};
   Fork fork(s, worth_a_fork(plan));
   const int st = launch_small<float, true>(plan, tab, Sources{}, mu, res, fork.stream());
   if (st != DAS_OK) return st;
   launch_ingest(plan, tab, fork, s, [&](const int4* chunks, int n, hipStream_t on) {
-    hipLaunchKernelGGL((ingest_kernel<float, true, true>), dim3(n), dim3(TPB), 0, on, (const NsMatrix*)(tab + plan->mat_at), chunks, Sources{}, mu,
+    hipLaunchKernelGGL((ingest_kernel<float, true>), dim3(n), dim3(TPB), 0, on, (const NsMatrix*)(tab + plan->mat_at), chunks, Sources{}, mu,
                        w.x[0], w.xt, w.part);
   });
   DAS_CHECK_LAUNCH();
-  return the_rest<true, true>(plan, tab, w, res, s, fork);
+  return the_rest<true>(plan, tab, w, res, s, fork);
 }

@@ -271,9 +271,9 @@ def orthogonalize(mats, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, out_dty
     """The orthogonal factor of every matrix of a list (or of one tensor) by `steps` Newton-Schulz products: for U = mats[i],
     X = U / (|U| + eps), then X <- (a I + b X X^T + c (X X^T)^2) X. 2-D tensors are one matrix, 3-D ones a stack; f32, bf16 or f16 (one
     type a call), any row / stack stride, unit column stride. Returns tensors of the same shapes.
-    out_dtype sets the precision too: bf16 (default) and f16 results come from products of f16 operands, 1e-3 off exact arithmetic for the
-    gradients of a training run (2-norm) and up to 5e-2 where the singular values span many orders of magnitude; f32 ones from
-    pairs of f16, 2e-4 off at most.
+    out_dtype: bfloat16 (default), float16 or float32; the arithmetic is the same and the result rounded once. With the default steps and
+    polynomial it is 2e-6 ... 5e-6 off exact arithmetic (2-norm) for gradients of full rank and up to 3e-4 for rank one, before that rounding; more or
+    steeper steps cost the product of the polynomial's slopes.
     plan: a NewtonSchulzPlan of these shapes (built here if None, which copies its tables to the device: keep one where the call
     repeats; inside a hipGraph capture it is required). Inf or NaN in a matrix makes that matrix NaN, no other. No gradient is recorded."""
     one = torch.is_tensor(mats)
@@ -304,7 +304,7 @@ def orthogonalize(mats, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, out_dty
             s.base, s.row_stride, s.batch_stride = t.data_ptr(), t.stride(-2), t.stride(0) if t.dim() == 3 else 0
         with _on(dev):
             lib = _lib.load()
-            ws = torch.empty(lib.das_ns_ws_bytes(C.byref(p), int(out_dtype == torch.float32)), dtype=torch.uint8, device=dev)
+            ws = torch.empty(lib.das_ns_ws_bytes(C.byref(p)), dtype=torch.uint8, device=dev)
             plan._used(tables)
             _lib.check(lib.das_orthogonalize(C.byref(p), _ptr(tables), src, len(live), dt, _ptr(out), _NS_DT[out_dtype], _ptr(ws),
                                              _stream_of(dev)), 'das_orthogonalize')
@@ -331,7 +331,7 @@ def muon_step(p, g, buf, plan, lr, momentum=0.95, weight_decay=0.0, nesterov=Tru
         raise _lib.DasHipError(f'muon_step: the plan reaches element {c_plan.extent} of buffers of {p.numel()}')
     with _on(p.device):
         lib = _lib.load()
-        ws = torch.empty(lib.das_ns_ws_bytes(C.byref(c_plan), 1), dtype=torch.uint8, device=p.device)
+        ws = torch.empty(lib.das_ns_ws_bytes(C.byref(c_plan)), dtype=torch.uint8, device=p.device)
         plan._used(tables)
         _lib.check(lib.das_muon_step(C.byref(c_plan), _ptr(tables), _ptr(p), _ptr(g), _ptr(buf), float(lr), float(momentum),
                                      float(weight_decay), int(bool(nesterov)), int(lr_scale != 'original'), float(grad_scale),

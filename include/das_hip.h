@@ -611,9 +611,9 @@ int das_sgd_momentum_step(float* p, const float* g, float* buf, long long n, flo
  * Newton-Schulz orthogonalisation of a ragged set of matrices. For each matrix U (rows x cols, m = min, n = max of the two,
  * transposed if rows > cols so that X is m x n):
  *   X = U / (|U|_F + eps);   steps times:  A = X X^T,  B = a I + b A + c A^2,  X = B X.
- * The precision follows the result's type. f16 / bf16 results of matrices with m > 64: products of f16 operands summed in f32, X, A and B rounded to f16 in between
- * (1e-3 off a 64-bit evaluation, in the 2-norm, for the gradients of a training run, up to 5e-2 for matrices whose singular values span
- * many orders of magnitude). f32 results, parameters and m <= 64: operands are pairs of f16 (22 bits), 2e-4 off at most. Sums of squares are
+ * Operands are pairs of f16 (22 bits) and sums f32, whatever the result's type; a result is rounded once. Five steps of the default polynomial are
+ * off a 64-bit evaluation, in the 2-norm, by 2e-6 ... 5e-6 for gradients of full rank and up to 3e-4 for rank one (4096 x 4096), where rounding
+ * errors outside U's row and column space grow by |a| a step; more or steeper steps cost the product of the polynomial's slopes. Sums of squares are
  * held in f32 by 64 x 64 blocks and added in f64. Results are the same bits from run to run.
  *
  * A plan lists the set once: das_ns_plan() checks the shapes and the polynomial and writes the tables (host memory) that the
@@ -631,7 +631,7 @@ typedef struct {
   long long x_elems, a_elems, thin_x_elems, thin_a_elems, thin_slots, gram_slots, product_slots, extent;            /* work areas (f16 elements); one past the last element of the flat buffers used */
   long long mat_at, chunk_at, gram_at, gram_join_at, product_at, product_join_at, update_at, slice_at, thin_at, table_bytes;   /* byte offsets of the tables */
   float coef[3 * DAS_NS_MAX_STEPS];              /* a, b, c of each step */
-  int phase_end[DAS_NS_MAX_STEPS];               /* f32 results: where a run of steps on the m x m matrices that starts here ends */
+  int phase_end[DAS_NS_MAX_STEPS];               /* where a run of steps on the m x m matrices that starts here ends */
   float eps;
 } DasNsPlan;
 /* One source tensor of das_orthogonalize: `count` matrices, element (i, r, c) at base[i * batch_stride + r * row_stride + c]. */
@@ -644,8 +644,8 @@ typedef struct {
  * [-16, 16] within `steps` steps or has |a + b s^2 + c s^4| > 64 there (f16 could overflow), eps < 0, or tables too small. */
 int das_ns_plan(const DasNsShape* shapes, int n, int steps, const float* coef, float eps, DasNsPlan* plan, void* tables,
                 long long table_bytes);
-/* f32_result: for das_muon_step, and for das_orthogonalize with out_dtype DAS_F32. */
-long long das_ns_ws_bytes(const DasNsPlan* plan, int f32_result);
+/* Workspace of a das_orthogonalize or das_muon_step call */
+long long das_ns_ws_bytes(const DasNsPlan* plan);
 /* out (flat, out_dtype DAS_F32 / DAS_BF16 / DAS_F16, plan offsets): the orthogonalised matrices; srcs: one per group of the plan, in_dtype
  * DAS_F32 / DAS_BF16 / DAS_F16. `ws`: das_ns_ws_bytes() of device memory, 16-byte aligned, in use until the call's kernels end. `out`, the
  * sources and ws do not overlap. Small and thin matrices of a set that holds many or large others run on a stream of the library's own (default priority,

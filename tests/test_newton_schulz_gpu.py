@@ -116,3 +116,22 @@ def test_f32_result_of_any_rank(shape, rank):
     from das_amd import train_ops as T
     u = low_rank(*shape, rank, seed=sum(shape) + rank)
     assert off(T.orthogonalize(u, out_dtype=torch.float32), u) <= pairs_bound(min(shape), rank)
+
+
+@pytest.mark.parametrize('out_dtype', [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('rank', [1, 4, 16, 128, 0])
+@pytest.mark.parametrize('shape', [(60, 64), (30, 3000), (256, 2304), (1030, 900), (2048, 2048)], ids=lambda s: '%dx%d' % s)
+def test_16_bit_result_is_the_f32_one_rounded(shape, rank, dtype, out_dtype):
+    """... so that it is off by its rounding alone: half a step, uniform in that, 3^-1/2 of it on the average; f16's subnormal numbers are half of
+    2^-24 apart, whatever the element"""
+    from das_amd import train_ops as T
+    u = low_rank(*shape, rank, seed=sum(shape) + rank)
+    u = (u / u.abs().max()).to(dtype)
+    got, f32 = T.orthogonalize(u, out_dtype=out_dtype), T.orthogonalize(u, out_dtype=torch.float32)
+    ref = polar64(u)
+    half = torch.finfo(out_dtype).eps / 2
+    tiny = 2.0 ** -25 * (shape[0] * shape[1] / 3) ** 0.5 / float(ref.norm()) if out_dtype == torch.float16 else 0
+    # (a 16-bit input is of full rank, by its own rounding, and counted as the f32 matrix that it came from)
+    assert off(got, u) <= (pairs_bound(min(shape), rank) ** 2 + half ** 2 / 3 + tiny ** 2) ** 0.5
+    assert torch.equal(got, f32.to(out_dtype))
