@@ -216,11 +216,8 @@ class NewtonSchulzPlan:
             self.device = torch.device('cuda', torch.cuda.current_device())
         if any(len(s) != 3 or min(s) < 0 for s in self.shapes) or not 1 <= int(steps) <= _lib.DAS_NS_MAX_STEPS:
             raise _lib.DasHipError(f'NewtonSchulzPlan: shapes are (rows, cols) or (count, rows, cols), steps 1 ... {_lib.DAS_NS_MAX_STEPS}')
-        co = [float(v) for t in coefficients for v in (t if hasattr(t, '__len__') else (t,))]
-        co = co * int(steps) if len(co) == 3 else co
-        if len(co) != 3 * int(steps):
-            raise _lib.DasHipError('NewtonSchulzPlan: one (a, b, c) triple, or one for every step')
         self.steps, self.eps = int(steps), float(eps)
+        self.coefficients = co = self._per_step(coefficients, self.steps)
         sizes = [k * r * c for k, r, c in self.shapes]
         if offsets is None:
             self.offsets = [sum(sizes[:i]) for i in range(len(sizes))]
@@ -238,6 +235,21 @@ class NewtonSchulzPlan:
                 self._out_size += (n + 7) // 8 * 8
             self._out = self._flat if self._out_offsets == self.offsets else \
                 self._build([(o, s) for o, s, n in zip(self._out_offsets, self.shapes, sizes) if n], co)
+
+    @staticmethod
+    def _per_step(coefficients, steps):
+        co = [float(v) for t in coefficients for v in (t if hasattr(t, '__len__') else (t,))]
+        co = co * steps if len(co) == 3 else co
+        if len(co) != 3 * steps:
+            raise _lib.DasHipError('NewtonSchulzPlan: one (a, b, c) triple, or one for every step')
+        return co
+
+    def _agrees(self, steps, coefficients, eps):
+        """Refuses arguments of a call (None: not given) that are not what this plan was made with."""
+        if not ((steps is None or int(steps) == self.steps) and (eps is None or float(eps) == self.eps) and
+                (coefficients is None or self._per_step(coefficients, self.steps) == self.coefficients)):
+            raise _lib.DasHipError(f'orthogonalize: the plan is for {self.steps} steps, coefficients {self.coefficients}, eps {self.eps}; got '
+                                   f'{steps}, {coefficients}, {eps}')
 
     def _build(self, entries, co):
         """-> (DasNsPlan, device tables), None for no entries"""
@@ -267,8 +279,9 @@ class NewtonSchulzPlan:
             tables.record_stream(torch.cuda.current_stream(self.device))
 
 
-def orthogonalize(mats, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, out_dtype=torch.bfloat16, plan=None):
-    """The orthogonal factor of every matrix of a list (or of one tensor) by `steps` Newton-Schulz products: for U = mats[i],
+def orthogonalize(mats, steps=None, coefficients=None, eps=None, out_dtype=torch.bfloat16, plan=None):
+    """The orthogonal factor of every matrix of a list (or of one tensor) by `steps` Newton-Schulz products (default 5, of NS_COEFFICIENTS, eps
+    1e-7; with a plan, the plan's: other ones beside it are refused): for U = mats[i],
     X = U / (|U| + eps), then X <- (a I + b X X^T + c (X X^T)^2) X. 2-D tensors are one matrix, 3-D ones a stack; f32, bf16 or f16 (one
     type a call), any row / stack stride, unit column stride. Returns tensors of the same shapes.
     out_dtype: bfloat16 (default), float16 or float32; the arithmetic is the same and the result rounded once. With the default steps and
@@ -289,7 +302,10 @@ def orthogonalize(mats, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, out_dty
     shapes = [tuple(t.shape) if t.dim() == 3 else (1,) + tuple(t.shape) for t in mats]
     dev = mats[0].device
     if plan is None:
-        plan = NewtonSchulzPlan(shapes, dev, steps=steps, coefficients=coefficients, eps=eps)
+        given = dict(steps=steps, coefficients=coefficients, eps=eps)
+        plan = NewtonSchulzPlan(shapes, dev, **{k: v for k, v in given.items() if v is not None})
+    else:
+        plan._agrees(steps, coefficients, eps)
     if plan.shapes != shapes or plan.device != dev:
         raise _lib.DasHipError(f'orthogonalize: the plan is for {plan.shapes} on {plan.device}, the tensors are {shapes} on {dev}')
     mats = [t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous() for t in mats]

@@ -31,3 +31,15 @@ def test_plan_tables_are_host_memory_whatever_the_default_device(monkeypatch, sh
         except (RuntimeError, AssertionError):
             pass                    # (no GPU to copy the tables to)
     assert rec.tables and rec.tables[0] and rec.tables[-1]
+
+
+def test_arguments_beside_a_plan_have_to_agree_with_it():
+    """(on a plan without tables: no GPU)"""
+    from das_amd import train_ops as T
+    from das_amd._lib import DasHipError
+    plan = T.NewtonSchulzPlan([(0, 5)], 'cuda:0', steps=4, eps=1e-6)
+    for kw in (dict(steps=5), dict(eps=1e-7), dict(coefficients=(1.5, -0.5, 0.0)), dict(coefficients=[T.NS_COEFFICIENTS] * 5)):
+        with pytest.raises(DasHipError):
+            plan._agrees(**{**dict(steps=None, coefficients=None, eps=None), **kw})
+    plan._agrees(None, None, None)
+    plan._agrees(4, [T.NS_COEFFICIENTS] * 4, 1e-6)

@@ -135,3 +135,18 @@ def test_16_bit_result_is_the_f32_one_rounded(shape, rank, dtype, out_dtype):
     # (a 16-bit input is of full rank, by its own rounding, and counted as the f32 matrix that it came from)
     assert off(got, u) <= (pairs_bound(min(shape), rank) ** 2 + half ** 2 / 3 + tiny ** 2) ** 0.5
     assert torch.equal(got, f32.to(out_dtype))
+
+
+def test_arguments_beside_a_plan():
+    """a plan has its steps, polynomial and eps: other ones are refused, the same ones are not"""
+    from das_amd import train_ops as T
+    from das_amd._lib import DasHipError
+    u = torch.randn(70, 90, generator=torch.Generator().manual_seed(0)).to(DEV)
+    plan = T.NewtonSchulzPlan([(70, 90)], DEV)
+    want = T.orthogonalize([u], plan=plan)[0]
+    for kw in (dict(steps=3), dict(coefficients=(1.5, -0.5, 0.0)), dict(coefficients=[COEF] * 4), dict(eps=1e-3), dict(steps=5, eps=0.0)):
+        with pytest.raises(DasHipError):
+            T.orthogonalize([u], plan=plan, **kw)
+    for kw in (dict(steps=5), dict(coefficients=COEF), dict(coefficients=[COEF] * 5, eps=1e-7), dict(steps=None)):
+        assert torch.equal(T.orthogonalize([u], plan=plan, **kw)[0], want)
+    assert torch.equal(T.orthogonalize([u])[0], want) and torch.equal(T.orthogonalize([u], steps=5, coefficients=COEF, eps=1e-7)[0], want)
