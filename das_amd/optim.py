@@ -506,6 +506,9 @@ class FlatSGD:
                 st = sd['state'].get(i, sd['state'].get(str(i)))
                 if st is not None and st.get('momentum_buffer') is not None:
                     mom[n] = st['momentum_buffer']
+            by = _written_by(sd)
+            if by not in (None, 'SGD'):
+                raise ValueError(f'optimizer state written by {by}: its moments are no SGD momentum')
             steps = int(sd.get('das_steps', 1 if mom else 0))
         for n, p, sl in zip(self._names, self._params, self.slots):
             dst = self.flat_m[sl.off:sl.off + sl.numel]
@@ -524,6 +527,20 @@ class FlatSGD:
 
     def grad_norm(self):
         return float(torch.sqrt(T.grad_sumsq(self.flat_g)).item()) / self.world
+
+
+def _written_by(sd):
+    """Which optimizer an optimizer state dict with state in it comes from ('SGD', 'AdamW', 'Muon'; None: cannot be told): what its entries hold, then
+    what its groups say (torch's SGD and this module's write dampening, FlatMuon's matrices momentum without it)"""
+    entries, groups = [e for e in sd['state'].values() if e], sd['param_groups']
+    if not entries:
+        return None
+    adam = ['exp_avg' in e for e in entries]
+    if all(adam):
+        return 'AdamW'
+    if any(adam) or any('nesterov' in g and 'dampening' not in g for g in groups):
+        return 'Muon'
+    return 'SGD' if any('dampening' in g for g in groups) else None
 
 
 def _state_entries(sd, model):
@@ -604,23 +621,28 @@ class FlatAdamW(FlatSGD):
         steps = {int(e['step']) for e in entries.values() if 'step' in e}
         if len(steps) > 1:
             raise ValueError(f'parameters at different steps ({sorted(steps)}): the flat optimizer keeps one step count')
+        if _written_by(sd) == 'SGD':
+            raise ValueError('optimizer state written by SGD: its momentum is no moment of this optimizer')
         matrix = next((g for g in self.groups if g['key'] == 'matrix'), None)
+        loads = []                      # (nothing is overwritten before the whole of it is known to fit)
         for n, p, sl in zip(self._names, self._params, self.slots):
             e = entries[n]
             is_matrix = matrix is not None and matrix['start'] <= sl.off < matrix['end']
             for flat, key in ((self.flat_m, 'momentum_buffer' if is_matrix else 'exp_avg'), (self.flat_v, None if is_matrix else 'exp_avg_sq')):
                 if key is None:
                     continue
-                if e and key not in e:
-                    raise ValueError(f'optimizer state of {n} has no {key}: written by another optimizer')
-                dst = flat[sl.off:sl.off + sl.numel]
-                if not e:              # (torch creates state at a parameter's first gradient: never stepped = none)
-                    dst.zero_()
-                elif sl.cl_shape is not None:
-                    O, KH, KW, I = sl.cl_shape
-                    dst.view(O, KH, KW, I).copy_(e[key].to(dst.device, torch.float32).permute(0, 2, 3, 1))
-                else:
-                    dst.copy_(e[key].to(dst.device, torch.float32).reshape(-1))
+                if e and (key not in e or e[key].shape != p.shape):
+                    raise ValueError(f'optimizer state of {n} has no {key} of shape {tuple(p.shape)}: written by another optimizer or for another model')
+                loads.append((sl, flat, e.get(key)))
+        for sl, flat, t in loads:
+            dst = flat[sl.off:sl.off + sl.numel]
+            if t is None:               # (torch creates state at a parameter's first gradient: never stepped = none)
+                dst.zero_()
+            elif sl.cl_shape is not None:
+                O, KH, KW, I = sl.cl_shape
+                dst.view(O, KH, KW, I).copy_(t.to(dst.device, torch.float32).permute(0, 2, 3, 1))
+            else:
+                dst.copy_(t.to(dst.device, torch.float32).reshape(-1))
         self.steps = int(sd.get('das_steps', max(steps) if steps else 0))
 
 

@@ -43,3 +43,79 @@ def test_arguments_beside_a_plan_have_to_agree_with_it():
             plan._agrees(**{**dict(steps=None, coefficients=None, eps=None), **kw})
     plan._agrees(None, None, None)
     plan._agrees(4, [T.NS_COEFFICIENTS] * 4, 1e-6)
+
+
+def nets():
+    """with matrices and the rest, and with matrices alone"""
+    import torch.nn as nn
+    torch.manual_seed(0)
+    yield lambda: nn.Sequential(nn.Conv2d(8, 16, 3), nn.BatchNorm2d(16), nn.Linear(64, 24))
+    yield lambda: nn.Sequential(nn.Linear(64, 24, bias=False), nn.Linear(24, 64, bias=False))
+
+
+def filled(opt, steps):
+    with torch.no_grad():
+        for sl in opt.slots:
+            opt.flat_m[sl.off:sl.off + sl.numel].normal_()
+            if hasattr(opt, 'flat_v') and sl.off < opt.flat_v.numel():
+                opt.flat_v[sl.off:sl.off + sl.numel].uniform_()
+    opt.steps = steps
+    return opt
+
+
+@pytest.mark.parametrize('which', [0, 1])
+@pytest.mark.parametrize('src', ['SGD', 'AdamW', 'Muon'])
+@pytest.mark.parametrize('dst', ['SGD', 'AdamW', 'Muon'])
+def test_state_of_another_optimizer_is_refused_whole(src, dst, which):
+    """no moment of one kind becomes a momentum of another, and a refused file leaves every buffer as it was"""
+    from das_amd.optim import build_optimizer
+    net = list(nets())[which]
+    sd = filled(build_optimizer(net(), dict(type=src, lr=1e-2)), 3).state_dict()
+    opt = filled(build_optimizer(net(), dict(type=dst, lr=1e-2)), 5)
+    before = [opt.flat_m.clone()] + ([opt.flat_v.clone()] if hasattr(opt, 'flat_v') else [])
+    if src == dst:
+        opt.load_state_dict(sd)
+        assert opt.steps == 3 and not torch.equal(opt.flat_m, before[0])
+        return
+    with pytest.raises(ValueError):
+        opt.load_state_dict(sd)
+    assert opt.steps == 5 and torch.equal(opt.flat_m, before[0]) and (len(before) == 1 or torch.equal(opt.flat_v, before[1]))
+
+
+def test_state_that_does_not_fit_is_refused_whole():
+    from das_amd.optim import build_optimizer
+    for kind in ('AdamW', 'Muon'):
+        net = list(nets())[0]
+        sd = filled(build_optimizer(net(), dict(type=kind, lr=1e-2)), 3).state_dict()
+        opt = filled(build_optimizer(net(), dict(type=kind, lr=1e-2)), 5)
+        m, v = opt.flat_m.clone(), opt.flat_v.clone()
+        last = len(sd['param_groups']) - 1
+        for bad in ({k: t[..., :-1] if k != 'step' else t for k, t in sd['state'][last].items()}, {'step': torch.tensor(3.0)}):
+            with pytest.raises(ValueError):
+                opt.load_state_dict(dict(sd, state={**sd['state'], last: bad}))
+            assert torch.equal(opt.flat_m, m) and torch.equal(opt.flat_v, v) and opt.steps == 5
+
+
+def test_state_of_torchs_optimizers():
+    """torch.optim.SGD's state goes into SGD, torch.optim.AdamW's into AdamW, each with one group for all parameters; a file without state anywhere"""
+    from das_amd.optim import build_optimizer
+    for net in nets():
+        for make, kind in ((lambda p: torch.optim.SGD(p, lr=0.1, momentum=0.9), 'SGD'), (lambda p: torch.optim.AdamW(p, lr=0.1), 'AdamW')):
+            m = net()
+            topt = make(m.parameters())
+            fresh = topt.state_dict()
+            for p in m.parameters():
+                p.grad = torch.randn_like(p)
+            topt.step()
+            for other in ('SGD', 'AdamW', 'Muon'):
+                opt = build_optimizer(net(), dict(type=other, lr=1e-2))
+                opt.load_state_dict(fresh)
+                assert opt.steps == 0 and not opt.flat_m.any()
+                if other == kind:
+                    opt.load_state_dict(topt.state_dict())
+                    dense = opt._dense_momentum()
+                    for n, p in m.named_parameters():
+                        assert torch.equal(dense[n], topt.state[p]['momentum_buffer' if kind == 'SGD' else 'exp_avg'])
+                else:
+                    with pytest.raises(ValueError):
+                        opt.load_state_dict(topt.state_dict())
