@@ -214,8 +214,9 @@ class NewtonSchulzPlan:
             raise _lib.DasHipError('das_amd ops run on the GPU only (no CPU fallback); got device ' + str(device))
         if self.device.index is None:
             self.device = torch.device('cuda', torch.cuda.current_device())
-        if any(len(s) != 3 or min(s) < 0 for s in self.shapes) or not 1 <= int(steps) <= _lib.DAS_NS_MAX_STEPS:
-            raise _lib.DasHipError(f'NewtonSchulzPlan: shapes are (rows, cols) or (count, rows, cols), steps 1 ... {_lib.DAS_NS_MAX_STEPS}')
+        # (2^31 - 1: the library's integers, which ctypes fills with the low bits of anything larger)
+        if any(len(s) != 3 or min(s) < 0 or max(s) > (1 << 31) - 1 for s in self.shapes) or not 1 <= int(steps) <= _lib.DAS_NS_MAX_STEPS:
+            raise _lib.DasHipError(f'NewtonSchulzPlan: shapes are (rows, cols) or (count, rows, cols) below 2^31, steps 1 ... {_lib.DAS_NS_MAX_STEPS}')
         self.steps, self.eps = int(steps), float(eps)
         self.coefficients = co = self._per_step(coefficients, self.steps)
         sizes = [k * r * c for k, r, c in self.shapes]
@@ -223,8 +224,8 @@ class NewtonSchulzPlan:
             self.offsets = [sum(sizes[:i]) for i in range(len(sizes))]
         else:
             self.offsets = [int(o) for o in offsets]
-            if len(self.offsets) != len(sizes):
-                raise _lib.DasHipError('NewtonSchulzPlan: one offset for every entry of shapes')
+            if len(self.offsets) != len(sizes) or any(abs(o) > 1 << 60 for o in self.offsets):
+                raise _lib.DasHipError('NewtonSchulzPlan: one offset for every entry of shapes, 2^60 at most')
         live = [(o, s) for o, s, n in zip(self.offsets, self.shapes, sizes) if n]
         self._flat = self._build(live, co)
         # orthogonalize()'s results: one flat output, every entry on a 16-byte boundary of it
@@ -263,7 +264,8 @@ class NewtonSchulzPlan:
         cf = (C.c_float * len(co))(*co)
         # (room for the tables of all but odd sets at the first try: the schedule is worked out once; pages not written cost nothing.
         # The library writes them from the host: host memory whatever torch's default device is)
-        host = torch.empty((1 << 20) + sum(k * r * c for _, (k, r, c) in entries) // 16, dtype=torch.uint8, device='cpu')
+        room = (1 << 20) + sum(k * r * c for _, (k, r, c) in entries) // 16
+        host = torch.empty(min(room, 1 << 28), dtype=torch.uint8, device='cpu')
         if lib.das_ns_plan(arr, len(entries), self.steps, cf, self.eps, C.byref(plan), _ptr(host), host.numel()) != _lib.DAS_OK:
             _lib.check(lib.das_ns_plan(arr, len(entries), self.steps, cf, self.eps, C.byref(plan), None, 0), 'das_ns_plan')
             host = torch.empty(plan.table_bytes, dtype=torch.uint8, device='cpu')

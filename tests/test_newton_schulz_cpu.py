@@ -119,3 +119,13 @@ def test_state_of_torchs_optimizers():
                 else:
                     with pytest.raises(ValueError):
                         opt.load_state_dict(topt.state_dict())
+
+
+def test_sizes_past_the_librarys_integers_are_refused():
+    """a count of 2^32 + 1 is not one matrix, and a set too large for a launch is a refusal, not a want of host memory"""
+    from das_amd import train_ops as T
+    from das_amd._lib import DasHipError
+    for shapes, kw in (([((1 << 32) + 1, 1, 1)], {}), ([(1, (1 << 32) + 8, 8)], {}), ([(8, (1 << 32) + 8)], {}), ([(8, 8)], dict(offsets=[1 << 64])),
+                       ([(8, 8)], dict(offsets=[(1 << 64) + 64])), ([(1 << 21, 1 << 14, 1 << 14)], {})):
+        with pytest.raises(DasHipError):
+            T.NewtonSchulzPlan(shapes, 'cuda:0', **kw)
