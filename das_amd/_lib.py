@@ -186,7 +186,7 @@ SIGNATURES = {
     'das_ns_plan': (i32, [C.POINTER(DasNsShape), i32, i32, C.POINTER(f32), f32, C.POINTER(DasNsPlan), vp, i64]),
     'das_ns_ws_bytes': (i64, [C.POINTER(DasNsPlan)]),
     'das_orthogonalize': (i32, [C.POINTER(DasNsPlan), vp, C.POINTER(DasNsSource), i32, i32, vp, i32, vp, vp]),
-    'das_muon_step': (i32, [C.POINTER(DasNsPlan), vp, vp, vp, vp, f32, f32, f32, i32, i32, f32, f32, vp, vp, vp]),
+    'das_muon_step': (i32, [C.POINTER(DasNsPlan), vp, vp, vp, vp, f64, f64, f64, i32, i32, f32, f32, vp, vp, vp]),
     'das_adamw_step': (i32, [vp, vp, vp, vp, i64, f64, f64, f64, f64, f64, i64, f32, f32, vp, vp]),
     'das_decode_cap': (i32, [C.POINTER(DasDecodeDesc)]),
     'das_decode_ws_bytes': (i64, [i32, i32, i32]),

@@ -112,7 +112,8 @@ struct Sources {            // das_orthogonalize's tensors, by value (no pointer
 struct MuonIn {
   const float* g;
   float* buf;
-  float momentum, grad_scale, max_norm;
+  float momentum, rest;     // mu, 1 - mu (each rounded once: 1 - f32(0.98) is 9e-7 off 0.02)
+  float grad_scale, max_norm;
   int nesterov;
   const float* sumsq;
 };
@@ -141,8 +142,8 @@ __device__ __forceinline__ float grad_factor(const MuonIn& mu) {
 // the momentum's new value in b, returns U
 __device__ __forceinline__ float muon_in(const MuonIn& mu, float f, float g, float& b) {
   g *= f;
-  b = mu.momentum * b + (1.f - mu.momentum) * g;
-  return mu.nesterov ? (1.f - mu.momentum) * g + mu.momentum * b : b;
+  b = mu.momentum * b + mu.rest * g;
+  return mu.nesterov ? mu.rest * g + mu.momentum * b : b;
 }
 
 template <typename T>
@@ -1971,12 +1972,12 @@ extern "C" int das_orthogonalize(const DasNsPlan* plan, const void* tables_dev, 
   return the_rest<false>(plan, tab, w, res, s, fork);
 }
 
-extern "C" int das_muon_step(const DasNsPlan* plan, const void* tables_dev, float* p, const float* g, float* buf, float lr,
-                             float momentum, float weight_decay, int nesterov, int lr_scale, float grad_scale, float max_norm,
+extern "C" int das_muon_step(const DasNsPlan* plan, const void* tables_dev, float* p, const float* g, float* buf, double lr,
+                             double momentum, double weight_decay, int nesterov, int lr_scale, float grad_scale, float max_norm,
                              const float* grad_sumsq, void* ws, void* stream) {
   DAS_PROF(stream);
-  if (!plan_valid(plan, tables_dev, ws) || !p || !g || !buf || !(momentum >= 0.f && momentum < 1.f) || !(lr >= 0.f) ||
-      !(weight_decay >= 0.f) || (max_norm > 0.f && !grad_sumsq) || lr_scale < 0 || lr_scale > 1)
+  if (!plan_valid(plan, tables_dev, ws) || !p || !g || !buf || !(momentum >= 0 && momentum < 1) || !(lr >= 0) ||
+      !(weight_decay >= 0) || (max_norm > 0.f && !grad_sumsq) || lr_scale < 0 || lr_scale > 1)
     return DAS_ERR_ARG;
   if (((uintptr_t)p | (uintptr_t)g | (uintptr_t)buf) & 3) return DAS_ERR_ARG;
   const long long bytes = 4 * plan->extent;
@@ -1984,8 +1985,8 @@ extern "C" int das_muon_step(const DasNsPlan* plan, const void* tables_dev, floa
   hipStream_t s = (hipStream_t)stream;
   const char* tab = (const char*)tables_dev;
   const Work w = carve(plan, ws);
-  const MuonIn mu = {g, buf, momentum, grad_scale, max_norm, nesterov, grad_sumsq};
-  const Result res = {nullptr, 0, p, (float)(1.0 - (double)lr * (double)weight_decay), lr, lr_scale};
+  const MuonIn mu = {g, buf, (float)momentum, (float)(1.0 - momentum), grad_scale, max_norm, nesterov, grad_sumsq};
+  const Result res = {nullptr, 0, p, (float)(1.0 - lr * weight_decay), (float)lr, lr_scale};
   Fork fork(s, worth_a_fork(plan));
   const int st = launch_small<float, true>(plan, tab, Sources{}, mu, res, fork.stream());
   if (st != DAS_OK) return st;

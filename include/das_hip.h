@@ -657,8 +657,8 @@ int das_orthogonalize(const DasNsPlan* plan, const void* tables_dev, const DasNs
  *   p = p * (1 - lr * weight_decay) - lr * f * orthogonalised(U),   f = sqrt(max(1, rows / cols)) (lr_scale 0) or
  *   0.2 * sqrt(max(rows, cols)) (lr_scale 1). Elements of p, g, buf outside the plan's matrices are not touched.
  * The three buffers (plan->extent elements each) do not overlap: DAS_ERR_ARG otherwise. */
-int das_muon_step(const DasNsPlan* plan, const void* tables_dev, float* p, const float* g, float* buf, float lr, float momentum,
-                  float weight_decay, int nesterov, int lr_scale, float grad_scale, float max_norm, const float* grad_sumsq,
+int das_muon_step(const DasNsPlan* plan, const void* tables_dev, float* p, const float* g, float* buf, double lr, double momentum,
+                  double weight_decay, int nesterov, int lr_scale, float grad_scale, float max_norm, const float* grad_sumsq,
                   void* ws, void* stream);
 /* AdamW on flat f32 buffers, g' as above, t = step >= 1:
  *   m = beta1 m + (1 - beta1) g';  v = beta2 v + (1 - beta2) g'^2;

@@ -150,3 +150,18 @@ def test_arguments_beside_a_plan():
     for kw in (dict(steps=5), dict(coefficients=COEF), dict(coefficients=[COEF] * 5, eps=1e-7), dict(steps=None)):
         assert torch.equal(T.orthogonalize([u], plan=plan, **kw)[0], want)
     assert torch.equal(T.orthogonalize([u])[0], want) and torch.equal(T.orthogonalize([u], steps=5, coefficients=COEF, eps=1e-7)[0], want)
+
+
+@pytest.mark.parametrize('shape', [(30, 50), (30, 4000), (200, 100)])
+@pytest.mark.parametrize('momentum', [0.98, 0.95, 0.9])
+def test_muons_average_is_as_exact_as_f32(momentum, shape):
+    """mu m + (1 - mu) g: the two factors, the two products and the sum are rounded once each, half a step (2^-24) at most, of terms whose sum of sizes
+    is |mu m| + |(1 - mu) g|: three of them on either way"""
+    from das_amd import train_ops as T
+    gen = torch.Generator().manual_seed(1)
+    n = shape[0] * shape[1]
+    p, g, m = (torch.randn(n, generator=gen).to(DEV) for _ in range(3))
+    m[::2] = 0
+    a, b = momentum * m.double(), (1 - momentum) * g.double()
+    T.muon_step(p, g, m, T.NewtonSchulzPlan([shape], DEV), lr=0.1, momentum=momentum)
+    assert ((m.double() - (a + b)).abs() <= 3 * 2.0 ** -24 * (a.abs() + b.abs())).all()
