@@ -652,7 +652,7 @@ class FlatMuon(FlatAdamW):
     A matrix is a 2-D weight, or a conv weight as output channels x (taps * input channels): the flat storage holds it as exactly that,
     dense, so one das_muon_step call updates them all in place (momentum average, Newton-Schulz orthogonalisation, decoupled decay).
     To AdamW go 1-D parameters, matrices with fewer than `min_side` rows or columns (a row alone would only be normalised: the
-    1- to 3-channel predictors, the flows' coordinates) and names that contain one of `adamw_params`.
+    1- to 3-channel predictors, the flows' coordinates) and names that contain one of `adamw_params` (several names, or one).
     lr drives the matrices, adamw_lr (default: lr) the rest; a schedule that sets lr scales both. lr_scale: 'original' or
     'match_rms_adamw' (train_ops.muon_step). `state_dict()`: momentum_buffer for matrices, AdamW's state for the rest.
     Several ranks: every rank updates every matrix from the summed gradient, to the same bits."""
@@ -664,7 +664,7 @@ class FlatMuon(FlatAdamW):
                  adamw_weight_decay=None, bias_lr_mult=1.0, bias_decay_mult=1.0, **kw):
         if not 0 <= momentum < 1 or lr_scale not in ('original', 'match_rms_adamw') or not lr > 0:
             raise ValueError(f"Muon: lr > 0, momentum in [0, 1), lr_scale 'original' or 'match_rms_adamw'; got {lr}, {momentum}, {lr_scale!r}")
-        self._min_side, self._adamw_names = int(min_side), tuple(adamw_params)
+        self._min_side, self._adamw_names = int(min_side), (adamw_params,) if isinstance(adamw_params, str) else tuple(adamw_params)
         ratio = 1.0 if adamw_lr is None else adamw_lr / lr
         rest_wd = weight_decay if adamw_weight_decay is None else adamw_weight_decay
         super().__init__(model, lr, betas=betas, eps=eps, weight_decay=rest_wd, bias_lr_mult=ratio * bias_lr_mult,

@@ -129,3 +129,12 @@ def test_sizes_past_the_librarys_integers_are_refused():
                        ([(8, 8)], dict(offsets=[(1 << 64) + 64])), ([(1 << 21, 1 << 14, 1 << 14)], {})):
         with pytest.raises(DasHipError):
             T.NewtonSchulzPlan(shapes, 'cuda:0', **kw)
+
+
+@pytest.mark.parametrize('names', ['2.w', ['2.w'], ('2.w', 'nothing')])
+def test_adamw_params_is_one_name_or_several(names):
+    """(a name alone is not its letters: '2.w' is part of no other name, but '.' is part of all)"""
+    from das_amd.optim import build_optimizer
+    opt = build_optimizer(list(nets())[0](), dict(type='Muon', lr=1e-2, adamw_params=names))
+    by = {n: next(g['key'] for g in opt.groups if g['start'] <= sl.off < g['end']) for n, sl in zip(opt._names, opt.slots)}
+    assert by['0.weight'] == 'matrix' and by['2.weight'] == 'main'
