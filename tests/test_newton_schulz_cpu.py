@@ -138,3 +138,21 @@ def test_adamw_params_is_one_name_or_several(names):
     opt = build_optimizer(list(nets())[0](), dict(type='Muon', lr=1e-2, adamw_params=names))
     by = {n: next(g['key'] for g in opt.groups if g['start'] <= sl.off < g['end']) for n, sl in zip(opt._names, opt.slots)}
     assert by['0.weight'] == 'matrix' and by['2.weight'] == 'main'
+
+
+@pytest.mark.parametrize('rank', [1, 16, 0])
+@pytest.mark.parametrize('shape', [(1, 64), (64, 64), (30, 3000), (300, 200)])
+def test_the_bounds_reject_wrong_results(monkeypatch, shape, rank):
+    """the limits of the GPU tests of five steps, on the CPU: zeros, the negated result, the normalised input, a step too few or too many and a tile
+    of 16 x 16 left out are all far outside; the result in f32 and its bf16 rounding are inside"""
+    import test_newton_schulz_gpu as g
+    monkeypatch.setattr(g, 'DEV', 'cpu')
+    u = g.low_rank(*shape, rank, 3)
+    ref = g.polar64(u)
+    limit, half = g.pairs_bound(min(shape), rank or min(shape)), (g.pairs_bound(min(shape), rank or min(shape)) ** 2 + 2.0 ** -16 / 3) ** 0.5
+    hole = ref.clone()
+    i = int(ref.abs().argmax())
+    hole[i // shape[1] // 16 * 16:][:16, i % shape[1] // 16 * 16:][:, :16] = 0
+    for wrong in (torch.zeros_like(ref), -ref, u.double() / u.double().norm(), g.polar64(u, steps=4), g.polar64(u, steps=6), hole):
+        assert g.off(wrong, u) > 5 * half > 5 * limit
+    assert g.off(ref.float(), u) <= limit and g.off(ref.bfloat16(), u) <= half

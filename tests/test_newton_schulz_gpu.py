@@ -165,3 +165,105 @@ def test_muons_average_is_as_exact_as_f32(momentum, shape):
     a, b = momentum * m.double(), (1 - momentum) * g.double()
     T.muon_step(p, g, m, T.NewtonSchulzPlan([shape], DEV), lr=0.1, momentum=momentum)
     assert ((m.double() - (a + b)).abs() <= 3 * 2.0 ** -24 * (a.abs() + b.abs())).all()
+
+
+# sets whose launches are of every form: (tile side, wave groups a tile, whether inner axes are split) of X X^T and of the m x m products, (tile side,
+# wave groups) of Q X; odd and ragged sizes
+FORMS = [([(1, 256, 2304)], (64, 4, True), (64, 4, False), (64, 4)),
+         ([(8, 145, 1547)], (64, 4, True), (64, 4, False), (128, 2)),
+         ([(12, 141, 1616), (9, 227, 1084)], (64, 4, False), (64, 4, False), (128, 1)),
+         ([(2, 998, 981)], (128, 2, True), (64, 4, False), (64, 4)),
+         ([(5, 530, 370), (6, 729, 387)], (128, 2, True), (64, 4, False), (128, 2)),
+         ([(9, 597, 929), (3, 284, 1781)], (128, 2, True), (128, 2, False), (128, 1)),
+         ([(2, 1805, 867), (12, 1164, 386)], (128, 2, True), (128, 2, True), (128, 1)),
+         ([(1, 2048, 2048)], (128, 2, False), (128, 2, False), (128, 2)),
+         ([(12, 297, 1921), (10, 974, 929)], (128, 1, True), (128, 1, False), (128, 1)),
+         ([(5, 802, 1142), (1, 1981, 186), (11, 918, 1057), (3, 64, 64), (2, 30, 3000), (1, 5000, 12)], (128, 1, True), (128, 1, True), (128, 1)),
+         ([(5, 64, 64), (2, 1, 256), (3, 30, 3000), (1, 5000, 12), (2, 64, 257)], None, None, None)]
+
+
+def stacks(shapes, seed):
+    gen = torch.Generator(DEV).manual_seed(seed)
+    out = []
+    for k, r, c in shapes:
+        pix = 2 * max(r, c)
+        d = torch.randn(k, r, pix, generator=gen, device=DEV) * torch.exp(torch.randn(k, r, 1, generator=gen, device=DEV))
+        x = (torch.randn(k, pix, c, generator=gen, device=DEV) + torch.randn(k, pix, 1, generator=gen, device=DEV)).relu()
+        out.append(d @ x)
+    return out
+
+
+def polar64_stack(u, steps, coef=COEF):
+    x = u.double() / (torch.linalg.matrix_norm(u.double())[:, None, None] + 1e-7)
+    x = x.mT.contiguous() if x.shape[1] > x.shape[2] else x
+    a, b, c = coef
+    for _ in range(steps):
+        g = x @ x.mT.contiguous()
+        x = a * x + (b * g + c * (g @ g)) @ x
+    return x.mT if u.shape[1] > u.shape[2] else x
+
+
+def check_stack(got, u, ref, what):
+    """every matrix of a stack; fewer steps than five lose less than pairs_bound has"""
+    d = torch.linalg.matrix_norm(got.double() - ref) / torch.linalg.matrix_norm(ref)
+    limit = pairs_bound(min(u.shape[1:]), min(u.shape[1:]))
+    assert (d <= limit).all(), (what, tuple(u.shape), d.tolist(), limit)
+
+
+@pytest.mark.parametrize('steps', [1, 2, 3, 4, 5])
+@pytest.mark.parametrize('form', range(len(FORMS)))
+def test_every_form_of_the_launches(form, steps):
+    """every matrix of sets that reach every kernel, with the forms named so that another schedule shows; Muon's results by a parameter of zero that
+    becomes -f X; bf16 results"""
+    from das_amd import train_ops as T
+    shapes, gram, product, update = FORMS[form]
+    plan = T.NewtonSchulzPlan(shapes, DEV, steps=steps)
+    p = plan._flat[0]
+    if gram:
+        assert (p.gram_tile, p.gram_kg, p.n_gram_join > 0) == gram and (p.update_tile, p.update_kg) == update
+        assert (p.product_tile, p.product_kg, p.n_product_join > 0) == product
+    mats = stacks(shapes, form)
+    refs = [polar64_stack(u, steps) for u in mats]
+    got = T.orthogonalize(mats, plan=plan, out_dtype=torch.float32)
+    for u, y, ref in zip(mats, got, refs):
+        check_stack(y, u, ref, 'f32')
+    for y, z in zip(got, T.orthogonalize(mats, plan=plan)):
+        assert torch.equal(z, y.bfloat16())
+    g = torch.cat([u.reshape(-1) for u in mats])
+    w, m = torch.zeros_like(g), torch.zeros_like(g)
+    T.muon_step(w, g, m, plan, lr=1.0, momentum=0.0, nesterov=False)
+    assert torch.equal(m, g)
+    at = 0
+    for u, ref in zip(mats, refs):
+        f = max(1.0, u.shape[1] / u.shape[2]) ** 0.5
+        check_stack(-w[at:at + u.numel()].view(u.shape) / f, u, ref, 'muon')
+        at += u.numel()
+
+
+@pytest.mark.parametrize('shape', [(60, 64), (50, 1200), (96, 160), (300, 200)], ids=lambda s: '%dx%d' % s)
+@pytest.mark.parametrize('kind', ['1e-30', '1e-12', '1e12', '1e30', 'spike', 'decay', 'strides', 'transposed', 'expanded', 'bf16 view'])
+def test_five_steps_on_hard_inputs(kind, shape):
+    """magnitudes at f32's ends, one entry over all, singular values over twelve decades, strides and starts: by the bound of a rank-one result"""
+    from das_amd import train_ops as T
+    r, c = shape
+    u, eps = low_rank(r, c, 0, 7), 1e-7
+    if kind[0] == '1':
+        u, eps = u / u.norm() * float(kind), 0.0 if float(kind) < 1 else 1e-7
+    elif kind == 'spike':
+        u = 1e-6 * u / u.norm()
+        u[r - 1, c - 1] = 1e6
+    elif kind == 'decay':
+        a, _, b = torch.linalg.svd(u.cpu().double(), full_matrices=False)
+        u = (a * torch.logspace(0, -12, min(r, c), dtype=torch.float64) @ b).float().to(DEV)
+    elif kind == 'strides':
+        u = low_rank(2 * r + 1, c + 7, 0, 7)[1::2, 3:-4]
+    elif kind == 'transposed':
+        u = low_rank(c, r, 0, 7).t()
+    elif kind == 'expanded':
+        u = u[:1].expand(r, -1)
+    elif kind == 'bf16 view':
+        u = low_rank(r, c + 1, 0, 7).bfloat16()[:, 1:]
+    assert u.shape == shape
+    got = T.orthogonalize(u, eps=eps, out_dtype=torch.float32)
+    assert off(got, u, eps=eps) <= pairs_bound(min(shape), 1)
+    assert torch.equal(T.orthogonalize(u, eps=eps), got.bfloat16())
