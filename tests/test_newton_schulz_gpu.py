@@ -267,3 +267,66 @@ def test_five_steps_on_hard_inputs(kind, shape):
     got = T.orthogonalize(u, eps=eps, out_dtype=torch.float32)
     assert off(got, u, eps=eps) <= pairs_bound(min(shape), 1)
     assert torch.equal(T.orthogonalize(u, eps=eps), got.bfloat16())
+
+
+def x_bound(x, m):
+    """2-norm error of X out of a Muon step: pairs_bound's for what grows (times 0.7, the norm it is over there), the same relative to X for what does
+    not; U's own rounding, four halves of an f32 step, grows like X's"""
+    return 0.7 * pairs_bound(m, 1) + pairs_bound(m, 16) * float(x.norm()) + 3.4445 ** 5 * 4 * 2.0 ** -24
+
+
+@pytest.mark.parametrize('nesterov,lr_scale', [(True, 'original'), (False, 'match_rms_adamw'), (True, 'match_rms_adamw')])
+@pytest.mark.parametrize('rank', [1, 16, 0])
+def test_muon_step_with_momentum_and_decay(nesterov, lr_scale, rank):
+    from das_amd import train_ops as T
+    shapes = [(64, 147), (300, 70), (1, 256), (30, 3000), (700, 513)]
+    n = sum(r * c for r, c in shapes)
+    gen = torch.Generator().manual_seed(rank)
+    g = torch.cat([low_rank(r, c, rank, 1).reshape(-1) for r, c in shapes])
+    m = 0.5 * torch.cat([low_rank(r, c, rank, 2).reshape(-1) for r, c in shapes])
+    p = torch.randn(n, generator=gen).to(DEV)
+    mu, lr, wd = 0.95, 0.5, 0.1
+    m64 = mu * m.double() + (1 - mu) * g.double()
+    u64 = (1 - mu) * g.double() + mu * m64 if nesterov else m64
+    p64 = p.double() * (1 - lr * wd)
+    T.muon_step(p, g, m, T.NewtonSchulzPlan(shapes, DEV), lr=lr, momentum=mu, weight_decay=wd, nesterov=nesterov, lr_scale=lr_scale)
+    at = 0
+    for r, c in shapes:
+        s = slice(at, at + r * c)
+        at += r * c
+        x = polar64(u64[s].view(r, c))
+        f = max(1.0, r / c) ** 0.5 if lr_scale == 'original' else 0.2 * max(r, c) ** 0.5
+        d = float((p[s].double() - p64[s] + lr * f * x.reshape(-1)).norm())
+        assert d <= lr * f * x_bound(x, min(r, c)) + 4 * 2.0 ** -24 * float(p64[s].norm() + lr * f * x.norm()), (r, c)
+
+
+def test_flat_muon_moves_a_detectors_matrices_by_their_orthogonal_factors():
+    """two clipped steps of a small detector: what each matrix moved by, over the learning rate, against 64 bits"""
+    from das_amd.optim import build_optimizer
+    from test_train_step_gpu import make
+    model, data = make('f32')
+    opt = build_optimizer(model, dict(optimizer=dict(type='Muon', lr=0.01, weight_decay=0.1, momentum=0.9, adamw_lr=1e-3),
+                                      optimizer_config=dict(grad_clip=dict(max_norm=35))))
+    group = next(g for g in opt.groups if g['key'] == 'matrix')
+    mats = [(n, p, sl) for n, p, sl in zip(opt._names, opt._params, opt.slots) if group['start'] <= sl.off < group['end']]
+    assert len(mats) > 20
+    m64 = {n: torch.zeros(sl.numel, dtype=torch.float64, device=DEV) for n, _, sl in mats}
+    moved = 0
+    for _ in range(2):
+        opt.zero_grad()
+        model.train_step(data, None)['loss'].backward()
+        opt.all_reduce_grads()
+        before, g = opt.flat_p.double(), opt.flat_g.double()
+        k = min(1.0, 35 / (float(g.norm()) + 1e-6))
+        opt.step(0.01)
+        for n, p, sl in mats:
+            s, r, c = slice(sl.off, sl.off + sl.numel), p.shape[0], p.numel() // p.shape[0]
+            m64[n] = 0.9 * m64[n] + 0.1 * k * g[s]
+            x = polar64((0.1 * k * g[s] + 0.9 * m64[n]).view(r, c))
+            f = max(1.0, r / c) ** 0.5
+            got = (before[s] * (1 - 0.01 * 0.1) - opt.flat_p[s].double()) / (0.01 * f)
+            # (the clip factor's own error scales U, which its norm takes out but for eps)
+            limit = x_bound(x, min(r, c)) + 2.0 ** -16 * float(x.norm()) + 3 * 2.0 ** -24 * float(before[s].norm()) / (0.01 * f)
+            assert float((got - x.reshape(-1)).norm()) <= limit, n
+            moved += float(x.norm()) > 0.5
+    assert moved > 30
