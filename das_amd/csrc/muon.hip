@@ -1416,10 +1416,15 @@ class Fork {
   hipStream_t main_;
   Side* side_ = nullptr;
 };
-// It pays beside launches of tens of microseconds (the detector's set 2276 -> 2216 us), that is with 128 x 128 tiles of the products. Its
-// events cost the host 80 us a call: as much as it hides beside 64 x 64 ones (182 us either way for seven small and thin matrices with two of
-// 129 x 1023 and one of 700 x 513), more where there are no tiles (60 -> 85 us for five small and thin ones).
-bool worth_a_fork(const DasNsPlan* p) { return p->product_tile == 128 && p->n_tile_chunks > 0 && p->n_small + p->n_thin > 0; }
+// It pays beside launches of tens of microseconds (the detector's set 2276 -> 2216 us), that is with 128 x 128 tiles of the products; beside 64 x 64
+// ones where there is a whole chain of eight launches to hide, of small and of thin matrices, and tiles to hide it under: 700 x 513 (45 tiles) with one
+// 64 x 64 and one 64 x 5000 254 -> 190 us in a queue of calls, 281 -> 248 alone; but 256 x 2304 (10 tiles) with one 16 x 16 and one 8 x 5000 161 -> 158 and 187 ->
+// 200, 128 x 256 with five 64 x 64 114 -> 118, 700 x 513 with two 1 x 256 185 -> 194: its events cost the host 50 ... 80 us a call. Without tiles
+// there is nothing to be beside (60 -> 85 us for five small and thin ones).
+bool worth_a_fork(const DasNsPlan* p) {
+  if (p->n_tile_chunks == 0 || p->n_small + p->n_thin == 0) return false;
+  return p->product_tile == 128 || (p->n_small > 0 && p->n_thin > 0 && p->n_product >= 32);
+}
 
 Steps steps_of(const DasNsPlan* p) {
   Steps st;

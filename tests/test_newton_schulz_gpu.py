@@ -330,3 +330,27 @@ def test_flat_muon_moves_a_detectors_matrices_by_their_orthogonal_factors():
             assert float((got - x.reshape(-1)).norm()) <= limit, n
             moved += float(x.norm()) > 0.5
     assert moved > 30
+
+
+def test_second_stream_beside_small_tiles():
+    """a chain of small and thin matrices beside 64 x 64 tiles: the same bits as captured, where one stream does all, with sources and results reused
+    at once behind the call"""
+    from das_amd import train_ops as T
+    shapes = [(1, 700, 513), (3, 64, 64), (2, 27, 2304), (1, 64, 5000)]
+    mats = stacks(shapes, 1)
+    plan = T.NewtonSchulzPlan(shapes, DEV)
+    assert plan._flat[0].product_tile == 64 and plan._flat[0].n_product >= 32 and plan._flat[0].n_small and plan._flat[0].n_thin
+    static, graph = [t.clone() for t in mats], torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        want = T.orthogonalize(static, plan=plan, out_dtype=torch.float32)
+    graph.replay()
+    for _ in range(20):
+        buf = [t.clone() for t in mats]
+        got = T.orthogonalize(buf, plan=plan, out_dtype=torch.float32)
+        for b in buf:
+            b.zero_()
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+    for u, y in zip(mats, got):
+        check_stack(y, u, polar64_stack(u, 5), 'second stream')
