@@ -4,21 +4,23 @@
 // X = (a I + b X X^T + c (X X^T)^2) X: in singular values s -> s (a + b s^2 + c s^4). All matrices of a set go through the same launches:
 // a table (built once on the host, das_ns_plan) lists every tile of every matrix, one workgroup per tile.
 //
-// Every operand is a pair of f16, high + low part, 22 bits, and a product is three (high high + high low + low high), whatever the result's type:
-// an error of X outside its row and column space grows by |a| a step, 485-fold in five default ones. Single f16 operands, 11 bits, would do for
-// gradients of full rank (2e-3 off 64-bit arithmetic in bf16 with its own rounding, and 1.4 to 2.1 times faster), but lose gradients out of few
-// pixels: rank 128 1e-2, rank 16 4e-2, rank one 0.2 off. Pairs, f32 result: full rank 2e-6 ... 5e-6, rank 16 2e-5 ... 6e-5, rank one 9e-5 (256 x 2304)
-// ... 3e-4 (4096 x 4096). More steps, or steeper ones, cost the product of the polynomial's slopes.
-// To pay for three products the m x n matrix is touched as seldom as possible: Z(G) commutes with G, so several steps can be taken on m x m
-// matrices alone,
+// Every operand is a pair of f16, high + low part, 22 bits, and a product is three (high high + high low + low high), whatever the
+// result's type: an error of X outside its row and column space grows by |a| a step, 485-fold in five default ones. Single f16 operands,
+// 11 bits, would do for gradients of full rank (2e-3 off 64-bit arithmetic in bf16 with its own rounding, and 1.4 to 2.1 times faster),
+// but lose gradients out of few pixels: rank 128 1e-2, rank 16 4e-2, rank one 0.2 off. Pairs, f32 result: full rank 2e-6 ... 5e-6, rank
+// 16 2e-5 ... 6e-5, rank one 9e-5 (256 x 2304) ... 3e-4 (4096 x 4096). More steps, or steeper ones, cost the product of the polynomial's
+// slopes. To pay for three products the m x n matrix is touched as seldom as possible: Z(G) commutes with G, so several steps can be
+// taken on m x m matrices alone,
 //   G = X X^T;  each step  Z = a I + b G + c G G,  Q = Z Q,  G = X' X'^T = Z G Z;  X' = Q X at the end of such a phase
-// 18 m m n + 42 m^3 flops for five steps (plain steps with three products: 45 m m n + 15 m^3; a symmetric product is computed on and below its
-// diagonal). A phase ends before an error of G, which grows by (a + b s^2 + c s^4)^2 a step in the direction of small singular values s while
-// G's true entries there grow alike but start smaller, has grown 256-fold: with the default polynomial three steps, then two.
+// 18 m m n + 42 m^3 flops for five steps (plain steps with three products: 45 m m n + 15 m^3; a symmetric product is computed on and
+// below its diagonal). A phase ends before an error of G, which grows by (a + b s^2 + c s^4)^2 a step in the direction of small singular
+// values s while G's true entries there grow alike but start smaller, has grown 256-fold: with the default polynomial three steps, then
+// two.
 //
-// Scales keep entries, and the low parts of pairs, among f16's normal numbers. X is kept times S, 2^15 over the bound of its norm: an entry of
-// a rank-one X is about (m n)^-1/2, and with S = sqrt(n) its low part was subnormal, 2^-25 off (4096 x 4096, f32 result: 8e-4 off instead of
-// 3e-4). G is kept times gscale, about m (its trace starts at one). Row lengths are padded with zeros (ldx, lda) to whole stages of the inner axis.
+// Scales keep entries, and the low parts of pairs, among f16's normal numbers. X is kept times S, 2^15 over the bound of its norm: an
+// entry of a rank-one X is about (m n)^-1/2, and with S = sqrt(n) its low part was subnormal, 2^-25 off (4096 x 4096, f32 result: 8e-4
+// off instead of 3e-4). G is kept times gscale, about m (its trace starts at one). Row lengths are padded with zeros (ldx, lda) to whole
+// stages of the inner axis.
 #include <algorithm>
 #include <cmath>
 #include <cstring>
@@ -320,8 +322,8 @@ __global__ __launch_bounds__(TPB) void normalise_kernel(const NsMatrix* __restri
 // swizzled by row, read with ds_read_tr16_b64 (four inner rows x 16 columns a 16-lane group, one column a lane).
 typedef short i16x4_t __attribute__((ext_vector_type(4)));
 
-// 16 bytes a lane, global -> LDS (lane 0's destination + 16 l). Issued from asm: for the builtin hipcc waits for every copy in flight in front
-// of the next LDS read. The waits are multiply()'s. M0 (the destination) is put back.
+// 16 bytes a lane, global -> LDS (lane 0's destination + 16 l). Issued from asm: for the builtin hipcc waits for every copy in flight in
+// front of the next LDS read. The waits are multiply()'s. M0 (the destination) is put back.
 __device__ __forceinline__ void copy16(const void* src, const char* lds_wave_base) {
   unsigned keep;
   const unsigned dst = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(const __attribute__((address_space(3))) char*)lds_wave_base);
@@ -742,11 +744,11 @@ __global__ __launch_bounds__(KG * TPB, KG == 1 ? 2 : KG) void update_kernel(cons
 // all steps of a phase on the m x m matrices in LDS and leaves Q; the pass over the slices that forms Q X also forms the parts of the next
 // X X^T: five launches after the first pass (16 x 1056 by tiles: 85 us).
 //
-// 16 waves, one 16 x 16 fragment of an m x m product a wave (2 x 2 fragments each on four waves: 20.4 us for 64 x 64 instead of 19.8,
-// the flows' and predictors' set, up to 64 x 256, 31.7 us instead of 25.0: one wave a SIMD hides no latency). m <= 32 leaves waves over: they divide the long inner axis of X X^T,
-// and Z Q and Z G are formed by different ones. LDS matrices: rows of pairs (32 high parts, 32 low parts, ...), row pitch 16 bytes past a multiple of 256;
-// 32 columns of X take 128 bytes as pairs and as floats: U, X and the result use the same place. Rows and columns up to the next
-// multiple of 16 are zero.
+// 16 waves, one 16 x 16 fragment of an m x m product a wave (2 x 2 fragments each on four waves: 20.4 us for 64 x 64 instead of 19.8, the
+// flows' and predictors' set, up to 64 x 256, 31.7 us instead of 25.0: one wave a SIMD hides no latency). m <= 32 leaves waves over: they
+// divide the long inner axis of X X^T, and Z Q and Z G are formed by different ones. LDS matrices: rows of pairs (32 high parts, 32 low
+// parts, ...), row pitch 16 bytes past a multiple of 256; 32 columns of X take 128 bytes as pairs and as floats: U, X and the result use
+// the same place. Rows and columns up to the next multiple of 16 are zero.
 constexpr int SMALL_M = 64, SMALL_TPB = 1024, SMALL_LDS = 155 * 1024;
 constexpr int PA = 2 * SMALL_M + 8;   // row pitch of the m x m matrices, f16 elements
 constexpr int SMALL_QUADS = 8;        // float4 of U, and 16 x 16 fragments of X, a thread / wave can have: m n <= 32 Ki (fewer where a set allows it: no spills)
@@ -838,8 +840,8 @@ struct Share {
     c0 = (f % n) * 16;
   }
 };
-// P Q^T's fragment stored transposed (four values of a lane are neighbours then), so that Q P^T is what lies there: f(row, col, four values)
-// may change them
+// P Q^T's fragment stored transposed (four values of a lane are neighbours then), so that Q P^T is what lies there: f(row, col, four
+// values) may change them
 template <typename F>
 __device__ __forceinline__ void frag_store(const Share& w, const f32x4_t& acc, _Float16* out, F f) {
   const int lane = threadIdx.x & 63, r = w.c0 + (lane & 15), c = w.r0 + (lane >> 4) * 4;
@@ -862,10 +864,10 @@ __device__ __forceinline__ void store_gram(const Share& w, f32x4_t acc, f32x4_t*
     });
   __syncthreads();
 }
-// Steps k ... end - 1 on the m x m matrices (the same products as iterate), G in A[0]; -> Q
-// The factors' order matters to rounding errors alone. Between the null space of X X^T, where Z is near 3.4, and the rest, where it is near 1, those
-// of Z G Z and of Z Q (Q's columns in the rest) grow by the product of both a step, those of Z Z G or Q Z by the larger one squared
-// (64 x 64 of rank one: 4e-4 off instead of 2e-5). The tiles' form has no order: it computes one half and mirrors it.
+// Steps k ... end - 1 on the m x m matrices (the same products as iterate), G in A[0]; -> Q.
+// The factors' order matters to rounding errors alone. Between the null space of X X^T, where Z is near 3.4, and the rest, where it is
+// near 1, those of Z G Z and of Z Q (Q's columns in the rest) grow by the product of both a step, those of Z Z G or Q Z by the larger one
+// squared (64 x 64 of rank one: 4e-4 off instead of 2e-5). The tiles' form has no order: it computes one half and mirrors it.
 template <int K>   // K inner steps of 32: m <= 32 K
 __device__ __forceinline__ _Float16* phase_chain(const Share& w, _Float16* const (&A)[N_AREAS], const Steps& st, int k, int end, float gscale) {
   const bool on = w.part == 0, second = w.part == (w.parts > 1 ? 1 : 0);
@@ -1268,7 +1270,8 @@ Work carve(const DasNsPlan* p, void* ws) {
   return w;
 }
 
-// Lets a kernel have a whole CU's dynamic LDS: asked of the runtime once a thread, device and kernel (in front of every launch: 0.4 us of host time each)
+// Lets a kernel have a whole CU's dynamic LDS: asked of the runtime once a thread, device and kernel (in front of every launch: 0.4 us of
+// host time each)
 void allow_lds(const void* kernel) {
   constexpr int KERNELS = 64;
   thread_local const void* seen[KERNELS];
@@ -1327,9 +1330,10 @@ int phase_end(const Bounds* bound, int steps, int k) {
   return end;
 }
 
-// A second stream for the small and thin matrices of a set that holds others too: a chain of short launches that leaves the GPU nearly empty,
-// beside the tiles' launches instead of before them, from their own part of the first pass on (fork and join by events; the caller's stream waits for the end). Streams of
-// default priority, from a pool: one call has one for itself. A call that is being captured stays on its stream.
+// A second stream for the small and thin matrices of a set that holds others too: a chain of short launches that leaves the GPU nearly
+// empty, beside the tiles' launches instead of before them, from their own part of the first pass on (fork and join by events; the
+// caller's stream waits for the end). Streams of default priority, from a pool: one call has one for itself. A call that is being
+// captured stays on its stream.
 struct Side {
   int dev = 0;
   hipStream_t stream = nullptr;
@@ -1416,11 +1420,12 @@ class Fork {
   hipStream_t main_;
   Side* side_ = nullptr;
 };
-// It pays beside launches of tens of microseconds (the detector's set 2276 -> 2216 us), that is with 128 x 128 tiles of the products; beside 64 x 64
-// ones where there is a whole chain of eight launches to hide, of small and of thin matrices, and tiles to hide it under: 700 x 513 (45 tiles) with one
-// 64 x 64 and one 64 x 5000 254 -> 190 us in a queue of calls, 281 -> 248 alone; but 256 x 2304 (10 tiles) with one 16 x 16 and one 8 x 5000 161 -> 158 and 187 ->
-// 200, 128 x 256 with five 64 x 64 114 -> 118, 700 x 513 with two 1 x 256 185 -> 194: its events cost the host 50 ... 80 us a call. Without tiles
-// there is nothing to be beside (60 -> 85 us for five small and thin ones).
+// It pays beside launches of tens of microseconds (the detector's set 2276 -> 2216 us), that is with 128 x 128 tiles of the products;
+// beside 64 x 64 ones where there is a whole chain of eight launches to hide, of small and of thin matrices, and tiles to hide it under:
+// 700 x 513 (45 tiles) with one 64 x 64 and one 64 x 5000 254 -> 190 us in a queue of calls, 281 -> 248 alone; but 256 x 2304 (10 tiles)
+// with one 16 x 16 and one 8 x 5000 161 -> 158 and 187 -> 200, 128 x 256 with five 64 x 64 114 -> 118, 700 x 513 with two 1 x 256 185 ->
+// 194: its events cost the host 50 ... 80 us a call. Without tiles there is nothing to be beside (60 -> 85 us for five small and thin
+// ones).
 bool worth_a_fork(const DasNsPlan* p) {
   if (p->n_tile_chunks == 0 || p->n_small + p->n_thin == 0) return false;
   return p->product_tile == 128 || (p->n_small > 0 && p->n_thin > 0 && p->n_product >= 32);
@@ -1660,8 +1665,9 @@ long long makespan(const std::vector<int>& pieces, int slots, long long limit, s
 // Symmetric tiles of a launch for `slots` workgroups at a time. Tiles that would end after the others are split along the inner axis
 // where that pays: 1056 equal tiles in 512 slots are two rounds and a sixteenth, and took the time of nearly three. A part costs 128 KiB
 // of traffic, the join a launch: 0.0125 and 1.2 steps of 64 inner elements (2.5 us with two workgroups on a CU; 13 us measured for 272
-// parts), six of the shorter steps of 64 x 64 tiles with four wave groups (4 ... 8 is level; 12: 8x 256 x 1024, Muon, 155 us instead of 150). A workgroup whose neighbour on the CU has ended runs up to twice as fast, so only half of what sticks out counts. A part has
-// at least 4 steps.
+// parts), six of the shorter steps of 64 x 64 tiles with four wave groups (4 ... 8 is level; 12: 8x 256 x 1024, Muon, 155 us instead of
+// 150). A workgroup whose neighbour on the CU has ended runs up to twice as fast, so only half of what sticks out counts. A part has at
+// least 4 steps.
 void schedule(const Tables& tab, const std::vector<Tile>& tiles, int slots, double join_cost, Launch& launch, std::vector<NsItem>& join, long long& n_slots) {
   auto item = [&](auto... v) { return tab.item(v...); };
   std::vector<int> order(tiles.size()), parts(tiles.size(), 1), late;
@@ -1829,15 +1835,15 @@ bool build(const DasNsShape* shapes, int n, double top, DasNsPlan* plan, Tables&
   const int tiled_end = (int)(t.mats.size() - t.thin.size());
   // Products and updates: 64 x 64 tiles whose inner axis four wave groups share while the 256 CUs have them in two rounds (9x 512x512,
   // Muon: 314 us, 372 with 128 x 128 ones), else 128 x 128 (24x 512x512: 435 us, 576 with 64 x 64 ones). Where a CU gets one of those,
-  // two wave groups share it: at most 256 of an update, which has no second round to fill (512-channel bottleneck, 272 tiles: 233 us, 254 with two
-  // groups), under 384 of a product, whose long ones are split (2048x2048, 136 tiles: 1084 -> 853 us).
+  // two wave groups share it: at most 256 of an update, which has no second round to fill (512-channel bottleneck, 272 tiles: 233 us, 254
+  // with two groups), under 384 of a product, whose long ones are split (2048x2048, 136 tiles: 1084 -> 853 us).
   plan->product_tile = lower64 > 512 ? 128 : 64;
   plan->product_kg = plan->product_tile == 64 ? 4 : lower128 >= 384 ? 1 : 2;
   plan->update_tile = all64 > 512 ? 128 : 64;
   plan->update_kg = plan->update_tile == 64 ? 4 : all128 > 256 ? 1 : 2;
-  // X X^T, whose inner axis is long and may be split: 64 x 64 tiles and four wave groups for one round of the CUs (256 x 2304 to bf16: 109 -> 99 us,
-  // 512 x 512 114 -> 99, 128 x 1152 Muon 109 -> 101; 12x 512 x 2048, 432 tiles: 470 us, 486 with 64 x 64 ones), then 128 x 128; where
-  // there are fewer than 384 of those, two wave groups share a tile (one workgroup a CU, not two)
+  // X X^T, whose inner axis is long and may be split: 64 x 64 tiles and four wave groups for one round of the CUs (256 x 2304 123 us, 131
+  // with 128 x 128 ones; 512 x 512 157, 165; 1024 x 1024 249, 254; but 12x 512 x 2048, 432 tiles: 486, 470 with 128 x 128 ones), then 128
+  // x 128; where there are fewer than 384 of those, two wave groups share a tile (one workgroup a CU, not two)
   plan->gram_tile = lower64 <= 256 ? 64 : 128;
   plan->gram_kg = lower64 <= 256 ? 4 : lower128 >= 384 ? 1 : 2;
   // blocks of up to 8 x 8 tiles, smaller where one would be more than a 16th of the launch (half of an XCD's part)

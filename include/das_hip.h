@@ -611,10 +611,11 @@ int das_sgd_momentum_step(float* p, const float* g, float* buf, long long n, flo
  * Newton-Schulz orthogonalisation of a ragged set of matrices. For each matrix U (rows x cols, m = min, n = max of the two,
  * transposed if rows > cols so that X is m x n):
  *   X = U / (|U|_F + eps);   steps times:  A = X X^T,  B = a I + b A + c A^2,  X = B X.
- * Operands are pairs of f16 (22 bits) and sums f32, whatever the result's type; a result is rounded once. Five steps of the default polynomial are
- * off a 64-bit evaluation, in the 2-norm, by 2e-6 ... 5e-6 for gradients of full rank and up to 3e-4 for rank one (4096 x 4096), where rounding
- * errors outside U's row and column space grow by |a| a step; more or steeper steps cost the product of the polynomial's slopes. Sums of squares are
- * held in f32 by 64 x 64 blocks and added in f64. Results are the same bits from run to run.
+ * Operands are pairs of f16 (22 bits) and sums f32, whatever the result's type; a result is rounded once. Five steps of the
+ * default polynomial are off a 64-bit evaluation, in the 2-norm, by 2e-6 ... 5e-6 for gradients of full rank and up to 3e-4 for rank
+ * one (4096 x 4096), where rounding errors outside U's row and column space grow by |a| a step; more or steeper steps cost the
+ * product of the polynomial's slopes. Sums of squares are held in f32 by 64 x 64 blocks and added in f64. Results are the same bits
+ * from run to run.
  *
  * A plan lists the set once: das_ns_plan() checks the shapes and the polynomial and writes the tables (host memory) that the
  * kernels walk; the caller copies them to the device and hands both to every call. Plans hold no pointers and no results. */
@@ -626,10 +627,13 @@ typedef struct {
   int reserved;
 } DasNsShape;
 typedef struct {
-  int n_groups, n_matrices, n_small, small_lds, small_quads, n_thin, n_slices, n_chunks, n_tile_chunks, n_gram, n_gram_join, n_product, n_product_join, n_update, steps;
+  int n_groups, n_matrices, n_small, small_lds, small_quads, n_thin, n_slices, n_chunks, n_tile_chunks;
+  int n_gram, n_gram_join, n_product, n_product_join, n_update, steps;
   int product_tile, update_tile, product_kg, update_kg, gram_tile, gram_kg;
-  long long x_elems, a_elems, thin_x_elems, thin_a_elems, thin_slots, gram_slots, product_slots, extent;            /* work areas (f16 elements); one past the last element of the flat buffers used */
-  long long mat_at, chunk_at, gram_at, gram_join_at, product_at, product_join_at, update_at, slice_at, thin_at, table_bytes;   /* byte offsets of the tables */
+  /* work areas (f16 elements); extent: one past the last element of the flat buffers used */
+  long long x_elems, a_elems, thin_x_elems, thin_a_elems, thin_slots, gram_slots, product_slots, extent;
+  /* byte offsets of the tables */
+  long long mat_at, chunk_at, gram_at, gram_join_at, product_at, product_join_at, update_at, slice_at, thin_at, table_bytes;
   float coef[3 * DAS_NS_MAX_STEPS];              /* a, b, c of each step */
   int phase_end[DAS_NS_MAX_STEPS];               /* where a run of steps on the m x m matrices that starts here ends */
   float eps;
@@ -640,16 +644,18 @@ typedef struct {
   long long batch_stride, row_stride;
 } DasNsSource;
 /* Fills *plan; with tables != NULL (plan->table_bytes host bytes) also the tables. DAS_ERR_ARG: n < 1, a shape without elements or
- * with a side over 1 << 20 or both over 1 << 15, an offset over 1 << 60, 1 << 22 matrices or 1 << 24 blocks of 64 x 64, overlapping matrices, steps outside 1 ... DAS_NS_MAX_STEPS, a polynomial that takes [0, 1] out of
- * [-16, 16] within `steps` steps or has |a + b s^2 + c s^4| > 64 there (f16 could overflow), eps < 0, or tables too small. */
+ * with a side over 1 << 20 or both over 1 << 15, an offset over 1 << 60, 1 << 22 matrices or 1 << 24 blocks of 64 x 64,
+ * overlapping matrices, steps outside 1 ... DAS_NS_MAX_STEPS, a polynomial that takes [0, 1] out of [-16, 16] within `steps` steps
+ * or has |a + b s^2 + c s^4| > 64 there (f16 could overflow), eps < 0, or tables too small. */
 int das_ns_plan(const DasNsShape* shapes, int n, int steps, const float* coef, float eps, DasNsPlan* plan, void* tables,
                 long long table_bytes);
 /* Workspace of a das_orthogonalize or das_muon_step call */
 long long das_ns_ws_bytes(const DasNsPlan* plan);
-/* out (flat, out_dtype DAS_F32 / DAS_BF16 / DAS_F16, plan offsets): the orthogonalised matrices; srcs: one per group of the plan, in_dtype
- * DAS_F32 / DAS_BF16 / DAS_F16. `ws`: das_ns_ws_bytes() of device memory, 16-byte aligned, in use until the call's kernels end. `out`, the
- * sources and ws do not overlap. Small and thin matrices of a set that holds many or large others run on a stream of the library's own (default priority,
- * created at first need, kept) beside `stream`, which waits for them; a call that is being captured uses `stream` alone. */
+/* out (flat, out_dtype DAS_F32 / DAS_BF16 / DAS_F16, plan offsets): the orthogonalised matrices; srcs: one per group of the plan,
+ * in_dtype DAS_F32 / DAS_BF16 / DAS_F16. `ws`: das_ns_ws_bytes() of device memory, 16-byte aligned, in use until the call's
+ * kernels end. `out`, the sources and ws do not overlap. Small and thin matrices of a set that holds many or large others may run
+ * on a stream of the library's own (default priority, created at first need, kept) beside `stream`, which waits for them; a call
+ * that is being captured uses `stream` alone. */
 int das_orthogonalize(const DasNsPlan* plan, const void* tables_dev, const DasNsSource* srcs, int n_srcs, int in_dtype, void* out,
                       int out_dtype, void* ws, void* stream);
 /* Muon: with g' = g * grad_scale * min(1, max_norm / (sqrt(*grad_sumsq) * grad_scale + 1e-6)) (no clipping for max_norm <= 0),
@@ -662,7 +668,8 @@ int das_muon_step(const DasNsPlan* plan, const void* tables_dev, float* p, const
                   void* ws, void* stream);
 /* AdamW on flat f32 buffers, g' as above, t = step >= 1:
  *   m = beta1 m + (1 - beta1) g';  v = beta2 v + (1 - beta2) g'^2;
- *   p = p (1 - lr weight_decay) - lr (m / (1 - beta1^t)) / (sqrt(v / (1 - beta2^t)) + eps). The four buffers do not overlap: DAS_ERR_ARG otherwise. */
+ *   p = p (1 - lr weight_decay) - lr (m / (1 - beta1^t)) / (sqrt(v / (1 - beta2^t)) + eps).
+ * The four buffers do not overlap: DAS_ERR_ARG otherwise. */
 int das_adamw_step(float* p, const float* g, float* m, float* v, long long n, double lr, double beta1, double beta2, double eps,
                    double weight_decay, long long step, float grad_scale, float max_norm, const float* grad_sumsq, void* stream);
 
