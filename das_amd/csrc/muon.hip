@@ -66,9 +66,10 @@ struct Partial {            // of one 64 x 64 block: sum of squares of (u 2^-e),
   int e;
 };
 
-// v as a pair of f16: v rounded, and what that leaves. Both parts come from one f32 value: the empty asm (no instruction) keeps hipcc from
-// fusing the multiplication that v comes from into one of two conversions of it. v_fma_mixlo_f16 rounds the product once, v_mul_f32 and
-// v_cvt_pk_f16_f32 round it twice: next to a tie they differ, and a high part with the low part of its neighbour is 2^-11 of v off.
+// v as a pair of f16: v rounded, and what that leaves. Both parts come from one f32 value: the empty asm (no instruction; what comes here is a
+// sum or a product formed by the vector unit, or was loaded) keeps hipcc from fusing the multiplication that v comes from into one of two
+// conversions of it. v_fma_mixlo_f16 rounds the product once, v_mul_f32 and v_cvt_pk_f16_f32 round it twice: next to a tie they differ, and
+// a high part with the low part of its neighbour is 2^-11 of v off (one element in 2^15; rank one, 256 x 2304: 7.4e-4 off instead of 1.3e-4).
 struct Pair {
   _Float16 high, low;
 };
